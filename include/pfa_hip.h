@@ -40,6 +40,7 @@ extern "C" {
 #define PFA_BF16 1
 #define PFA_F16 2
 #define PFA_I8 3   /* symmetric int8 with a float scale per head */
+#define PFA_E4M3 4 /* 8-bit float (OCP e4m3), cells of pfa_kv_pages only */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int pfa_version(void);
@@ -632,6 +633,91 @@ int pfa_int8_kv_attn_fwd(pfa_tensor4 q, pfa_tensor4 out, int64_t T, int H, int D
                          const float* v_scale, const int32_t* key_pos, int S,
                          int causal, float scale, void* workspace,
                          size_t ws_bytes, void* stream);
+
+/* ====================================================================
+ * Paged key-value cache and the attention of one new token over it.  No
+ * counterpart in the reference, whose forward takes whole sequences.
+ *
+ * A pool holds n_pages pages of page_size tokens (16, 32, 64, 128 or 256)
+ * for kv_heads heads of head_dim (16, 32, 64 or 128): cells k and v
+ * [page][head][slot][d] in `dtype` (PFA_F32 / PFA_BF16 / PFA_F16 / PFA_I8 /
+ * PFA_E4M3), pages k_page / v_page cells apart (inner dimensions dense, rows
+ * 16-byte aligned).  PFA_I8 and PFA_E4M3 cells have one f32 scale per token
+ * and head, k_scale and v_scale [page][head][slot].  k_bounds, or NULL, are
+ * the least and the largest stored key of every channel of a page's head,
+ * [page][head][2][d], in the cells' type, or f32 for 8-bit cells.
+ *
+ * Position t of sequence b lies in slot t % page_size of page
+ * table[b * table_stride + t / page_size].  A row of the table has
+ * table_pages entries.  Entries that name no page of the pool (-1, say) hold
+ * no keys: nothing is written there, zeros are read, attention leaves them
+ * out.  Two entries with the same page share its keys; two writes to it in
+ * one call leave either's.
+ * ==================================================================== */
+typedef struct pfa_kv_pages {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  void* k_bounds;
+  int64_t k_page, v_page;
+  int n_pages, kv_heads, page_size, head_dim, dtype;
+} pfa_kv_pages;
+
+/* New tokens k, v [b][h][t][d] (n for each of B sequences, dtype PFA_F32 /
+ * PFA_BF16 / PFA_F16: the cells' own, or any of the three for 8-bit cells)
+ * into their pages: token i < counts[b] (all n where counts is NULL) goes to
+ * position starts[b] + i.  Positions below zero or behind the table's last
+ * page are left out.  8-bit cells: scale = max(absmax / top, 1e-6), top 127
+ * (PFA_I8) or 448 (PFA_E4M3), cell = x / scale rounded to nearest even; a row
+ * with a value that is not finite gets scale NaN and zero cells.  k_bounds of
+ * a page's head, where the pool has them: those of the written keys as they
+ * are stored (a NaN among them gives NaN), joined with what stood there
+ * unless the page is written from its first slot on. */
+int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4 v, int dtype,
+                       int B, int64_t n, const int32_t* table, int64_t table_stride,
+                       int table_pages, const int32_t* starts, const int32_t* counts,
+                       void* stream);
+
+/* Positions starts[b] .. starts[b] + counts[b] - 1 (counts NULL: n of them)
+ * of every sequence as values, k_out and v_out (B, n, kv_heads, head_dim) in
+ * out_dtype: cell * scale rounded once.  Rows i >= counts[b], and those
+ * without a page, are zero. */
+int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int32_t* table,
+                      int64_t table_stride, int table_pages, const int32_t* starts,
+                      const int32_t* counts, void* k_out, void* v_out, int out_dtype,
+                      void* stream);
+
+/* Attention of one new token a sequence: q [b][h][d] (H query heads, H a
+ * multiple of kv_heads, head h reads key-value head h / (H / kv_heads); s_t
+ * unused) over positions starts[b] (NULL: 0) .. lengths[b] - 1, or, with
+ * n_selected >= 0, over those of them that lie in the entries of the
+ * sequence's table row that `selected` (B, kv_heads, n_selected) lists
+ * (entries outside of it are left out, an entry listed twice counts twice);
+ * n_selected < 0: no list.  out (B, H, D) dense, in q's type
+ * (PFA_F32 / PFA_BF16 / PFA_F16: the cells' own, or any of the three for
+ * 8-bit cells).  A row that sees no key is zero, and so is one all of whose
+ * scores are -inf.  Sums and softmax statistics are f32. */
+int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int head_dim, int page_size,
+                                  int table_pages, int n_selected, size_t* bytes);
+int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages,
+                       const int32_t* table, int64_t table_stride, int table_pages,
+                       const int32_t* lengths, const int32_t* starts,
+                       const int32_t* selected, int n_selected, float scale, void* out,
+                       void* workspace, size_t ws_bytes, void* stream);
+
+/* The `count` pages of each sequence and key-value head with the best bound on
+ * a score: chosen (B, kv_heads, count) int32, entries of the sequence's table
+ * row in ascending order, -1 behind the last.  A page's score is the largest,
+ * over the group's query heads, of sum_d q_d * (q_d > 0 ? max_d : min_d),
+ * summed in 64 bits and held in 32; NaN counts below everything.  The `first`
+ * first and `last` last entries that hold positions starts[b] ..
+ * lengths[b] - 1 come before all others, then the better score, then the
+ * lower entry; entries without a page are never chosen. */
+int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes);
+int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages,
+                        const int32_t* table, int64_t table_stride, int table_pages,
+                        const int32_t* lengths, const int32_t* starts, int count, int first,
+                        int last, int32_t* chosen, void* workspace, size_t ws_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }

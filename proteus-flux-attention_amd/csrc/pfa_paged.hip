@@ -1,0 +1,505 @@
+// Paged key-value cache: write, read, page selection and the attention of one
+// new token over it.
+#include "pfa_paged.h"
+
+namespace pfa {
+
+using namespace paged;
+
+int paged_check(const pfa_kv_pages* pg, const int32_t* table, int64_t table_stride, int table_pages, int B, Pages* p,
+                Table* t) {
+  PFA_CHECK_ARG(pg->dtype == PFA_F32 || pg->dtype == PFA_BF16 || pg->dtype == PFA_F16 || is8(pg->dtype),
+                "pages: unknown cell type %d", pg->dtype);
+  PFA_CHECK_ARG(pg->head_dim == 16 || pg->head_dim == 32 || pg->head_dim == 64 || pg->head_dim == 128,
+                "pages: head_dim must be 16, 32, 64 or 128 (got %d)", pg->head_dim);
+  PFA_CHECK_ARG(pg->page_size >= 16 && pg->page_size <= 256 && (pg->page_size & (pg->page_size - 1)) == 0,
+                "pages: page_size must be 16, 32, 64, 128 or 256 (got %d)", pg->page_size);
+  PFA_CHECK_ARG(pg->n_pages > 0 && pg->kv_heads > 0 && pg->kv_heads <= 65535 && pg->k && pg->v,
+                "pages: an empty pool");
+  PFA_CHECK_ARG(!is8(pg->dtype) || (pg->k_scale && pg->v_scale), "pages: 8-bit cells need k_scale and v_scale");
+  const int64_t cells = (int64_t)pg->kv_heads * pg->page_size * pg->head_dim;
+  const int e = cell_bytes(pg->dtype);
+  PFA_CHECK_ARG(pg->n_pages == 1 || (pg->k_page >= cells && pg->v_page >= cells), "pages: pages overlap");
+  PFA_CHECK_ARG((uintptr_t)pg->k % 16 == 0 && (uintptr_t)pg->v % 16 == 0 && pg->k_page * e % 16 == 0 &&
+                    pg->v_page * e % 16 == 0 && (uintptr_t)pg->k_scale % 16 == 0 && (uintptr_t)pg->v_scale % 16 == 0 &&
+                    (uintptr_t)pg->k_bounds % 16 == 0,
+                "pages: rows must be 16-byte aligned");
+  PFA_CHECK_ARG(B >= 0 && B <= 65535, "pages: 0 <= B <= 65535 sequences (got %d)", B);
+  PFA_CHECK_ARG(table_pages >= 0 && (int64_t)table_pages * pg->page_size <= (1ll << 30) &&
+                    (table || table_pages == 0 || B == 0),
+                "pages: a block table of up to 2^30 positions (got %d pages)", table_pages);
+  int shift = 4;
+  while ((1 << shift) < pg->page_size) ++shift;
+  *p = Pages{pg->k, pg->v, pg->k_scale, pg->v_scale, pg->k_bounds, pg->k_page, pg->v_page,
+             pg->n_pages, pg->kv_heads, pg->page_size, shift};
+  *t = Table{table, table_stride, table_pages};
+  return PFA_OK;
+}
+
+namespace {
+
+// ---------------------------------------------------------------------
+// Write.  A workgroup takes the tokens of one page and head.  D / 8 lanes
+// hold a row, eight values each: absmax by lane exchanges, the cells in one
+// store, the page's bounds in registers over the rows and joined over the
+// lanes and waves at the end, so no atomics and the same bits in any split of
+// the tokens over calls.
+// ---------------------------------------------------------------------
+__device__ __forceinline__ float min_nan(float a, float b) { return a != a || a < b ? a : b; }
+__device__ __forceinline__ float max_nan(float a, float b) { return a != a || a > b ? a : b; }
+
+struct NewRows {
+  const void* p;
+  int64_t s_b, s_h, s_t;
+  int vec;  // rows aligned to eight elements
+};
+
+template <int DT>
+__device__ __forceinline__ void row8(const NewRows& r, int64_t at, float (&o)[8]) {
+  using T = typename Elem<DT>::T;
+  const T* p = (const T*)r.p + at;
+  if (r.vec) load8<DT>(p, o);
+  else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = load_f<DT>(p + i);
+  }
+}
+
+// Eight values of a row of `lanes` lanes into its cells; x comes back as the
+// values that the cells stand for.
+template <int DT, int CT>
+__device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at, bool first, int lanes, float (&x)[8]) {
+  if constexpr (!is8(CT)) {
+    store8<CT>(dst, x);
+  } else {
+    float m = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      m = fmaxf(m, fabsf(x[i]));
+      finite = finite && fabsf(x[i]) < INFINITY;
+    }
+    if (!finite) m = INFINITY;
+    for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const bool ok = m < INFINITY;
+    const float s = ok ? fmaxf(m / top_of(CT), kLeastScale) : __builtin_nanf("");
+    if (first) *scale_at = s;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = ok ? x[4 * i + j] / s : 0.0f;
+      if constexpr (CT == PFA_I8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float r = rintf(c[j]);
+          w[i] |= ((uint32_t)(int)r & 0xffu) << (8 * j);
+          x[4 * i + j] = r * s;
+        }
+      } else {
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+        p = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], p, true);
+        w[i] = (uint32_t)p;
+        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(p, 0) * s;
+        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(p, 1) * s;
+        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(p, 2) * s;
+        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(p, 3) * s;
+      }
+    }
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  }
+}
+
+template <int DT, int CT>
+__global__ void __launch_bounds__(256) write_kernel(Pages pg, Table tab, NewRows k, NewRows v, int D, int64_t n,
+                                                    const int32_t* __restrict__ starts,
+                                                    const int32_t* __restrict__ counts) {
+  using CellT = typename Cell<CT>::T;
+  const int64_t b = blockIdx.z;
+  const int h = blockIdx.y;
+  const int64_t start = starts[b];
+  int64_t count = counts ? (int64_t)counts[b] : n;
+  count = count < 0 ? 0 : count < n ? count : n;
+  const int64_t first = start < 0 ? 0 : start;  // positions written: [first, end)
+  const int64_t end = start + count;
+  const int64_t ordinal = (first >> pg.shift) + blockIdx.x;
+  const int64_t base = ordinal << pg.shift;
+  const int64_t from = first > base ? first : base, to = end < base + pg.ps ? end : base + pg.ps;
+  if (from >= to) return;
+  const int id = page_at(tab, pg, b, ordinal);
+  if (id < 0) return;
+
+  const int lanes = D / 8, rows = blockDim.x / lanes;
+  const int lane = threadIdx.x % lanes, row = threadIdx.x / lanes;
+  const int64_t kpage = id * pg.k_page + (int64_t)h * pg.ps * D, vpage = id * pg.v_page + (int64_t)h * pg.ps * D;
+  const int64_t spage = ((int64_t)id * pg.H + h) * pg.ps;
+  float lo[8], hi[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+  for (int64_t pos = from + row; pos < to; pos += rows) {
+    const int slot = (int)(pos - base);
+    const int64_t i = pos - start;
+    float x[8], y[8];
+    row8<DT>(k, b * k.s_b + h * k.s_h + i * k.s_t + 8 * lane, x);
+    row8<DT>(v, b * v.s_b + h * v.s_h + i * v.s_t + 8 * lane, y);
+    put8<DT, CT>((CellT*)pg.k + kpage + slot * D + 8 * lane, pg.k_scale + spage + slot, lane == 0, lanes, x);
+    put8<DT, CT>((CellT*)pg.v + vpage + slot * D + 8 * lane, pg.v_scale + spage + slot, lane == 0, lanes, y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], x[j]), hi[j] = max_nan(hi[j], x[j]);
+  }
+  if (!pg.bounds) return;
+  __shared__ float part[2][4][128];
+  for (int o = lanes; o < kWave; o <<= 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo[j] = min_nan(lo[j], __shfl_xor(lo[j], o));
+      hi[j] = max_nan(hi[j], __shfl_xor(hi[j], o));
+    }
+  }
+  const int wave = threadIdx.x / kWave;
+  if (threadIdx.x % kWave < lanes) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[0][wave][8 * lane + j] = lo[j], part[1][wave][8 * lane + j] = hi[j];
+  }
+  __syncthreads();
+  constexpr int BT = bound_dtype(CT);
+  using BoundT = typename Elem<BT>::T;
+  BoundT* out = (BoundT*)pg.bounds + ((int64_t)id * pg.H + h) * 2 * D;
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float a = part[0][0][d], z = part[1][0][d];
+    for (int w = 1; w < (int)blockDim.x / kWave; ++w) a = min_nan(a, part[0][w][d]), z = max_nan(z, part[1][w][d]);
+    if (from > base) a = min_nan(a, load_f<BT>(out + d)), z = max_nan(z, load_f<BT>(out + D + d));
+    store_f<BT>(out + d, a);
+    store_f<BT>(out + D + d, z);
+  }
+}
+
+// ---------------------------------------------------------------------
+// Read: eight values a thread.
+// ---------------------------------------------------------------------
+template <int CT, int OT>
+__global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int D, int64_t n, int64_t total,
+                                                   const int32_t* __restrict__ starts,
+                                                   const int32_t* __restrict__ counts, void* k_out, void* v_out) {
+  using CellT = typename Cell<CT>::T;
+  using OutT = typename Elem<OT>::T;
+  const int lanes = D / 8;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+    const int lane = (int)(at % lanes);
+    int64_t rest = at / lanes;
+    const int h = (int)(rest % pg.H);
+    rest /= pg.H;
+    const int64_t i = rest % n, b = rest / n;
+    const int64_t pos = starts[b] + i;
+    const int id = i < (counts ? (int64_t)counts[b] : n) && pos >= 0 ? page_at(tab, pg, b, pos >> pg.shift) : -1;
+    float x[8] = {}, y[8] = {};
+    if (id >= 0) {
+      const int64_t slot = (int64_t)h * pg.ps + (pos & (pg.ps - 1));
+      cells8<CT>((const CellT*)pg.k + id * pg.k_page + slot * D + 8 * lane, x);
+      cells8<CT>((const CellT*)pg.v + id * pg.v_page + slot * D + 8 * lane, y);
+      if constexpr (is8(CT)) {
+        const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
+        const float a = pg.k_scale[s], c = pg.v_scale[s];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= a, y[j] *= c;
+      }
+    }
+    store8<OT>((OutT*)k_out + 8 * at, x);
+    store8<OT>((OutT*)v_out + 8 * at, y);
+  }
+}
+
+// ---------------------------------------------------------------------
+// Selection.  Scores: a wave per (sequence, head, page), then the rank of a
+// page by counting the better ones.
+// ---------------------------------------------------------------------
+template <int QT, int BT>
+__global__ void __launch_bounds__(64) score_kernel(Pages pg, Table tab, pfa_tensor4 q, int G, int D,
+                                                   const int32_t* __restrict__ lengths,
+                                                   const int32_t* __restrict__ starts, int first, int last,
+                                                   uint32_t* __restrict__ keys) {
+  const int64_t b = blockIdx.z;
+  const int h = blockIdx.y, page = blockIdx.x, lane = threadIdx.x;
+  const int64_t len = length_at(lengths, tab, pg, b);
+  const int64_t start = starts && starts[b] > 0 ? starts[b] : 0;
+  uint32_t* key = keys + (b * pg.H + h) * tab.P + page;
+  const int64_t p0 = start >> pg.shift, pe = (len + pg.ps - 1) >> pg.shift;
+  const int id = start < len && page >= p0 && page < pe ? page_at(tab, pg, b, page) : -1;
+  if (id < 0) {
+    if (lane == 0) *key = 0;  // no candidate
+    return;
+  }
+  const typename Elem<BT>::T* lo = (const typename Elem<BT>::T*)pg.bounds + ((int64_t)id * pg.H + h) * 2 * D;
+  float best = -INFINITY;
+  bool nan = false;
+  for (int g = 0; g < G; ++g) {
+    const typename Elem<QT>::T* qp = (const typename Elem<QT>::T*)q.ptr + b * q.s_b + (int64_t)(h * G + g) * q.s_h;
+    double s = 0.0;
+    for (int d = lane; d < D; d += kWave) {
+      const float x = load_f<QT>(qp + d);
+      s += (double)x * (double)load_f<BT>(lo + (x > 0.0f ? D : 0) + d);
+    }
+    for (int o = 1; o < kWave; o <<= 1) s += __shfl_xor(s, o);
+    const float f = (float)s;
+    nan = nan || f != f;
+    best = fmaxf(best, f);
+  }
+  if (lane) return;
+  uint32_t u = __float_as_uint(best);
+  u = u & 0x80000000u ? ~u : u | 0x80000000u;
+  if (nan) u = 1;
+  if (page < p0 + first || page >= pe - last) u = 0xffffffffu;
+  *key = u;
+}
+
+__global__ void __launch_bounds__(256) rank_kernel(int P, int H, int count, const uint32_t* __restrict__ keys,
+                                                   int32_t* __restrict__ chosen) {
+  const uint32_t* key = keys + (int64_t)blockIdx.x * P;
+  int32_t* out = chosen + (int64_t)blockIdx.x * count;
+  __shared__ int taken[256];
+  int base = 0;
+  for (int p0 = 0; p0 < P; p0 += 256) {
+    const int p = p0 + threadIdx.x;
+    const uint32_t mine = p < P ? key[p] : 0;
+    int before = 0;
+    if (mine) {
+      for (int o = 0; o < P; ++o) before += key[o] > mine || (key[o] == mine && o < p);
+    }
+    taken[threadIdx.x] = mine && before < count;
+    __syncthreads();
+    int rank = base, all = base;
+    for (int i = 0; i < 256; ++i) {
+      rank += i < (int)threadIdx.x ? taken[i] : 0;
+      all += taken[i];
+    }
+    if (taken[threadIdx.x]) out[rank] = p;
+    base = all;
+    __syncthreads();
+  }
+  for (int i = base + threadIdx.x; i < count; i += 256) out[i] = -1;
+}
+
+// ---------------------------------------------------------------------
+// Attention, one wave per (sequence, query head), a key at a time.
+// ---------------------------------------------------------------------
+template <int QT, int CT>
+__global__ void __launch_bounds__(64) attend_kernel(Pages pg, Table tab, pfa_tensor4 q, int H, int D,
+                                                    const int32_t* __restrict__ lengths,
+                                                    const int32_t* __restrict__ starts,
+                                                    const int32_t* __restrict__ selected, int S, float scale,
+                                                    void* out) {
+  using CellT = typename Cell<CT>::T;
+  const int64_t b = blockIdx.y;
+  const int hq = blockIdx.x, h = hq / (H / pg.H), lane = threadIdx.x;
+  const int64_t len = length_at(lengths, tab, pg, b);
+  const int64_t start = starts && starts[b] > 0 ? starts[b] : 0;
+  const typename Elem<QT>::T* qp = (const typename Elem<QT>::T*)q.ptr + b * q.s_b + hq * q.s_h;
+  const int d0 = lane, d1 = lane + 64;
+  const float q0 = d0 < D ? load_f<QT>(qp + d0) : 0.0f, q1 = d1 < D ? load_f<QT>(qp + d1) : 0.0f;
+  float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  const int64_t entries = S >= 0 ? S : ((len + pg.ps - 1) >> pg.shift);
+  for (int64_t e = 0; e < entries; ++e) {
+    const int64_t ordinal = S >= 0 ? (int64_t)selected[(b * pg.H + h) * S + e] : e;
+    const int id = page_at(tab, pg, b, ordinal);
+    if (id < 0) continue;
+    for (int slot = 0; slot < pg.ps; ++slot) {
+      const int64_t pos = (ordinal << pg.shift) + slot;
+      if (pos < start || pos >= len) continue;
+      const int64_t at = (int64_t)h * pg.ps + slot;
+      const CellT* kp = (const CellT*)pg.k + id * pg.k_page + at * D;
+      const CellT* vp = (const CellT*)pg.v + id * pg.v_page + at * D;
+      float s = (d0 < D ? q0 * cell_f<CT>(kp + d0) : 0.0f) + (d1 < D ? q1 * cell_f<CT>(kp + d1) : 0.0f);
+      for (int o = 1; o < kWave; o <<= 1) s += __shfl_xor(s, o);
+      float vs = 1.0f;
+      s *= scale;
+      if constexpr (is8(CT)) {
+        const int64_t a = (int64_t)id * pg.H * pg.ps + at;
+        s *= pg.k_scale[a];
+        vs = pg.v_scale[a];
+      }
+      const float top = fmaxf(m, s);
+      const float old = m == -INFINITY ? 0.0f : expf(m - top);
+      const float p = s == -INFINITY ? 0.0f : expf(s - top);
+      m = top;
+      l = l * old + p;
+      o0 = o0 * old + (d0 < D ? p * vs * cell_f<CT>(vp + d0) : 0.0f);
+      o1 = o1 * old + (d1 < D ? p * vs * cell_f<CT>(vp + d1) : 0.0f);
+    }
+  }
+  typename Elem<QT>::T* op = (typename Elem<QT>::T*)out + (b * H + hq) * D;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (d0 < D) store_f<QT>(op + d0, o0 * inv);
+  if (d1 < D) store_f<QT>(op + d1, o1 * inv);
+}
+
+// Calls f with the (values, cells) types as template arguments: the cells' own
+// float type, or any of the three with 8-bit cells.
+template <typename F>
+void by_types(int dt, int ct, F&& f) {
+#define PFA_PAIR(A, C) \
+  if (dt == A && ct == C) return f(std::integral_constant<int, A>{}, std::integral_constant<int, C>{});
+  PFA_PAIR(PFA_F32, PFA_F32) PFA_PAIR(PFA_BF16, PFA_BF16) PFA_PAIR(PFA_F16, PFA_F16)
+  PFA_PAIR(PFA_F32, PFA_I8) PFA_PAIR(PFA_BF16, PFA_I8) PFA_PAIR(PFA_F16, PFA_I8)
+  PFA_PAIR(PFA_F32, PFA_E4M3) PFA_PAIR(PFA_BF16, PFA_E4M3) PFA_PAIR(PFA_F16, PFA_E4M3)
+#undef PFA_PAIR
+}
+
+int types_check(int dt, int ct) {
+  PFA_CHECK_ARG(dt == PFA_F32 || dt == PFA_BF16 || dt == PFA_F16, "pages: unknown value type %d", dt);
+  PFA_CHECK_ARG(is8(ct) || dt == ct, "pages: values of type %d for cells of type %d", dt, ct);
+  return PFA_OK;
+}
+
+}  // namespace
+}  // namespace pfa
+
+using namespace pfa;
+
+extern "C" int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4 v, int dtype, int B, int64_t n,
+                                  const int32_t* table, int64_t table_stride, int table_pages, const int32_t* starts,
+                                  const int32_t* counts, void* stream) {
+  clear_error();
+  Pages p;
+  Table t;
+  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = types_check(dtype, pages.dtype)) return rc;
+  PFA_CHECK_ARG(n >= 0 && n <= (1 << 30), "kv_pages_write: 0 <= n <= 2^30 tokens");
+  if (B == 0 || n == 0 || table_pages == 0) return PFA_OK;
+  PFA_CHECK_ARG(k.ptr && v.ptr && starts, "kv_pages_write: null argument");
+  const int D = pages.head_dim;
+  const int e = cell_bytes(dtype);
+  auto rows = [&](const pfa_tensor4& x) {
+    const bool vec = (uintptr_t)x.ptr % 16 == 0 && x.s_b * e % 16 == 0 && x.s_h * e % 16 == 0 && x.s_t * e % 16 == 0;
+    return NewRows{x.ptr, x.s_b, x.s_h, x.s_t, vec};
+  };
+  const int64_t touched = (n + p.ps - 2) / p.ps + 1;
+  const int64_t at_once = (n < p.ps ? n : p.ps) * (D / 8);
+  const int threads = at_once <= 64 ? 64 : at_once <= 128 ? 128 : 256;
+  by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
+    write_kernel<decltype(dt)::value, decltype(ct)::value>
+        <<<dim3((unsigned)touched, p.H, B), threads, 0, as_stream(stream)>>>(p, t, rows(k), rows(v), D, n, starts,
+                                                                             counts);
+  });
+  PFA_CHECK_LAUNCH("kv_pages_write");
+  return PFA_OK;
+}
+
+extern "C" int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int32_t* table, int64_t table_stride,
+                                 int table_pages, const int32_t* starts, const int32_t* counts, void* k_out,
+                                 void* v_out, int out_dtype, void* stream) {
+  clear_error();
+  Pages p;
+  Table t;
+  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  PFA_CHECK_ARG(out_dtype == PFA_F32 || out_dtype == PFA_BF16 || out_dtype == PFA_F16,
+                "kv_pages_read: unknown value type %d", out_dtype);
+  PFA_CHECK_ARG(n >= 0 && n <= (1 << 30), "kv_pages_read: 0 <= n <= 2^30 tokens");
+  if (B == 0 || n == 0) return PFA_OK;
+  PFA_CHECK_ARG(k_out && v_out && starts && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
+                "kv_pages_read: null or unaligned argument");
+  const int D = pages.head_dim;
+  const int64_t total = (int64_t)B * n * p.H * (D / 8);
+  const int64_t blocks = (total + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
+  auto launch = [&](auto ct, auto ot) {
+    read_kernel<decltype(ct)::value, decltype(ot)::value>
+        <<<grid, 256, 0, as_stream(stream)>>>(p, t, D, n, total, starts, counts, k_out, v_out);
+  };
+  auto by_out = [&](auto ct) {
+    if (out_dtype == PFA_F32) launch(ct, std::integral_constant<int, PFA_F32>{});
+    else if (out_dtype == PFA_BF16) launch(ct, std::integral_constant<int, PFA_BF16>{});
+    else launch(ct, std::integral_constant<int, PFA_F16>{});
+  };
+  switch (pages.dtype) {
+    case PFA_F32: by_out(std::integral_constant<int, PFA_F32>{}); break;
+    case PFA_BF16: by_out(std::integral_constant<int, PFA_BF16>{}); break;
+    case PFA_F16: by_out(std::integral_constant<int, PFA_F16>{}); break;
+    case PFA_I8: by_out(std::integral_constant<int, PFA_I8>{}); break;
+    default: by_out(std::integral_constant<int, PFA_E4M3>{}); break;
+  }
+  PFA_CHECK_LAUNCH("kv_pages_read");
+  return PFA_OK;
+}
+
+namespace {
+
+int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H, const pfa_kv_pages& pages,
+                const int32_t* lengths) {
+  if (int rc = types_check(dtype, pages.dtype)) return rc;
+  PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages.kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
+                pages.kv_heads);
+  PFA_CHECK_ARG(B == 0 || (q.ptr && lengths), "%s: null argument", what);
+  return PFA_OK;
+}
+
+}  // namespace
+
+extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes) {
+  clear_error();
+  PFA_CHECK_ARG(bytes && B >= 0 && kv_heads > 0 && table_pages >= 0, "kv_pages_select: bad sizes");
+  *bytes = (size_t)B * kv_heads * table_pages * 4;
+  return PFA_OK;
+}
+
+extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages, const int32_t* table,
+                                   int64_t table_stride, int table_pages, const int32_t* lengths,
+                                   const int32_t* starts, int count, int first, int last, int32_t* chosen,
+                                   void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  Pages p;
+  Table t;
+  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = query_check("kv_pages_select", q, dtype, B, H, pages, lengths)) return rc;
+  PFA_CHECK_ARG(pages.k_bounds, "kv_pages_select: the pool has no key bounds");
+  PFA_CHECK_ARG(count > 0 && first >= 0 && last >= 0 && first <= count && last <= count - first,
+                "kv_pages_select: count > 0 pages, the %d first and %d last among them (got %d)", first, last, count);
+  if (B == 0) return PFA_OK;
+  PFA_CHECK_ARG(chosen, "kv_pages_select: null argument");
+  size_t need = 0;
+  pfa_kv_pages_select_workspace_size(B, p.H, table_pages, &need);
+  if (ws_bytes < need || (need && !workspace)) {
+    set_error("kv_pages_select: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    return PFA_E_WORKSPACE;
+  }
+  uint32_t* keys = (uint32_t*)workspace;
+  if (table_pages > 0) {
+    by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
+      score_kernel<decltype(dt)::value, bound_dtype(decltype(ct)::value)>
+          <<<dim3(table_pages, p.H, B), 64, 0, as_stream(stream)>>>(p, t, q, H / p.H, pages.head_dim, lengths, starts,
+                                                                    first, last, keys);
+    });
+  }
+  rank_kernel<<<B * p.H, 256, 0, as_stream(stream)>>>(table_pages, p.H, count, keys, chosen);
+  PFA_CHECK_LAUNCH("kv_pages_select");
+  return PFA_OK;
+}
+
+extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int head_dim, int page_size, int table_pages,
+                                             int n_selected, size_t* bytes) {
+  clear_error();
+  PFA_CHECK_ARG(bytes && B >= 0 && H > 0 && kv_heads > 0 && head_dim > 0 && page_size > 0 && table_pages >= 0,
+                "paged_attn: bad sizes");
+  *bytes = 0;
+  return PFA_OK;
+}
+
+extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages, const int32_t* table,
+                                  int64_t table_stride, int table_pages, const int32_t* lengths, const int32_t* starts,
+                                  const int32_t* selected, int n_selected, float scale, void* out, void* workspace,
+                                  size_t ws_bytes, void* stream) {
+  clear_error();
+  Pages p;
+  Table t;
+  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = query_check("paged_attn", q, dtype, B, H, pages, lengths)) return rc;
+  PFA_CHECK_ARG(n_selected <= 0 || selected, "paged_attn: null argument");
+  if (B == 0) return PFA_OK;
+  PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "paged_attn: null or unaligned argument");
+  by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
+    attend_kernel<decltype(dt)::value, decltype(ct)::value><<<dim3(H, B), 64, 0, as_stream(stream)>>>(
+        p, t, q, H, pages.head_dim, lengths, starts, selected, n_selected, scale, out);
+  });
+  PFA_CHECK_LAUNCH("paged_attn");
+  return PFA_OK;
+}

@@ -6,6 +6,15 @@ hand-written gfx950 HIP kernels in ``lib/libpfa_hip.so`` (C ABI declared in
 ``include/pfa_hip.h``).
 """
 
+from .kernels.paged_attn import (
+    KVPages,
+    new_kv_pages,
+    paged_attention,
+    paged_sparse_attention,
+    read_kv_pages,
+    select_kv_pages,
+    write_kv_pages,
+)
 from .kernels.sparse_attn import aspa_sparse_attention, get_last_backend, get_last_backend_info
 from .models.aspa import (
     MLP,
@@ -36,6 +45,13 @@ __all__ = [
     "ChunkedShortlistMetrics",
     "ChunkedShortlistResult",
     "ChunkedShortlistRunner",
+    "KVPages",
+    "new_kv_pages",
+    "write_kv_pages",
+    "read_kv_pages",
+    "select_kv_pages",
+    "paged_attention",
+    "paged_sparse_attention",
     "__version__",
 ]
 

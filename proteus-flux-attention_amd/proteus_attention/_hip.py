@@ -15,7 +15,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libpfa_hip.so"
 
-PFA_F32, PFA_BF16, PFA_F16, PFA_I8 = 0, 1, 2, 3
+PFA_F32, PFA_BF16, PFA_F16, PFA_I8, PFA_E4M3 = 0, 1, 2, 3, 4
 
 _DTYPE_TAG = {
     torch.float32: PFA_F32,
@@ -73,6 +73,12 @@ EXPORTED_SYMBOLS = (
     "pfa_rope_rows_inplace",
     "pfa_int8_kv_attn_workspace_size",
     "pfa_int8_kv_attn_fwd",
+    "pfa_kv_pages_write",
+    "pfa_kv_pages_read",
+    "pfa_paged_attn_workspace_size",
+    "pfa_paged_attn_fwd",
+    "pfa_kv_pages_select_workspace_size",
+    "pfa_kv_pages_select",
 )
 
 
@@ -84,6 +90,25 @@ class Tensor4(ctypes.Structure):
         ("s_b", ctypes.c_int64),
         ("s_h", ctypes.c_int64),
         ("s_t", ctypes.c_int64),
+    ]
+
+
+class KVPagesC(ctypes.Structure):
+    """pfa_kv_pages: the pool of a paged key-value cache."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_bounds", ctypes.c_void_p),
+        ("k_page", ctypes.c_int64),
+        ("v_page", ctypes.c_int64),
+        ("n_pages", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("dtype", ctypes.c_int),
     ]
 
 
@@ -164,6 +189,14 @@ _SIGNATURES = {
     "pfa_int8_kv_attn_workspace_size": ([_i64, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_int8_kv_attn_fwd": ([Tensor4, Tensor4, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp,
                               _sz, _vp], _i32),
+    "pfa_kv_pages_write": ([KVPagesC, Tensor4, Tensor4, _i32, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp], _i32),
+    "pfa_kv_pages_read": ([KVPagesC, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
+    "pfa_paged_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
+    "pfa_paged_attn_fwd": ([Tensor4, _i32, _i32, _i32, KVPagesC, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _vp,
+                            _sz, _vp], _i32),
+    "pfa_kv_pages_select_workspace_size": ([_i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
+    "pfa_kv_pages_select": ([Tensor4, _i32, _i32, _i32, KVPagesC, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _vp,
+                             _vp, _sz, _vp], _i32),
 }
 
 
