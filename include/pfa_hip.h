@@ -696,8 +696,8 @@ int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int32_t* table
  * (PFA_F32 / PFA_BF16 / PFA_F16: the cells' own, or any of the three for
  * 8-bit cells).  A row that sees no key is zero, and so is one all of whose
  * scores are -inf.  Sums and softmax statistics are f32. */
-int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int head_dim, int page_size,
-                                  int table_pages, int n_selected, size_t* bytes);
+int pfa_paged_attn_workspace_size(int B, int H, pfa_kv_pages pages, int table_pages,
+                                  int n_selected, size_t* bytes);
 int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages,
                        const int32_t* table, int64_t table_stride, int table_pages,
                        const int32_t* lengths, const int32_t* starts,

@@ -1,6 +1,7 @@
 // Paged key-value cache: write, read, page selection and the attention of one
 // new token over it.
 #include "pfa_paged.h"
+#include "pfa_paged_attn.h"
 
 namespace pfa {
 
@@ -280,59 +281,6 @@ __global__ void __launch_bounds__(256) rank_kernel(int P, int H, int count, cons
   for (int i = base + threadIdx.x; i < count; i += 256) out[i] = -1;
 }
 
-// ---------------------------------------------------------------------
-// Attention, one wave per (sequence, query head), a key at a time.
-// ---------------------------------------------------------------------
-template <int QT, int CT>
-__global__ void __launch_bounds__(64) attend_kernel(Pages pg, Table tab, pfa_tensor4 q, int H, int D,
-                                                    const int32_t* __restrict__ lengths,
-                                                    const int32_t* __restrict__ starts,
-                                                    const int32_t* __restrict__ selected, int S, float scale,
-                                                    void* out) {
-  using CellT = typename Cell<CT>::T;
-  const int64_t b = blockIdx.y;
-  const int hq = blockIdx.x, h = hq / (H / pg.H), lane = threadIdx.x;
-  const int64_t len = length_at(lengths, tab, pg, b);
-  const int64_t start = starts && starts[b] > 0 ? starts[b] : 0;
-  const typename Elem<QT>::T* qp = (const typename Elem<QT>::T*)q.ptr + b * q.s_b + hq * q.s_h;
-  const int d0 = lane, d1 = lane + 64;
-  const float q0 = d0 < D ? load_f<QT>(qp + d0) : 0.0f, q1 = d1 < D ? load_f<QT>(qp + d1) : 0.0f;
-  float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  const int64_t entries = S >= 0 ? S : ((len + pg.ps - 1) >> pg.shift);
-  for (int64_t e = 0; e < entries; ++e) {
-    const int64_t ordinal = S >= 0 ? (int64_t)selected[(b * pg.H + h) * S + e] : e;
-    const int id = page_at(tab, pg, b, ordinal);
-    if (id < 0) continue;
-    for (int slot = 0; slot < pg.ps; ++slot) {
-      const int64_t pos = (ordinal << pg.shift) + slot;
-      if (pos < start || pos >= len) continue;
-      const int64_t at = (int64_t)h * pg.ps + slot;
-      const CellT* kp = (const CellT*)pg.k + id * pg.k_page + at * D;
-      const CellT* vp = (const CellT*)pg.v + id * pg.v_page + at * D;
-      float s = (d0 < D ? q0 * cell_f<CT>(kp + d0) : 0.0f) + (d1 < D ? q1 * cell_f<CT>(kp + d1) : 0.0f);
-      for (int o = 1; o < kWave; o <<= 1) s += __shfl_xor(s, o);
-      float vs = 1.0f;
-      s *= scale;
-      if constexpr (is8(CT)) {
-        const int64_t a = (int64_t)id * pg.H * pg.ps + at;
-        s *= pg.k_scale[a];
-        vs = pg.v_scale[a];
-      }
-      const float top = fmaxf(m, s);
-      const float old = m == -INFINITY ? 0.0f : expf(m - top);
-      const float p = s == -INFINITY ? 0.0f : expf(s - top);
-      m = top;
-      l = l * old + p;
-      o0 = o0 * old + (d0 < D ? p * vs * cell_f<CT>(vp + d0) : 0.0f);
-      o1 = o1 * old + (d1 < D ? p * vs * cell_f<CT>(vp + d1) : 0.0f);
-    }
-  }
-  typename Elem<QT>::T* op = (typename Elem<QT>::T*)out + (b * H + hq) * D;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (d0 < D) store_f<QT>(op + d0, o0 * inv);
-  if (d1 < D) store_f<QT>(op + d1, o1 * inv);
-}
-
 // Calls f with the (values, cells) types as template arguments: the cells' own
 // float type, or any of the three with 8-bit cells.
 template <typename F>
@@ -364,7 +312,7 @@ extern "C" int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4
   Table t;
   if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
   if (int rc = types_check(dtype, pages.dtype)) return rc;
-  PFA_CHECK_ARG(n >= 0 && n <= (1 << 30), "kv_pages_write: 0 <= n <= 2^30 tokens");
+  PFA_CHECK_ARG(n >= 0 && n <= (1 << 26), "kv_pages_write: 0 <= n <= 2^26 tokens");
   if (B == 0 || n == 0 || table_pages == 0) return PFA_OK;
   PFA_CHECK_ARG(k.ptr && v.ptr && starts, "kv_pages_write: null argument");
   const int D = pages.head_dim;
@@ -429,6 +377,7 @@ int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H,
   if (int rc = types_check(dtype, pages.dtype)) return rc;
   PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages.kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
                 pages.kv_heads);
+  PFA_CHECK_ARG((int64_t)B * H <= 1 << 23, "%s: up to 2^23 rows (got %d x %d)", what, B, H);
   PFA_CHECK_ARG(B == 0 || (q.ptr && lengths), "%s: null argument", what);
   return PFA_OK;
 }
@@ -475,12 +424,16 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
   return PFA_OK;
 }
 
-extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int head_dim, int page_size, int table_pages,
-                                             int n_selected, size_t* bytes) {
+extern "C" int pfa_paged_attn_workspace_size(int B, int H, pfa_kv_pages pages, int table_pages, int n_selected,
+                                             size_t* bytes) {
   clear_error();
-  PFA_CHECK_ARG(bytes && B >= 0 && H > 0 && kv_heads > 0 && head_dim > 0 && page_size > 0 && table_pages >= 0,
-                "paged_attn: bad sizes");
-  *bytes = 0;
+  Pages p;
+  Table t;
+  if (int rc = paged_check(&pages, nullptr, 0, 0, B, &p, &t)) return rc;
+  PFA_CHECK_ARG(bytes && H > 0 && H % p.H == 0 && table_pages >= 0, "paged_attn: bad sizes");
+  *bytes = attend_plan(B, H, p.H, pages.head_dim, p.shift, table_pages, n_selected,
+                       attend_tile(pages.dtype, pages.head_dim))
+               .bytes;
   return PFA_OK;
 }
 
@@ -494,12 +447,23 @@ extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv
   if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
   if (int rc = query_check("paged_attn", q, dtype, B, H, pages, lengths)) return rc;
   PFA_CHECK_ARG(n_selected <= 0 || selected, "paged_attn: null argument");
+  PFA_CHECK_ARG((int64_t)n_selected << p.shift <= (1ll << 30), "paged_attn: lists of up to 2^30 positions");
+  const float c = scale * 1.44269504088896340736f;
+  PFA_CHECK_ARG(c > 0.0f && c < INFINITY, "paged_attn: scale must be positive and finite");
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "paged_attn: null or unaligned argument");
-  by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
-    attend_kernel<decltype(dt)::value, decltype(ct)::value><<<dim3(H, B), 64, 0, as_stream(stream)>>>(
-        p, t, q, H, pages.head_dim, lengths, starts, selected, n_selected, scale, out);
-  });
+  const int S = n_selected < 0 ? -1 : n_selected;
+  const Plan plan = attend_plan(B, H, p.H, pages.head_dim, p.shift, table_pages, S,
+                                attend_tile(pages.dtype, pages.head_dim));
+  if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
+    set_error("paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, plan.bytes);
+    return PFA_E_WORKSPACE;
+  }
+  const AttendCall a{p, table, table_stride, table_pages, B, H, pages.head_dim, q, lengths, starts, selected, S, c, out,
+                     (float*)workspace, as_stream(stream)};
+  if (pages.dtype == PFA_I8) attend_i8(dtype, a);
+  else if (pages.dtype == PFA_E4M3) attend_e4m3(dtype, a);
+  else attend_float(dtype, a);
   PFA_CHECK_LAUNCH("paged_attn");
   return PFA_OK;
 }

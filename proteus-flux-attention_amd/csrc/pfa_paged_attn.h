@@ -1,0 +1,712 @@
+// Attention of one new token over a paged cache, on the matrix cores.
+//
+// For a key-value head h and the G query heads that share it:
+//   S = K Q^T (keys x heads),  m = max S,  P = exp(S - m),  O = V^T P / sum P.
+//
+// Every key and value is read once, so the cache's bytes are the bound (G is
+// small: 4 D G operations for 2 D cells).  The kernel is built around loads
+// that need no shuffle behind them:
+//
+// - A wave takes 32 keys at a time.  S^T = K Q^T puts keys in the rows of the
+//   product: lane (n, g), n = lane % 16, g = lane / 16, loads 16-byte units of
+//   key n's row, 16 keys x 64 bytes a load, which is the operand as it stands
+//   (the order of the channels is free as long as Q's is the same).
+// - S comes back with head n in lane (n, g) and keys 4g .. 4g + 3 of each 16 in
+//   its registers.  The second product contracts over keys, whose order is free
+//   too: O^T = V^T P^T with lane group g holding keys 4g .. 4g + 3 of both 16s is
+//   P as it stands.
+// - V's operand needs eight keys of one channel in a lane.  Lane (n, g) loads
+//   D / 16 neighbouring channels of each of its eight keys (a row is 16 lanes,
+//   in one piece), and byte permutes between registers of the same lane turn
+//   keys and channels around: one for every two cells.
+// - O^T has head n in lane (n, g) again, so the running maximum's correction is
+//   one factor a lane, and lane (n, g) ends with D / 4 neighbouring channels.
+//
+// No LDS, no barrier and no lane exchange but the maximum over g, two row
+// swaps, until a workgroup's four waves are joined.
+//
+// Precision: f32 stays on v_mfma_f32_16x16x4f32.  8-bit cells are whole in
+// bf16; their scales multiply S and P in f32.  Queries of f16 or f32 on 8-bit
+// cells are split into two or three bf16 parts, which hold all their bits.  P
+// goes in parts of its own, each what the ones before leave: two parts (bf16: 16
+// bits, f16: 22) where the result has 8 or 11 bits, three (24 bits) where it is
+// f32.  f16 parts are scaled by 2^15, so that a probability is whole down to
+// 2^-39 of the row's largest.
+#pragma once
+
+#include "pfa_paged.h"
+
+namespace pfa {
+namespace paged {
+
+constexpr int kWaves = 4;  // of a workgroup
+
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4_t;
+typedef __attribute__((__vector_size__(8 * sizeof(_Float16)))) _Float16 f16x8_t;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// BYTES (1, 2, 4, 8, 16 or 32) at p, into dwords.
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* o) {
+  if constexpr (BYTES == 1) o[0] = *p;
+  else if constexpr (BYTES == 2) o[0] = *reinterpret_cast<const uint16_t*>(p);
+  else if constexpr (BYTES == 4) o[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (BYTES == 8) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
+    o[0] = a.x, o[1] = a.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 a = reinterpret_cast<const uint4*>(p)[i];
+      o[4 * i] = a.x, o[4 * i + 1] = a.y, o[4 * i + 2] = a.z, o[4 * i + 3] = a.w;
+    }
+  }
+}
+
+// Two f32 that bf16 holds, or that are rounded to it, in one dword.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;
+  return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2_t;
+  return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+}
+
+// Cells 2i and 2i + 1 of a dword of 8-bit cells as bf16, exactly.
+template <int CT>
+__device__ __forceinline__ uint32_t cells2_bf16(uint32_t w, int i) {
+  if constexpr (CT == PFA_I8) {
+    const float a = (float)(int8_t)(w >> (16 * i)), b = (float)(int8_t)(w >> (16 * i + 8));
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);  // the upper halves
+  } else {
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2_;
+    const f32x2_ f = i ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+    return __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302);
+  }
+}
+
+// Cells of a call's kernel, by the types of queries and cells and the head's width.
+template <int QT_, int CT_, int D_>
+struct Form {
+  static constexpr int QT = QT_, CT = CT_, D = D_;
+  static constexpr int E = cell_bytes(CT);
+  static constexpr bool F32 = CT == PFA_F32, F16 = CT == PFA_F16;
+  static constexpr int NQ = !is8(CT) || QT == PFA_BF16 ? 1 : QT == PFA_F16 ? 2 : 3;  // parts of Q
+  static constexpr int NP = QT == PFA_F32 ? 3 : 2;                                    // parts of P
+  static constexpr int EL = D / 4;                     // channels of a lane in S
+  static constexpr int U = EL < 16 / E ? EL : 16 / E;  // of one load
+  static constexpr int KW = EL * E / 4;                // dwords of a lane's share of 16 keys
+  static constexpr int NC = F32 ? EL : EL < 8 ? 1 : EL / 8;  // products over it
+  static constexpr int VD = D / 16;                    // channels of a lane in O
+  static constexpr int VB = VD * E;                    // their bytes of a key
+  static constexpr int VW = VB < 4 ? 1 : VB / 4;
+  // 32-key groups that a wave loads at once: 8 KB of keys for rows of 64 bytes
+  // and more
+  static constexpr int NG = D * E >= 256 ? 1 : D * E >= 128 ? 2 : 4;
+  static constexpr int TILE = 32 * NG;
+  static constexpr float PSCALE = F16 ? 32768.0f : 1.0f;
+};
+
+// 16 keys in a row of a page: the position of the first, far behind every
+// length where there are none.
+struct Block {
+  int id, slot, pos;
+};
+constexpr int kNowhere = 0x7fffff00;
+
+// One sequence and key-value head.
+struct Row {
+  const int32_t* ids;   // the sequence's row of the table
+  const int32_t* list;  // the listed entries, where S >= 0
+  int S, P, n_pages, shift, start, len;
+
+  // `key` counts positions, or the slots of the listed pages
+  __device__ __forceinline__ Block block(int key) const {
+    int ordinal = key >> shift;
+    if (S >= 0) ordinal = ordinal < S ? list[ordinal] : -1;
+    ordinal = __builtin_amdgcn_readfirstlane(ordinal);
+    int id = (uint32_t)ordinal < (uint32_t)P ? ids[ordinal] : -1;
+    id = __builtin_amdgcn_readfirstlane(id);
+    const int slot = key & ((1 << shift) - 1);
+    if ((uint32_t)id >= (uint32_t)n_pages) return Block{0, slot, kNowhere};
+    return Block{id, slot, (ordinal << shift) + slot};
+  }
+};
+
+template <typename F>
+struct Tile {
+  Block b[2 * F::NG];
+  __device__ __forceinline__ void find(const Row& r, int tile) {
+#pragma unroll
+    for (int i = 0; i < F::NG; ++i) {
+      const int key = tile * F::TILE + 32 * i;
+      b[2 * i] = r.block(key);
+      if (r.shift > 4) b[2 * i + 1] = Block{b[2 * i].id, b[2 * i].slot + 16, b[2 * i].pos + 16};
+      else b[2 * i + 1] = r.block(key + 16);
+    }
+  }
+  // whether all its keys are seen
+  __device__ __forceinline__ bool whole(const Row& r) const {
+    bool w = true;
+#pragma unroll
+    for (int i = 0; i < 2 * F::NG; ++i) w = w && b[i].pos >= r.start && b[i].pos + 16 <= r.len;
+    return w;
+  }
+};
+
+// A wave's running state: O^T of head n in lane (n, g), channels
+// VD * (4g + i) + j, and the row's maximum and sum (of the lane's own keys).
+template <typename F>
+struct State {
+  f32x4_t o[F::VD];
+  float m, l;
+};
+
+template <typename F>
+struct Wave {
+  int n, g;
+  u32x4_t q[F::F32 ? 1 : F::NQ][F::F32 ? 1 : F::NC];
+  float qf[F::F32 ? F::EL : 1];
+  uint32_t k[2 * F::NG][F::KW];
+
+  // Channel of a lane's element x: unit x / U of 4U channels, one U a lane group.
+  __device__ __forceinline__ int channel(int x) const { return x / F::U * 4 * F::U + g * F::U + x % F::U; }
+
+  __device__ __forceinline__ void load_q(const typename Elem<F::QT>::T* p, bool row) {
+    if constexpr (F::F32) {
+#pragma unroll
+      for (int x = 0; x < F::EL; ++x) qf[x] = row ? p[channel(x)] : 0.0f;
+    } else {
+#pragma unroll
+      for (int c = 0; c < F::NC; ++c) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = row && 8 * c + e < F::EL ? load_f<F::QT>(p + channel(8 * c + e)) : 0.0f;
+        parts<F::NQ, F::F16>(x, [&](int part, u32x4_t w) { q[part][c] = w; });
+      }
+    }
+  }
+
+  // Eight f32 as N 16-bit operands, each what the ones before leave.
+  template <int N, bool HALF, typename Put>
+  static __device__ __forceinline__ void parts(float (&x)[8], Put&& put) {
+#pragma unroll
+    for (int part = 0; part < N; ++part) {
+      u32x4_t w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = HALF ? pack_f16(x[2 * i], x[2 * i + 1]) : pack_bf16(x[2 * i], x[2 * i + 1]);
+        w[i] = u;
+        if (part + 1 < N) {
+          if constexpr (HALF) {
+            x[2 * i] -= f16_to_f32((uint16_t)u), x[2 * i + 1] -= f16_to_f32((uint16_t)(u >> 16));
+          } else {
+            x[2 * i] -= __uint_as_float(u << 16), x[2 * i + 1] -= __uint_as_float(u & 0xffff0000u);
+          }
+        }
+      }
+      put(part, w);
+    }
+  }
+
+  static __device__ __forceinline__ f32x4_t mma(u32x4_t a, u32x4_t b, f32x4_t c) {
+    if constexpr (F::F16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                    0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                     0, 0, 0);
+  }
+
+  __device__ __forceinline__ void load_k(const Pages& pg, int h, const Tile<F>& t) {
+    const int lane_at = (n * F::D + g * F::U) * F::E;
+#pragma unroll
+    for (int i = 0; i < 2 * F::NG; ++i) {
+      const uint8_t* base =
+          (const uint8_t*)pg.k + ((int64_t)t.b[i].id * pg.k_page + (int64_t)(h * pg.ps + t.b[i].slot) * F::D) * F::E;
+#pragma unroll
+      for (int u = 0; u < F::EL / F::U; ++u)
+        load_bytes<F::U * F::E>(base + lane_at + u * 4 * F::U * F::E, &k[i][u * F::U * F::E / 4]);
+    }
+  }
+
+  // S of the 16 keys of block i.
+  __device__ __forceinline__ f32x4_t scores(int i) const {
+    f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (F::F32) {
+      f32x4_t s2 = s;
+#pragma unroll
+      for (int x = 0; x < F::EL; x += 2) {
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][x]), qf[x], s, 0, 0, 0);
+        s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i][x + 1]), qf[x + 1], s2, 0, 0, 0);
+      }
+      s += s2;
+    } else {
+#pragma unroll
+      for (int c = 0; c < F::NC; ++c) {
+        u32x4_t a = {0, 0, 0, 0};
+        if constexpr (is8(F::CT)) {
+#pragma unroll
+          for (int w = 0; w < (F::EL < 8 ? 2 : 4); ++w) a[w] = cells2_bf16<F::CT>(k[i][2 * c + w / 2], w & 1);
+        } else {
+#pragma unroll
+          for (int w = 0; w < (F::EL < 8 ? 2 : 4); ++w) a[w] = k[i][4 * c + w];
+        }
+#pragma unroll
+        for (int part = F::NQ - 1; part >= 0; --part) s = mma(a, q[part][c], s);
+      }
+    }
+    return s;
+  }
+
+  // One tile: V loads, S from the keys that are in registers, the next tile's
+  // keys, P, and O.
+  __device__ __forceinline__ void step(const Pages& pg, const Row& r, int h, float c, const Tile<F>& t, bool more,
+                                       const Tile<F>& next, State<F>& st) {
+    uint32_t v[2 * F::NG][4][F::VW];
+    f32x4_t s[2 * F::NG], vs[2 * F::NG];
+    const int lane_at = 4 * g * F::D * F::E + n * F::VB;
+#pragma unroll
+    for (int i = 0; i < 2 * F::NG; ++i) {
+      const int64_t slot = (int64_t)(h * pg.ps + t.b[i].slot);
+      const uint8_t* base = (const uint8_t*)pg.v + ((int64_t)t.b[i].id * pg.v_page + slot * F::D) * F::E;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) load_bytes<F::VB>(base + lane_at + y * F::D * F::E, v[i][y]);
+      if constexpr (is8(F::CT)) {
+        const int64_t at = ((int64_t)t.b[i].id * pg.H) * pg.ps + slot + 4 * g;
+        s[i] = *reinterpret_cast<const f32x4_t*>(pg.k_scale + at) * c;
+        vs[i] = *reinterpret_cast<const f32x4_t*>(pg.v_scale + at);
+      }
+    }
+    // t = S * c (with the key's scale): base-2 logarithms of the weights
+#pragma unroll
+    for (int i = 0; i < 2 * F::NG; ++i) {
+      if constexpr (is8(F::CT)) s[i] = scores(i) * s[i];
+      else s[i] = scores(i);
+    }
+    if (more) load_k(pg, h, next);
+    const float cc = is8(F::CT) ? 1.0f : c;
+    if (!t.whole(r)) {
+      // keys that are not seen: no weight, and nothing of what stands there
+#pragma unroll
+      for (int i = 0; i < 2 * F::NG; ++i) {
+        const int pos = t.b[i].pos + 4 * g;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const bool seen = pos + y >= r.start && pos + y < r.len;
+          s[i][y] = seen ? s[i][y] : -INFINITY;
+          if constexpr (is8(F::CT)) vs[i][y] = seen ? vs[i][y] : 0.0f;
+#pragma unroll
+          for (int w = 0; w < F::VW; ++w) v[i][y][w] = seen ? v[i][y][w] : 0u;
+        }
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 2 * F::NG; ++i)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) top = fmaxf(top, s[i][y]);
+    top = max_over_rows4(top) * cc;
+    if (__any(top > st.m)) {
+      const float m = fmaxf(st.m, top);
+      const float alpha = m == -INFINITY ? 1.0f : exp2_(st.m - m);
+      st.m = m;
+      st.l *= alpha;
+#pragma unroll
+      for (int j = 0; j < F::VD; ++j) st.o[j] *= alpha;
+    }
+    const float m = st.m == -INFINITY ? 0.0f : st.m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * F::NG; ++i)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const float p = exp2_(fmaf(s[i][y], cc, -m));
+        sum += p;
+        s[i][y] = is8(F::CT) ? p * vs[i][y] : p * F::PSCALE;
+      }
+    st.l += sum;
+    if constexpr (F::F32) {
+#pragma unroll
+      for (int i = 0; i < 2 * F::NG; ++i)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int j = 0; j < F::VD; ++j)
+            st.o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[i][y][j]), s[i][y], st.o[j], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * F::NG; i += 2) {
+        float x[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) x[y] = s[i + y / 4][y & 3];
+        u32x4_t p[F::NP];
+        parts<F::NP, F::F16>(x, [&](int part, u32x4_t w) { p[part] = w; });
+        // channels 2jj, 2jj + 1 of the eight keys, as pairs of 16-bit cells
+        constexpr int PAIRS = F::VD < 2 ? 1 : F::VD / 2;
+#pragma unroll
+        for (int jj = 0; jj < PAIRS; ++jj) {
+          uint32_t w[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            if constexpr (is8(F::CT)) w[y] = cells2_bf16<F::CT>(v[i + y / 4][y & 3][jj / 2], jj & 1);
+            else w[y] = v[i + y / 4][y & 3][jj];
+          }
+#pragma unroll
+          for (int e = 0; e < (F::VD < 2 ? 1 : 2); ++e) {
+            u32x4_t a;
+#pragma unroll
+            for (int x2 = 0; x2 < 4; ++x2)
+              a[x2] = __builtin_amdgcn_perm(w[2 * x2 + 1], w[2 * x2], e ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int part = F::NP - 1; part >= 0; --part) st.o[2 * jj + e] = mma(a, p[part], st.o[2 * jj + e]);
+          }
+        }
+      }
+    }
+  }
+};
+
+// What a workgroup's waves, and then a row's workgroups, are joined by: the
+// weight of a part with maximum m and sum l under the common maximum.  A part
+// without a score above -inf weighs nothing, unless a NaN is in it.
+__device__ __forceinline__ float part_weight(float m, float l, float top) {
+  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2_(m - top);
+}
+
+// How the tiles of all rows are dealt out: a pair is a sequence and 16 heads
+// at most of one key-value head, R pairs a sequence, `tiles` of a sequence for
+// each of its pairs; all in one line, sequence by sequence and pair by pair,
+// cut in `chunk`s, one a workgroup.
+struct Deal {
+  int B, R, RT;      // sequences; pairs of one; pairs of one of its heads
+  int S, shift, P;   // listed entries or -1; the pages
+  int tile;          // keys of a tile
+  int least;         // tiles of a chunk, at least
+  int groups;        // workgroups
+
+  __device__ __forceinline__ int first_tile(int start) const { return S >= 0 || start <= 0 ? 0 : start / tile; }
+  __device__ __forceinline__ int tiles(int start, int len) const {
+    if (S >= 0) return (int)((((int64_t)S << shift) + tile - 1) / tile);
+    return start >= len ? 0 : (len + tile - 1) / tile - first_tile(start);
+  }
+  __device__ __forceinline__ int length(const int32_t* lengths, int b) const {
+    const int64_t n = lengths[b], most = (int64_t)P << shift;
+    return (int)(n < 0 ? 0 : n < most ? n : most);
+  }
+  __device__ __forceinline__ int begin(const int32_t* starts, int b) const {
+    return starts && starts[b] > 0 ? starts[b] : 0;
+  }
+  __device__ __forceinline__ int64_t chunk(int64_t total) const {
+    const int64_t c = (total + groups - 1) / groups;
+    return c < least ? least : c;
+  }
+};
+
+// A value that all lanes share, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                   (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+// Parts of pairs that several workgroups share: slot 2w, the pair that
+// workgroup w continues, 2w + 1, the one that it starts and does not end.
+// O (rows, D), then the maxima and the sums.
+__device__ __forceinline__ float* part_slot(float* parts, int64_t slot, int rows, int D) {
+  return parts + slot * rows * (D + 2);
+}
+
+template <typename F>
+__global__ void __launch_bounds__(64 * kWaves) attend_kernel(
+    Pages pg, Deal deal, const int32_t* __restrict__ table, int64_t table_stride,
+    const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int G,
+    const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts, const int32_t* __restrict__ selected,
+    float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws) {
+  constexpr int D = F::D;
+  __shared__ float so[kWaves][16][D + 4];
+  __shared__ float sm[kWaves][16], sl[kWaves][16];
+  __shared__ int64_t sums[kWaves];
+  __shared__ int64_t found[2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Wave<F> w;
+  w.n = lane & 15, w.g = lane >> 4;
+  const int rows = G < 16 ? G : 16;
+
+  // the workgroup's chunk: [f, f1) of the line, f in pair `r` of sequence b,
+  // whose pairs' first tile is `at` on the line
+  int64_t f, f1, at;
+  int b;
+  if (parts_ws) {
+    int64_t mine = 0;
+    for (int i = tid; i < deal.B; i += 64 * kWaves) mine += deal.tiles(deal.begin(starts, i), deal.length(lengths, i));
+    mine = wave_sum(mine);
+    if (lane == 0) sums[wave] = mine;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) total += sums[i];
+    total = uniform(total) * deal.R;
+    const int64_t chunk = deal.chunk(total);
+    f = blockIdx.x * chunk;
+    if (f >= total) return;
+    f1 = f + chunk < total ? f + chunk : total;
+    int64_t before = 0;
+    for (int base = 0; base < deal.B; base += 64 * kWaves) {
+      const int i = base + tid;
+      const int64_t nt = i < deal.B ? deal.tiles(deal.begin(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
+      int64_t incl = nt;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int64_t x = __shfl_up(incl, o);
+        if (lane >= o) incl += x;
+      }
+      __syncthreads();
+      if (lane == 63) sums[wave] = incl;
+      __syncthreads();
+      int64_t all = 0;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) {
+        if (j < wave) incl += sums[j];
+        all += sums[j];
+      }
+      if (nt > 0 && before + incl - nt <= f && f < before + incl) found[0] = i, found[1] = before + incl - nt;
+      before += all;
+      if (f < before) break;
+    }
+    __syncthreads();
+    b = (int)uniform(found[0]);
+    at = uniform(found[1]);
+  } else {  // a workgroup a pair
+    b = blockIdx.x / deal.R;
+    f = (int64_t)(blockIdx.x % deal.R) * deal.tiles(deal.begin(starts, b), deal.length(lengths, b));
+    f1 = f + 1;
+    at = 0;
+  }
+  const bool lone = !parts_ws;
+
+  while (f < f1) {
+    const int start = deal.begin(starts, b), len = deal.length(lengths, b);
+    const int nt = deal.tiles(start, len);
+    if (!lone && nt == 0) {
+      ++b;
+      continue;
+    }
+    const int pair = lone ? blockIdx.x % deal.R : (int)uniform((f - at) / nt);
+    const int64_t pair_at = at + (int64_t)pair * nt;
+    const int ta = lone ? 0 : (int)(f - pair_at);
+    const int tb = lone || f1 - pair_at > nt ? nt : (int)(f1 - pair_at);
+    const int h = pair / deal.RT, row0 = h * G + 16 * (pair % deal.RT);
+    const int here = (h + 1) * G - row0 < 16 ? (h + 1) * G - row0 : 16;
+
+    w.load_q(q + b * q_b + (row0 + w.n) * q_h, w.n < here);
+    State<F> st;
+#pragma unroll
+    for (int j = 0; j < F::VD; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    st.m = -INFINITY, st.l = 0.0f;
+    Row r{table + b * table_stride, selected + ((int64_t)b * pg.H + h) * (deal.S > 0 ? deal.S : 0), deal.S, deal.P,
+          pg.n_pages, deal.shift, start, len};
+    const int t0 = deal.first_tile(start);
+    int t = t0 + ta + wave;
+    const int te = t0 + tb;
+    if (t < te) {
+      Tile<F> cur, next;
+      cur.find(r, t);
+      w.load_k(pg, h, cur);
+      next = cur;
+      for (; t < te; t += kWaves) {
+        const bool more = t + kWaves < te;
+        if (more) next.find(r, t + kWaves);
+        w.step(pg, r, h, c, cur, more, next, st);
+        cur = next;
+      }
+    }
+
+    // join the waves
+    float l = st.l;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (w.n < here) {
+      if (w.g == 0) sm[wave][w.n] = st.m, sl[wave][w.n] = l;
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int j = 0; j < F::VD; ++j) so[wave][w.n][F::VD * (4 * w.g + y) + j] = st.o[j][y];
+    }
+    __syncthreads();
+    const bool ends = tb == nt, whole = ta == 0 && ends;
+    float* slot = whole ? nullptr : part_slot(parts_ws, 2 * (int64_t)blockIdx.x + (ta == 0), rows, D);
+    for (int i = tid; i < here * D; i += 64 * kWaves) {
+      const int row = i / D, d = i % D;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) top = fmaxf(top, sm[j][row]);
+      float o = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) {
+        const float a = part_weight(sm[j][row], sl[j][row], top);
+        o += a == 0.0f ? 0.0f : a * so[j][row][d];
+        sum += a == 0.0f ? 0.0f : a * sl[j][row];
+      }
+      if (whole) {
+        store_f<F::QT>(out + ((int64_t)b * (deal.R / deal.RT) * G + row0 + row) * D + d,
+                       sum == 0.0f ? 0.0f : o / (sum * F::PSCALE));
+      } else {
+        slot[i] = o;
+        if (d == 0) slot[rows * D + row] = top, slot[rows * (D + 1) + row] = sum;
+      }
+    }
+    if (lone) return;
+    f = pair_at + tb;
+    if (ends && pair + 1 == deal.R) {
+      at = f;
+      ++b;
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the parts of one row; writes the rows of sequences that see nothing.
+template <int QT>
+__global__ void __launch_bounds__(256) join_kernel(Deal deal, int G, int D, float pscale,
+                                                   const int32_t* __restrict__ lengths,
+                                                   const int32_t* __restrict__ starts, float* __restrict__ parts,
+                                                   typename Elem<QT>::T* __restrict__ out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x / deal.R, pair = blockIdx.x % deal.R;
+  const int h = pair / deal.RT, row = blockIdx.y, head = h * G + 16 * (pair % deal.RT) + row;
+  if (head >= (h + 1) * G) return;
+  __shared__ int64_t sums[2][4];
+  int64_t total = 0, before = 0;
+  for (int i = tid; i < deal.B; i += 256) {
+    const int nt = deal.tiles(deal.begin(starts, i), deal.length(lengths, i));
+    total += nt;
+    before += i < b ? nt : 0;
+  }
+  total = wave_sum(total), before = wave_sum(before);
+  if (lane == 0) sums[0][wave] = total, sums[1][wave] = before;
+  __syncthreads();
+  total = (sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3]) * deal.R;
+  const int nt = deal.tiles(deal.begin(starts, b), deal.length(lengths, b));
+  typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head) * D;
+  if (nt == 0) {
+    for (int d = tid; d < D; d += 256) store_f<QT>(to + d, 0.0f);
+    return;
+  }
+  before = (sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3]) * deal.R + (int64_t)pair * nt;
+  const int64_t chunk = deal.chunk(total);
+  const int64_t w0 = before / chunk, w1 = (before + nt - 1) / chunk;
+  if (w0 == w1) return;  // written by its one workgroup
+  const int rows = G < 16 ? G : 16;
+  // part i of the row is workgroup w0 + i's
+  auto slot = [&](int64_t i) { return part_slot(parts, 2 * (w0 + i) + (i == 0), rows, D); };
+  const int n = (int)(w1 - w0) + 1;
+  __shared__ float red[4];
+  __shared__ float acc[256], accl[256];
+  float top = -INFINITY;
+  for (int i = tid; i < n; i += 256) top = fmaxf(top, slot(i)[rows * D + row]);
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  // D threads a part, 256 / D parts at once
+  const int d = tid % D, lot = tid / D, lots = 256 / D;
+  float o = 0.0f, sum = 0.0f;
+  for (int i = lot; i < n; i += lots) {
+    const float* s = slot(i);
+    const float l = s[rows * (D + 1) + row], a = part_weight(s[rows * D + row], l, top);
+    if (a != 0.0f) o += a * s[row * D + d], sum += a * l;
+  }
+  acc[tid] = o, accl[tid] = sum;
+  __syncthreads();
+  if (lot) return;
+  for (int i = 1; i < lots; ++i) o += acc[i * D + d], sum += accl[i * D + d];
+  store_f<QT>(to + d, sum == 0.0f ? 0.0f : o / (sum * pscale));
+}
+
+// A call's arguments behind its checks.
+struct AttendCall {
+  Pages pg;
+  const int32_t* table;
+  int64_t table_stride;
+  int P, B, H, D;
+  pfa_tensor4 q;
+  const int32_t *lengths, *starts, *selected;
+  int S;
+  float c;  // scale * log2(e)
+  void* out;
+  float* parts;
+  hipStream_t stream;
+};
+
+// Workgroups of a call that shares its rows out.
+constexpr int kGroups = 1024;
+constexpr int kLeast = 8;   // tiles of a chunk
+constexpr int kLone = 16;   // tiles that one workgroup takes rather than two launches
+
+struct Plan {
+  Deal deal;
+  size_t bytes;  // of the parts; 0: a workgroup a pair
+};
+
+inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int S, int tile) {
+  Plan p{};
+  const int G = H / kv_heads, RT = (G + 15) / 16;
+  const int64_t keys = (int64_t)(S >= 0 ? S : P) << shift, most = (keys + tile - 1) / tile;
+  p.deal = Deal{B, kv_heads * RT, RT, S, shift, P, tile, kLeast, 0};
+  if (most > kLone) {
+    const int64_t chunks = (most * B * p.deal.R + kLeast - 1) / kLeast;
+    p.deal.groups = (int)(chunks < kGroups ? chunks : kGroups);
+    p.bytes = (size_t)p.deal.groups * 2 * (G < 16 ? G : 16) * (D + 2) * 4;
+  }
+  return p;
+}
+
+// Keys of a tile, as Form has them.
+inline int attend_tile(int ct, int D) {
+  const int bytes = D * cell_bytes(ct);
+  return bytes >= 256 ? 32 : bytes >= 128 ? 64 : 128;
+}
+
+template <int QT, int CT, int D>
+void attend_launch(const AttendCall& a) {
+  using F = Form<QT, CT, D>;
+  using T = typename Elem<QT>::T;
+  const Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE);
+  const Deal& deal = p.deal;
+  const int G = a.H / a.pg.H;
+  const unsigned pairs = (unsigned)(a.B * deal.R);
+  attend_kernel<F><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
+      a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, G, a.lengths, a.starts, a.selected, a.c,
+      (T*)a.out, p.bytes ? a.parts : nullptr);
+  if (p.bytes)
+    join_kernel<QT><<<dim3(pairs, G < 16 ? G : 16), 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts,
+                                                                        a.parts, (T*)a.out);
+}
+
+template <int QT, int CT>
+void attend_by_width(const AttendCall& a) {
+  switch (a.D) {
+    case 16: return attend_launch<QT, CT, 16>(a);
+    case 32: return attend_launch<QT, CT, 32>(a);
+    case 64: return attend_launch<QT, CT, 64>(a);
+    default: return attend_launch<QT, CT, 128>(a);
+  }
+}
+
+// One translation unit each, by the cells' type.
+void attend_float(int qt, const AttendCall& a);
+void attend_i8(int qt, const AttendCall& a);
+void attend_e4m3(int qt, const AttendCall& a);
+
+}  // namespace paged
+}  // namespace pfa

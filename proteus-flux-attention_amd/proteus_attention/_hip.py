@@ -191,7 +191,7 @@ _SIGNATURES = {
                               _sz, _vp], _i32),
     "pfa_kv_pages_write": ([KVPagesC, Tensor4, Tensor4, _i32, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp], _i32),
     "pfa_kv_pages_read": ([KVPagesC, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
-    "pfa_paged_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
+    "pfa_paged_attn_workspace_size": ([_i32, _i32, KVPagesC, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_paged_attn_fwd": ([Tensor4, _i32, _i32, _i32, KVPagesC, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _vp,
                             _sz, _vp], _i32),
     "pfa_kv_pages_select_workspace_size": ([_i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),

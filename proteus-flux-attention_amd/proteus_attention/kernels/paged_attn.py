@@ -272,7 +272,7 @@ def _attend(a: _Query, selected: Optional[torch.Tensor], scale: float) -> torch.
     lib = _hip.lib()
     size = ctypes.c_size_t(0)
     P, S = a.table.shape[1], -1 if selected is None else selected.shape[2]
-    _hip.check(lib.pfa_paged_attn_workspace_size(B, H, a.pool.kv_heads, D, a.pool.page_size, P, S, ctypes.byref(size)),
+    _hip.check(lib.pfa_paged_attn_workspace_size(B, H, a.pool, P, S, ctypes.byref(size)),
                "pfa_paged_attn_workspace_size")
     ws = _workspace(size.value, a.device)
     out = torch.empty(B, H, D, dtype=a.q.dtype, device=a.device)
