@@ -2,6 +2,7 @@
 // new token over it.
 #include "pfa_paged.h"
 #include "pfa_paged_attn.h"
+#include "pfa_paged_select.h"
 
 namespace pfa {
 
@@ -211,76 +212,6 @@ __global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int D, i
   }
 }
 
-// ---------------------------------------------------------------------
-// Selection.  Scores: a wave per (sequence, head, page), then the rank of a
-// page by counting the better ones.
-// ---------------------------------------------------------------------
-template <int QT, int BT>
-__global__ void __launch_bounds__(64) score_kernel(Pages pg, Table tab, pfa_tensor4 q, int G, int D,
-                                                   const int32_t* __restrict__ lengths,
-                                                   const int32_t* __restrict__ starts, int first, int last,
-                                                   uint32_t* __restrict__ keys) {
-  const int64_t b = blockIdx.z;
-  const int h = blockIdx.y, page = blockIdx.x, lane = threadIdx.x;
-  const int64_t len = length_at(lengths, tab, pg, b);
-  const int64_t start = starts && starts[b] > 0 ? starts[b] : 0;
-  uint32_t* key = keys + (b * pg.H + h) * tab.P + page;
-  const int64_t p0 = start >> pg.shift, pe = (len + pg.ps - 1) >> pg.shift;
-  const int id = start < len && page >= p0 && page < pe ? page_at(tab, pg, b, page) : -1;
-  if (id < 0) {
-    if (lane == 0) *key = 0;  // no candidate
-    return;
-  }
-  const typename Elem<BT>::T* lo = (const typename Elem<BT>::T*)pg.bounds + ((int64_t)id * pg.H + h) * 2 * D;
-  float best = -INFINITY;
-  bool nan = false;
-  for (int g = 0; g < G; ++g) {
-    const typename Elem<QT>::T* qp = (const typename Elem<QT>::T*)q.ptr + b * q.s_b + (int64_t)(h * G + g) * q.s_h;
-    double s = 0.0;
-    for (int d = lane; d < D; d += kWave) {
-      const float x = load_f<QT>(qp + d);
-      s += (double)x * (double)load_f<BT>(lo + (x > 0.0f ? D : 0) + d);
-    }
-    for (int o = 1; o < kWave; o <<= 1) s += __shfl_xor(s, o);
-    const float f = (float)s;
-    nan = nan || f != f;
-    best = fmaxf(best, f);
-  }
-  if (lane) return;
-  uint32_t u = __float_as_uint(best);
-  u = u & 0x80000000u ? ~u : u | 0x80000000u;
-  if (nan) u = 1;
-  if (page < p0 + first || page >= pe - last) u = 0xffffffffu;
-  *key = u;
-}
-
-__global__ void __launch_bounds__(256) rank_kernel(int P, int H, int count, const uint32_t* __restrict__ keys,
-                                                   int32_t* __restrict__ chosen) {
-  const uint32_t* key = keys + (int64_t)blockIdx.x * P;
-  int32_t* out = chosen + (int64_t)blockIdx.x * count;
-  __shared__ int taken[256];
-  int base = 0;
-  for (int p0 = 0; p0 < P; p0 += 256) {
-    const int p = p0 + threadIdx.x;
-    const uint32_t mine = p < P ? key[p] : 0;
-    int before = 0;
-    if (mine) {
-      for (int o = 0; o < P; ++o) before += key[o] > mine || (key[o] == mine && o < p);
-    }
-    taken[threadIdx.x] = mine && before < count;
-    __syncthreads();
-    int rank = base, all = base;
-    for (int i = 0; i < 256; ++i) {
-      rank += i < (int)threadIdx.x ? taken[i] : 0;
-      all += taken[i];
-    }
-    if (taken[threadIdx.x]) out[rank] = p;
-    base = all;
-    __syncthreads();
-  }
-  for (int i = base + threadIdx.x; i < count; i += 256) out[i] = -1;
-}
-
 // Calls f with the (values, cells) types as template arguments: the cells' own
 // float type, or any of the three with 8-bit cells.
 template <typename F>
@@ -377,7 +308,7 @@ int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H,
   if (int rc = types_check(dtype, pages.dtype)) return rc;
   PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages.kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
                 pages.kv_heads);
-  PFA_CHECK_ARG((int64_t)B * H <= 1 << 23, "%s: up to 2^23 rows (got %d x %d)", what, B, H);
+  PFA_CHECK_ARG((int64_t)B * H <= 1 << 21, "%s: up to 2^21 rows (got %d x %d)", what, B, H);
   PFA_CHECK_ARG(B == 0 || (q.ptr && lengths), "%s: null argument", what);
   return PFA_OK;
 }
@@ -412,14 +343,32 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
     return PFA_E_WORKSPACE;
   }
   uint32_t* keys = (uint32_t*)workspace;
-  if (table_pages > 0) {
+  const int D = pages.head_dim, P = table_pages, rows = B * p.H;
+  if (P > 0) {
     by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
-      score_kernel<decltype(dt)::value, bound_dtype(decltype(ct)::value)>
-          <<<dim3(table_pages, p.H, B), 64, 0, as_stream(stream)>>>(p, t, q, H / p.H, pages.head_dim, lengths, starts,
-                                                                    first, last, keys);
+      constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
+      auto score = [&](auto width) {
+        constexpr int W = decltype(width)::value;
+        constexpr int at_once = 4 * (kWave / (W / 8)) * kSteps;
+        score_kernel<QT, BT, W><<<dim3((P + at_once - 1) / at_once, p.H, B), 256, 0, as_stream(stream)>>>(
+            p, table, table_stride, P, (const typename Elem<QT>::T*)q.ptr, q.s_b, q.s_h, H / p.H, lengths, starts, first,
+            last, keys);
+      };
+      if (D == 16) score(std::integral_constant<int, 16>{});
+      else if (D == 32) score(std::integral_constant<int, 32>{});
+      else if (D == 64) score(std::integral_constant<int, 64>{});
+      else score(std::integral_constant<int, 128>{});
     });
   }
-  rank_kernel<<<B * p.H, 256, 0, as_stream(stream)>>>(table_pages, p.H, count, keys, chosen);
+  auto choose = [&](auto threads, auto rounds) {
+    choose_kernel<decltype(threads)::value, decltype(rounds)::value>
+        <<<rows, decltype(threads)::value, 0, as_stream(stream)>>>(p.H, P, p.shift, count, lengths, starts, keys, chosen);
+  };
+  using std::integral_constant;
+  if (P <= 1024) choose(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (P <= 4096) choose(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  else if (P <= 16384) choose(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+  else choose(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
   PFA_CHECK_LAUNCH("kv_pages_select");
   return PFA_OK;
 }
