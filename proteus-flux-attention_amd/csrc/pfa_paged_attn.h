@@ -87,6 +87,9 @@ __device__ __forceinline__ uint32_t cells2_bf16(uint32_t w, int i) {
   }
 }
 
+// 32-key groups of a tile.
+__host__ __device__ constexpr int tile_groups(int ct, int D) { return D * cell_bytes(ct) >= 128 ? 1 : 2; }
+
 // Cells of a call's kernel, by the types of queries and cells and the head's width.
 template <int QT_, int CT_, int D_>
 struct Form {
@@ -102,10 +105,10 @@ struct Form {
   static constexpr int VD = D / 16;                    // channels of a lane in O
   static constexpr int VB = VD * E;                    // their bytes of a key
   static constexpr int VW = VB < 4 ? 1 : VB / 4;
-  // 32-key groups that a wave loads at once: 8 KB of keys for rows of 64 bytes
-  // and more
-  static constexpr int NG = D * E >= 256 ? 1 : D * E >= 128 ? 2 : 4;
+  static constexpr int NG = tile_groups(CT, D);  // 32-key groups that a wave loads at once
   static constexpr int TILE = 32 * NG;
+  // waves of a SIMD, at least, that the registers leave without spills
+  static constexpr int AT_LEAST = QT == PFA_F32 && D == 128 ? 2 : 3;
   static constexpr float PSCALE = F16 ? 32768.0f : 1.0f;
 };
 
@@ -377,9 +380,13 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 }
 
 // How the tiles of all rows are dealt out: a pair is a sequence and 16 heads
-// at most of one key-value head, R pairs a sequence, `tiles` of a sequence for
-// each of its pairs; all in one line, sequence by sequence and pair by pair,
-// cut in `chunk`s, one a workgroup.
+// at most of one key-value head, R pairs a sequence.  All pairs lie in one line,
+// sequence by sequence, kStart places and one for each of its tiles long, and the
+// line is cut in `chunk`s, one a workgroup.  The kStart places stand for what a
+// pair costs before its first key arrives and after its last: without them a
+// workgroup with a dozen one-tile pairs was the last to end.
+constexpr int kStart = 8;
+
 struct Deal {
   int B, R, RT;      // sequences; pairs of one; pairs of one of its heads
   int S, shift, P;   // listed entries or -1; the pages
@@ -398,6 +405,11 @@ struct Deal {
   }
   __device__ __forceinline__ int begin(const int32_t* starts, int b) const {
     return starts && starts[b] > 0 ? starts[b] : 0;
+  }
+  // places of a pair
+  __device__ __forceinline__ int places(int start, int len) const {
+    const int n = tiles(start, len);
+    return n > 0 ? n + kStart : 0;
   }
   __device__ __forceinline__ int64_t chunk(int64_t total) const {
     const int64_t c = (total + groups - 1) / groups;
@@ -425,7 +437,7 @@ __device__ __forceinline__ float* part_slot(float* parts, int64_t slot, int rows
 }
 
 template <typename F>
-__global__ void __launch_bounds__(64 * kWaves) attend_kernel(
+__global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     Pages pg, Deal deal, const int32_t* __restrict__ table, int64_t table_stride,
     const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int G,
     const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts, const int32_t* __restrict__ selected,
@@ -441,13 +453,13 @@ __global__ void __launch_bounds__(64 * kWaves) attend_kernel(
   w.n = lane & 15, w.g = lane >> 4;
   const int rows = G < 16 ? G : 16;
 
-  // the workgroup's chunk: [f, f1) of the line, f in pair `r` of sequence b,
-  // whose pairs' first tile is `at` on the line
+  // the workgroup's chunk: [f, f1) of the line, f in a pair of sequence b, whose
+  // first pair begins at `at`
   int64_t f, f1, at;
   int b;
   if (parts_ws) {
     int64_t mine = 0;
-    for (int i = tid; i < deal.B; i += 64 * kWaves) mine += deal.tiles(deal.begin(starts, i), deal.length(lengths, i));
+    for (int i = tid; i < deal.B; i += 64 * kWaves) mine += deal.places(deal.begin(starts, i), deal.length(lengths, i));
     mine = wave_sum(mine);
     if (lane == 0) sums[wave] = mine;
     __syncthreads();
@@ -462,7 +474,7 @@ __global__ void __launch_bounds__(64 * kWaves) attend_kernel(
     int64_t before = 0;
     for (int base = 0; base < deal.B; base += 64 * kWaves) {
       const int i = base + tid;
-      const int64_t nt = i < deal.B ? deal.tiles(deal.begin(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
+      const int64_t nt = i < deal.B ? deal.places(deal.begin(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
       int64_t incl = nt;
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) {
@@ -495,15 +507,21 @@ __global__ void __launch_bounds__(64 * kWaves) attend_kernel(
 
   while (f < f1) {
     const int start = deal.begin(starts, b), len = deal.length(lengths, b);
-    const int nt = deal.tiles(start, len);
+    const int nt = deal.tiles(start, len), np = deal.places(start, len);
     if (!lone && nt == 0) {
       ++b;
       continue;
     }
-    const int pair = lone ? blockIdx.x % deal.R : (int)uniform((f - at) / nt);
-    const int64_t pair_at = at + (int64_t)pair * nt;
-    const int ta = lone ? 0 : (int)(f - pair_at);
-    const int tb = lone || f1 - pair_at > nt ? nt : (int)(f1 - pair_at);
+    const int pair = lone ? blockIdx.x % deal.R : (int)uniform((f - at) / np);
+    // the pair's first tile on the line, and its tiles [ta, tb) in the chunk
+    const int64_t pair_at = at + (int64_t)pair * np + kStart;
+    const int ta = lone || f < pair_at ? 0 : (int)(f - pair_at);
+    const int tb = lone || f1 - pair_at > nt ? nt : f1 < pair_at ? 0 : (int)(f1 - pair_at);
+    if (!lone) {
+      if (tb == 0) return;  // the chunk ends before the pair's first tile
+      f = pair_at + tb;
+      if (tb == nt && pair + 1 == deal.R) at = f;
+    }
     const int h = pair / deal.RT, row0 = h * G + 16 * (pair % deal.RT);
     const int here = (h + 1) * G - row0 < 16 ? (h + 1) * G - row0 : 16;
 
@@ -565,72 +583,85 @@ __global__ void __launch_bounds__(64 * kWaves) attend_kernel(
       }
     }
     if (lone) return;
-    f = pair_at + tb;
-    if (ends && pair + 1 == deal.R) {
-      at = f;
-      ++b;
-    }
+    if (ends && pair + 1 == deal.R) ++b;
     __syncthreads();
   }
 }
 
-// Joins the parts of one row; writes the rows of sequences that see nothing.
-template <int QT>
-__global__ void __launch_bounds__(256) join_kernel(Deal deal, int G, int D, float pscale,
-                                                   const int32_t* __restrict__ lengths,
-                                                   const int32_t* __restrict__ starts, float* __restrict__ parts,
-                                                   typename Elem<QT>::T* __restrict__ out) {
+// Joins the parts of a row, a workgroup a row; writes the rows of sequences that
+// see nothing.  A wave takes every WAVESth part, a lane D / 64 channels of it (one
+// of 64 / D parts for narrow heads).
+template <int QT, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float pscale,
+                                                       const int32_t* __restrict__ lengths,
+                                                       const int32_t* __restrict__ starts, float* __restrict__ parts,
+                                                       typename Elem<QT>::T* __restrict__ out) {
+  constexpr int WAVES = THREADS / kWave;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / deal.R, pair = blockIdx.x % deal.R;
   const int h = pair / deal.RT, row = blockIdx.y, head = h * G + 16 * (pair % deal.RT) + row;
   if (head >= (h + 1) * G) return;
-  __shared__ int64_t sums[2][4];
+  __shared__ int64_t sums[2][WAVES];
+  __shared__ float red[WAVES];
+  __shared__ float acc[WAVES][128];
+  __shared__ float accl[WAVES];
   int64_t total = 0, before = 0;
-  for (int i = tid; i < deal.B; i += 256) {
-    const int nt = deal.tiles(deal.begin(starts, i), deal.length(lengths, i));
-    total += nt;
-    before += i < b ? nt : 0;
+  for (int i = tid; i < deal.B; i += THREADS) {
+    const int n = deal.places(deal.begin(starts, i), deal.length(lengths, i));
+    total += n;
+    before += i < b ? n : 0;
   }
+  const int nt = deal.tiles(deal.begin(starts, b), deal.length(lengths, b));
   total = wave_sum(total), before = wave_sum(before);
   if (lane == 0) sums[0][wave] = total, sums[1][wave] = before;
   __syncthreads();
-  total = (sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3]) * deal.R;
-  const int nt = deal.tiles(deal.begin(starts, b), deal.length(lengths, b));
+  total = before = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) total += sums[0][w], before += sums[1][w];
   typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head) * D;
   if (nt == 0) {
-    for (int d = tid; d < D; d += 256) store_f<QT>(to + d, 0.0f);
+    for (int d = tid; d < D; d += THREADS) store_f<QT>(to + d, 0.0f);
     return;
   }
-  before = (sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3]) * deal.R + (int64_t)pair * nt;
-  const int64_t chunk = deal.chunk(total);
-  const int64_t w0 = before / chunk, w1 = (before + nt - 1) / chunk;
+  const int64_t chunk = deal.chunk(total * deal.R);
+  const int64_t first = before * deal.R + (int64_t)pair * (nt + kStart) + kStart;  // the pair's first tile
+  const int64_t w0 = first / chunk, w1 = (first + nt - 1) / chunk;
   if (w0 == w1) return;  // written by its one workgroup
   const int rows = G < 16 ? G : 16;
-  // part i of the row is workgroup w0 + i's
-  auto slot = [&](int64_t i) { return part_slot(parts, 2 * (w0 + i) + (i == 0), rows, D); };
   const int n = (int)(w1 - w0) + 1;
-  __shared__ float red[4];
-  __shared__ float acc[256], accl[256];
+  // part i of the row is workgroup w0 + i's
+  auto slot = [&](int i) { return part_slot(parts, 2 * (w0 + i) + (i == 0), rows, D); };
   float top = -INFINITY;
-  for (int i = tid; i < n; i += 256) top = fmaxf(top, slot(i)[rows * D + row]);
+  for (int i = tid; i < n; i += THREADS) top = fmaxf(top, slot(i)[rows * D + row]);
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
   if (lane == 0) red[wave] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  // D threads a part, 256 / D parts at once
-  const int d = tid % D, lot = tid / D, lots = 256 / D;
-  float o = 0.0f, sum = 0.0f;
-  for (int i = lot; i < n; i += lots) {
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, red[w]);
+  const int d = lane % D, per = D < kWave ? kWave / D : 1, mine = D < kWave ? lane / D : 0;
+  const bool two = D > kWave;
+  float o0 = 0.0f, o1 = 0.0f, sum = 0.0f;
+#pragma unroll 8
+  for (int i = wave * per + mine; i < n; i += WAVES * per) {
     const float* s = slot(i);
     const float l = s[rows * (D + 1) + row], a = part_weight(s[rows * D + row], l, top);
-    if (a != 0.0f) o += a * s[row * D + d], sum += a * l;
+    const float x = s[row * D + d], y = two ? s[row * D + 64 + d] : 0.0f;
+    o0 += a == 0.0f ? 0.0f : a * x, o1 += a == 0.0f ? 0.0f : a * y, sum += a == 0.0f ? 0.0f : a * l;
   }
-  acc[tid] = o, accl[tid] = sum;
+  for (int o = D; o < kWave; o <<= 1) o0 += __shfl_xor(o0, o), sum += __shfl_xor(sum, o);
+  if (lane < D) {
+    acc[wave][d] = o0;
+    if (two) acc[wave][64 + d] = o1;
+  }
+  if (lane == 0) accl[wave] = sum;
   __syncthreads();
-  if (lot) return;
-  for (int i = 1; i < lots; ++i) o += acc[i * D + d], sum += accl[i * D + d];
-  store_f<QT>(to + d, sum == 0.0f ? 0.0f : o / (sum * pscale));
+  for (int c = tid; c < D; c += THREADS) {
+    float o = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) o += acc[w][c], l += accl[w];
+    store_f<QT>(to + c, l == 0.0f ? 0.0f : o / (l * pscale));
+  }
 }
 
 // A call's arguments behind its checks.
@@ -648,9 +679,10 @@ struct AttendCall {
   hipStream_t stream;
 };
 
-// Workgroups of a call that shares its rows out.
+// Workgroups of a call that shares its rows out: as many as the chip holds at
+// once, at most kGroups.
 constexpr int kGroups = 1024;
-constexpr int kLeast = 8;   // tiles of a chunk
+constexpr int kLeast = 16;  // places of a chunk
 constexpr int kLone = 16;   // tiles that one workgroup takes rather than two launches
 
 struct Plan {
@@ -664,33 +696,45 @@ inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int
   const int64_t keys = (int64_t)(S >= 0 ? S : P) << shift, most = (keys + tile - 1) / tile;
   p.deal = Deal{B, kv_heads * RT, RT, S, shift, P, tile, kLeast, 0};
   if (most > kLone) {
-    const int64_t chunks = (most * B * p.deal.R + kLeast - 1) / kLeast;
+    const int64_t chunks = ((most + kStart) * B * p.deal.R + kLeast - 1) / kLeast;
     p.deal.groups = (int)(chunks < kGroups ? chunks : kGroups);
     p.bytes = (size_t)p.deal.groups * 2 * (G < 16 ? G : 16) * (D + 2) * 4;
   }
   return p;
 }
 
-// Keys of a tile, as Form has them.
-inline int attend_tile(int ct, int D) {
-  const int bytes = D * cell_bytes(ct);
-  return bytes >= 256 ? 32 : bytes >= 128 ? 64 : 128;
+inline int attend_tile(int ct, int D) { return 32 * tile_groups(ct, D); }
+
+// Workgroups of a kernel that the chip holds at once.
+inline int resident(const void* kernel, int threads) {
+  int device = 0, units = 0, each = 0;
+  if (hipGetDevice(&device) != hipSuccess ||
+      hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+      hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, threads, 0) != hipSuccess || units * each <= 0)
+    return kGroups;
+  return units * each;
 }
 
 template <int QT, int CT, int D>
 void attend_launch(const AttendCall& a) {
   using F = Form<QT, CT, D>;
   using T = typename Elem<QT>::T;
-  const Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE);
-  const Deal& deal = p.deal;
+  Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE);
+  Deal& deal = p.deal;
+  static const int at_once = resident(reinterpret_cast<const void*>(&attend_kernel<F>), 64 * kWaves);
+  if (deal.groups > at_once) deal.groups = at_once;
   const int G = a.H / a.pg.H;
   const unsigned pairs = (unsigned)(a.B * deal.R);
   attend_kernel<F><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
       a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, G, a.lengths, a.starts, a.selected, a.c,
       (T*)a.out, p.bytes ? a.parts : nullptr);
-  if (p.bytes)
-    join_kernel<QT><<<dim3(pairs, G < 16 ? G : 16), 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts,
-                                                                        a.parts, (T*)a.out);
+  if (!p.bytes) return;
+  const dim3 rows(pairs, G < 16 ? G : 16);
+  // a row of a few pairs has parts by the hundred
+  if (pairs >= 64)
+    join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, (T*)a.out);
+  else
+    join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, (T*)a.out);
 }
 
 template <int QT, int CT>
