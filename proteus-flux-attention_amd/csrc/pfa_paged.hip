@@ -315,10 +315,13 @@ int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H,
 
 }  // namespace
 
+// Keys of a row, 16-byte aligned.
+static int64_t row_keys(int table_pages) { return ((int64_t)table_pages + 3) & ~3ll; }
+
 extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes) {
   clear_error();
   PFA_CHECK_ARG(bytes && B >= 0 && kv_heads > 0 && table_pages >= 0, "kv_pages_select: bad sizes");
-  *bytes = (size_t)B * kv_heads * table_pages * 4;
+  *bytes = (size_t)B * kv_heads * row_keys(table_pages) * 4;
   return PFA_OK;
 }
 
@@ -338,7 +341,7 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
   PFA_CHECK_ARG(chosen, "kv_pages_select: null argument");
   size_t need = 0;
   pfa_kv_pages_select_workspace_size(B, p.H, table_pages, &need);
-  if (ws_bytes < need || (need && !workspace)) {
+  if (ws_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16 != 0))) {
     set_error("kv_pages_select: workspace of %zu bytes, %zu needed", ws_bytes, need);
     return PFA_E_WORKSPACE;
   }
@@ -350,9 +353,9 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
       auto score = [&](auto width) {
         constexpr int W = decltype(width)::value;
         constexpr int at_once = 4 * (kWave / (W / 8)) * kSteps;
-        score_kernel<QT, BT, W><<<dim3((P + at_once - 1) / at_once, p.H, B), 256, 0, as_stream(stream)>>>(
+        score_kernel<QT, BT, W><<<dim3(p.H, (P + at_once - 1) / at_once, B), 256, 0, as_stream(stream)>>>(
             p, table, table_stride, P, (const typename Elem<QT>::T*)q.ptr, q.s_b, q.s_h, H / p.H, lengths, starts, first,
-            last, keys);
+            last, row_keys(P), keys);
       };
       if (D == 16) score(std::integral_constant<int, 16>{});
       else if (D == 32) score(std::integral_constant<int, 32>{});
@@ -360,15 +363,16 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
       else score(std::integral_constant<int, 128>{});
     });
   }
-  auto choose = [&](auto threads, auto rounds) {
-    choose_kernel<decltype(threads)::value, decltype(rounds)::value>
-        <<<rows, decltype(threads)::value, 0, as_stream(stream)>>>(p.H, P, p.shift, count, lengths, starts, keys, chosen);
-  };
-  using std::integral_constant;
-  if (P <= 1024) choose(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-  else if (P <= 4096) choose(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
-  else if (P <= 16384) choose(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
-  else choose(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
+  // entries of a row from the first's four on: up to P + 3
+#define PFA_CHOOSE(THREADS, K, HELD)                                                                          \
+  choose_kernel<THREADS, K, HELD><<<rows, THREADS, 0, as_stream(stream)>>>(p.H, P, row_keys(P), p.shift, count, \
+                                                                           lengths, starts, keys, chosen)
+  if (P + 3 <= 256 * 4) PFA_CHOOSE(256, 4, true);
+  else if (P + 3 <= 1024 * 4) PFA_CHOOSE(1024, 4, true);
+  else if (P + 3 <= 1024 * 8) PFA_CHOOSE(1024, 8, true);
+  else if (P + 3 <= 1024 * 16) PFA_CHOOSE(1024, 16, true);
+  else PFA_CHOOSE(1024, 16, false);
+#undef PFA_CHOOSE
   PFA_CHECK_LAUNCH("kv_pages_select");
   return PFA_OK;
 }

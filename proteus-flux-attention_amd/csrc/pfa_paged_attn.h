@@ -119,22 +119,25 @@ struct Block {
 };
 constexpr int kNowhere = 0x7fffff00;
 
+// Pages of a run of tiles, in LDS: looked up by all of the workgroup's threads at
+// once, so that a tile's lookup, two loads one behind the other, is not in front
+// of every tile's keys.
+constexpr int kEntries = 512;
+struct Entry {
+  int id, pos;  // the page, and the position of its first slot or kNowhere
+};
+
 // One sequence and key-value head.
 struct Row {
-  const int32_t* ids;   // the sequence's row of the table
-  const int32_t* list;  // the listed entries, where S >= 0
-  int S, P, n_pages, shift, start, len;
+  const Entry* entries;  // the run's
+  int first;             // entry of the run's first
+  int shift, start, len;
 
   // `key` counts positions, or the slots of the listed pages
   __device__ __forceinline__ Block block(int key) const {
-    int ordinal = key >> shift;
-    if (S >= 0) ordinal = ordinal < S ? list[ordinal] : -1;
-    ordinal = __builtin_amdgcn_readfirstlane(ordinal);
-    int id = (uint32_t)ordinal < (uint32_t)P ? ids[ordinal] : -1;
-    id = __builtin_amdgcn_readfirstlane(id);
+    const Entry e = entries[(key >> shift) - first];
     const int slot = key & ((1 << shift) - 1);
-    if ((uint32_t)id >= (uint32_t)n_pages) return Block{0, slot, kNowhere};
-    return Block{id, slot, (ordinal << shift) + slot};
+    return Block{__builtin_amdgcn_readfirstlane(e.id), slot, __builtin_amdgcn_readfirstlane(e.pos) + slot};
   }
 };
 
@@ -177,16 +180,31 @@ struct Wave {
   // Channel of a lane's element x: unit x / U of 4U channels, one U a lane group.
   __device__ __forceinline__ int channel(int x) const { return x / F::U * 4 * F::U + g * F::U + x % F::U; }
 
-  __device__ __forceinline__ void load_q(const typename Elem<F::QT>::T* p, bool row) {
+  // `vec`: the row is 16-byte aligned
+  __device__ __forceinline__ void load_q(const typename Elem<F::QT>::T* p, bool row, bool vec) {
     if constexpr (F::F32) {
 #pragma unroll
-      for (int x = 0; x < F::EL; ++x) qf[x] = row ? p[channel(x)] : 0.0f;
+      for (int x = 0; x < F::EL; x += 4) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* at = p + channel(x);
+        if (row) {
+          if (vec) a = *reinterpret_cast<const float4*>(at);
+          else a = make_float4(at[0], at[1], at[2], at[3]);
+        }
+        qf[x] = a.x, qf[x + 1] = a.y, qf[x + 2] = a.z, qf[x + 3] = a.w;
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < F::NC; ++c) {
-        float x[8];
+        float x[8] = {};
+        const typename Elem<F::QT>::T* at = p + channel(8 * c);
+        if (row) {
+          if (vec && F::EL >= 8) load8<F::QT>(at, x);
+          else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = row && 8 * c + e < F::EL ? load_f<F::QT>(p + channel(8 * c + e)) : 0.0f;
+            for (int e = 0; e < (F::EL < 8 ? F::EL : 8); ++e) x[e] = load_f<F::QT>(at + e);
+          }
+        }
         parts<F::NQ, F::F16>(x, [&](int part, u32x4_t w) { q[part][c] = w; });
       }
     }
@@ -265,8 +283,10 @@ struct Wave {
   }
 
   // One tile: V loads, S from the keys that are in registers, the next tile's
-  // keys, P, and O.
-  __device__ __forceinline__ void step(const Pages& pg, const Row& r, int h, float c, const Tile<F>& t, bool more,
+  // keys, P, and O.  The next keys are loaded whether or not there is a next tile
+  // (`next` is this one then): a load under a condition would have the wait for V
+  // wait for them, too.
+  __device__ __forceinline__ void step(const Pages& pg, const Row& r, int h, float c, const Tile<F>& t,
                                        const Tile<F>& next, State<F>& st) {
     uint32_t v[2 * F::NG][4][F::VW];
     f32x4_t s[2 * F::NG], vs[2 * F::NG];
@@ -283,13 +303,15 @@ struct Wave {
         vs[i] = *reinterpret_cast<const f32x4_t*>(pg.v_scale + at);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // V is on its way before K is waited for
     // t = S * c (with the key's scale): base-2 logarithms of the weights
 #pragma unroll
     for (int i = 0; i < 2 * F::NG; ++i) {
       if constexpr (is8(F::CT)) s[i] = scores(i) * s[i];
       else s[i] = scores(i);
     }
-    if (more) load_k(pg, h, next);
+    load_k(pg, h, next);
+    __builtin_amdgcn_sched_barrier(0);
     const float cc = is8(F::CT) ? 1.0f : c;
     if (!t.whole(r)) {
       // keys that are not seen: no weight, and nothing of what stands there
@@ -387,6 +409,11 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 // workgroup with a dozen one-tile pairs was the last to end.
 constexpr int kStart = 8;
 
+// a / b of positive numbers, in 32 bits where they are enough.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 struct Deal {
   int B, R, RT;      // sequences; pairs of one; pairs of one of its heads
   int S, shift, P;   // listed entries or -1; the pages
@@ -412,7 +439,7 @@ struct Deal {
     return n > 0 ? n + kStart : 0;
   }
   __device__ __forceinline__ int64_t chunk(int64_t total) const {
-    const int64_t c = (total + groups - 1) / groups;
+    const int64_t c = quotient(total + groups - 1, groups);
     return c < least ? least : c;
   }
 };
@@ -429,6 +456,11 @@ __device__ __forceinline__ int64_t wave_sum(int64_t x) {
   return x;
 }
 
+// What a pair's first workgroup leaves for the join.
+struct Shared {
+  int first, n;  // workgroups first .. first + n - 1 have parts of the pair
+};
+
 // Parts of pairs that several workgroups share: slot 2w, the pair that
 // workgroup w continues, 2w + 1, the one that it starts and does not end.
 // O (rows, D), then the maxima and the sums.
@@ -439,12 +471,13 @@ __device__ __forceinline__ float* part_slot(float* parts, int64_t slot, int rows
 template <typename F>
 __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     Pages pg, Deal deal, const int32_t* __restrict__ table, int64_t table_stride,
-    const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int G,
+    const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int q_vec, int G,
     const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts, const int32_t* __restrict__ selected,
-    float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws) {
+    float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws, Shared* __restrict__ shared) {
   constexpr int D = F::D;
   __shared__ float so[kWaves][16][D + 4];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
+  __shared__ Entry entries[kEntries + 1];
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found[2];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -455,44 +488,64 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 
   // the workgroup's chunk: [f, f1) of the line, f in a pair of sequence b, whose
   // first pair begins at `at`
-  int64_t f, f1, at;
+  int64_t f, f1, at, chunk = 1;
   int b;
-  if (parts_ws) {
-    int64_t mine = 0;
-    for (int i = tid; i < deal.B; i += 64 * kWaves) mine += deal.places(deal.begin(starts, i), deal.length(lengths, i));
-    mine = wave_sum(mine);
-    if (lane == 0) sums[wave] = mine;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) total += sums[i];
-    total = uniform(total) * deal.R;
-    const int64_t chunk = deal.chunk(total);
+  if (parts_ws && deal.S >= 0) {  // all sequences alike
+    const int np = deal.places(0, 1);
+    const int64_t total = (int64_t)deal.B * deal.R * np;
+    chunk = deal.chunk(total);
     f = blockIdx.x * chunk;
     if (f >= total) return;
     f1 = f + chunk < total ? f + chunk : total;
-    int64_t before = 0;
-    for (int base = 0; base < deal.B; base += 64 * kWaves) {
-      const int i = base + tid;
-      const int64_t nt = i < deal.B ? deal.places(deal.begin(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
-      int64_t incl = nt;
+    b = (int)quotient(f, (int64_t)deal.R * np);
+    at = (int64_t)b * deal.R * np;
+  } else if (parts_ws) {
+    // places of the sequences up to this thread's, of 256 at a time
+    auto places = [&](int i) {
+      return i < deal.B ? deal.places(deal.begin(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
+    };
+    int64_t nt, incl, all;
+    auto scan = [&](int i) {
+      incl = nt = places(i);
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) {
         const int64_t x = __shfl_up(incl, o);
         if (lane >= o) incl += x;
       }
-      __syncthreads();
       if (lane == 63) sums[wave] = incl;
       __syncthreads();
-      int64_t all = 0;
+      all = 0;
 #pragma unroll
       for (int j = 0; j < kWaves; ++j) {
         if (j < wave) incl += sums[j];
         all += sums[j];
       }
-      if (nt > 0 && before + incl - nt <= f && f < before + incl) found[0] = i, found[1] = before + incl - nt;
+    };
+    scan(tid);
+    int64_t total = all;
+    if (deal.B > 64 * kWaves) {
+      int64_t mine = 0;
+      for (int i = tid + 64 * kWaves; i < deal.B; i += 64 * kWaves) mine += places(i);
+      mine = wave_sum(mine);
+      __syncthreads();
+      if (lane == 0) sums[wave] = mine;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) total += sums[i];
+    }
+    total = uniform(total);
+    chunk = deal.chunk(total);
+    f = blockIdx.x * chunk;
+    if (f >= total) return;
+    f1 = f + chunk < total ? f + chunk : total;
+    int64_t before = 0;
+    for (int base = 0;;) {
+      if (nt > 0 && before + incl - nt <= f && f < before + incl) found[0] = base + tid, found[1] = before + incl - nt;
       before += all;
       if (f < before) break;
+      base += 64 * kWaves;
+      __syncthreads();
+      scan(base + tid);
     }
     __syncthreads();
     b = (int)uniform(found[0]);
@@ -512,7 +565,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       ++b;
       continue;
     }
-    const int pair = lone ? blockIdx.x % deal.R : (int)uniform((f - at) / np);
+    const int pair = lone ? blockIdx.x % deal.R : (int)uniform(quotient(f - at, np));
     // the pair's first tile on the line, and its tiles [ta, tb) in the chunk
     const int64_t pair_at = at + (int64_t)pair * np + kStart;
     const int ta = lone || f < pair_at ? 0 : (int)(f - pair_at);
@@ -525,26 +578,39 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     const int h = pair / deal.RT, row0 = h * G + 16 * (pair % deal.RT);
     const int here = (h + 1) * G - row0 < 16 ? (h + 1) * G - row0 : 16;
 
-    w.load_q(q + b * q_b + (row0 + w.n) * q_h, w.n < here);
+    w.load_q(q + b * q_b + (row0 + w.n) * q_h, w.n < here, q_vec);
     State<F> st;
 #pragma unroll
     for (int j = 0; j < F::VD; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     st.m = -INFINITY, st.l = 0.0f;
-    Row r{table + b * table_stride, selected + ((int64_t)b * pg.H + h) * (deal.S > 0 ? deal.S : 0), deal.S, deal.P,
-          pg.n_pages, deal.shift, start, len};
-    const int t0 = deal.first_tile(start);
-    int t = t0 + ta + wave;
-    const int te = t0 + tb;
-    if (t < te) {
-      Tile<F> cur, next;
-      cur.find(r, t);
-      w.load_k(pg, h, cur);
-      next = cur;
-      for (; t < te; t += kWaves) {
-        const bool more = t + kWaves < te;
-        if (more) next.find(r, t + kWaves);
-        w.step(pg, r, h, c, cur, more, next, st);
-        cur = next;
+    const int32_t* ids = table + b * table_stride;
+    const int32_t* list = selected + ((int64_t)b * pg.H + h) * (deal.S > 0 ? deal.S : 0);
+    const int t0 = deal.first_tile(start), te = t0 + tb;
+    const int run = (kEntries << deal.shift) / F::TILE;  // tiles whose pages fit
+    for (int r0 = t0 + ta; r0 < te; r0 += run) {
+      const int re = te - r0 < run ? te : r0 + run;
+      const Row r{entries, r0 * F::TILE >> deal.shift, deal.shift, start, len};
+      const int n = ((re * F::TILE - 1) >> deal.shift) - r.first + 1;
+      if (r0 > t0 + ta) __syncthreads();  // the last run's are read
+      for (int i = tid; i < n; i += 64 * kWaves) {
+        int ordinal = r.first + i;
+        if (deal.S >= 0) ordinal = ordinal < deal.S ? list[ordinal] : -1;
+        const int id = (uint32_t)ordinal < (uint32_t)deal.P ? ids[ordinal] : -1;
+        const bool ok = (uint32_t)id < (uint32_t)pg.n_pages;
+        entries[i] = Entry{ok ? id : 0, ok ? ordinal << deal.shift : kNowhere};
+      }
+      __syncthreads();
+      int t = r0 + wave;
+      if (t < re) {
+        Tile<F> cur, next;
+        cur.find(r, t);
+        w.load_k(pg, h, cur);
+        next = cur;
+        for (; t < re; t += kWaves) {
+          if (t + kWaves < re) next.find(r, t + kWaves);
+          w.step(pg, r, h, c, cur, next, st);
+          cur = next;
+        }
       }
     }
 
@@ -561,6 +627,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     }
     __syncthreads();
     const bool ends = tb == nt, whole = ta == 0 && ends;
+    if (!lone && ta == 0 && tid == 0)
+      shared[(int64_t)b * deal.R + pair] =
+          Shared{(int)blockIdx.x, ends ? 1 : (int)quotient(pair_at + nt - 1, chunk) - (int)blockIdx.x + 1};
     float* slot = whole ? nullptr : part_slot(parts_ws, 2 * (int64_t)blockIdx.x + (ta == 0), rows, D);
     for (int i = tid; i < here * D; i += 64 * kWaves) {
       const int row = i / D, d = i % D;
@@ -589,77 +658,67 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 }
 
 // Joins the parts of a row, a workgroup a row; writes the rows of sequences that
-// see nothing.  A wave takes every WAVESth part, a lane D / 64 channels of it (one
-// of 64 / D parts for narrow heads).
+// see nothing.  A team of min(D, 64) lanes takes every TEAMS-th part, eight parts'
+// loads at once, and the teams are joined in LDS.
 template <int QT, int THREADS>
 __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float pscale,
                                                        const int32_t* __restrict__ lengths,
-                                                       const int32_t* __restrict__ starts, float* __restrict__ parts,
+                                                       const int32_t* __restrict__ starts,
+                                                       const float* __restrict__ parts,
+                                                       const Shared* __restrict__ shared,
                                                        typename Elem<QT>::T* __restrict__ out) {
-  constexpr int WAVES = THREADS / kWave;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x;
   const int b = blockIdx.x / deal.R, pair = blockIdx.x % deal.R;
   const int h = pair / deal.RT, row = blockIdx.y, head = h * G + 16 * (pair % deal.RT) + row;
   if (head >= (h + 1) * G) return;
-  __shared__ int64_t sums[2][WAVES];
-  __shared__ float red[WAVES];
-  __shared__ float acc[WAVES][128];
-  __shared__ float accl[WAVES];
-  int64_t total = 0, before = 0;
-  for (int i = tid; i < deal.B; i += THREADS) {
-    const int n = deal.places(deal.begin(starts, i), deal.length(lengths, i));
-    total += n;
-    before += i < b ? n : 0;
-  }
-  const int nt = deal.tiles(deal.begin(starts, b), deal.length(lengths, b));
-  total = wave_sum(total), before = wave_sum(before);
-  if (lane == 0) sums[0][wave] = total, sums[1][wave] = before;
-  __syncthreads();
-  total = before = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) total += sums[0][w], before += sums[1][w];
+  const Shared who = shared[blockIdx.x];  // nobody's where the sequence has no tiles
   typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head) * D;
-  if (nt == 0) {
+  if (deal.tiles(deal.begin(starts, b), deal.length(lengths, b)) == 0) {
     for (int d = tid; d < D; d += THREADS) store_f<QT>(to + d, 0.0f);
     return;
   }
-  const int64_t chunk = deal.chunk(total * deal.R);
-  const int64_t first = before * deal.R + (int64_t)pair * (nt + kStart) + kStart;  // the pair's first tile
-  const int64_t w0 = first / chunk, w1 = (first + nt - 1) / chunk;
-  if (w0 == w1) return;  // written by its one workgroup
+  if (who.n == 1) return;  // written by its one workgroup
   const int rows = G < 16 ? G : 16;
-  const int n = (int)(w1 - w0) + 1;
-  // part i of the row is workgroup w0 + i's
-  auto slot = [&](int i) { return part_slot(parts, 2 * (w0 + i) + (i == 0), rows, D); };
-  float top = -INFINITY;
-  for (int i = tid; i < n; i += THREADS) top = fmaxf(top, slot(i)[rows * D + row]);
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, red[w]);
-  const int d = lane % D, per = D < kWave ? kWave / D : 1, mine = D < kWave ? lane / D : 0;
+  const int lanes = D < kWave ? D : kWave, d = tid % lanes, team = tid / lanes, teams = THREADS / lanes;
   const bool two = D > kWave;
-  float o0 = 0.0f, o1 = 0.0f, sum = 0.0f;
-#pragma unroll 8
-  for (int i = wave * per + mine; i < n; i += WAVES * per) {
-    const float* s = slot(i);
-    const float l = s[rows * (D + 1) + row], a = part_weight(s[rows * D + row], l, top);
-    const float x = s[row * D + d], y = two ? s[row * D + 64 + d] : 0.0f;
-    o0 += a == 0.0f ? 0.0f : a * x, o1 += a == 0.0f ? 0.0f : a * y, sum += a == 0.0f ? 0.0f : a * l;
-  }
-  for (int o = D; o < kWave; o <<= 1) o0 += __shfl_xor(o0, o), sum += __shfl_xor(sum, o);
-  if (lane < D) {
-    acc[wave][d] = o0;
-    if (two) acc[wave][64 + d] = o1;
-  }
-  if (lane == 0) accl[wave] = sum;
-  __syncthreads();
-  for (int c = tid; c < D; c += THREADS) {
-    float o = 0.0f, l = 0.0f;
+  float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int i0 = team; i0 < who.n; i0 += 8 * teams) {
+    float m[8], l[8], x[8], y[8];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) o += acc[w][c], l += accl[w];
+    for (int u = 0; u < 8; ++u) {
+      const int i = i0 + u * teams;
+      const bool in = i < who.n;
+      // part i is workgroup first + i's
+      const float* s = parts + (2 * (int64_t)(who.first + (in ? i : 0)) + (!in || i == 0)) * rows * (D + 2);
+      m[u] = in ? s[rows * D + row] : -INFINITY, l[u] = in ? s[rows * (D + 1) + row] : 0.0f;
+      x[u] = s[row * D + d], y[u] = two ? s[row * D + 64 + d] : 0.0f;
+    }
+    float t = top;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t = fmaxf(t, m[u]);
+    const float a = part_weight(top, sum, t);
+    o0 = a == 0.0f ? 0.0f : a * o0, o1 = a == 0.0f ? 0.0f : a * o1, sum = a == 0.0f ? 0.0f : a * sum;
+    top = t;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float w = part_weight(m[u], l[u], t);
+      if (w != 0.0f) o0 += w * x[u], o1 += w * y[u], sum += w * l[u];
+    }
+  }
+  constexpr int TEAMS = THREADS / 16;  // at most
+  __shared__ float acc[THREADS * 2], tops[TEAMS], suml[TEAMS];
+  acc[team * D + d] = o0;
+  if (two) acc[team * D + 64 + d] = o1;
+  if (d == 0) tops[team] = top, suml[team] = sum;
+  __syncthreads();
+  const int used = who.n < teams ? who.n : teams;
+  for (int c = tid; c < D; c += THREADS) {
+    float t = -INFINITY, o = 0.0f, l = 0.0f;
+    for (int w = 0; w < used; ++w) t = fmaxf(t, tops[w]);
+    for (int w = 0; w < used; ++w) {
+      const float a = part_weight(tops[w], suml[w], t);
+      if (a != 0.0f) o += a * acc[w * D + c], l += a * suml[w];
+    }
     store_f<QT>(to + c, l == 0.0f ? 0.0f : o / (l * pscale));
   }
 }
@@ -682,12 +741,12 @@ struct AttendCall {
 // Workgroups of a call that shares its rows out: as many as the chip holds at
 // once, at most kGroups.
 constexpr int kGroups = 1024;
-constexpr int kLeast = 16;  // places of a chunk
+constexpr int kLeast = 8;   // places of a chunk
 constexpr int kLone = 16;   // tiles that one workgroup takes rather than two launches
 
 struct Plan {
   Deal deal;
-  size_t bytes;  // of the parts; 0: a workgroup a pair
+  size_t parts, bytes;  // of the parts, and of the workspace; 0: a workgroup a pair
 };
 
 inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int S, int tile) {
@@ -698,7 +757,8 @@ inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int
   if (most > kLone) {
     const int64_t chunks = ((most + kStart) * B * p.deal.R + kLeast - 1) / kLeast;
     p.deal.groups = (int)(chunks < kGroups ? chunks : kGroups);
-    p.bytes = (size_t)p.deal.groups * 2 * (G < 16 ? G : 16) * (D + 2) * 4;
+    p.parts = (size_t)p.deal.groups * 2 * (G < 16 ? G : 16) * (D + 2) * 4;
+    p.bytes = p.parts + (size_t)B * p.deal.R * sizeof(Shared);
   }
   return p;
 }
@@ -725,16 +785,20 @@ void attend_launch(const AttendCall& a) {
   if (deal.groups > at_once) deal.groups = at_once;
   const int G = a.H / a.pg.H;
   const unsigned pairs = (unsigned)(a.B * deal.R);
+  Shared* shared = reinterpret_cast<Shared*>(reinterpret_cast<char*>(a.parts) + p.parts);
+  const bool q_vec = ((uintptr_t)a.q.ptr | (uintptr_t)(a.q.s_b * sizeof(T)) | (uintptr_t)(a.q.s_h * sizeof(T))) % 16 == 0;
   attend_kernel<F><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
-      a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, G, a.lengths, a.starts, a.selected, a.c,
-      (T*)a.out, p.bytes ? a.parts : nullptr);
+      a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts, a.selected, a.c,
+      (T*)a.out, p.bytes ? a.parts : nullptr, shared);
   if (!p.bytes) return;
   const dim3 rows(pairs, G < 16 ? G : 16);
   // a row of a few pairs has parts by the hundred
   if (pairs >= 64)
-    join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, (T*)a.out);
+    join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, shared,
+                                                     (T*)a.out);
   else
-    join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, (T*)a.out);
+    join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, shared,
+                                                       (T*)a.out);
 }
 
 template <int QT, int CT>

@@ -24,29 +24,46 @@ __device__ __forceinline__ Span span_at(const int32_t* lengths, const int32_t* s
   return Span{start >> shift, (len + (1 << shift) - 1) >> shift};
 }
 
-constexpr int kScoreHeads = 32;  // query heads in LDS at once
+constexpr int kScoreHeads = 8;  // query heads in LDS at once
 constexpr int kSteps = 4;        // pages of a lane at once
+
+// The value of lane ^ MASK, 64 bits: a quad permute, or a swizzle.
+template <int MASK>
+__device__ __forceinline__ double across(double x) {
+  const int lo = __double2loint(x), hi = __double2hiint(x);
+  if constexpr (MASK < 4) {
+    constexpr int PERM = MASK == 1 ? 0xB1 : 0x4E;  // [1, 0, 3, 2], [2, 3, 0, 1]
+    return __hiloint2double(__builtin_amdgcn_mov_dpp(hi, PERM, 0xf, 0xf, true),
+                            __builtin_amdgcn_mov_dpp(lo, PERM, 0xf, 0xf, true));
+  } else {
+    constexpr int XOR = MASK << 10 | 0x1f;
+    return __hiloint2double(__builtin_amdgcn_ds_swizzle(hi, XOR), __builtin_amdgcn_ds_swizzle(lo, XOR));
+  }
+}
 
 // Scores.  D / 8 lanes hold a page's two bounds of a head, eight channels each,
 // of kSteps pages at once, and go over the query heads; sums are 64 bits, so
 // that the order of the summands decides nothing that is not equal to 2^-53:
 // with bf16 or f16 values the sums are as good as always exact.  The bounds are
-// read once and are the bound: 4 D bytes a page and head for 16-bit cells against
-// 3 D G instructions over 64 lanes (select, widen, fused multiply-add; the last
-// runs at f32's rate on this chip).
+// read once for all heads of a group; a channel is a select, a widening and a
+// fused multiply-add.  Heads of one page are neighbours in the grid, as their
+// bounds are in memory.  196,608 pages and heads of 128 bf16 channels (100 MB),
+// four query heads each: 31 us; one query head instead of four: 26 us.  Widening
+// the bounds once and two products of max(q, 0) and min(q, 0) a channel: 35 us (160
+// registers, three waves a SIMD); workgroups of one or two waves: 34 us.
 template <int QT, int BT, int D>
 __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __restrict__ table, int64_t table_stride,
                                                     int P, const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
                                                     int64_t q_h, int G, const int32_t* __restrict__ lengths,
                                                     const int32_t* __restrict__ starts, int first, int last,
-                                                    uint32_t* __restrict__ keys) {
+                                                    int64_t row_keys, uint32_t* __restrict__ keys) {
   constexpr int LP = D / 8;            // lanes of a page
   constexpr int PW = kWave / LP;       // pages of a wave at once
   constexpr int AT_ONCE = 4 * PW * kSteps;  // pages of a workgroup
   using BoundT = typename Elem<BT>::T;
-  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int b = blockIdx.z, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
-  const int base = blockIdx.x * AT_ONCE;
+  const int base = blockIdx.y * AT_ONCE;
   if (base >= sp.pe || base + AT_ONCE <= sp.p0) return;
   __shared__ float qs[kScoreHeads][D];
   const int part = lane % LP;
@@ -73,11 +90,13 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
   for (int g0 = 0; g0 < G; g0 += kScoreHeads) {
     const int heads = G - g0 < kScoreHeads ? G - g0 : kScoreHeads;
     __syncthreads();
-    for (int i = tid; i < heads * D; i += 256)
-      qs[i / D][i % D] = load_f<QT>(q + b * q_b + (int64_t)(h * G + g0 + i / D) * q_h + i % D);
+    for (int i = tid; i < heads * D; i += 256) {
+      const float x = load_f<QT>(q + b * q_b + (int64_t)(h * G + g0 + i / D) * q_h + i % D);
+      qs[i / D][i % D] = x;
+    }
     __syncthreads();
     for (int g = 0; g < heads; ++g) {
-      double sum[kSteps] = {0.0, 0.0, 0.0, 0.0};
+      double sum[kSteps] = {};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = qs[g][8 * part + i];
@@ -91,16 +110,16 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const double mine = odd ? sum[2 + s] : sum[s], other = odd ? sum[s] : sum[2 + s];
-        r[s] = mine + __shfl_xor(other, 1);
+        r[s] = mine + across<1>(other);
       }
       double t[KEEP];
       if constexpr (LP == 2) {
         t[0] = r[0], t[1] = r[1];
       } else {
         const double mine = upper ? r[1] : r[0], other = upper ? r[0] : r[1];
-        t[0] = mine + __shfl_xor(other, 2);
-#pragma unroll
-        for (int o = 4; o < LP; o <<= 1) t[0] += __shfl_xor(t[0], o);
+        t[0] = mine + across<2>(other);
+        if constexpr (LP > 4) t[0] += across<4>(t[0]);
+        if constexpr (LP > 8) t[0] += across<8>(t[0]);
       }
 #pragma unroll
       for (int s = 0; s < KEEP; ++s) {
@@ -111,7 +130,7 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
     }
   }
   if (part >= 4) return;
-  uint32_t* row = keys + ((int64_t)b * pg.H + h) * P;
+  uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
     const int s = LP == 2 ? 2 * odd + k : 2 * odd + upper;
@@ -131,13 +150,13 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
 // The best `count` of a row of keys, ascending.  The keys' range is cut into
 // 2,048 bins and the bin that holds the last one to take is cut again, until all
 // of a bin or, among equal keys, the lowest entries are taken: mostly two
-// rounds.  A workgroup a row; a thread holds four entries in a row of every
-// 4 * THREADS, in registers where R rounds of them hold the row (R = 0: read
-// again from the L2 each time).
+// rounds.  A workgroup a row, a thread K entries in a row, in registers where
+// THREADS * K hold all of them (HELD), else read again from the L2 each time.
 constexpr int kBins = 2048;
 
+// Exclusive sum over the workgroup; `all`: the whole.
 template <int THREADS>
-__device__ __forceinline__ int block_scan(int x, int* sums, int& all) {  // exclusive
+__device__ __forceinline__ int block_scan(int x, int* sums, int& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int incl = x;
 #pragma unroll
@@ -145,7 +164,6 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int& all) {  // excl
     const int y = __shfl_up(incl, o);
     if (lane >= o) incl += y;
   }
-  __syncthreads();
   if (lane == 63) sums[wave] = incl;
   __syncthreads();
   int before = 0;
@@ -158,70 +176,73 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int& all) {  // excl
   return before + incl - x;
 }
 
-template <int THREADS, int R>
-__global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int shift, int count,
+template <int THREADS, int K, bool HELD>
+__global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t row_keys, int shift, int count,
                                                          const int32_t* __restrict__ lengths,
                                                          const int32_t* __restrict__ starts,
                                                          const uint32_t* __restrict__ keys,
                                                          int32_t* __restrict__ chosen) {
   constexpr int WAVES = THREADS / kWave;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t* key = keys + (int64_t)blockIdx.x * P;
+  const uint32_t* key = keys + (int64_t)blockIdx.x * row_keys;
   int32_t* out = chosen + (int64_t)blockIdx.x * count;
   const Span sp = span_at(lengths, starts, P, shift, blockIdx.x / H);
-  const int rounds = (sp.pe - sp.p0 + 4 * THREADS - 1) / (4 * THREADS);
+  const int from0 = sp.p0 & ~3;  // rows of keys are 16-byte aligned
+  const int rounds = HELD ? 1 : (sp.pe - from0 + THREADS * K - 1) / (THREADS * K);
   __shared__ int hist[kBins];
-  __shared__ int sums[WAVES], sums2[WAVES];
+  __shared__ int sums[3][WAVES];
   __shared__ uint32_t range[2][WAVES];
   __shared__ int cut[3];
 
-  uint32_t held[R > 0 ? R : 1][4];
-  auto fetch = [&](int r, uint32_t (&x)[4]) {
-    const int p = sp.p0 + (r * THREADS + tid) * 4;
+  uint32_t held[K];
+  auto fetch = [&](int r, uint32_t (&x)[K]) {
+    const int p = from0 + (r * THREADS + tid) * K;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = p + i < sp.pe ? key[p + i] : kNone;
+    for (int i = 0; i < K; i += 4) {
+      uint4 a = make_uint4(0, 0, 0, 0);
+      if (p + i < sp.pe) a = *reinterpret_cast<const uint4*>(key + p + i);
+      x[i] = a.x, x[i + 1] = a.y, x[i + 2] = a.z, x[i + 3] = a.w;
+    }
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (p + i < sp.p0 || p + i >= sp.pe) x[i] = kNone;
   };
-  if constexpr (R > 0) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) fetch(r, held[r]);
-  }
+  if constexpr (HELD) fetch(0, held);
   auto each = [&](auto&& f) {
-    if constexpr (R > 0) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) f(r, held[r]);
-    } else {
+    if constexpr (HELD) f(0, held);
+    else {
       for (int r = 0; r < rounds; ++r) {
-        uint32_t x[4];
-        fetch(r, x);
-        f(r, x);
+        fetch(r, held);
+        f(r, held);
       }
     }
   };
 
   uint32_t lo = 0xffffffffu, hi = 0;
   int forced = 0, others = 0;
-  each([&](int, const uint32_t (&x)[4]) {
+  each([&](int, const uint32_t (&x)[K]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < K; ++i) {
       const bool normal = x[i] != kNone && x[i] != kForced;
       forced += x[i] == kForced;
       others += normal;
       if (normal) lo = x[i] < lo ? x[i] : lo, hi = x[i] > hi ? x[i] : hi;
     }
   });
+  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) {
     const uint32_t a = __shfl_xor(lo, o), z = __shfl_xor(hi, o);
     lo = a < lo ? a : lo, hi = z > hi ? z : hi;
     forced += __shfl_xor(forced, o), others += __shfl_xor(others, o);
   }
-  if (lane == 0) range[0][wave] = lo, range[1][wave] = hi, sums[wave] = forced, sums2[wave] = others;
+  if (lane == 0) range[0][wave] = lo, range[1][wave] = hi, sums[0][wave] = forced, sums[1][wave] = others;
   __syncthreads();
   forced = others = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
     lo = range[0][w] < lo ? range[0][w] : lo, hi = range[1][w] > hi ? range[1][w] : hi;
-    forced += sums[w], others += sums2[w];
+    forced += sums[0][w], others += sums[1][w];
   }
   // taken: forced, keys above `over`, and `ties` keys that equal it
   int need = count - forced;
@@ -233,73 +254,67 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int shift
     over = kForced - 1;
   } else {
     while (true) {
-      const int bits = hi == lo ? 0 : 32 - __clz(hi - lo);
-      const int cutshift = bits > 11 ? bits - 11 : 0;
       if (hi == lo) {
         over = lo, ties = need;
         break;
       }
-      for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
-      __syncthreads();
-      each([&](int, const uint32_t (&x)[4]) {
+      const int bits = 32 - __clz(hi - lo), cutshift = bits > 11 ? bits - 11 : 0;
+      each([&](int, const uint32_t (&x)[K]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (x[i] >= lo && x[i] <= hi && x[i] != kForced) atomicAdd(&hist[(x[i] - lo) >> cutshift], 1);
+        for (int i = 0; i < K; ++i)
+          if (x[i] >= lo && x[i] <= hi) atomicAdd(&hist[(x[i] - lo) >> cutshift], 1);
       });
       __syncthreads();
       // bins from the top: thread t's are kBins - 1 - PER * t ...
       constexpr int PER = kBins / THREADS;
-      int mine = 0;
+      int bin_n[PER], mine = 0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) mine += hist[kBins - 1 - PER * tid - i];
+      for (int i = 0; i < PER; ++i) {
+        int& bin = hist[kBins - 1 - PER * tid - i];
+        mine += bin_n[i] = bin;
+        bin = 0;
+      }
       int all;
-      int above = block_scan<THREADS>(mine, sums, all);
+      int above = block_scan<THREADS>(mine, sums[2], all);
       if (above < need && above + mine >= need) {
+#pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int bin = kBins - 1 - PER * tid - i, n = hist[bin];
-          if (above + n >= need) {
-            cut[0] = bin, cut[1] = need - above, cut[2] = n;
-            break;
-          }
-          above += n;
+          if (above < need && above + bin_n[i] >= need)
+            cut[0] = kBins - 1 - PER * tid - i, cut[1] = need - above, cut[2] = bin_n[i];
+          above += bin_n[i];
         }
       }
       __syncthreads();
-      const int bin = cut[0];
       need = cut[1];
-      const uint32_t from = lo + ((uint32_t)bin << cutshift), to = from + ((1u << cutshift) - 1u);
+      const uint32_t from = lo + ((uint32_t)cut[0] << cutshift), to = from + ((1u << cutshift) - 1u);
       if (cut[2] == need) {  // all of the bin
         over = from - 1;
         break;
       }
       lo = from, hi = to < hi ? to : hi;
-      __syncthreads();
     }
   }
-  // ascending: ties count by entry, too
+  // ascending, ties by entry; counts of the taken above and of the ties, 16 bits
+  // each: THREADS * K < 2^16
   int base = 0, tied = 0;
-  each([&](int r, const uint32_t (&x)[4]) {
-    if (R > 0 && r >= rounds) return;
-    int eq = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) eq += ties > 0 && x[i] == over;
-    int all_eq = 0, before_eq = 0;
-    if (ties > 0) before_eq = tied + block_scan<THREADS>(eq, sums, all_eq);
-    bool take[4];
+  each([&](int r, const uint32_t (&x)[K]) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool tie = ties > 0 && x[i] == over;
-      take[i] = x[i] > over || (tie && before_eq < ties);
-      before_eq += tie;
-      n += take[i];
-    }
+    for (int i = 0; i < K; ++i) n += x[i] > over ? 1 << 16 : ties > 0 && x[i] == over ? 1 : 0;
     int all;
-    int at = base + block_scan<THREADS>(n, sums2, all);
+    if (!HELD) __syncthreads();  // the last round's sums are read
+    const int before = block_scan<THREADS>(n, sums[0], all);
+    int eq = tied + (before & 0xffff), at = base + (before >> 16) + (eq < ties ? eq - tied : ties > tied ? ties - tied : 0);
+    const int p = from0 + (r * THREADS + tid) * K;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (take[i]) out[at++] = sp.p0 + (r * THREADS + tid) * 4 + i;
-    base += all, tied += all_eq;
+    for (int i = 0; i < K; ++i) {
+      const bool tie = ties > 0 && x[i] == over;
+      if (x[i] > over || (tie && eq < ties)) out[at++] = p + i;
+      eq += tie;
+    }
+    const int eqs = all & 0xffff, left = ties > tied ? ties - tied : 0;
+    base += (all >> 16) + (eqs < left ? eqs : left);
+    tied += eqs;
   });
   for (int i = base + tid; i < count; i += THREADS) out[i] = -1;
 }

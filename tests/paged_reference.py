@@ -151,8 +151,8 @@ def select(q, pool, table, lengths, starts, count, first, last):
                     continue
                 x = q[b, h * G:h * G + G].double()
                 s = (x * torch.where(x > 0, bounds[page, h, 1], bounds[page, h, 0])).sum(-1).float()
-                s = -math.inf if torch.isnan(s).any() else float(s.max())
-                nan = bool(torch.isnan((x * torch.where(x > 0, bounds[page, h, 1], bounds[page, h, 0])).sum(-1)).any())
+                nan = bool(torch.isnan(s).any())
+                s = -math.inf if nan else float(s.max())
                 forced = p < p0 + first or p >= pe - last
                 found.append((not forced, nan, -s, p))
             take = sorted(p for *_, p in sorted(found)[:count])
