@@ -672,7 +672,7 @@ typedef struct pfa_kv_pages {
  * a page's head, where the pool has them: those of the written keys as they
  * are stored (a NaN among them gives NaN), joined with what stood there
  * unless the page is written from its first slot on. */
-int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4 v, int dtype,
+int pfa_kv_pages_write(const pfa_kv_pages* pages, pfa_tensor4 k, pfa_tensor4 v, int dtype,
                        int B, int64_t n, const int32_t* table, int64_t table_stride,
                        int table_pages, const int32_t* starts, const int32_t* counts,
                        void* stream);
@@ -681,7 +681,7 @@ int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4 v, int dty
  * of every sequence as values, k_out and v_out (B, n, kv_heads, head_dim) in
  * out_dtype: cell * scale rounded once.  Rows i >= counts[b], and those
  * without a page, are zero. */
-int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int32_t* table,
+int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t* table,
                       int64_t table_stride, int table_pages, const int32_t* starts,
                       const int32_t* counts, void* k_out, void* v_out, int out_dtype,
                       void* stream);
@@ -696,9 +696,10 @@ int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int32_t* table
  * (PFA_F32 / PFA_BF16 / PFA_F16: the cells' own, or any of the three for
  * 8-bit cells).  A row that sees no key is zero, and so is one all of whose
  * scores are -inf.  Sums and softmax statistics are f32. */
-int pfa_paged_attn_workspace_size(int B, int H, pfa_kv_pages pages, int table_pages,
-                                  int n_selected, size_t* bytes);
-int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages,
+int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
+                                  int cell_dtype, int table_pages, int n_selected,
+                                  size_t* bytes);
+int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages,
                        const int32_t* table, int64_t table_stride, int table_pages,
                        const int32_t* lengths, const int32_t* starts,
                        const int32_t* selected, int n_selected, float scale, void* out,
@@ -713,7 +714,7 @@ int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages page
  * lengths[b] - 1 come before all others, then the better score, then the
  * lower entry; entries without a page are never chosen. */
 int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes);
-int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages,
+int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages,
                         const int32_t* table, int64_t table_stride, int table_pages,
                         const int32_t* lengths, const int32_t* starts, int count, int first,
                         int last, int32_t* chosen, void* workspace, size_t ws_bytes,

@@ -8,16 +8,31 @@ namespace pfa {
 
 using namespace paged;
 
+static int shift_of(int page_size) {
+  int shift = 4;
+  while ((1 << shift) < page_size) ++shift;
+  return shift;
+}
+
+static int sizes_check(int kv_heads, int page_size, int head_dim, int dtype, int table_pages, int B) {
+  PFA_CHECK_ARG(dtype == PFA_F32 || dtype == PFA_BF16 || dtype == PFA_F16 || is8(dtype), "pages: unknown cell type %d",
+                dtype);
+  PFA_CHECK_ARG(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128,
+                "pages: head_dim must be 16, 32, 64 or 128 (got %d)", head_dim);
+  PFA_CHECK_ARG(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
+                "pages: page_size must be 16, 32, 64, 128 or 256 (got %d)", page_size);
+  PFA_CHECK_ARG(kv_heads > 0 && kv_heads <= 65535, "pages: 1 to 65535 heads (got %d)", kv_heads);
+  PFA_CHECK_ARG(B >= 0 && B <= 65535, "pages: 0 <= B <= 65535 sequences (got %d)", B);
+  PFA_CHECK_ARG(table_pages >= 0 && (int64_t)table_pages * page_size <= (1ll << 30),
+                "pages: a block table of up to 2^30 positions (got %d pages)", table_pages);
+  return PFA_OK;
+}
+
 int paged_check(const pfa_kv_pages* pg, const int32_t* table, int64_t table_stride, int table_pages, int B, Pages* p,
                 Table* t) {
-  PFA_CHECK_ARG(pg->dtype == PFA_F32 || pg->dtype == PFA_BF16 || pg->dtype == PFA_F16 || is8(pg->dtype),
-                "pages: unknown cell type %d", pg->dtype);
-  PFA_CHECK_ARG(pg->head_dim == 16 || pg->head_dim == 32 || pg->head_dim == 64 || pg->head_dim == 128,
-                "pages: head_dim must be 16, 32, 64 or 128 (got %d)", pg->head_dim);
-  PFA_CHECK_ARG(pg->page_size >= 16 && pg->page_size <= 256 && (pg->page_size & (pg->page_size - 1)) == 0,
-                "pages: page_size must be 16, 32, 64, 128 or 256 (got %d)", pg->page_size);
-  PFA_CHECK_ARG(pg->n_pages > 0 && pg->kv_heads > 0 && pg->kv_heads <= 65535 && pg->k && pg->v,
-                "pages: an empty pool");
+  PFA_CHECK_ARG(pg, "pages: null argument");
+  if (int rc = sizes_check(pg->kv_heads, pg->page_size, pg->head_dim, pg->dtype, table_pages, B)) return rc;
+  PFA_CHECK_ARG(pg->n_pages > 0 && pg->k && pg->v, "pages: an empty pool");
   PFA_CHECK_ARG(!is8(pg->dtype) || (pg->k_scale && pg->v_scale), "pages: 8-bit cells need k_scale and v_scale");
   const int64_t cells = (int64_t)pg->kv_heads * pg->page_size * pg->head_dim;
   const int e = cell_bytes(pg->dtype);
@@ -26,14 +41,9 @@ int paged_check(const pfa_kv_pages* pg, const int32_t* table, int64_t table_stri
                     pg->v_page * e % 16 == 0 && (uintptr_t)pg->k_scale % 16 == 0 && (uintptr_t)pg->v_scale % 16 == 0 &&
                     (uintptr_t)pg->k_bounds % 16 == 0,
                 "pages: rows must be 16-byte aligned");
-  PFA_CHECK_ARG(B >= 0 && B <= 65535, "pages: 0 <= B <= 65535 sequences (got %d)", B);
-  PFA_CHECK_ARG(table_pages >= 0 && (int64_t)table_pages * pg->page_size <= (1ll << 30) &&
-                    (table || table_pages == 0 || B == 0),
-                "pages: a block table of up to 2^30 positions (got %d pages)", table_pages);
-  int shift = 4;
-  while ((1 << shift) < pg->page_size) ++shift;
+  PFA_CHECK_ARG(table || table_pages == 0 || B == 0, "pages: null argument");
   *p = Pages{pg->k, pg->v, pg->k_scale, pg->v_scale, pg->k_bounds, pg->k_page, pg->v_page,
-             pg->n_pages, pg->kv_heads, pg->page_size, shift};
+             pg->n_pages, pg->kv_heads, pg->page_size, shift_of(pg->page_size)};
   *t = Table{table, table_stride, table_pages};
   return PFA_OK;
 }
@@ -235,18 +245,18 @@ int types_check(int dt, int ct) {
 
 using namespace pfa;
 
-extern "C" int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4 v, int dtype, int B, int64_t n,
+extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, pfa_tensor4 k, pfa_tensor4 v, int dtype, int B, int64_t n,
                                   const int32_t* table, int64_t table_stride, int table_pages, const int32_t* starts,
                                   const int32_t* counts, void* stream) {
   clear_error();
   Pages p;
   Table t;
-  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
-  if (int rc = types_check(dtype, pages.dtype)) return rc;
+  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = types_check(dtype, pages->dtype)) return rc;
   PFA_CHECK_ARG(n >= 0 && n <= (1 << 26), "kv_pages_write: 0 <= n <= 2^26 tokens");
   if (B == 0 || n == 0 || table_pages == 0) return PFA_OK;
   PFA_CHECK_ARG(k.ptr && v.ptr && starts, "kv_pages_write: null argument");
-  const int D = pages.head_dim;
+  const int D = pages->head_dim;
   const int e = cell_bytes(dtype);
   auto rows = [&](const pfa_tensor4& x) {
     const bool vec = (uintptr_t)x.ptr % 16 == 0 && x.s_b * e % 16 == 0 && x.s_h * e % 16 == 0 && x.s_t * e % 16 == 0;
@@ -255,7 +265,7 @@ extern "C" int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4
   const int64_t touched = (n + p.ps - 2) / p.ps + 1;
   const int64_t at_once = (n < p.ps ? n : p.ps) * (D / 8);
   const int threads = at_once <= 64 ? 64 : at_once <= 128 ? 128 : 256;
-  by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
+  by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
     write_kernel<decltype(dt)::value, decltype(ct)::value>
         <<<dim3((unsigned)touched, p.H, B), threads, 0, as_stream(stream)>>>(p, t, rows(k), rows(v), D, n, starts,
                                                                              counts);
@@ -264,20 +274,20 @@ extern "C" int pfa_kv_pages_write(pfa_kv_pages pages, pfa_tensor4 k, pfa_tensor4
   return PFA_OK;
 }
 
-extern "C" int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int32_t* table, int64_t table_stride,
+extern "C" int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t* table, int64_t table_stride,
                                  int table_pages, const int32_t* starts, const int32_t* counts, void* k_out,
                                  void* v_out, int out_dtype, void* stream) {
   clear_error();
   Pages p;
   Table t;
-  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
   PFA_CHECK_ARG(out_dtype == PFA_F32 || out_dtype == PFA_BF16 || out_dtype == PFA_F16,
                 "kv_pages_read: unknown value type %d", out_dtype);
   PFA_CHECK_ARG(n >= 0 && n <= (1 << 30), "kv_pages_read: 0 <= n <= 2^30 tokens");
   if (B == 0 || n == 0) return PFA_OK;
   PFA_CHECK_ARG(k_out && v_out && starts && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                 "kv_pages_read: null or unaligned argument");
-  const int D = pages.head_dim;
+  const int D = pages->head_dim;
   const int64_t total = (int64_t)B * n * p.H * (D / 8);
   const int64_t blocks = (total + 255) / 256;
   const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
@@ -290,7 +300,7 @@ extern "C" int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int
     else if (out_dtype == PFA_BF16) launch(ct, std::integral_constant<int, PFA_BF16>{});
     else launch(ct, std::integral_constant<int, PFA_F16>{});
   };
-  switch (pages.dtype) {
+  switch (pages->dtype) {
     case PFA_F32: by_out(std::integral_constant<int, PFA_F32>{}); break;
     case PFA_BF16: by_out(std::integral_constant<int, PFA_BF16>{}); break;
     case PFA_F16: by_out(std::integral_constant<int, PFA_F16>{}); break;
@@ -303,11 +313,11 @@ extern "C" int pfa_kv_pages_read(pfa_kv_pages pages, int B, int64_t n, const int
 
 namespace {
 
-int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H, const pfa_kv_pages& pages,
+int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H, const pfa_kv_pages* pages,
                 const int32_t* lengths) {
-  if (int rc = types_check(dtype, pages.dtype)) return rc;
-  PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages.kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
-                pages.kv_heads);
+  if (int rc = types_check(dtype, pages->dtype)) return rc;
+  PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages->kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
+                pages->kv_heads);
   PFA_CHECK_ARG((int64_t)B * H <= 1 << 21, "%s: up to 2^21 rows (got %d x %d)", what, B, H);
   PFA_CHECK_ARG(B == 0 || (q.ptr && lengths), "%s: null argument", what);
   return PFA_OK;
@@ -325,16 +335,16 @@ extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table
   return PFA_OK;
 }
 
-extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages, const int32_t* table,
+extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
                                    int64_t table_stride, int table_pages, const int32_t* lengths,
                                    const int32_t* starts, int count, int first, int last, int32_t* chosen,
                                    void* workspace, size_t ws_bytes, void* stream) {
   clear_error();
   Pages p;
   Table t;
-  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
   if (int rc = query_check("kv_pages_select", q, dtype, B, H, pages, lengths)) return rc;
-  PFA_CHECK_ARG(pages.k_bounds, "kv_pages_select: the pool has no key bounds");
+  PFA_CHECK_ARG(pages->k_bounds, "kv_pages_select: the pool has no key bounds");
   PFA_CHECK_ARG(count > 0 && first >= 0 && last >= 0 && first <= count && last <= count - first,
                 "kv_pages_select: count > 0 pages, the %d first and %d last among them (got %d)", first, last, count);
   if (B == 0) return PFA_OK;
@@ -346,9 +356,9 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
     return PFA_E_WORKSPACE;
   }
   uint32_t* keys = (uint32_t*)workspace;
-  const int D = pages.head_dim, P = table_pages, rows = B * p.H;
+  const int D = pages->head_dim, P = table_pages, rows = B * p.H;
   if (P > 0) {
-    by_types(dtype, pages.dtype, [&](auto dt, auto ct) {
+    by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
       constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
       auto score = [&](auto width) {
         constexpr int W = decltype(width)::value;
@@ -377,27 +387,25 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, pfa_k
   return PFA_OK;
 }
 
-extern "C" int pfa_paged_attn_workspace_size(int B, int H, pfa_kv_pages pages, int table_pages, int n_selected,
-                                             size_t* bytes) {
+extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim, int cell_dtype,
+                                             int table_pages, int n_selected, size_t* bytes) {
   clear_error();
-  Pages p;
-  Table t;
-  if (int rc = paged_check(&pages, nullptr, 0, 0, B, &p, &t)) return rc;
-  PFA_CHECK_ARG(bytes && H > 0 && H % p.H == 0 && table_pages >= 0, "paged_attn: bad sizes");
-  *bytes = attend_plan(B, H, p.H, pages.head_dim, p.shift, table_pages, n_selected,
-                       attend_tile(pages.dtype, pages.head_dim))
+  if (int rc = sizes_check(kv_heads, page_size, head_dim, cell_dtype, table_pages, B)) return rc;
+  PFA_CHECK_ARG(bytes && H > 0 && H % kv_heads == 0, "paged_attn: bad sizes");
+  *bytes = attend_plan(B, H, kv_heads, head_dim, shift_of(page_size), table_pages, n_selected < 0 ? -1 : n_selected,
+                       attend_tile(cell_dtype, head_dim))
                .bytes;
   return PFA_OK;
 }
 
-extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv_pages pages, const int32_t* table,
+extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
                                   int64_t table_stride, int table_pages, const int32_t* lengths, const int32_t* starts,
                                   const int32_t* selected, int n_selected, float scale, void* out, void* workspace,
                                   size_t ws_bytes, void* stream) {
   clear_error();
   Pages p;
   Table t;
-  if (int rc = paged_check(&pages, table, table_stride, table_pages, B, &p, &t)) return rc;
+  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
   if (int rc = query_check("paged_attn", q, dtype, B, H, pages, lengths)) return rc;
   PFA_CHECK_ARG(n_selected <= 0 || selected, "paged_attn: null argument");
   PFA_CHECK_ARG((int64_t)n_selected << p.shift <= (1ll << 30), "paged_attn: lists of up to 2^30 positions");
@@ -406,16 +414,16 @@ extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, pfa_kv
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "paged_attn: null or unaligned argument");
   const int S = n_selected < 0 ? -1 : n_selected;
-  const Plan plan = attend_plan(B, H, p.H, pages.head_dim, p.shift, table_pages, S,
-                                attend_tile(pages.dtype, pages.head_dim));
+  const Plan plan = attend_plan(B, H, p.H, pages->head_dim, p.shift, table_pages, S,
+                                attend_tile(pages->dtype, pages->head_dim));
   if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
     set_error("paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, plan.bytes);
     return PFA_E_WORKSPACE;
   }
-  const AttendCall a{p, table, table_stride, table_pages, B, H, pages.head_dim, q, lengths, starts, selected, S, c, out,
+  const AttendCall a{p, table, table_stride, table_pages, B, H, pages->head_dim, q, lengths, starts, selected, S, c, out,
                      (float*)workspace, as_stream(stream)};
-  if (pages.dtype == PFA_I8) attend_i8(dtype, a);
-  else if (pages.dtype == PFA_E4M3) attend_e4m3(dtype, a);
+  if (pages->dtype == PFA_I8) attend_i8(dtype, a);
+  else if (pages->dtype == PFA_E4M3) attend_e4m3(dtype, a);
   else attend_float(dtype, a);
   PFA_CHECK_LAUNCH("paged_attn");
   return PFA_OK;

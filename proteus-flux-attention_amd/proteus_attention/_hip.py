@@ -93,25 +93,6 @@ class Tensor4(ctypes.Structure):
     ]
 
 
-class KVPagesC(ctypes.Structure):
-    """pfa_kv_pages: the pool of a paged key-value cache."""
-
-    _fields_ = [
-        ("k", ctypes.c_void_p),
-        ("v", ctypes.c_void_p),
-        ("k_scale", ctypes.c_void_p),
-        ("v_scale", ctypes.c_void_p),
-        ("k_bounds", ctypes.c_void_p),
-        ("k_page", ctypes.c_int64),
-        ("v_page", ctypes.c_int64),
-        ("n_pages", ctypes.c_int),
-        ("kv_heads", ctypes.c_int),
-        ("page_size", ctypes.c_int),
-        ("head_dim", ctypes.c_int),
-        ("dtype", ctypes.c_int),
-    ]
-
-
 class HipLibraryError(RuntimeError):
     """Raised when libpfa_hip.so cannot be loaded or a call fails."""
 
@@ -189,13 +170,13 @@ _SIGNATURES = {
     "pfa_int8_kv_attn_workspace_size": ([_i64, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_int8_kv_attn_fwd": ([Tensor4, Tensor4, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp,
                               _sz, _vp], _i32),
-    "pfa_kv_pages_write": ([KVPagesC, Tensor4, Tensor4, _i32, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp], _i32),
-    "pfa_kv_pages_read": ([KVPagesC, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
-    "pfa_paged_attn_workspace_size": ([_i32, _i32, KVPagesC, _i32, _i32, ctypes.POINTER(_sz)], _i32),
-    "pfa_paged_attn_fwd": ([Tensor4, _i32, _i32, _i32, KVPagesC, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _vp,
+    "pfa_kv_pages_write": ([_vp, Tensor4, Tensor4, _i32, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp], _i32),
+    "pfa_kv_pages_read": ([_vp, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
+    "pfa_paged_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
+    "pfa_paged_attn_fwd": ([Tensor4, _i32, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _f32, _vp, _vp,
                             _sz, _vp], _i32),
     "pfa_kv_pages_select_workspace_size": ([_i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
-    "pfa_kv_pages_select": ([Tensor4, _i32, _i32, _i32, KVPagesC, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _vp,
+    "pfa_kv_pages_select": ([Tensor4, _i32, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _vp,
                              _vp, _sz, _vp], _i32),
 }
 

@@ -22,14 +22,15 @@ the package this is the inference path: tensors that require a gradient raise
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from .. import _hip
-from .sparse_attn import _workspace
+from .sparse_attn import _size_out
 
 HEAD_DIMS = (16, 32, 64, 128)
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -77,66 +78,80 @@ def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *
     return KVPages(k, v, *scales, kb)
 
 
+# pfa_kv_pages of include/pfa_hip.h
+_POOL = struct.Struct("PPPPPqqiiiii4x")
+
+
 def _dense(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, name: str) -> int:
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
     return t.data_ptr()
 
 
-def _pool(pages: KVPages) -> "_hip.KVPagesC":
+def _pool(pages: KVPages) -> Tuple[bytes, int, int, int]:
+    """The pool for the library, and its heads, page size and head dim."""
+
     k, v, k_scale, v_scale, bounds = pages
-    dtype = k.dtype
+    dtype, shape = k.dtype, k.shape
     tag = _CELL_TAG.get(dtype)
     if tag is None or v.dtype != dtype:
         raise ValueError(f"k and v pages must share one of {tuple(_CELL_TAG)} (got {dtype}, {v.dtype})")
-    if k.dim() != 4 or v.shape != k.shape:
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("k and v pages must be (pages, kv_heads, page_size, head_dim) tensors of one shape")
-    N, H, ps, D = shape = tuple(k.shape)
+    N, H, ps, D = shape
     if D not in HEAD_DIMS or ps not in PAGE_SIZES:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS} and page_size one of {PAGE_SIZES} (got {D}, {ps})")
     if N == 0 or H == 0:
         raise ValueError("an empty pool")
-    for t in (k, v):
-        s = t.stride()
-        if s[3] != 1 or s[2] != D or (H > 1 and s[1] != ps * D):
-            raise ValueError("a page's heads, slots and channels must be dense")
-    ks = vs = kb = None
+    ks, vs = k.stride(), v.stride()
+    dense = (ps * D, D, 1)
+    if ks[1:] != dense or vs[1:] != dense:
+        for s in (ks, vs):
+            if s[2:] != dense[1:] or (H > 1 and s[1] != dense[0]):
+                raise ValueError("a page's heads, slots and channels must be dense")
+    a = c = b = 0
+    bound_dtype = dtype
     if dtype in _EIGHT_BITS:
         if k_scale is None or v_scale is None:
             raise ValueError("8-bit pages need k_scale and v_scale")
-        ks = _dense(k_scale, shape[:3], torch.float32, "k_scale")
-        vs = _dense(v_scale, shape[:3], torch.float32, "v_scale")
+        a = _dense(k_scale, shape[:3], torch.float32, "k_scale")
+        c = _dense(v_scale, shape[:3], torch.float32, "v_scale")
+        bound_dtype = torch.float32
     if bounds is not None:
-        kb = _dense(bounds, (N, H, 2, D), torch.float32 if dtype in _EIGHT_BITS else dtype, "k_bounds")
-    return _hip.KVPagesC(k.data_ptr(), v.data_ptr(), ks, vs, kb, k.stride(0), v.stride(0), N, H, ps, D, tag)
+        b = _dense(bounds, (N, H, 2, D), bound_dtype, "k_bounds")
+    return _POOL.pack(k.data_ptr(), v.data_ptr(), a, c, b, ks[0], vs[0], N, H, ps, D, tag), H, ps, D
 
 
-def _table(block_table: torch.Tensor) -> torch.Tensor:
-    if block_table.dim() != 2 or block_table.dtype != torch.int32:
-        raise ValueError("block_table must be a (B, P) int32 tensor")
-    return block_table if block_table.stride(1) == 1 or block_table.shape[1] <= 1 else block_table.contiguous()
+def _table(block_table: torch.Tensor, B: int) -> torch.Tensor:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != B or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table must be a ({B}, P) int32 tensor")
+    return block_table if block_table.stride(1) == 1 or shape[1] <= 1 else block_table.contiguous()
 
 
-def _per_sequence(t: Optional[torch.Tensor], B: int, name: str) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    if t.dim() != 1 or t.shape[0] != B or t.dtype != torch.int32:
+def _per_sequence(t: torch.Tensor, B: int, name: str) -> torch.Tensor:
+    if t.shape != (B,) or t.dtype != torch.int32:
         raise ValueError(f"{name} must be a ({B},) int32 tensor")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _inference(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
+def _device(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """The index of the one device that all tensors are on."""
+
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or index < 0):
+            _hip.require_device(*tensors, what=what)
+    return index
 
 
 class _OnDevice:
-    """Makes a tensor's device the current one for a call, where it is not."""
+    """Makes a device the current one for a call, where it is not."""
 
     __slots__ = ("index", "before")
 
-    def __init__(self, device: torch.device) -> None:
-        self.index = device.index
+    def __init__(self, index: int) -> None:
+        self.index = index
 
     def __enter__(self):
         now = torch.cuda.current_device()
@@ -148,6 +163,31 @@ class _OnDevice:
         if self.before >= 0:
             torch.cuda.set_device(self.before)
         return False
+
+
+@functools.lru_cache(maxsize=256)
+def _attend_bytes(*sizes: int) -> int:
+    """Workspace of one-token attention: B, query heads, kv heads, page size,
+    head dim, cell tag, the table's pages, listed pages or -1."""
+
+    return _size_out(_hip.lib().pfa_paged_attn_workspace_size, *sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _select_bytes(*sizes: int) -> int:
+    """Workspace of selection: B, kv heads, the table's pages."""
+
+    return _size_out(_hip.lib().pfa_kv_pages_select_workspace_size, *sizes)
+
+
+def _scratch(nbytes: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int]]:
+    """A workspace of the call's own, from torch's allocator on the current
+    stream, and its address."""
+
+    if nbytes == 0:
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr()
 
 
 def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor,
@@ -166,31 +206,36 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     Two sequences of one call must not write to one page.
     """
 
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v must be (B, n, kv_heads, head_dim) tensors of one shape and dtype")
-    B, n, H, D = k.shape
-    pool = _pool(pages)
-    if H != pool.kv_heads or D != pool.head_dim:
-        raise ValueError(f"k and v have {H} heads of {D}, the pages {pool.kv_heads} of {pool.head_dim}")
-    tag = _VALUE_TAG.get(k.dtype)
-    if tag is None or (pages.k.dtype not in _EIGHT_BITS and pages.k.dtype != k.dtype):
-        raise ValueError(f"values of {k.dtype} for pages of {pages.k.dtype}")
-    table = _table(block_table)
-    starts, counts = _per_sequence(starts, B, "starts"), _per_sequence(counts, B, "counts")
-    if starts is None or table.shape[0] != B:
-        raise ValueError("block_table and starts need one row per sequence")
-    _inference("write_kv_pages", k, v)
-    device = _hip.require_device(*pages, k, v, table, starts, counts, what="write_kv_pages")
-    if k.stride(3) != 1:
+    B, n, H, D = shape
+    pool, pool_heads, _, pool_dim = _pool(pages)
+    if H != pool_heads or D != pool_dim:
+        raise ValueError(f"k and v have {H} heads of {D}, the pages {pool_heads} of {pool_dim}")
+    tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
+    if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
+        raise ValueError(f"values of {dtype} for pages of {cells}")
+    table, starts = _table(block_table, B), _per_sequence(starts, B, "starts")
+    if counts is not None:
+        counts = _per_sequence(counts, B, "counts")
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError("write_kv_pages has no backward pass: call it under torch.no_grad()")
+    index = _device("write_kv_pages", k, v, *pages, table, starts, counts)
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1:
         k = k.contiguous()
-    if v.stride(3) != 1:
+        ks = k.stride()
+    if vs[3] != 1:
         v = v.contiguous()
-    with _OnDevice(device), _hip.TIMER.timed("kv_pages_write"):
+        vs = v.stride()
+    with _OnDevice(index), _hip.TIMER.timed("kv_pages_write"):
         rc = _hip.lib().pfa_kv_pages_write(
-            pool, _hip.Tensor4(k.data_ptr(), k.stride(0), k.stride(2), k.stride(1)),
-            _hip.Tensor4(v.data_ptr(), v.stride(0), v.stride(2), v.stride(1)), tag, B, n, table.data_ptr(),
-            table.stride(0), table.shape[1], starts.data_ptr(), _hip.ptr(counts), _hip.stream_ptr(device))
-    _hip.check(rc, "pfa_kv_pages_write")
+            pool, _hip.Tensor4(k.data_ptr(), ks[0], ks[2], ks[1]), _hip.Tensor4(v.data_ptr(), vs[0], vs[2], vs[1]), tag,
+            B, n, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(),
+            None if counts is None else counts.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _hip.check(rc, "pfa_kv_pages_write")
 
 
 def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tensor, counts: Optional[torch.Tensor],
@@ -200,87 +245,89 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     ``dtype`` (default: the pages' type, f32 for 8-bit pages).  Rows
     i >= ``counts[b]``, and those without a page, are zero."""
 
-    pool = _pool(pages)
-    table = _table(block_table)
-    B, n = table.shape[0], int(n)
-    starts, counts = _per_sequence(starts, B, "starts"), _per_sequence(counts, B, "counts")
-    if starts is None:
-        raise ValueError("starts needs one entry per sequence")
+    pool, H, _, D = _pool(pages)
+    B, n = block_table.shape[0] if block_table.dim() else 0, int(n)
+    table, starts = _table(block_table, B), _per_sequence(starts, B, "starts")
+    if counts is not None:
+        counts = _per_sequence(counts, B, "counts")
     if n < 0:
         raise ValueError("n must not be negative")
     if dtype is None:
-        dtype = torch.float32 if pages.k.dtype in _EIGHT_BITS else pages.k.dtype
+        dtype = torch.float32 if pages[0].dtype in _EIGHT_BITS else pages[0].dtype
     tag = _VALUE_TAG.get(dtype)
     if tag is None:
         raise ValueError(f"unsupported value dtype {dtype}")
-    device = _hip.require_device(*pages, table, starts, counts, what="read_kv_pages")
-    k, v = (torch.empty(B, n, pool.kv_heads, pool.head_dim, dtype=dtype, device=device) for _ in range(2))
-    with _OnDevice(device), _hip.TIMER.timed("kv_pages_read"):
-        rc = _hip.lib().pfa_kv_pages_read(pool, B, n, table.data_ptr(), table.stride(0), table.shape[1],
-                                          starts.data_ptr(), _hip.ptr(counts), k.data_ptr(), v.data_ptr(), tag,
-                                          _hip.stream_ptr(device))
-    _hip.check(rc, "pfa_kv_pages_read")
+    index = _device("read_kv_pages", *pages, table, starts, counts)
+    device = table.device
+    k = torch.empty((B, n, H, D), dtype=dtype, device=device)
+    v = torch.empty((B, n, H, D), dtype=dtype, device=device)
+    with _OnDevice(index), _hip.TIMER.timed("kv_pages_read"):
+        rc = _hip.lib().pfa_kv_pages_read(
+            pool, B, n, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(),
+            None if counts is None else counts.data_ptr(), k.data_ptr(), v.data_ptr(), tag,
+            torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _hip.check(rc, "pfa_kv_pages_read")
     return k, v
 
 
-class _Query(NamedTuple):
-    """The checked arguments that selection and attention share."""
+class _Query:
+    """The checked arguments that selection and attention share, for the
+    library in ``args``; the tensors stay referenced until the calls are made."""
 
-    pool: "_hip.KVPagesC"
-    q: torch.Tensor
-    q4: "_hip.Tensor4"
-    tag: int
-    table: torch.Tensor
-    lengths: torch.Tensor
-    starts: Optional[torch.Tensor]
-    device: torch.device
+    __slots__ = ("args", "B", "H", "Hkv", "ps", "D", "P", "tag", "cells", "q", "table", "lengths", "starts", "index")
+
+    def __init__(self, what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
+                 starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None) -> None:
+        shape, dtype = q.shape, q.dtype
+        if len(shape) != 3:
+            raise ValueError("q must be a (B, heads, head_dim) tensor: one new token a sequence")
+        self.B, self.H, self.D = B, H, D = shape
+        pool, self.Hkv, self.ps, pool_dim = _pool(pages)
+        if D != pool_dim or H == 0 or H % self.Hkv:
+            raise ValueError(f"q has {H} heads of {D}, the pages {self.Hkv} of {pool_dim}")
+        tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
+        if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
+            raise ValueError(f"queries of {dtype} for pages of {cells}")
+        self.tag, self.cells = tag, _CELL_TAG[cells]
+        self.table = table = _table(block_table, B)
+        self.P = table.shape[1]
+        self.lengths = lengths = _per_sequence(lengths, B, "lengths")
+        self.starts = starts = None if starts is None else _per_sequence(starts, B, "starts")
+        if q.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
+        self.index = _device(what, q, *pages, table, lengths, starts, selected)
+        s = q.stride()
+        if s[2] != 1:
+            q = q.contiguous()
+            s = q.stride()
+        self.q = q
+        self.args = (_hip.Tensor4(q.data_ptr(), s[0], s[1], 0), tag, B, H, pool, table.data_ptr(), table.stride(0),
+                     self.P, lengths.data_ptr(), None if starts is None else starts.data_ptr())
 
 
-def _query(what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
-           starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None) -> _Query:
-    if q.dim() != 3:
-        raise ValueError("q must be a (B, heads, head_dim) tensor: one new token a sequence")
-    B, H, D = q.shape
-    pool = _pool(pages)
-    if D != pool.head_dim or H == 0 or H % pool.kv_heads:
-        raise ValueError(f"q has {H} heads of {D}, the pages {pool.kv_heads} of {pool.head_dim}")
-    tag = _VALUE_TAG.get(q.dtype)
-    if tag is None or (pages.k.dtype not in _EIGHT_BITS and pages.k.dtype != q.dtype):
-        raise ValueError(f"queries of {q.dtype} for pages of {pages.k.dtype}")
-    table = _table(block_table)
-    lengths, starts = _per_sequence(lengths, B, "lengths"), _per_sequence(starts, B, "starts")
-    if lengths is None or table.shape[0] != B:
-        raise ValueError("block_table and lengths need one row per sequence")
-    _inference(what, q)
-    device = _hip.require_device(q, *pages, table, lengths, starts, selected, what=what)
-    if q.stride(2) != 1:
-        q = q.contiguous()
-    return _Query(pool, q, _hip.Tensor4(q.data_ptr(), q.stride(0), q.stride(1), 0), tag, table, lengths, starts, device)
-
-
-def _scale(scale: Optional[float], D: int) -> float:
+def _scale(scale: Optional[float]) -> Optional[float]:
     if scale is None:
-        return 1.0 / math.sqrt(D)
+        return None
     scale = float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("scale must be positive and finite")
     return scale
 
 
-def _attend(a: _Query, selected: Optional[torch.Tensor], scale: float) -> torch.Tensor:
-    B, H, D = a.q.shape
-    lib = _hip.lib()
-    size = ctypes.c_size_t(0)
-    P, S = a.table.shape[1], -1 if selected is None else selected.shape[2]
-    _hip.check(lib.pfa_paged_attn_workspace_size(B, H, a.pool, P, S, ctypes.byref(size)),
-               "pfa_paged_attn_workspace_size")
-    ws = _workspace(size.value, a.device)
-    out = torch.empty(B, H, D, dtype=a.q.dtype, device=a.device)
-    with _OnDevice(a.device), _hip.TIMER.timed("paged_attn_fwd"):
-        rc = lib.pfa_paged_attn_fwd(a.q4, a.tag, B, H, a.pool, a.table.data_ptr(), a.table.stride(0), P,
-                                    a.lengths.data_ptr(), _hip.ptr(a.starts), _hip.ptr(selected), S, scale,
-                                    out.data_ptr(), ws.data_ptr(), ws.numel(), _hip.stream_ptr(a.device))
-    _hip.check(rc, "pfa_paged_attn_fwd")
+def _attend(a: _Query, selected: Optional[torch.Tensor], scale: Optional[float]) -> torch.Tensor:
+    if scale is None:
+        scale = 1.0 / math.sqrt(a.D)
+    S = -1 if selected is None else selected.shape[2]
+    device = a.table.device
+    ws, ws_ptr = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
+    out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
+    with _OnDevice(a.index), _hip.TIMER.timed("paged_attn_fwd"):
+        rc = _hip.lib().pfa_paged_attn_fwd(*a.args, None if selected is None else selected.data_ptr(), S, scale,
+                                           out.data_ptr(), ws_ptr, 0 if ws is None else ws.numel(),
+                                           torch._C._cuda_getCurrentRawStream(a.index))
+    if rc:
+        _hip.check(rc, "pfa_paged_attn_fwd")
     return out
 
 
@@ -299,33 +346,36 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     none with a score above -inf, is zero.
     """
 
-    a = _query("paged_attention", q, pages, block_table, lengths, starts, selected)
+    if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32):
+        raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
+    scale = _scale(scale)
+    a = _Query("paged_attention", q, pages, block_table, lengths, starts, selected)
     if selected is not None:
-        if selected.dim() != 3 or selected.shape[:2] != (q.shape[0], a.pool.kv_heads) or selected.dtype != torch.int32:
+        if selected.shape[:2] != (a.B, a.Hkv):
             raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
         selected = selected.contiguous()
-    return _attend(a, selected, _scale(scale, q.shape[2]))
+    return _attend(a, selected, scale)
 
 
-def _select(a: _Query, pages: KVPages, count: int, first: int, last: int) -> torch.Tensor:
-    B, H, _ = a.q.shape
+def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, int, int]:
     count, first, last = int(count), int(first), int(last)
-    if pages.k_bounds is None:
+    if pages[4] is None:
         raise ValueError("selection needs pages with k_bounds")
     if count < 1 or first < 0 or last < 0 or first + last > count:
         raise ValueError("count must be positive and hold the first and last pages")
-    lib = _hip.lib()
-    size = ctypes.c_size_t(0)
-    P = a.table.shape[1]
-    _hip.check(lib.pfa_kv_pages_select_workspace_size(B, a.pool.kv_heads, P, ctypes.byref(size)),
-               "pfa_kv_pages_select_workspace_size")
-    ws = _workspace(size.value, a.device)
-    chosen = torch.empty(B, a.pool.kv_heads, count, dtype=torch.int32, device=a.device)
-    with _OnDevice(a.device), _hip.TIMER.timed("kv_pages_select"):
-        rc = lib.pfa_kv_pages_select(a.q4, a.tag, B, H, a.pool, a.table.data_ptr(), a.table.stride(0), P,
-                                     a.lengths.data_ptr(), _hip.ptr(a.starts), count, first, last, chosen.data_ptr(),
-                                     ws.data_ptr(), ws.numel(), _hip.stream_ptr(a.device))
-    _hip.check(rc, "pfa_kv_pages_select")
+    return count, first, last
+
+
+def _select(a: _Query, count: int, first: int, last: int) -> torch.Tensor:
+    device = a.table.device
+    ws, ws_ptr = _scratch(_select_bytes(a.B, a.Hkv, a.P), device)
+    chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
+    with _OnDevice(a.index), _hip.TIMER.timed("kv_pages_select"):
+        rc = _hip.lib().pfa_kv_pages_select(*a.args, count, first, last, chosen.data_ptr(), ws_ptr,
+                                            0 if ws is None else ws.numel(),
+                                            torch._C._cuda_getCurrentRawStream(a.index))
+    if rc:
+        _hip.check(rc, "pfa_kv_pages_select")
     return chosen
 
 
@@ -343,7 +393,8 @@ def select_kv_pages(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     better score wins, ties the lower entry.
     """
 
-    return _select(_query("select_kv_pages", q, pages, block_table, lengths, starts), pages, count, first, last)
+    sizes = _counted(pages, count, first, last)
+    return _select(_Query("select_kv_pages", q, pages, block_table, lengths, starts), *sizes)
 
 
 def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -352,10 +403,11 @@ def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.T
     """:func:`paged_attention` over the pages that :func:`select_kv_pages`
     chooses.  Returns the output and the chosen entries."""
 
-    a = _query("paged_sparse_attention", q, pages, block_table, lengths, starts)
-    sc = _scale(scale, q.shape[2])
-    chosen = _select(a, pages, count, first, last)
-    return _attend(a, chosen, sc), chosen
+    sizes = _counted(pages, count, first, last)
+    scale = _scale(scale)
+    a = _Query("paged_sparse_attention", q, pages, block_table, lengths, starts)
+    chosen = _select(a, *sizes)
+    return _attend(a, chosen, scale), chosen
 
 
 __all__ = [

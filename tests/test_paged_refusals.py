@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import pytest
 import torch
@@ -87,10 +88,8 @@ def test_pools_that_do_not_fit():
     lambda p: select_kv_pages(Q, p._replace(k_bounds=None), TABLE, ONE, 3),
 ])
 def test_arguments_that_do_not_fit(call):
-    with pytest.raises((ValueError, _hip.HipLibraryError)) as e:
+    with pytest.raises(ValueError):
         call(_new())
-    if isinstance(e.value, _hip.HipLibraryError):  # refused for the device first: the C entry refuses it again
-        assert "ROCm device" in str(e.value)
 
 
 def test_no_backward():
@@ -104,7 +103,7 @@ def _c_pool(**kw):
     a = dict(k=256, v=256, k_scale=None, v_scale=None, k_bounds=None, k_page=2 * 16 * 32, v_page=2 * 16 * 32, n_pages=4,
              kv_heads=2, page_size=16, head_dim=32, dtype=_hip.PFA_F32)
     a.update(kw)
-    return _hip.KVPagesC(*a.values())
+    return struct.pack("PPPPPqqiiiii4x", *(x or 0 for x in a.values()))
 
 
 def test_c_entries_refuse_before_any_launch():
@@ -129,6 +128,10 @@ def test_c_entries_refuse_before_any_launch():
     assert bad == [-1] * len(bad)
     rc = lib.pfa_kv_pages_select(t4, 0, 1, 2, _c_pool(k_bounds=256), p, 2, 2, p, None, 2, 1, 1, p, p, 4, None)
     assert rc == -3
+    size = ctypes.c_size_t(0)
+    sizes = [(1, 4, 2, 16, 32, _hip.PFA_F32, 100, -1), (1, 3, 2, 16, 32, 0, 100, -1), (1, 4, 2, 24, 32, 0, 100, -1),
+             (1, 4, 2, 16, 48, 0, 100, -1), (1, 4, 2, 16, 32, 7, 100, -1), (-1, 4, 2, 16, 32, 0, 100, -1)]
+    assert [lib.pfa_paged_attn_workspace_size(*x, ctypes.byref(size)) for x in sizes] == [0] + [-1] * 5
     # nothing to do: no launch, no error
     assert attend(_c_pool(), B=0) == 0
     assert lib.pfa_kv_pages_write(_c_pool(), t4, t4, 0, 1, 0, p, 2, 2, p, p, None) == 0
