@@ -331,7 +331,7 @@ static int64_t row_keys(int table_pages) { return ((int64_t)table_pages + 3) & ~
 extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes) {
   clear_error();
   PFA_CHECK_ARG(bytes && B >= 0 && kv_heads > 0 && table_pages >= 0, "kv_pages_select: bad sizes");
-  *bytes = (size_t)B * kv_heads * row_keys(table_pages) * 4;
+  *bytes = table_pages <= kFused ? 0 : (size_t)B * kv_heads * row_keys(table_pages) * 4;
   return PFA_OK;
 }
 
@@ -357,27 +357,31 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const
   }
   uint32_t* keys = (uint32_t*)workspace;
   const int D = pages->head_dim, P = table_pages, rows = B * p.H;
-  if (P > 0) {
-    by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
-      constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
-      auto score = [&](auto width) {
-        constexpr int W = decltype(width)::value;
-        constexpr int at_once = 4 * (kWave / (W / 8)) * kSteps;
-        score_kernel<QT, BT, W><<<dim3(p.H, (P + at_once - 1) / at_once, B), 256, 0, as_stream(stream)>>>(
-            p, table, table_stride, P, (const typename Elem<QT>::T*)q.ptr, q.s_b, q.s_h, H / p.H, lengths, starts, first,
-            last, row_keys(P), keys);
-      };
-      if (D == 16) score(std::integral_constant<int, 16>{});
-      else if (D == 32) score(std::integral_constant<int, 32>{});
-      else if (D == 64) score(std::integral_constant<int, 64>{});
-      else score(std::integral_constant<int, 128>{});
-    });
-  }
+  by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
+    constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
+    const auto* qp = (const typename Elem<QT>::T*)q.ptr;
+    auto launch = [&](auto width) {
+      constexpr int W = decltype(width)::value;
+      if (P <= kFused)
+        select_kernel<QT, BT, W><<<rows, 1024, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q.s_b, q.s_h,
+                                                                       H / p.H, lengths, starts, first, last, count,
+                                                                       chosen);
+      else
+        score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W) - 1) / score_span(4, W), B), 256, 0,
+                                  as_stream(stream)>>>(p, table, table_stride, P, qp, q.s_b, q.s_h, H / p.H, lengths,
+                                                       starts, first, last, row_keys(P), keys);
+    };
+    if (D == 16) launch(std::integral_constant<int, 16>{});
+    else if (D == 32) launch(std::integral_constant<int, 32>{});
+    else if (D == 64) launch(std::integral_constant<int, 64>{});
+    else launch(std::integral_constant<int, 128>{});
+  });
   // entries of a row from the first's four on: up to P + 3
 #define PFA_CHOOSE(THREADS, K, HELD)                                                                          \
   choose_kernel<THREADS, K, HELD><<<rows, THREADS, 0, as_stream(stream)>>>(p.H, P, row_keys(P), p.shift, count, \
                                                                            lengths, starts, keys, chosen)
-  if (P + 3 <= 256 * 4) PFA_CHOOSE(256, 4, true);
+  if (P <= kFused) {
+  } else if (P + 3 <= 256 * 4) PFA_CHOOSE(256, 4, true);
   else if (P + 3 <= 1024 * 4) PFA_CHOOSE(1024, 4, true);
   else if (P + 3 <= 1024 * 8) PFA_CHOOSE(1024, 8, true);
   else if (P + 3 <= 1024 * 16) PFA_CHOOSE(1024, 16, true);

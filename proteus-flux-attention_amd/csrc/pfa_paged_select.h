@@ -51,30 +51,24 @@ __device__ __forceinline__ double across(double x) {
 // four query heads each: 31 us; one query head instead of four: 26 us.  Widening
 // the bounds once and two products of max(q, 0) and min(q, 0) a channel: 35 us (160
 // registers, three waves a SIMD); workgroups of one or two waves: 34 us.
-template <int QT, int BT, int D>
-__global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __restrict__ table, int64_t table_stride,
-                                                    int P, const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
-                                                    int64_t q_h, int G, const int32_t* __restrict__ lengths,
-                                                    const int32_t* __restrict__ starts, int first, int last,
-                                                    int64_t row_keys, uint32_t* __restrict__ keys) {
-  constexpr int LP = D / 8;            // lanes of a page
-  constexpr int PW = kWave / LP;       // pages of a wave at once
-  constexpr int AT_ONCE = 4 * PW * kSteps;  // pages of a workgroup
+//
+// Pages base .. base + WAVES * 64 / (D / 8) * kSteps - 1 of a workgroup's row; put
+// gets each page of the span and its key.
+template <int QT, int BT, int D, int WAVES, typename Put>
+__device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __restrict__ ids, const Span& sp, int h,
+                                            const typename Elem<QT>::T* __restrict__ q, int64_t q_h, int G, int first,
+                                            int last, int base, float (&qs)[kScoreHeads][D], Put&& put) {
+  constexpr int LP = D / 8;       // lanes of a page
+  constexpr int PW = kWave / LP;  // pages of a wave at once
   using BoundT = typename Elem<BT>::T;
-  const int b = blockIdx.z, h = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const Span sp = span_at(lengths, starts, P, pg.shift, b);
-  const int base = blockIdx.y * AT_ONCE;
-  if (base >= sp.pe || base + AT_ONCE <= sp.p0) return;
-  __shared__ float qs[kScoreHeads][D];
-  const int part = lane % LP;
-  // page of step s: base + (4 waves x kSteps + s) x PW + lane / LP
-  const int page0 = base + (tid >> 6) * kSteps * PW + lane / LP;
+  const int tid = threadIdx.x, lane = tid & 63, part = lane % LP;
+  const int page0 = base + (tid >> 6) * kSteps * PW + lane / LP;  // of step s: + s * PW
   float lo[kSteps][8], hi[kSteps][8];
   bool have[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     const int page = page0 + s * PW;
-    const int id = page >= sp.p0 && page < sp.pe ? table[b * table_stride + page] : -1;
+    const int id = page >= sp.p0 && page < sp.pe ? ids[page] : -1;
     have[s] = (uint32_t)id < (uint32_t)pg.n_pages;
     const BoundT* at = (const BoundT*)pg.bounds + ((int64_t)(have[s] ? id : 0) * pg.H + h) * 2 * D + 8 * part;
     load8<BT>(at, lo[s]);
@@ -90,10 +84,8 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
   for (int g0 = 0; g0 < G; g0 += kScoreHeads) {
     const int heads = G - g0 < kScoreHeads ? G - g0 : kScoreHeads;
     __syncthreads();
-    for (int i = tid; i < heads * D; i += 256) {
-      const float x = load_f<QT>(q + b * q_b + (int64_t)(h * G + g0 + i / D) * q_h + i % D);
-      qs[i / D][i % D] = x;
-    }
+    for (int i = tid; i < heads * D; i += WAVES * kWave)
+      qs[i / D][i % D] = load_f<QT>(q + (int64_t)(h * G + g0 + i / D) * q_h + i % D);
     __syncthreads();
     for (int g = 0; g < heads; ++g) {
       double sum[kSteps] = {};
@@ -130,7 +122,6 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
     }
   }
   if (part >= 4) return;
-  uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
     const int s = LP == 2 ? 2 * odd + k : 2 * odd + upper;
@@ -143,8 +134,27 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
     u = u & 0x80000000u ? ~u : u | 0x80000000u;  // -inf is 0x007fffff, +inf 0xff800000
     if (nan[k]) u = kNan;
     if (page - sp.p0 < first || sp.pe - page <= last) u = kForced;
-    row[page] = ok ? u : kNone;
+    put(page, ok ? u : kNone);
   }
+}
+
+// Pages of a workgroup of `waves` waves at once.
+__host__ __device__ constexpr int score_span(int waves, int D) { return waves * (kWave / (D / 8)) * kSteps; }
+
+template <int QT, int BT, int D>
+__global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __restrict__ table, int64_t table_stride,
+                                                    int P, const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
+                                                    int64_t q_h, int G, const int32_t* __restrict__ lengths,
+                                                    const int32_t* __restrict__ starts, int first, int last,
+                                                    int64_t row_keys, uint32_t* __restrict__ keys) {
+  const int b = blockIdx.z, h = blockIdx.x;
+  const Span sp = span_at(lengths, starts, P, pg.shift, b);
+  const int base = blockIdx.y * score_span(4, D);
+  if (base >= sp.pe || base + score_span(4, D) <= sp.p0) return;
+  __shared__ float qs[kScoreHeads][D];
+  uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
+  score_pages<QT, BT, D, 4>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
+                            [&](int page, uint32_t key) { row[page] = key; });
 }
 
 // The best `count` of a row of keys, ascending.  The keys' range is cut into
@@ -176,37 +186,18 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int& all) {
   return before + incl - x;
 }
 
-template <int THREADS, int K, bool HELD>
-__global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t row_keys, int shift, int count,
-                                                         const int32_t* __restrict__ lengths,
-                                                         const int32_t* __restrict__ starts,
-                                                         const uint32_t* __restrict__ keys,
-                                                         int32_t* __restrict__ chosen) {
+// fetch(r, x): the K keys of the thread's entries from + (r * THREADS + thread) * K
+// on in round r, kNone where there are none.
+template <int THREADS, int K, bool HELD, typename Fetch>
+__device__ __forceinline__ void choose_best(int from0, int rounds, int count, int32_t* __restrict__ out, Fetch&& fetch) {
   constexpr int WAVES = THREADS / kWave;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t* key = keys + (int64_t)blockIdx.x * row_keys;
-  int32_t* out = chosen + (int64_t)blockIdx.x * count;
-  const Span sp = span_at(lengths, starts, P, shift, blockIdx.x / H);
-  const int from0 = sp.p0 & ~3;  // rows of keys are 16-byte aligned
-  const int rounds = HELD ? 1 : (sp.pe - from0 + THREADS * K - 1) / (THREADS * K);
   __shared__ int hist[kBins];
   __shared__ int sums[3][WAVES];
   __shared__ uint32_t range[2][WAVES];
   __shared__ int cut[3];
 
   uint32_t held[K];
-  auto fetch = [&](int r, uint32_t (&x)[K]) {
-    const int p = from0 + (r * THREADS + tid) * K;
-#pragma unroll
-    for (int i = 0; i < K; i += 4) {
-      uint4 a = make_uint4(0, 0, 0, 0);
-      if (p + i < sp.pe) a = *reinterpret_cast<const uint4*>(key + p + i);
-      x[i] = a.x, x[i + 1] = a.y, x[i + 2] = a.z, x[i + 3] = a.w;
-    }
-#pragma unroll
-    for (int i = 0; i < K; ++i)
-      if (p + i < sp.p0 || p + i >= sp.pe) x[i] = kNone;
-  };
   if constexpr (HELD) fetch(0, held);
   auto each = [&](auto&& f) {
     if constexpr (HELD) f(0, held);
@@ -317,6 +308,55 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
     tied += eqs;
   });
   for (int i = base + tid; i < count; i += THREADS) out[i] = -1;
+}
+
+template <int THREADS, int K, bool HELD>
+__global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t row_keys, int shift, int count,
+                                                         const int32_t* __restrict__ lengths,
+                                                         const int32_t* __restrict__ starts,
+                                                         const uint32_t* __restrict__ keys,
+                                                         int32_t* __restrict__ chosen) {
+  const uint32_t* key = keys + (int64_t)blockIdx.x * row_keys;
+  const Span sp = span_at(lengths, starts, P, shift, blockIdx.x / H);
+  const int from0 = sp.p0 & ~3;  // rows of keys are 16-byte aligned
+  const int rounds = HELD ? 1 : (sp.pe - from0 + THREADS * K - 1) / (THREADS * K);
+  choose_best<THREADS, K, HELD>(from0, rounds, count, chosen + (int64_t)blockIdx.x * count,
+                                [&](int r, uint32_t (&x)[K]) {
+    const int p = from0 + (r * THREADS + (int)threadIdx.x) * K;
+#pragma unroll
+    for (int i = 0; i < K; i += 4) {
+      uint4 a = make_uint4(0, 0, 0, 0);
+      if (p + i < sp.pe) a = *reinterpret_cast<const uint4*>(key + p + i);
+      x[i] = a.x, x[i + 1] = a.y, x[i + 2] = a.z, x[i + 3] = a.w;
+    }
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (p + i < sp.p0 || p + i >= sp.pe) x[i] = kNone;
+  });
+}
+
+// Both for rows of up to kFused pages, a workgroup a row with the keys in LDS: a
+// launch (3.5 us of the host) less, in no more time (251 pages of 64
+// channels, 8 rows: 9.1 us against 4.0 + 5.4).
+constexpr int kFused = 512;
+
+template <int QT, int BT, int D>
+__global__ void __launch_bounds__(1024) select_kernel(Pages pg, const int32_t* __restrict__ table,
+                                                      int64_t table_stride, int P,
+                                                      const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
+                                                      int64_t q_h, int G, const int32_t* __restrict__ lengths,
+                                                      const int32_t* __restrict__ starts, int first, int last,
+                                                      int count, int32_t* __restrict__ chosen) {
+  const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H, tid = threadIdx.x;
+  const Span sp = span_at(lengths, starts, P, pg.shift, b);
+  __shared__ float qs[kScoreHeads][D];
+  __shared__ uint32_t keys[kFused];
+  for (int base = sp.p0; base < sp.pe; base += score_span(16, D))
+    score_pages<QT, BT, D, 16>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
+                               [&](int page, uint32_t key) { keys[page - sp.p0] = key; });
+  __syncthreads();
+  choose_best<1024, 1, true>(sp.p0, 1, count, chosen + (int64_t)blockIdx.x * count,
+                             [&](int, uint32_t (&x)[1]) { x[0] = tid < sp.pe - sp.p0 ? keys[tid] : kNone; });
 }
 
 }  // namespace paged

@@ -237,7 +237,8 @@ def test_selection(pair, D):
     dt, cell = pair
     g = torch.Generator().manual_seed(6)
     for H, G, ps, lengths, starts in ((1, 1, 16, [1, 160, 161, 0], None), (2, 4, 16, [4000, 900], [0, 333]),
-                                      (3, 5, 64, [5000, 64, 640], [70, 64, 9]), (1, 17, 32, [1200], None)):
+                                      (3, 5, 64, [5000, 64, 640], [70, 64, 9]), (1, 17, 32, [1200], None),
+                                      (1, 3, 16, [20011, 9000, 8193], [37, 0, 8192])):
         N = sum(-(-n // ps) for n in lengths) + 1
         pool = R.make_pool(N, H, ps, D, cell, g, bounds=True)
         table = R.make_table(lengths, ps, N, g)
@@ -258,7 +259,7 @@ def test_selection_of_equal_pages():
     """All pages alike: the lowest entries, whatever the number of pages."""
     from proteus_attention import KVPages, select_kv_pages
 
-    for P in (1, 63, 1000, 5000):
+    for P in (1, 63, 511, 512, 513, 1021, 1022, 4094, 5000, 8190, 16381, 16382, 40000):
         z = torch.zeros(1, 1, 16, 16, device=DEV)
         pages = KVPages(k=z, v=z.clone(), k_bounds=torch.ones(1, 1, 2, 16, device=DEV))
         q = torch.randn(1, 2, 16, device=DEV)

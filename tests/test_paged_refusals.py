@@ -126,7 +126,7 @@ def test_c_entries_refuse_before_any_launch():
            lib.pfa_kv_pages_write(_c_pool(), t4, t4, _hip.PFA_F16, 1, 3, p, 2, 2, p, p, None),
            lib.pfa_kv_pages_write(_c_pool(), t4, t4, _hip.PFA_F32, 1, 3, p, 2, 2, None, p, None)]
     assert bad == [-1] * len(bad)
-    rc = lib.pfa_kv_pages_select(t4, 0, 1, 2, _c_pool(k_bounds=256), p, 2, 2, p, None, 2, 1, 1, p, p, 4, None)
+    rc = lib.pfa_kv_pages_select(t4, 0, 1, 2, _c_pool(k_bounds=256), p, 600, 600, p, None, 2, 1, 1, p, p, 4, None)
     assert rc == -3
     size = ctypes.c_size_t(0)
     sizes = [(1, 4, 2, 16, 32, _hip.PFA_F32, 100, -1), (1, 3, 2, 16, 32, 0, 100, -1), (1, 4, 2, 24, 32, 0, 100, -1),
