@@ -367,7 +367,7 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const
                                                                        H / p.H, lengths, starts, first, last, count,
                                                                        chosen);
       else
-        score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W) - 1) / score_span(4, W), B), 256, 0,
+        score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W, BT) - 1) / score_span(4, W, BT), B), 256, 0,
                                   as_stream(stream)>>>(p, table, table_stride, P, qp, q.s_b, q.s_h, H / p.H, lengths,
                                                        starts, first, last, row_keys(P), keys);
     };

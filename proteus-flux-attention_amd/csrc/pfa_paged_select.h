@@ -25,7 +25,9 @@ __device__ __forceinline__ Span span_at(const int32_t* lengths, const int32_t* s
 }
 
 constexpr int kScoreHeads = 8;  // query heads in LDS at once
-constexpr int kSteps = 4;        // pages of a lane at once
+constexpr int kPair = 1;         // query heads at once
+// pages of a lane at once
+__host__ __device__ constexpr int steps_of(int bt) { return bt == PFA_F32 ? 4 : 4; }
 
 // The value of lane ^ MASK, 64 bits: a quad permute, or a swizzle.
 template <int MASK>
@@ -41,8 +43,28 @@ __device__ __forceinline__ double across(double x) {
   }
 }
 
+// One exchange of `spread`s: N sums of a lane become N / 2, or, where one is left,
+// the sum of both lanes'.
+template <int MASK, int N, int LP>
+__device__ __forceinline__ void spread(double* sum, int lane) {
+  if constexpr (MASK < LP) {
+    if constexpr (N > 1) {
+      const bool up = lane & MASK;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const double mine = up ? sum[N / 2 + i] : sum[i], other = up ? sum[i] : sum[N / 2 + i];
+        sum[i] = mine + across<MASK>(other);
+      }
+      spread<2 * MASK, N / 2, LP>(sum, lane);
+    } else {
+      sum[0] += across<MASK>(sum[0]);
+      spread<2 * MASK, 1, LP>(sum, lane);
+    }
+  }
+}
+
 // Scores.  D / 8 lanes hold a page's two bounds of a head, eight channels each,
-// of kSteps pages at once, and go over the query heads; sums are 64 bits, so
+// of `steps_of` pages at once, and go over the query heads; sums are 64 bits, so
 // that the order of the summands decides nothing that is not equal to 2^-53:
 // with bf16 or f16 values the sums are as good as always exact.  The bounds are
 // read once for all heads of a group; a channel is a select, a widening and a
@@ -62,74 +84,97 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
   constexpr int PW = kWave / LP;  // pages of a wave at once
   using BoundT = typename Elem<BT>::T;
   const int tid = threadIdx.x, lane = tid & 63, part = lane % LP;
-  const int page0 = base + (tid >> 6) * kSteps * PW + lane / LP;  // of step s: + s * PW
-  float lo[kSteps][8], hi[kSteps][8];
-  bool have[kSteps];
+  constexpr int STEPS = steps_of(BT);
+  const int page0 = base + (tid >> 6) * STEPS * PW + lane / LP;  // of step s: + s * PW
+  // the first heads' queries, on their way before the bounds are waited for
+  constexpr int QN = kScoreHeads * D / (WAVES * kWave) > 0 ? kScoreHeads * D / (WAVES * kWave) : 1;
+  float qr[QN];
+  auto load_q = [&](int g0, int heads) {
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
+    for (int u = 0; u < QN; ++u) {
+      const int i = tid + u * WAVES * kWave;
+      qr[u] = i < heads * D ? load_f<QT>(q + (int64_t)(h * G + g0 + i / D) * q_h + i % D) : 0.0f;
+    }
+  };
+  auto store_q = [&](int heads) {
+#pragma unroll
+    for (int u = 0; u < QN; ++u) {
+      const int i = tid + u * WAVES * kWave;
+      if (i < heads * D) qs[i / D][i % D] = qr[u];
+    }
+  };
+  const int heads0 = G < kScoreHeads ? G : kScoreHeads;
+  int id[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
     const int page = page0 + s * PW;
-    const int id = page >= sp.p0 && page < sp.pe ? ids[page] : -1;
-    have[s] = (uint32_t)id < (uint32_t)pg.n_pages;
-    const BoundT* at = (const BoundT*)pg.bounds + ((int64_t)(have[s] ? id : 0) * pg.H + h) * 2 * D + 8 * part;
+    id[s] = page >= sp.p0 && page < sp.pe ? ids[page] : -1;
+  }
+  load_q(0, heads0);
+  float lo[STEPS][8], hi[STEPS][8];
+  bool have[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    have[s] = (uint32_t)id[s] < (uint32_t)pg.n_pages;
+    const BoundT* at = (const BoundT*)pg.bounds + ((int64_t)(have[s] ? id[s] : 0) * pg.H + h) * 2 * D + 8 * part;
     load8<BT>(at, lo[s]);
     load8<BT>(at + D, hi[s]);
   }
-  // after the exchanges a lane holds the sums of KEEP steps
-  constexpr int KEEP = LP == 2 ? 2 : 1;
+  // NV sums of a lane, heads first; each exchange leaves a lane half of them, until
+  // one is left or the lanes are through: KEEP of them, from value `mine` on
+  constexpr int NV = kPair * STEPS, SPLITS = LP >= NV ? NV : LP, KEEP = NV / SPLITS;
   float best[KEEP];
   bool nan[KEEP];
 #pragma unroll
   for (int s = 0; s < KEEP; ++s) best[s] = -INFINITY, nan[s] = false;
-  const bool odd = lane & 1, upper = lane & 2;
   for (int g0 = 0; g0 < G; g0 += kScoreHeads) {
     const int heads = G - g0 < kScoreHeads ? G - g0 : kScoreHeads;
+    if (g0 > 0) load_q(g0, heads);
     __syncthreads();
-    for (int i = tid; i < heads * D; i += WAVES * kWave)
-      qs[i / D][i % D] = load_f<QT>(q + (int64_t)(h * G + g0 + i / D) * q_h + i % D);
+    store_q(heads);
     __syncthreads();
-    for (int g = 0; g < heads; ++g) {
-      double sum[kSteps] = {};
+    for (int g = 0; g < heads; g += kPair) {
+      double sum[NV] = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = qs[g][8 * part + i];
-        const bool up = x > 0.0f;
-        const double xd = x;
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) sum[s] = fma(xd, (double)(up ? hi[s][i] : lo[s][i]), sum[s]);
-      }
-      // lanes 2a, 2a + 1 share the steps out, then pairs of pairs
-      double r[2];
+        for (int u = 0; u < kPair; ++u) {
+          const float x = qs[g + u < heads ? g + u : heads - 1][8 * part + i];  // an odd last head counts twice
+          const bool up = x > 0.0f;
+          const double xd = x;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const double mine = odd ? sum[2 + s] : sum[s], other = odd ? sum[s] : sum[2 + s];
-        r[s] = mine + across<1>(other);
-      }
-      double t[KEEP];
-      if constexpr (LP == 2) {
-        t[0] = r[0], t[1] = r[1];
-      } else {
-        const double mine = upper ? r[1] : r[0], other = upper ? r[0] : r[1];
-        t[0] = mine + across<2>(other);
-        if constexpr (LP > 4) t[0] += across<4>(t[0]);
-        if constexpr (LP > 8) t[0] += across<8>(t[0]);
-      }
+          for (int s = 0; s < STEPS; ++s)
+            sum[u * STEPS + s] = fma(xd, (double)(up ? hi[s][i] : lo[s][i]), sum[u * STEPS + s]);
+        }
+      spread<1, NV, LP>(sum, lane);
 #pragma unroll
       for (int s = 0; s < KEEP; ++s) {
-        const float f = (float)t[s];
+        const float f = (float)sum[s];
         nan[s] = nan[s] || f != f;
         best[s] = fmaxf(best[s], f);
       }
     }
   }
-  if (part >= 4) return;
+  // value of sum[0]: lane bit 0 chose between halves, bit 1 between quarters, ...
+  int mine = 0;
+#pragma unroll
+  for (int o = 1; o < SPLITS; o <<= 1) mine += part & o ? NV / (2 * o) : 0;
+  if constexpr (kPair == 2) {
+#pragma unroll
+    for (int s = 0; s < KEEP; ++s) {
+      best[s] = fmaxf(best[s], __shfl_xor(best[s], 1));
+      nan[s] = nan[s] | (bool)__shfl_xor((int)nan[s], 1);
+    }
+  }
+  if (part >= SPLITS || mine >= STEPS) return;
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
-    const int s = LP == 2 ? 2 * odd + k : 2 * odd + upper;
+    const int s = mine + k;
     const int page = page0 + s * PW;
-    if (page < sp.p0 || page >= sp.pe) continue;
+    if (s >= STEPS || page < sp.p0 || page >= sp.pe) continue;
     bool ok = false;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) ok = i == s ? have[i] : ok;
+    for (int i = 0; i < STEPS; ++i) ok = i == s ? have[i] : ok;
     uint32_t u = __float_as_uint(best[k]);
     u = u & 0x80000000u ? ~u : u | 0x80000000u;  // -inf is 0x007fffff, +inf 0xff800000
     if (nan[k]) u = kNan;
@@ -139,7 +184,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
 }
 
 // Pages of a workgroup of `waves` waves at once.
-__host__ __device__ constexpr int score_span(int waves, int D) { return waves * (kWave / (D / 8)) * kSteps; }
+__host__ __device__ constexpr int score_span(int waves, int D, int bt) { return waves * (kWave / (D / 8)) * steps_of(bt); }
 
 template <int QT, int BT, int D>
 __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __restrict__ table, int64_t table_stride,
@@ -149,8 +194,8 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
                                                     int64_t row_keys, uint32_t* __restrict__ keys) {
   const int b = blockIdx.z, h = blockIdx.x;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
-  const int base = blockIdx.y * score_span(4, D);
-  if (base >= sp.pe || base + score_span(4, D) <= sp.p0) return;
+  const int base = blockIdx.y * score_span(4, D, BT);
+  if (base >= sp.pe || base + score_span(4, D, BT) <= sp.p0) return;
   __shared__ float qs[kScoreHeads][D];
   uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
   score_pages<QT, BT, D, 4>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
@@ -351,7 +396,7 @@ __global__ void __launch_bounds__(1024) select_kernel(Pages pg, const int32_t* _
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
   __shared__ uint32_t keys[kFused];
-  for (int base = sp.p0; base < sp.pe; base += score_span(16, D))
+  for (int base = sp.p0; base < sp.pe; base += score_span(16, D, BT))
     score_pages<QT, BT, D, 16>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
                                [&](int page, uint32_t key) { keys[page - sp.p0] = key; });
   __syncthreads();
