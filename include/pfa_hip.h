@@ -672,7 +672,7 @@ typedef struct pfa_kv_pages {
  * a page's head, where the pool has them: those of the written keys as they
  * are stored (a NaN among them gives NaN), joined with what stood there
  * unless the page is written from its first slot on. */
-int pfa_kv_pages_write(const pfa_kv_pages* pages, pfa_tensor4 k, pfa_tensor4 v, int dtype,
+int pfa_kv_pages_write(const pfa_kv_pages* pages, const pfa_tensor4* k, const pfa_tensor4* v, int dtype,
                        int B, int64_t n, const int32_t* table, int64_t table_stride,
                        int table_pages, const int32_t* starts, const int32_t* counts,
                        void* stream);
@@ -699,7 +699,7 @@ int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t
 int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
                                   int cell_dtype, int table_pages, int n_selected,
                                   size_t* bytes);
-int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages,
+int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
                        const int32_t* table, int64_t table_stride, int table_pages,
                        const int32_t* lengths, const int32_t* starts,
                        const int32_t* selected, int n_selected, float scale, void* out,
@@ -714,7 +714,7 @@ int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_page
  * lengths[b] - 1 come before all others, then the better score, then the
  * lower entry; entries without a page are never chosen. */
 int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes);
-int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages,
+int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
                         const int32_t* table, int64_t table_stride, int table_pages,
                         const int32_t* lengths, const int32_t* starts, int count, int first,
                         int last, int32_t* chosen, void* workspace, size_t ws_bytes,

@@ -245,7 +245,7 @@ int types_check(int dt, int ct) {
 
 using namespace pfa;
 
-extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, pfa_tensor4 k, pfa_tensor4 v, int dtype, int B, int64_t n,
+extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, const pfa_tensor4* k, const pfa_tensor4* v, int dtype, int B, int64_t n,
                                   const int32_t* table, int64_t table_stride, int table_pages, const int32_t* starts,
                                   const int32_t* counts, void* stream) {
   clear_error();
@@ -255,7 +255,7 @@ extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, pfa_tensor4 k, pfa_
   if (int rc = types_check(dtype, pages->dtype)) return rc;
   PFA_CHECK_ARG(n >= 0 && n <= (1 << 26), "kv_pages_write: 0 <= n <= 2^26 tokens");
   if (B == 0 || n == 0 || table_pages == 0) return PFA_OK;
-  PFA_CHECK_ARG(k.ptr && v.ptr && starts, "kv_pages_write: null argument");
+  PFA_CHECK_ARG(k && v && k->ptr && v->ptr && starts, "kv_pages_write: null argument");
   const int D = pages->head_dim;
   const int e = cell_bytes(dtype);
   auto rows = [&](const pfa_tensor4& x) {
@@ -267,7 +267,7 @@ extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, pfa_tensor4 k, pfa_
   const int threads = at_once <= 64 ? 64 : at_once <= 128 ? 128 : 256;
   by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
     write_kernel<decltype(dt)::value, decltype(ct)::value>
-        <<<dim3((unsigned)touched, p.H, B), threads, 0, as_stream(stream)>>>(p, t, rows(k), rows(v), D, n, starts,
+        <<<dim3((unsigned)touched, p.H, B), threads, 0, as_stream(stream)>>>(p, t, rows(*k), rows(*v), D, n, starts,
                                                                              counts);
   });
   PFA_CHECK_LAUNCH("kv_pages_write");
@@ -313,13 +313,13 @@ extern "C" int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, co
 
 namespace {
 
-int query_check(const char* what, const pfa_tensor4& q, int dtype, int B, int H, const pfa_kv_pages* pages,
+int query_check(const char* what, const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
                 const int32_t* lengths) {
   if (int rc = types_check(dtype, pages->dtype)) return rc;
   PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages->kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
                 pages->kv_heads);
   PFA_CHECK_ARG((int64_t)B * H <= 1 << 21, "%s: up to 2^21 rows (got %d x %d)", what, B, H);
-  PFA_CHECK_ARG(B == 0 || (q.ptr && lengths), "%s: null argument", what);
+  PFA_CHECK_ARG(B == 0 || (q && q->ptr && lengths), "%s: null argument", what);
   return PFA_OK;
 }
 
@@ -335,7 +335,7 @@ extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table
   return PFA_OK;
 }
 
-extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
+extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
                                    int64_t table_stride, int table_pages, const int32_t* lengths,
                                    const int32_t* starts, int count, int first, int last, int32_t* chosen,
                                    void* workspace, size_t ws_bytes, void* stream) {
@@ -359,16 +359,16 @@ extern "C" int pfa_kv_pages_select(pfa_tensor4 q, int dtype, int B, int H, const
   const int D = pages->head_dim, P = table_pages, rows = B * p.H;
   by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
     constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
-    const auto* qp = (const typename Elem<QT>::T*)q.ptr;
+    const auto* qp = (const typename Elem<QT>::T*)q->ptr;
     auto launch = [&](auto width) {
       constexpr int W = decltype(width)::value;
       if (P <= kFused)
-        select_kernel<QT, BT, W><<<rows, 1024, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q.s_b, q.s_h,
+        select_kernel<QT, BT, W><<<rows, 1024, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h,
                                                                        H / p.H, lengths, starts, first, last, count,
                                                                        chosen);
       else
         score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W, BT) - 1) / score_span(4, W, BT), B), 256, 0,
-                                  as_stream(stream)>>>(p, table, table_stride, P, qp, q.s_b, q.s_h, H / p.H, lengths,
+                                  as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths,
                                                        starts, first, last, row_keys(P), keys);
     };
     if (D == 16) launch(std::integral_constant<int, 16>{});
@@ -402,7 +402,7 @@ extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int pag
   return PFA_OK;
 }
 
-extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
+extern "C" int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
                                   int64_t table_stride, int table_pages, const int32_t* lengths, const int32_t* starts,
                                   const int32_t* selected, int n_selected, float scale, void* out, void* workspace,
                                   size_t ws_bytes, void* stream) {
@@ -424,7 +424,7 @@ extern "C" int pfa_paged_attn_fwd(pfa_tensor4 q, int dtype, int B, int H, const 
     set_error("paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, plan.bytes);
     return PFA_E_WORKSPACE;
   }
-  const AttendCall a{p, table, table_stride, table_pages, B, H, pages->head_dim, q, lengths, starts, selected, S, c, out,
+  const AttendCall a{p, table, table_stride, table_pages, B, H, pages->head_dim, *q, lengths, starts, selected, S, c, out,
                      (float*)workspace, as_stream(stream)};
   if (pages->dtype == PFA_I8) attend_i8(dtype, a);
   else if (pages->dtype == PFA_E4M3) attend_e4m3(dtype, a);

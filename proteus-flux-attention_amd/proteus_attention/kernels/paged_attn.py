@@ -78,8 +78,9 @@ def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *
     return KVPages(k, v, *scales, kb)
 
 
-# pfa_kv_pages of include/pfa_hip.h
+# pfa_kv_pages and pfa_tensor4 of include/pfa_hip.h
 _POOL = struct.Struct("PPPPPqqiiiii4x")
+_TENSOR4 = struct.Struct("Pqqq")
 
 
 def _dense(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, name: str) -> int:
@@ -145,24 +146,22 @@ def _device(what: str, *tensors: Optional[torch.Tensor]) -> int:
     return index
 
 
-class _OnDevice:
-    """Makes a device the current one for a call, where it is not."""
+def _call(index: int, name: str, fn, *args) -> None:
+    """fn(*args, stream) on a device's current stream, the device the current one
+    for the call where it is not."""
 
-    __slots__ = ("index", "before")
-
-    def __init__(self, index: int) -> None:
-        self.index = index
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        self.before = -1 if now == self.index else now
-        if self.before >= 0:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before >= 0:
-            torch.cuda.set_device(self.before)
-        return False
+    now = torch._C._cuda_getDevice()
+    if now != index:
+        with torch.cuda.device(index):
+            return _call(index, name, fn, *args)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if _hip.TIMER.enabled:
+        with _hip.TIMER.timed(name):
+            rc = fn(*args, stream)
+    else:
+        rc = fn(*args, stream)
+    if rc:
+        _hip.check(rc, fn.__name__)
 
 
 @functools.lru_cache(maxsize=256)
@@ -229,13 +228,10 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     if vs[3] != 1:
         v = v.contiguous()
         vs = v.stride()
-    with _OnDevice(index), _hip.TIMER.timed("kv_pages_write"):
-        rc = _hip.lib().pfa_kv_pages_write(
-            pool, _hip.Tensor4(k.data_ptr(), ks[0], ks[2], ks[1]), _hip.Tensor4(v.data_ptr(), vs[0], vs[2], vs[1]), tag,
-            B, n, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(),
-            None if counts is None else counts.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _hip.check(rc, "pfa_kv_pages_write")
+    _call(index, "kv_pages_write", _hip.lib().pfa_kv_pages_write, pool,
+          _TENSOR4.pack(k.data_ptr(), ks[0], ks[2], ks[1]), _TENSOR4.pack(v.data_ptr(), vs[0], vs[2], vs[1]), tag, B, n,
+          table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(),
+          None if counts is None else counts.data_ptr())
 
 
 def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tensor, counts: Optional[torch.Tensor],
@@ -261,13 +257,9 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     device = table.device
     k = torch.empty((B, n, H, D), dtype=dtype, device=device)
     v = torch.empty((B, n, H, D), dtype=dtype, device=device)
-    with _OnDevice(index), _hip.TIMER.timed("kv_pages_read"):
-        rc = _hip.lib().pfa_kv_pages_read(
-            pool, B, n, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(),
-            None if counts is None else counts.data_ptr(), k.data_ptr(), v.data_ptr(), tag,
-            torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        _hip.check(rc, "pfa_kv_pages_read")
+    _call(index, "kv_pages_read", _hip.lib().pfa_kv_pages_read, pool, B, n, table.data_ptr(), table.stride(0),
+          table.shape[1], starts.data_ptr(), None if counts is None else counts.data_ptr(), k.data_ptr(), v.data_ptr(),
+          tag)
     return k, v
 
 
@@ -302,7 +294,7 @@ class _Query:
             q = q.contiguous()
             s = q.stride()
         self.q = q
-        self.args = (_hip.Tensor4(q.data_ptr(), s[0], s[1], 0), tag, B, H, pool, table.data_ptr(), table.stride(0),
+        self.args = (_TENSOR4.pack(q.data_ptr(), s[0], s[1], 0), tag, B, H, pool, table.data_ptr(), table.stride(0),
                      self.P, lengths.data_ptr(), None if starts is None else starts.data_ptr())
 
 
@@ -322,12 +314,9 @@ def _attend(a: _Query, selected: Optional[torch.Tensor], scale: Optional[float])
     device = a.table.device
     ws, ws_ptr = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
     out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
-    with _OnDevice(a.index), _hip.TIMER.timed("paged_attn_fwd"):
-        rc = _hip.lib().pfa_paged_attn_fwd(*a.args, None if selected is None else selected.data_ptr(), S, scale,
-                                           out.data_ptr(), ws_ptr, 0 if ws is None else ws.numel(),
-                                           torch._C._cuda_getCurrentRawStream(a.index))
-    if rc:
-        _hip.check(rc, "pfa_paged_attn_fwd")
+    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, *a.args,
+          None if selected is None else selected.data_ptr(), S, scale, out.data_ptr(), ws_ptr,
+          0 if ws is None else ws.numel())
     return out
 
 
@@ -370,12 +359,8 @@ def _select(a: _Query, count: int, first: int, last: int) -> torch.Tensor:
     device = a.table.device
     ws, ws_ptr = _scratch(_select_bytes(a.B, a.Hkv, a.P), device)
     chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
-    with _OnDevice(a.index), _hip.TIMER.timed("kv_pages_select"):
-        rc = _hip.lib().pfa_kv_pages_select(*a.args, count, first, last, chosen.data_ptr(), ws_ptr,
-                                            0 if ws is None else ws.numel(),
-                                            torch._C._cuda_getCurrentRawStream(a.index))
-    if rc:
-        _hip.check(rc, "pfa_kv_pages_select")
+    _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, *a.args, count, first, last, chosen.data_ptr(),
+          ws_ptr, 0 if ws is None else ws.numel())
     return chosen
 
 

@@ -108,7 +108,7 @@ def _c_pool(**kw):
 
 def test_c_entries_refuse_before_any_launch():
     lib = _hip.lib()
-    t4 = _hip.Tensor4(256, 64, 32, 32)
+    t4 = struct.pack("Pqqq", 256, 64, 32, 32)
     p = ctypes.c_void_p(256)  # never dereferenced
 
     def attend(pool, q=t4, tag=_hip.PFA_F32, B=1, H=2, P=2, n=-1, out=p, lengths=p):
