@@ -679,8 +679,8 @@ int pfa_kv_pages_write(const pfa_kv_pages* pages, const pfa_tensor4* k, const pf
 
 /* Positions starts[b] .. starts[b] + counts[b] - 1 (counts NULL: n of them)
  * of every sequence as values, k_out and v_out (B, n, kv_heads, head_dim) in
- * out_dtype: cell * scale rounded once.  Rows i >= counts[b], and those
- * without a page, are zero. */
+ * out_dtype: cell * scale in f32, then rounded to it.  Rows i >= counts[b], and
+ * those without a page, are zero. */
 int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t* table,
                       int64_t table_stride, int table_pages, const int32_t* starts,
                       const int32_t* counts, void* k_out, void* v_out, int out_dtype,

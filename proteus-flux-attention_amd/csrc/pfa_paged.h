@@ -49,6 +49,11 @@ __device__ __forceinline__ int64_t length_at(const int32_t* lengths, const Table
   return n < 0 ? 0 : n < most ? n : most;
 }
 
+// a / b of positive numbers, in 32 bits where they are enough.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // One e4m3 cell as f32: v_cvt_f32_fp8 (OCP form on gfx950).
 __device__ __forceinline__ float e4m3_to_f32(uint8_t b) { return __builtin_amdgcn_cvt_f32_fp8((int)b, 0); }
 

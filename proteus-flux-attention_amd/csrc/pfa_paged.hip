@@ -56,9 +56,29 @@ namespace {
 // store, the page's bounds in registers over the rows and joined over the
 // lanes and waves at the end, so no atomics and the same bits in any split of
 // the tokens over calls.
+//
+// A copy's bytes bound it, if the arithmetic stays out of the way: quotients by
+// the row's scale come from its one reciprocal with two corrections by fused
+// multiply-adds (Markstein 1990), the same bits as a division in 5 instructions
+// for 11, and int8 from the sum with 1.5 * 2^23, whose low bits are the rounded
+// quotient.  25,600 rows of 8 heads of 128 bf16 values into int8 pages with bounds:
+// 41 to 52 us, 162 MB (58 with divisions and selects for NaN).
 // ---------------------------------------------------------------------
-__device__ __forceinline__ float min_nan(float a, float b) { return a != a || a < b ? a : b; }
-__device__ __forceinline__ float max_nan(float a, float b) { return a != a || a > b ? a : b; }
+__device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The largest over 2, 4, 8 or 16 lanes that lie together.
+template <int LANES>
+__device__ __forceinline__ float max_lanes(float x) {
+  auto step = [&](auto ctrl) {
+    x = max_nan(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)));
+  };
+  step(std::integral_constant<int, 0xB1>{});                             // the neighbour
+  if constexpr (LANES > 2) step(std::integral_constant<int, 0x4E>{});   // the other pair
+  if constexpr (LANES > 4) step(std::integral_constant<int, 0x141>{});  // mirrored in eight
+  if constexpr (LANES > 8) step(std::integral_constant<int, 0x140>{});  // mirrored in sixteen
+  return x;
+}
 
 struct NewRows {
   const void* p;
@@ -77,148 +97,197 @@ __device__ __forceinline__ void row8(const NewRows& r, int64_t at, float (&o)[8]
   }
 }
 
-// Eight values of a row of `lanes` lanes into its cells; x comes back as the
-// values that the cells stand for.
-template <int DT, int CT>
-__device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at, bool first, int lanes, float (&x)[8]) {
+// Eight values of a row of LANES lanes into its cells; with `back`, x comes back as
+// the values that the cells stand for.
+template <int CT, int LANES>
+__device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at, bool first, bool back, float (&x)[8]) {
   if constexpr (!is8(CT)) {
     store8<CT>(dst, x);
   } else {
     float m = 0.0f;
-    bool finite = true;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      m = fmaxf(m, fabsf(x[i]));
-      finite = finite && fabsf(x[i]) < INFINITY;
-    }
-    if (!finite) m = INFINITY;
-    for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
+    m = max_lanes<LANES>(m);
     const bool ok = m < INFINITY;
     const float s = ok ? fmaxf(m / top_of(CT), kLeastScale) : __builtin_nanf("");
     if (first) *scale_at = s;
-    uint32_t w[2] = {0, 0};
+    // x / s to nearest: s >= 1e-6 and at most 448 in size, so that nothing that
+    // decides a cell underflows
+    const float y = 1.0f / s;
+    float c[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float c[4];
+    for (int i = 0; i < 8; ++i) {
+      float q = x[i] * y;
+      q = fmaf(fmaf(-q, s, x[i]), y, q);
+      q = fmaf(fmaf(-q, s, x[i]), y, q);
+      c[i] = ok ? q : 0.0f;
+    }
+    uint32_t w[2];
+    if constexpr (CT == PFA_I8) {
+      constexpr float kRound = 12582912.0f;  // 1.5 * 2^23
+      uint32_t u[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = ok ? x[4 * i + j] / s : 0.0f;
-      if constexpr (CT == PFA_I8) {
+      for (int i = 0; i < 8; ++i) {
+        const float r = c[i] + kRound;
+        u[i] = __float_as_uint(r);
+        if (back) x[i] = (r - kRound) * s;
+      }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float r = rintf(c[j]);
-          w[i] |= ((uint32_t)(int)r & 0xffu) << (8 * j);
-          x[4 * i + j] = r * s;
-        }
-      } else {
-        int p = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
-        p = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], p, true);
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t a = __builtin_amdgcn_perm(u[4 * i + 1], u[4 * i], 0x0c0c0400);
+        const uint32_t b = __builtin_amdgcn_perm(u[4 * i + 3], u[4 * i + 2], 0x0c0c0400);
+        w[i] = a | b << 16;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * i], c[4 * i + 1], 0, false);
+        p = __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * i + 2], c[4 * i + 3], p, true);
         w[i] = (uint32_t)p;
-        x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(p, 0) * s;
-        x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(p, 1) * s;
-        x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(p, 2) * s;
-        x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(p, 3) * s;
+        if (back) {
+          x[4 * i] = __builtin_amdgcn_cvt_f32_fp8(p, 0) * s;
+          x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(p, 1) * s;
+          x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(p, 2) * s;
+          x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(p, 3) * s;
+        }
       }
     }
     *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
   }
 }
 
-template <int DT, int CT>
-__global__ void __launch_bounds__(256) write_kernel(Pages pg, Table tab, NewRows k, NewRows v, int D, int64_t n,
+template <int DT, int CT, int D>
+__global__ void __launch_bounds__(256) write_kernel(Pages pg, Table tab, NewRows k, NewRows v, int64_t n,
+                                                    int64_t units,
                                                     const int32_t* __restrict__ starts,
                                                     const int32_t* __restrict__ counts) {
   using CellT = typename Cell<CT>::T;
-  const int64_t b = blockIdx.z;
-  const int h = blockIdx.y;
+  constexpr int LANES = D / 8;
+  const int64_t b = blockIdx.y;
   const int64_t start = starts[b];
   int64_t count = counts ? (int64_t)counts[b] : n;
   count = count < 0 ? 0 : count < n ? count : n;
   const int64_t first = start < 0 ? 0 : start;  // positions written: [first, end)
   const int64_t end = start + count;
-  const int64_t ordinal = (first >> pg.shift) + blockIdx.x;
-  const int64_t base = ordinal << pg.shift;
-  const int64_t from = first > base ? first : base, to = end < base + pg.ps ? end : base + pg.ps;
-  if (from >= to) return;
-  const int id = page_at(tab, pg, b, ordinal);
-  if (id < 0) return;
+  const int lane = threadIdx.x % LANES, rows = blockDim.x / LANES, wave = threadIdx.x / kWave;
+  const bool back = pg.bounds != nullptr;
+  __shared__ float part[2][4][D];
+  // heads of one page are neighbours, as their new rows are in memory
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const int64_t touched = quotient(unit, pg.H);
+    const int h = (int)(unit - touched * pg.H);
+    const int64_t ordinal = (first >> pg.shift) + touched, base = ordinal << pg.shift;
+    const int64_t from = first > base ? first : base, to = end < base + pg.ps ? end : base + pg.ps;
+    if (from >= to) continue;
+    const int id = page_at(tab, pg, b, ordinal);
+    if (id < 0) continue;
 
-  const int lanes = D / 8, rows = blockDim.x / lanes;
-  const int lane = threadIdx.x % lanes, row = threadIdx.x / lanes;
-  const int64_t kpage = id * pg.k_page + (int64_t)h * pg.ps * D, vpage = id * pg.v_page + (int64_t)h * pg.ps * D;
-  const int64_t spage = ((int64_t)id * pg.H + h) * pg.ps;
-  float lo[8], hi[8];
+    const int64_t kpage = id * pg.k_page + (int64_t)h * pg.ps * D, vpage = id * pg.v_page + (int64_t)h * pg.ps * D;
+    const int64_t spage = ((int64_t)id * pg.H + h) * pg.ps;
+    const int64_t k_at = b * k.s_b + h * k.s_h + 8 * lane, v_at = b * v.s_b + h * v.s_h + 8 * lane;
+    float lo[8], hi[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-  for (int64_t pos = from + row; pos < to; pos += rows) {
-    const int slot = (int)(pos - base);
-    const int64_t i = pos - start;
-    float x[8], y[8];
-    row8<DT>(k, b * k.s_b + h * k.s_h + i * k.s_t + 8 * lane, x);
-    row8<DT>(v, b * v.s_b + h * v.s_h + i * v.s_t + 8 * lane, y);
-    put8<DT, CT>((CellT*)pg.k + kpage + slot * D + 8 * lane, pg.k_scale + spage + slot, lane == 0, lanes, x);
-    put8<DT, CT>((CellT*)pg.v + vpage + slot * D + 8 * lane, pg.v_scale + spage + slot, lane == 0, lanes, y);
+    for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+    for (int64_t pos = from + threadIdx.x / LANES; pos < to; pos += rows) {
+      const int slot = (int)(pos - base);
+      const int64_t i = pos - start;
+      float x[8], y[8];
+      row8<DT>(k, k_at + i * k.s_t, x);
+      row8<DT>(v, v_at + i * v.s_t, y);
+      put8<CT, LANES>((CellT*)pg.k + kpage + slot * D + 8 * lane, pg.k_scale + spage + slot, lane == 0, back, x);
+      put8<CT, LANES>((CellT*)pg.v + vpage + slot * D + 8 * lane, pg.v_scale + spage + slot, lane == 0, false, y);
+      if (back) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], x[j]), hi[j] = max_nan(hi[j], x[j]);
-  }
-  if (!pg.bounds) return;
-  __shared__ float part[2][4][128];
-  for (int o = lanes; o < kWave; o <<= 1) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo[j] = min_nan(lo[j], __shfl_xor(lo[j], o));
-      hi[j] = max_nan(hi[j], __shfl_xor(hi[j], o));
+        for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], x[j]), hi[j] = max_nan(hi[j], x[j]);
+      }
     }
-  }
-  const int wave = threadIdx.x / kWave;
-  if (threadIdx.x % kWave < lanes) {
+    if (!back) continue;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) part[0][wave][8 * lane + j] = lo[j], part[1][wave][8 * lane + j] = hi[j];
-  }
-  __syncthreads();
-  constexpr int BT = bound_dtype(CT);
-  using BoundT = typename Elem<BT>::T;
-  BoundT* out = (BoundT*)pg.bounds + ((int64_t)id * pg.H + h) * 2 * D;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float a = part[0][0][d], z = part[1][0][d];
-    for (int w = 1; w < (int)blockDim.x / kWave; ++w) a = min_nan(a, part[0][w][d]), z = max_nan(z, part[1][w][d]);
-    if (from > base) a = min_nan(a, load_f<BT>(out + d)), z = max_nan(z, load_f<BT>(out + D + d));
-    store_f<BT>(out + d, a);
-    store_f<BT>(out + D + d, z);
+    for (int o = LANES; o < kWave; o <<= 1) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lo[j] = min_nan(lo[j], __shfl_xor(lo[j], o));
+        hi[j] = max_nan(hi[j], __shfl_xor(hi[j], o));
+      }
+    }
+    if (threadIdx.x % kWave < LANES) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[0][wave][8 * lane + j] = lo[j], part[1][wave][8 * lane + j] = hi[j];
+    }
+    __syncthreads();
+    constexpr int BT = bound_dtype(CT);
+    using BoundT = typename Elem<BT>::T;
+    BoundT* out = (BoundT*)pg.bounds + ((int64_t)id * pg.H + h) * 2 * D;
+    for (int d = threadIdx.x; d < D; d += blockDim.x) {
+      float a = part[0][0][d], z = part[1][0][d];
+      for (int w = 1; w < (int)blockDim.x / kWave; ++w) a = min_nan(a, part[0][w][d]), z = max_nan(z, part[1][w][d]);
+      if (from > base) a = min_nan(a, load_f<BT>(out + d)), z = max_nan(z, load_f<BT>(out + D + d));
+      store_f<BT>(out + d, a);
+      store_f<BT>(out + D + d, z);
+    }
+    __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------
-// Read: eight values a thread.
+// Read: eight values a thread and row, one row or two of each of k and v at
+// once, rows in the output's order.  A copy's bytes bound it.  The place of a workgroup's
+// first row is divided out once for all its threads.
 // ---------------------------------------------------------------------
-template <int CT, int OT>
-__global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int D, int64_t n, int64_t total,
+// 262,144 rows of 8 heads of 128 e4m3 cells into bf16: two rows 305 us, one 320;
+// 25,600 of int8 into f32: 67 and 59; 3,000 of 8 heads of 32 bf16: 5.0 and 4.2.
+__host__ __device__ constexpr int read_rows(int ct, int ot) { return is8(ct) && ot != PFA_F32 ? 2 : 1; }
+
+template <int CT, int OT, int D>
+__global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int64_t n, int64_t blocks,
                                                    const int32_t* __restrict__ starts,
-                                                   const int32_t* __restrict__ counts, void* k_out, void* v_out) {
+                                                   const int32_t* __restrict__ counts, void* __restrict__ k_out,
+                                                   void* __restrict__ v_out) {
   using CellT = typename Cell<CT>::T;
   using OutT = typename Elem<OT>::T;
-  const int lanes = D / 8;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
-    const int lane = (int)(at % lanes);
-    int64_t rest = at / lanes;
-    const int h = (int)(rest % pg.H);
-    rest /= pg.H;
-    const int64_t i = rest % n, b = rest / n;
-    const int64_t pos = starts[b] + i;
-    const int id = i < (counts ? (int64_t)counts[b] : n) && pos >= 0 ? page_at(tab, pg, b, pos >> pg.shift) : -1;
-    float x[8] = {}, y[8] = {};
-    if (id >= 0) {
-      const int64_t slot = (int64_t)h * pg.ps + (pos & (pg.ps - 1));
-      cells8<CT>((const CellT*)pg.k + id * pg.k_page + slot * D + 8 * lane, x);
-      cells8<CT>((const CellT*)pg.v + id * pg.v_page + slot * D + 8 * lane, y);
-      if constexpr (is8(CT)) {
-        const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
-        const float a = pg.k_scale[s], c = pg.v_scale[s];
+  constexpr int LANES = D / 8, ROWS = 256 / LANES, kReadRows = read_rows(CT, OT);
+  const int64_t b = blockIdx.y, rows = n * pg.H;
+  const int64_t start = starts[b];
+  int64_t count = counts ? (int64_t)counts[b] : n;
+  const int lane = threadIdx.x % LANES;
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const int64_t r0 = block * (ROWS * kReadRows), i0 = quotient(r0, pg.H);
+    const uint32_t h0 = (uint32_t)(r0 - i0 * pg.H);
+    float x[kReadRows][8], y[kReadRows][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= a, y[j] *= c;
+    for (int u = 0; u < kReadRows; ++u) {
+      const uint32_t at = threadIdx.x / LANES + u * ROWS;
+      const uint32_t skip = (h0 + at) / (uint32_t)pg.H;
+      const int h = (int)(h0 + at - skip * pg.H);
+      const int64_t i = i0 + skip, pos = start + i;
+      const int id = i < n && i < count && pos >= 0 ? page_at(tab, pg, b, pos >> pg.shift) : -1;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[u][j] = y[u][j] = 0.0f;
+      if (id >= 0) {
+        const int64_t slot = (int64_t)h * pg.ps + (pos & (pg.ps - 1));
+        cells8<CT>((const CellT*)pg.k + id * pg.k_page + slot * D + 8 * lane, x[u]);
+        cells8<CT>((const CellT*)pg.v + id * pg.v_page + slot * D + 8 * lane, y[u]);
+        if constexpr (is8(CT)) {
+          const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
+          const float a = pg.k_scale[s], c = pg.v_scale[s];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[u][j] *= a, y[u][j] *= c;
+            // f16: the product is rounded to f32 before its rounding to 16 bits, as
+            // with the other types (v_fma_mixlo_f16 would do with one)
+            if constexpr (OT == PFA_F16) asm("" : "+v"(x[u][j]), "+v"(y[u][j]));
+          }
+        }
       }
     }
-    store8<OT>((OutT*)k_out + 8 * at, x);
-    store8<OT>((OutT*)v_out + 8 * at, y);
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+      const int64_t r = r0 + threadIdx.x / LANES + u * ROWS;
+      if (r >= rows) continue;
+      const int64_t to = (b * rows + r) * D + 8 * lane;
+      store8<OT>((OutT*)k_out + to, x[u]);
+      store8<OT>((OutT*)v_out + to, y[u]);
+    }
   }
 }
 
@@ -232,6 +301,15 @@ void by_types(int dt, int ct, F&& f) {
   PFA_PAIR(PFA_F32, PFA_I8) PFA_PAIR(PFA_BF16, PFA_I8) PFA_PAIR(PFA_F16, PFA_I8)
   PFA_PAIR(PFA_F32, PFA_E4M3) PFA_PAIR(PFA_BF16, PFA_E4M3) PFA_PAIR(PFA_F16, PFA_E4M3)
 #undef PFA_PAIR
+}
+
+// Calls f with the head's width as a template argument.
+template <typename F>
+void by_width(int D, F&& f) {
+  if (D == 16) f(std::integral_constant<int, 16>{});
+  else if (D == 32) f(std::integral_constant<int, 32>{});
+  else if (D == 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
 }
 
 int types_check(int dt, int ct) {
@@ -265,10 +343,13 @@ extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, const pfa_tensor4* 
   const int64_t touched = (n + p.ps - 2) / p.ps + 1;
   const int64_t at_once = (n < p.ps ? n : p.ps) * (D / 8);
   const int threads = at_once <= 64 ? 64 : at_once <= 128 ? 128 : 256;
+  const int64_t units = touched * p.H;
+  const dim3 grid((unsigned)(units < (1 << 22) ? units : 1 << 22), B);
   by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
-    write_kernel<decltype(dt)::value, decltype(ct)::value>
-        <<<dim3((unsigned)touched, p.H, B), threads, 0, as_stream(stream)>>>(p, t, rows(*k), rows(*v), D, n, starts,
-                                                                             counts);
+    by_width(D, [&](auto width) {
+      write_kernel<decltype(dt)::value, decltype(ct)::value, decltype(width)::value>
+          <<<grid, threads, 0, as_stream(stream)>>>(p, t, rows(*k), rows(*v), n, units, starts, counts);
+    });
   });
   PFA_CHECK_LAUNCH("kv_pages_write");
   return PFA_OK;
@@ -288,12 +369,14 @@ extern "C" int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, co
   PFA_CHECK_ARG(k_out && v_out && starts && (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0,
                 "kv_pages_read: null or unaligned argument");
   const int D = pages->head_dim;
-  const int64_t total = (int64_t)B * n * p.H * (D / 8);
-  const int64_t blocks = (total + 255) / 256;
-  const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
   auto launch = [&](auto ct, auto ot) {
-    read_kernel<decltype(ct)::value, decltype(ot)::value>
-        <<<grid, 256, 0, as_stream(stream)>>>(p, t, D, n, total, starts, counts, k_out, v_out);
+    const int at_once = 256 / (D / 8) * read_rows(decltype(ct)::value, decltype(ot)::value);
+    const int64_t blocks = (n * p.H + at_once - 1) / at_once;
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20), B);
+    by_width(D, [&](auto width) {
+      read_kernel<decltype(ct)::value, decltype(ot)::value, decltype(width)::value>
+          <<<grid, 256, 0, as_stream(stream)>>>(p, t, n, blocks, starts, counts, k_out, v_out);
+    });
   };
   auto by_out = [&](auto ct) {
     if (out_dtype == PFA_F32) launch(ct, std::integral_constant<int, PFA_F32>{});
@@ -360,7 +443,7 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
   by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
     constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
     const auto* qp = (const typename Elem<QT>::T*)q->ptr;
-    auto launch = [&](auto width) {
+    by_width(D, [&](auto width) {
       constexpr int W = decltype(width)::value;
       if (P <= kFused)
         select_kernel<QT, BT, W><<<rows, 1024, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h,
@@ -370,11 +453,7 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
         score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W, BT) - 1) / score_span(4, W, BT), B), 256, 0,
                                   as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths,
                                                        starts, first, last, row_keys(P), keys);
-    };
-    if (D == 16) launch(std::integral_constant<int, 16>{});
-    else if (D == 32) launch(std::integral_constant<int, 32>{});
-    else if (D == 64) launch(std::integral_constant<int, 64>{});
-    else launch(std::integral_constant<int, 128>{});
+    });
   });
   // entries of a row from the first's four on: up to P + 3
 #define PFA_CHOOSE(THREADS, K, HELD)                                                                          \

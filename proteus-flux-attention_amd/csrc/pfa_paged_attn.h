@@ -409,11 +409,6 @@ __device__ __forceinline__ float part_weight(float m, float l, float top) {
 // workgroup with a dozen one-tile pairs was the last to end.
 constexpr int kStart = 8;
 
-// a / b of positive numbers, in 32 bits where they are enough.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
-
 struct Deal {
   int B, R, RT;      // sequences; pairs of one; pairs of one of its heads
   int S, shift, P;   // listed entries or -1; the pages
