@@ -157,7 +157,7 @@ __device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at,
 }
 
 template <int DT, int CT, int D>
-__global__ void __launch_bounds__(256) write_kernel(Pages pg, Table tab, NewRows k, NewRows v, int64_t n,
+__global__ void __launch_bounds__(1024) write_kernel(Pages pg, Table tab, NewRows k, NewRows v, int64_t n,
                                                     int64_t units,
                                                     const int32_t* __restrict__ starts,
                                                     const int32_t* __restrict__ counts) {
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256) write_kernel(Pages pg, Table tab, NewRows
   const int64_t end = start + count;
   const int lane = threadIdx.x % LANES, rows = blockDim.x / LANES, wave = threadIdx.x / kWave;
   const bool back = pg.bounds != nullptr;
-  __shared__ float part[2][4][D];
+  __shared__ float part[2][16][D];
   // heads of one page are neighbours, as their new rows are in memory
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const int64_t touched = quotient(unit, pg.H);
@@ -342,7 +342,10 @@ extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, const pfa_tensor4* 
   };
   const int64_t touched = (n + p.ps - 2) / p.ps + 1;
   const int64_t at_once = (n < p.ps ? n : p.ps) * (D / 8);
-  const int threads = at_once <= 64 ? 64 : at_once <= 128 ? 128 : 256;
+  // a page's rows at once where there are few pages, else four waves each
+  const int most = touched * p.H * B < 2048 ? 1024 : 256;
+  int threads = 64;
+  while (threads < at_once && threads < most) threads *= 2;
   const int64_t units = touched * p.H;
   const dim3 grid((unsigned)(units < (1 << 22) ? units : 1 << 22), B);
   by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
@@ -445,10 +448,12 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
     const auto* qp = (const typename Elem<QT>::T*)q->ptr;
     by_width(D, [&](auto width) {
       constexpr int W = decltype(width)::value;
-      if (P <= kFused)
-        select_kernel<QT, BT, W><<<rows, 1024, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h,
-                                                                       H / p.H, lengths, starts, first, last, count,
-                                                                       chosen);
+      if (P <= kFusedSmall)
+        select_kernel<QT, BT, W, 256><<<rows, 256, 0, as_stream(stream)>>>(
+            p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
+      else if (P <= kFused)
+        select_kernel<QT, BT, W, 1024><<<rows, 1024, 0, as_stream(stream)>>>(
+            p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else
         score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W, BT) - 1) / score_span(4, W, BT), B), 256, 0,
                                   as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths,

@@ -153,6 +153,17 @@ struct Tile {
       else b[2 * i + 1] = r.block(key + 16);
     }
   }
+  // the first of tiles t, t + kWaves, ... before `end` that has a key to see
+  __device__ __forceinline__ int find_seen(const Row& r, int t, int end) {
+    for (; t < end; t += kWaves) {
+      find(r, t);
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < 2 * F::NG; ++i) any = any || (b[i].pos < r.len && b[i].pos + 16 > r.start);
+      if (any) break;
+    }
+    return t;
+  }
   // whether all its keys are seen
   __device__ __forceinline__ bool whole(const Row& r) const {
     bool w = true;
@@ -595,14 +606,15 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
         entries[i] = Entry{ok ? id : 0, ok ? ordinal << deal.shift : kNowhere};
       }
       __syncthreads();
-      int t = r0 + wave;
+      Tile<F> cur, next;
+      int t = cur.find_seen(r, r0 + wave, re);
       if (t < re) {
-        Tile<F> cur, next;
-        cur.find(r, t);
         w.load_k(pg, h, cur);
-        next = cur;
-        for (; t < re; t += kWaves) {
-          if (t + kWaves < re) next.find(r, t + kWaves);
+        while (t < re) {
+          next = cur;
+          Tile<F> found;
+          t = found.find_seen(r, t + kWaves, re);
+          if (t < re) next = found;
           w.step(pg, r, h, c, cur, next, st);
           cur = next;
         }
@@ -652,8 +664,8 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   }
 }
 
-// Joins the parts of a row, a workgroup a row; writes the rows of sequences that
-// see nothing.  A team of min(D, 64) lanes takes every TEAMS-th part, eight parts'
+// Joins the parts of a pair's rows, a workgroup a row, or a pair where there are
+// many; writes the rows of sequences that see nothing.  A team of min(D, 64) lanes takes every TEAMS-th part, eight parts'
 // loads at once, and the teams are joined in LDS.
 template <int QT, int THREADS>
 __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float pscale,
@@ -664,57 +676,59 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
                                                        typename Elem<QT>::T* __restrict__ out) {
   const int tid = threadIdx.x;
   const int b = blockIdx.x / deal.R, pair = blockIdx.x % deal.R;
-  const int h = pair / deal.RT, row = blockIdx.y, head = h * G + 16 * (pair % deal.RT) + row;
-  if (head >= (h + 1) * G) return;
+  const int h = pair / deal.RT, head0 = h * G + 16 * (pair % deal.RT);
+  const int rows = G < 16 ? G : 16, here = (h + 1) * G - head0 < 16 ? (h + 1) * G - head0 : 16;
   const Shared who = shared[blockIdx.x];  // nobody's where the sequence has no tiles
-  typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head) * D;
+  typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head0) * D;
   if (deal.tiles(deal.begin(starts, b), deal.length(lengths, b)) == 0) {
-    for (int d = tid; d < D; d += THREADS) store_f<QT>(to + d, 0.0f);
+    for (int i = blockIdx.y * D + tid; i < here * D; i += THREADS * gridDim.y) store_f<QT>(to + i, 0.0f);
     return;
   }
   if (who.n == 1) return;  // written by its one workgroup
-  const int rows = G < 16 ? G : 16;
   const int lanes = D < kWave ? D : kWave, d = tid % lanes, team = tid / lanes, teams = THREADS / lanes;
   const bool two = D > kWave;
-  float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int i0 = team; i0 < who.n; i0 += 8 * teams) {
-    float m[8], l[8], x[8], y[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = i0 + u * teams;
-      const bool in = i < who.n;
-      // part i is workgroup first + i's
-      const float* s = parts + (2 * (int64_t)(who.first + (in ? i : 0)) + (!in || i == 0)) * rows * (D + 2);
-      m[u] = in ? s[rows * D + row] : -INFINITY, l[u] = in ? s[rows * (D + 1) + row] : 0.0f;
-      x[u] = s[row * D + d], y[u] = two ? s[row * D + 64 + d] : 0.0f;
-    }
-    float t = top;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) t = fmaxf(t, m[u]);
-    const float a = part_weight(top, sum, t);
-    o0 = a == 0.0f ? 0.0f : a * o0, o1 = a == 0.0f ? 0.0f : a * o1, sum = a == 0.0f ? 0.0f : a * sum;
-    top = t;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float w = part_weight(m[u], l[u], t);
-      if (w != 0.0f) o0 += w * x[u], o1 += w * y[u], sum += w * l[u];
-    }
-  }
   constexpr int TEAMS = THREADS / 16;  // at most
   __shared__ float acc[THREADS * 2], tops[TEAMS], suml[TEAMS];
-  acc[team * D + d] = o0;
-  if (two) acc[team * D + 64 + d] = o1;
-  if (d == 0) tops[team] = top, suml[team] = sum;
-  __syncthreads();
-  const int used = who.n < teams ? who.n : teams;
-  for (int c = tid; c < D; c += THREADS) {
-    float t = -INFINITY, o = 0.0f, l = 0.0f;
-    for (int w = 0; w < used; ++w) t = fmaxf(t, tops[w]);
-    for (int w = 0; w < used; ++w) {
-      const float a = part_weight(tops[w], suml[w], t);
-      if (a != 0.0f) o += a * acc[w * D + c], l += a * suml[w];
+  for (int row = blockIdx.y; row < here; row += gridDim.y) {
+    float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int i0 = team; i0 < who.n; i0 += 8 * teams) {
+      float m[8], l[8], x[8], y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * teams;
+        const bool in = i < who.n;
+        // part i is workgroup first + i's
+        const float* s = parts + (2 * (int64_t)(who.first + (in ? i : 0)) + (!in || i == 0)) * rows * (D + 2);
+        m[u] = in ? s[rows * D + row] : -INFINITY, l[u] = in ? s[rows * (D + 1) + row] : 0.0f;
+        x[u] = s[row * D + d], y[u] = two ? s[row * D + 64 + d] : 0.0f;
+      }
+      float t = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t = fmaxf(t, m[u]);
+      const float a = part_weight(top, sum, t);
+      o0 = a == 0.0f ? 0.0f : a * o0, o1 = a == 0.0f ? 0.0f : a * o1, sum = a == 0.0f ? 0.0f : a * sum;
+      top = t;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = part_weight(m[u], l[u], t);
+        if (w != 0.0f) o0 += w * x[u], o1 += w * y[u], sum += w * l[u];
+      }
     }
-    store_f<QT>(to + c, l == 0.0f ? 0.0f : o / (l * pscale));
+    acc[team * D + d] = o0;
+    if (two) acc[team * D + 64 + d] = o1;
+    if (d == 0) tops[team] = top, suml[team] = sum;
+    __syncthreads();
+    const int used = who.n < teams ? who.n : teams;
+    for (int c = tid; c < D; c += THREADS) {
+      float t = -INFINITY, o = 0.0f, l = 0.0f;
+      for (int w = 0; w < used; ++w) t = fmaxf(t, tops[w]);
+      for (int w = 0; w < used; ++w) {
+        const float a = part_weight(tops[w], suml[w], t);
+        if (a != 0.0f) o += a * acc[w * D + c], l += a * suml[w];
+      }
+      store_f<QT>(to + row * D + c, l == 0.0f ? 0.0f : o / (l * pscale));
+    }
+    __syncthreads();
   }
 }
 
@@ -737,7 +751,9 @@ struct AttendCall {
 // once, at most kGroups.
 constexpr int kGroups = 1024;
 constexpr int kLeast = 8;   // places of a chunk
-constexpr int kLone = 16;   // tiles that one workgroup takes rather than two launches
+// Tiles of a pair that one workgroup takes rather than two launches; with pairs for
+// every second unit, more.
+constexpr int kLone = 16, kLoneMany = 32, kMany = 256;
 
 struct Plan {
   Deal deal;
@@ -749,7 +765,7 @@ inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int
   const int G = H / kv_heads, RT = (G + 15) / 16;
   const int64_t keys = (int64_t)(S >= 0 ? S : P) << shift, most = (keys + tile - 1) / tile;
   p.deal = Deal{B, kv_heads * RT, RT, S, shift, P, tile, kLeast, 0};
-  if (most > kLone) {
+  if (most > ((int64_t)B * p.deal.R >= kMany ? kLoneMany : kLone)) {
     const int64_t chunks = ((most + kStart) * B * p.deal.R + kLeast - 1) / kLeast;
     p.deal.groups = (int)(chunks < kGroups ? chunks : kGroups);
     p.parts = (size_t)p.deal.groups * 2 * (G < 16 ? G : 16) * (D + 2) * 4;
@@ -786,7 +802,7 @@ void attend_launch(const AttendCall& a) {
       a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts, a.selected, a.c,
       (T*)a.out, p.bytes ? a.parts : nullptr, shared);
   if (!p.bytes) return;
-  const dim3 rows(pairs, G < 16 ? G : 16);
+  const dim3 rows(pairs, pairs >= kMany ? 1 : G < 16 ? G : 16);
   // a row of a few pairs has parts by the hundred
   if (pairs >= 64)
     join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, shared,

@@ -383,10 +383,10 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
 // Both for rows of up to kFused pages, a workgroup a row with the keys in LDS: a
 // launch (3.5 us of the host) less, in no more time (251 pages of 64
 // channels, 8 rows: 9.1 us against 4.0 + 5.4).
-constexpr int kFused = 512;
+constexpr int kFused = 512, kFusedSmall = 128;  // 256 threads up to the latter
 
-template <int QT, int BT, int D>
-__global__ void __launch_bounds__(1024) select_kernel(Pages pg, const int32_t* __restrict__ table,
+template <int QT, int BT, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t* __restrict__ table,
                                                       int64_t table_stride, int P,
                                                       const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
                                                       int64_t q_h, int G, const int32_t* __restrict__ lengths,
@@ -395,13 +395,13 @@ __global__ void __launch_bounds__(1024) select_kernel(Pages pg, const int32_t* _
   const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H, tid = threadIdx.x;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
-  __shared__ uint32_t keys[kFused];
-  for (int base = sp.p0; base < sp.pe; base += score_span(16, D, BT))
-    score_pages<QT, BT, D, 16>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
+  __shared__ uint32_t keys[THREADS];
+  for (int base = sp.p0; base < sp.pe; base += score_span(THREADS / kWave, D, BT))
+    score_pages<QT, BT, D, THREADS / kWave>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
                                [&](int page, uint32_t key) { keys[page - sp.p0] = key; });
   __syncthreads();
-  choose_best<1024, 1, true>(sp.p0, 1, count, chosen + (int64_t)blockIdx.x * count,
-                             [&](int, uint32_t (&x)[1]) { x[0] = tid < sp.pe - sp.p0 ? keys[tid] : kNone; });
+  choose_best<THREADS, 1, true>(sp.p0, 1, count, chosen + (int64_t)blockIdx.x * count,
+                                [&](int, uint32_t (&x)[1]) { x[0] = tid < sp.pe - sp.p0 ? keys[tid] : kNone; });
 }
 
 }  // namespace paged
