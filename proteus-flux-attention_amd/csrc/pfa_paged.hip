@@ -448,7 +448,8 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
     const auto* qp = (const typename Elem<QT>::T*)q->ptr;
     by_width(D, [&](auto width) {
       constexpr int W = decltype(width)::value;
-      if (P <= kFusedSmall)
+      // four waves where two rounds of theirs cover a row
+      if (P <= 2 * score_span(4, W, BT) && P <= kFused)
         select_kernel<QT, BT, W, 256><<<rows, 256, 0, as_stream(stream)>>>(
             p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else if (P <= kFused)

@@ -665,8 +665,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 }
 
 // Joins the parts of a pair's rows, a workgroup a row, or a pair where there are
-// many; writes the rows of sequences that see nothing.  A team of min(D, 64) lanes takes every TEAMS-th part, eight parts'
-// loads at once, and the teams are joined in LDS.
+// many; writes the rows of sequences that see nothing.  Up to 16 parts are a team
+// of min(D, 64) lanes' for each row; of more, every team takes some of a row's, and
+// the teams are joined in LDS.  Eight parts' loads go out at once.
 template <int QT, int THREADS>
 __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float pscale,
                                                        const int32_t* __restrict__ lengths,
@@ -687,44 +688,61 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
   if (who.n == 1) return;  // written by its one workgroup
   const int lanes = D < kWave ? D : kWave, d = tid % lanes, team = tid / lanes, teams = THREADS / lanes;
   const bool two = D > kWave;
-  constexpr int TEAMS = THREADS / 16;  // at most
-  __shared__ float acc[THREADS * 2], tops[TEAMS], suml[TEAMS];
-  for (int row = blockIdx.y; row < here; row += gridDim.y) {
-    float top = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int i0 = team; i0 < who.n; i0 += 8 * teams) {
+  struct Sum {
+    float m, l, o0, o1;
+  };
+  // parts i0, i0 + step, ... of a row, this lane's channels
+  auto gather = [&](int row, int i0, int step) {
+    Sum a{-INFINITY, 0.0f, 0.0f, 0.0f};
+    for (; i0 < who.n; i0 += 8 * step) {
       float m[8], l[8], x[8], y[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * teams;
+        const int i = i0 + u * step;
         const bool in = i < who.n;
         // part i is workgroup first + i's
         const float* s = parts + (2 * (int64_t)(who.first + (in ? i : 0)) + (!in || i == 0)) * rows * (D + 2);
         m[u] = in ? s[rows * D + row] : -INFINITY, l[u] = in ? s[rows * (D + 1) + row] : 0.0f;
         x[u] = s[row * D + d], y[u] = two ? s[row * D + 64 + d] : 0.0f;
       }
-      float t = top;
+      float t = a.m;
 #pragma unroll
       for (int u = 0; u < 8; ++u) t = fmaxf(t, m[u]);
-      const float a = part_weight(top, sum, t);
-      o0 = a == 0.0f ? 0.0f : a * o0, o1 = a == 0.0f ? 0.0f : a * o1, sum = a == 0.0f ? 0.0f : a * sum;
-      top = t;
+      const float w = part_weight(a.m, a.l, t);
+      a.o0 = w == 0.0f ? 0.0f : w * a.o0, a.o1 = w == 0.0f ? 0.0f : w * a.o1, a.l = w == 0.0f ? 0.0f : w * a.l;
+      a.m = t;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float w = part_weight(m[u], l[u], t);
-        if (w != 0.0f) o0 += w * x[u], o1 += w * y[u], sum += w * l[u];
+        const float p = part_weight(m[u], l[u], t);
+        if (p != 0.0f) a.o0 += p * x[u], a.o1 += p * y[u], a.l += p * l[u];
       }
     }
-    acc[team * D + d] = o0;
-    if (two) acc[team * D + 64 + d] = o1;
-    if (d == 0) tops[team] = top, suml[team] = sum;
+    return a;
+  };
+  if (who.n <= 16) {  // a team a row
+    for (int row = blockIdx.y * teams + team; row < here; row += gridDim.y * teams) {
+      const Sum a = gather(row, 0, 1);
+      const float inv = a.l == 0.0f ? 0.0f : 1.0f / (a.l * pscale);
+      store_f<QT>(to + row * D + d, a.o0 * inv);
+      if (two) store_f<QT>(to + row * D + 64 + d, a.o1 * inv);
+    }
+    return;
+  }
+  constexpr int TEAMS = THREADS / 16;  // at most
+  __shared__ float acc[THREADS * 2], tops[TEAMS], suml[TEAMS];
+  for (int row = blockIdx.y; row < here; row += gridDim.y) {
+    const Sum a = gather(row, team, teams);
+    acc[team * D + d] = a.o0;
+    if (two) acc[team * D + 64 + d] = a.o1;
+    if (d == 0) tops[team] = a.m, suml[team] = a.l;
     __syncthreads();
     const int used = who.n < teams ? who.n : teams;
     for (int c = tid; c < D; c += THREADS) {
       float t = -INFINITY, o = 0.0f, l = 0.0f;
       for (int w = 0; w < used; ++w) t = fmaxf(t, tops[w]);
       for (int w = 0; w < used; ++w) {
-        const float a = part_weight(tops[w], suml[w], t);
-        if (a != 0.0f) o += a * acc[w * D + c], l += a * suml[w];
+        const float p = part_weight(tops[w], suml[w], t);
+        if (p != 0.0f) o += p * acc[w * D + c], l += p * suml[w];
       }
       store_f<QT>(to + row * D + c, l == 0.0f ? 0.0f : o / (l * pscale));
     }

@@ -104,6 +104,8 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
     }
   };
   const int heads0 = G < kScoreHeads ? G : kScoreHeads;
+  const int wave0 = base + __builtin_amdgcn_readfirstlane(tid >> 6) * STEPS * PW;
+  const bool busy = wave0 < sp.pe && wave0 + STEPS * PW > sp.p0;  // the wave has pages
   int id[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
@@ -133,7 +135,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
     __syncthreads();
     store_q(heads);
     __syncthreads();
-    for (int g = 0; g < heads; g += kPair) {
+    for (int g = 0; g < (busy ? heads : 0); g += kPair) {
       double sum[NV] = {};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -383,7 +385,7 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
 // Both for rows of up to kFused pages, a workgroup a row with the keys in LDS: a
 // launch (3.5 us of the host) less, in no more time (251 pages of 64
 // channels, 8 rows: 9.1 us against 4.0 + 5.4).
-constexpr int kFused = 512, kFusedSmall = 128;  // 256 threads up to the latter
+constexpr int kFused = 512;
 
 template <int QT, int BT, int D, int THREADS>
 __global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t* __restrict__ table,
@@ -395,13 +397,16 @@ __global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t
   const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H, tid = threadIdx.x;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
-  __shared__ uint32_t keys[THREADS];
+  __shared__ uint32_t keys[kFused];
   for (int base = sp.p0; base < sp.pe; base += score_span(THREADS / kWave, D, BT))
     score_pages<QT, BT, D, THREADS / kWave>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
                                [&](int page, uint32_t key) { keys[page - sp.p0] = key; });
   __syncthreads();
-  choose_best<THREADS, 1, true>(sp.p0, 1, count, chosen + (int64_t)blockIdx.x * count,
-                                [&](int, uint32_t (&x)[1]) { x[0] = tid < sp.pe - sp.p0 ? keys[tid] : kNone; });
+  constexpr int K = kFused / THREADS > 0 ? kFused / THREADS : 1;
+  choose_best<THREADS, K, true>(sp.p0, 1, count, chosen + (int64_t)blockIdx.x * count, [&](int, uint32_t (&x)[K]) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) x[i] = K * tid + i < sp.pe - sp.p0 ? keys[K * tid + i] : kNone;
+  });
 }
 
 }  // namespace paged
