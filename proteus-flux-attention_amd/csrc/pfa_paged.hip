@@ -448,6 +448,7 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
     const auto* qp = (const typename Elem<QT>::T*)q->ptr;
     by_width(D, [&](auto width) {
       constexpr int W = decltype(width)::value;
+      const int spans = (P + score_span(4, W, BT) - 1) / score_span(4, W, BT);
       // four waves where two rounds of theirs cover a row
       if (P <= 2 * score_span(4, W, BT) && P <= kFused)
         select_kernel<QT, BT, W, 256><<<rows, 256, 0, as_stream(stream)>>>(
@@ -456,8 +457,7 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
         select_kernel<QT, BT, W, 1024><<<rows, 1024, 0, as_stream(stream)>>>(
             p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else
-        score_kernel<QT, BT, W><<<dim3(p.H, (P + score_span(4, W, BT) - 1) / score_span(4, W, BT), B), 256, 0,
-                                  as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths,
+        score_kernel<QT, BT, W><<<dim3(p.H, spans < 65535 ? spans : 65535, B), 256, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths,
                                                        starts, first, last, row_keys(P), keys);
     });
   });

@@ -117,7 +117,7 @@ struct Form {
 struct Block {
   int id, slot, pos;
 };
-constexpr int kNowhere = 0x7fffff00;
+constexpr int kNowhere = 0x7ffff000;  // positions are below 2^30; no sum with a tile's keys overflows
 
 // Pages of a run of tiles, in LDS: looked up by all of the workgroup's threads at
 // once, so that a tile's lookup, two loads one behind the other, is not in front

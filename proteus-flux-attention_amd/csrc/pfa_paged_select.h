@@ -196,12 +196,14 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
                                                     int64_t row_keys, uint32_t* __restrict__ keys) {
   const int b = blockIdx.z, h = blockIdx.x;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
-  const int base = blockIdx.y * score_span(4, D, BT);
-  if (base >= sp.pe || base + score_span(4, D, BT) <= sp.p0) return;
+  constexpr int SPAN = score_span(4, D, BT);
   __shared__ float qs[kScoreHeads][D];
   uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
-  score_pages<QT, BT, D, 4>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
-                            [&](int page, uint32_t key) { row[page] = key; });
+  for (int base = blockIdx.y * SPAN; base < sp.pe; base += gridDim.y * SPAN) {
+    if (base + SPAN <= sp.p0) continue;
+    score_pages<QT, BT, D, 4>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
+                              [&](int page, uint32_t key) { row[page] = key; });
+  }
 }
 
 // The best `count` of a row of keys, ascending.  The keys' range is cut into
