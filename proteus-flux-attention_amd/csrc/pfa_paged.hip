@@ -457,19 +457,18 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
         select_kernel<QT, BT, W, 1024><<<rows, 1024, 0, as_stream(stream)>>>(
             p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else
-        score_kernel<QT, BT, W><<<dim3(p.H, spans < 65535 ? spans : 65535, B), 256, 0, as_stream(stream)>>>(p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths,
-                                                       starts, first, last, row_keys(P), keys);
+        score_kernel<QT, BT, W><<<dim3(p.H, spans < 65535 ? spans : 65535, B), 256, 0, as_stream(stream)>>>(
+            p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, row_keys(P), keys);
     });
   });
-  // entries of a row from the first's four on: up to P + 3
 #define PFA_CHOOSE(THREADS, K, HELD)                                                                          \
   choose_kernel<THREADS, K, HELD><<<rows, THREADS, 0, as_stream(stream)>>>(p.H, P, row_keys(P), p.shift, count, \
                                                                            lengths, starts, keys, chosen)
   if (P <= kFused) {
-  } else if (P + 3 <= 256 * 4) PFA_CHOOSE(256, 4, true);
-  else if (P + 3 <= 1024 * 4) PFA_CHOOSE(1024, 4, true);
-  else if (P + 3 <= 1024 * 8) PFA_CHOOSE(1024, 8, true);
-  else if (P + 3 <= 1024 * 16) PFA_CHOOSE(1024, 16, true);
+  } else if (P <= 256 * 4) PFA_CHOOSE(256, 4, true);
+  else if (P <= 1024 * 4) PFA_CHOOSE(1024, 4, true);
+  else if (P <= 1024 * 8) PFA_CHOOSE(1024, 8, true);
+  else if (P <= 1024 * 16) PFA_CHOOSE(1024, 16, true);
   else PFA_CHOOSE(1024, 16, false);
 #undef PFA_CHOOSE
   PFA_CHECK_LAUNCH("kv_pages_select");

@@ -77,7 +77,7 @@ __device__ __forceinline__ void spread(double* sum, int lane) {
 // Pages base .. base + WAVES * 64 / (D / 8) * kSteps - 1 of a workgroup's row; put
 // gets each page of the span and its key.
 template <int QT, int BT, int D, int WAVES, typename Put>
-__device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __restrict__ ids, const Span& sp, int h,
+__device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __restrict__ ids, int P, const Span& sp, int h,
                                             const typename Elem<QT>::T* __restrict__ q, int64_t q_h, int G, int first,
                                             int last, int base, float (&qs)[kScoreHeads][D], Put&& put) {
   constexpr int LP = D / 8;       // lanes of a page
@@ -110,14 +110,15 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     const int page = page0 + s * PW;
-    id[s] = page >= sp.p0 && page < sp.pe ? ids[page] : -1;
+    id[s] = page < P ? ids[page] : -1;  // before the span is known: a load less in a row
   }
   load_q(0, heads0);
   float lo[STEPS][8], hi[STEPS][8];
   bool have[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
-    have[s] = (uint32_t)id[s] < (uint32_t)pg.n_pages;
+    const int page = page0 + s * PW;
+    have[s] = page >= sp.p0 && page < sp.pe && (uint32_t)id[s] < (uint32_t)pg.n_pages;
     const BoundT* at = (const BoundT*)pg.bounds + ((int64_t)(have[s] ? id[s] : 0) * pg.H + h) * 2 * D + 8 * part;
     load8<BT>(at, lo[s]);
     load8<BT>(at + D, hi[s]);
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
   uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
   for (int base = blockIdx.y * SPAN; base < sp.pe; base += gridDim.y * SPAN) {
     if (base + SPAN <= sp.p0) continue;
-    score_pages<QT, BT, D, 4>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
+    score_pages<QT, BT, D, 4>(pg, table + b * table_stride, P, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
                               [&](int page, uint32_t key) { row[page] = key; });
   }
 }
@@ -367,15 +368,16 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
                                                          int32_t* __restrict__ chosen) {
   const uint32_t* key = keys + (int64_t)blockIdx.x * row_keys;
   const Span sp = span_at(lengths, starts, P, shift, blockIdx.x / H);
-  const int from0 = sp.p0 & ~3;  // rows of keys are 16-byte aligned
+  const int from0 = HELD ? 0 : sp.p0 & ~3;  // rows of keys are 16-byte aligned
   const int rounds = HELD ? 1 : (sp.pe - from0 + THREADS * K - 1) / (THREADS * K);
   choose_best<THREADS, K, HELD>(from0, rounds, count, chosen + (int64_t)blockIdx.x * count,
                                 [&](int r, uint32_t (&x)[K]) {
     const int p = from0 + (r * THREADS + (int)threadIdx.x) * K;
 #pragma unroll
     for (int i = 0; i < K; i += 4) {
+      // held rows before the span is known: what lies outside of it is masked
       uint4 a = make_uint4(0, 0, 0, 0);
-      if (p + i < sp.pe) a = *reinterpret_cast<const uint4*>(key + p + i);
+      if (p + i < (HELD ? P : sp.pe)) a = *reinterpret_cast<const uint4*>(key + p + i);
       x[i] = a.x, x[i + 1] = a.y, x[i + 2] = a.z, x[i + 3] = a.w;
     }
 #pragma unroll
@@ -400,14 +402,14 @@ __global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
   __shared__ uint32_t keys[kFused];
-  for (int base = sp.p0; base < sp.pe; base += score_span(THREADS / kWave, D, BT))
-    score_pages<QT, BT, D, THREADS / kWave>(pg, table + b * table_stride, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
-                               [&](int page, uint32_t key) { keys[page - sp.p0] = key; });
+  for (int base = 0; base < P; base += score_span(THREADS / kWave, D, BT))
+    score_pages<QT, BT, D, THREADS / kWave>(pg, table + b * table_stride, P, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
+                               [&](int page, uint32_t key) { keys[page] = key; });
   __syncthreads();
   constexpr int K = kFused / THREADS > 0 ? kFused / THREADS : 1;
-  choose_best<THREADS, K, true>(sp.p0, 1, count, chosen + (int64_t)blockIdx.x * count, [&](int, uint32_t (&x)[K]) {
+  choose_best<THREADS, K, true>(0, 1, count, chosen + (int64_t)blockIdx.x * count, [&](int, uint32_t (&x)[K]) {
 #pragma unroll
-    for (int i = 0; i < K; ++i) x[i] = K * tid + i < sp.pe - sp.p0 ? keys[K * tid + i] : kNone;
+    for (int i = 0; i < K; ++i) x[i] = K * tid + i >= sp.p0 && K * tid + i < sp.pe ? keys[K * tid + i] : kNone;
   });
 }
 
