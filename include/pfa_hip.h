@@ -690,8 +690,8 @@ int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t
  * multiple of kv_heads, head h reads key-value head h / (H / kv_heads); s_t
  * unused) over positions starts[b] (NULL: 0) .. lengths[b] - 1, or, with
  * n_selected >= 0, over those of them that lie in the entries of the
- * sequence's table row that `selected` (B, kv_heads, n_selected) lists
- * (entries outside of it are left out, an entry listed twice counts twice);
+ * sequence's table row that `selected` (B, kv_heads, n_selected; rows
+ * selected_stride apart) lists (entries outside of it are left out, an entry listed twice counts twice);
  * n_selected < 0: no list.  out (B, H, D) dense, in q's type
  * (PFA_F32 / PFA_BF16 / PFA_F16: the cells' own, or any of the three for
  * 8-bit cells).  A row that sees no key is zero, and so is one all of whose
@@ -702,7 +702,8 @@ int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int page_size, int
 int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
                        const int32_t* table, int64_t table_stride, int table_pages,
                        const int32_t* lengths, const int32_t* starts,
-                       const int32_t* selected, int n_selected, float scale, void* out,
+                       const int32_t* selected, int64_t selected_stride, int n_selected,
+                       float scale, void* out,
                        void* workspace, size_t ws_bytes, void* stream);
 
 /* The `count` pages of each sequence and key-value head with the best bound on

@@ -488,14 +488,14 @@ extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int pag
 
 extern "C" int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
                                   int64_t table_stride, int table_pages, const int32_t* lengths, const int32_t* starts,
-                                  const int32_t* selected, int n_selected, float scale, void* out, void* workspace,
-                                  size_t ws_bytes, void* stream) {
+                                  const int32_t* selected, int64_t selected_stride, int n_selected, float scale,
+                                  void* out, void* workspace, size_t ws_bytes, void* stream) {
   clear_error();
   Pages p;
   Table t;
   if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
   if (int rc = query_check("paged_attn", q, dtype, B, H, pages, lengths)) return rc;
-  PFA_CHECK_ARG(n_selected <= 0 || selected, "paged_attn: null argument");
+  PFA_CHECK_ARG(n_selected <= 0 || (selected && selected_stride >= n_selected), "paged_attn: lists that are null or overlap");
   PFA_CHECK_ARG((int64_t)n_selected << p.shift <= (1ll << 30), "paged_attn: lists of up to 2^30 positions");
   const float c = scale * 1.44269504088896340736f;
   PFA_CHECK_ARG(c > 0.0f && c < INFINITY, "paged_attn: scale must be positive and finite");
@@ -508,7 +508,8 @@ extern "C" int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H,
     set_error("paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, plan.bytes);
     return PFA_E_WORKSPACE;
   }
-  const AttendCall a{p, table, table_stride, table_pages, B, H, pages->head_dim, *q, lengths, starts, selected, S, c, out,
+  const AttendCall a{p, table, table_stride, table_pages, B, H, pages->head_dim, *q, lengths, starts, selected,
+                     selected_stride, S, c, out,
                      (float*)workspace, as_stream(stream)};
   if (pages->dtype == PFA_I8) attend_i8(dtype, a);
   else if (pages->dtype == PFA_E4M3) attend_e4m3(dtype, a);

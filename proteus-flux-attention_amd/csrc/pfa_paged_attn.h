@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     Pages pg, Deal deal, const int32_t* __restrict__ table, int64_t table_stride,
     const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int q_vec, int G,
     const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts, const int32_t* __restrict__ selected,
-    float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws, Shared* __restrict__ shared) {
+    int64_t selected_stride, float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws, Shared* __restrict__ shared) {
   constexpr int D = F::D;
   __shared__ float so[kWaves][16][D + 4];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     for (int j = 0; j < F::VD; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     st.m = -INFINITY, st.l = 0.0f;
     const int32_t* ids = table + b * table_stride;
-    const int32_t* list = selected + ((int64_t)b * pg.H + h) * (deal.S > 0 ? deal.S : 0);
+    const int32_t* list = selected + ((int64_t)b * pg.H + h) * selected_stride;
     const int t0 = deal.first_tile(start), te = t0 + tb;
     const int run = (kEntries << deal.shift) / F::TILE;  // tiles whose pages fit
     for (int r0 = t0 + ta; r0 < te; r0 += run) {
@@ -758,6 +758,7 @@ struct AttendCall {
   int P, B, H, D;
   pfa_tensor4 q;
   const int32_t *lengths, *starts, *selected;
+  int64_t selected_stride;
   int S;
   float c;  // scale * log2(e)
   void* out;
@@ -817,7 +818,8 @@ void attend_launch(const AttendCall& a) {
   Shared* shared = reinterpret_cast<Shared*>(reinterpret_cast<char*>(a.parts) + p.parts);
   const bool q_vec = ((uintptr_t)a.q.ptr | (uintptr_t)(a.q.s_b * sizeof(T)) | (uintptr_t)(a.q.s_h * sizeof(T))) % 16 == 0;
   attend_kernel<F><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
-      a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts, a.selected, a.c,
+      a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts, a.selected,
+      a.selected_stride, a.c,
       (T*)a.out, p.bytes ? a.parts : nullptr, shared);
   if (!p.bytes) return;
   const dim3 rows(pairs, pairs >= kMany ? 1 : G < 16 ? G : 16);

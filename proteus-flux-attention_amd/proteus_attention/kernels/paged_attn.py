@@ -307,16 +307,17 @@ def _scale(scale: Optional[float]) -> Optional[float]:
     return scale
 
 
-def _attend(a: _Query, selected: Optional[torch.Tensor], scale: Optional[float]) -> torch.Tensor:
+def _attend(a: _Query, selected: Optional[torch.Tensor], scale: Optional[float], S: int = -1) -> torch.Tensor:
+    """S: the entries of each list that count."""
+
     if scale is None:
         scale = 1.0 / math.sqrt(a.D)
-    S = -1 if selected is None else selected.shape[2]
     device = a.table.device
     ws, ws_ptr = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
     out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
     _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, *a.args,
-          None if selected is None else selected.data_ptr(), S, scale, out.data_ptr(), ws_ptr,
-          0 if ws is None else ws.numel())
+          None if selected is None else selected.data_ptr(), 0 if selected is None else selected.shape[2], S, scale,
+          out.data_ptr(), ws_ptr, 0 if ws is None else ws.numel())
     return out
 
 
@@ -342,8 +343,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     if selected is not None:
         if selected.shape[:2] != (a.B, a.Hkv):
             raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
-        selected = selected.contiguous()
-    return _attend(a, selected, scale)
+        return _attend(a, selected.contiguous(), scale, selected.shape[2])
+    return _attend(a, None, scale)
 
 
 def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, int, int]:
@@ -392,7 +393,7 @@ def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.T
     scale = _scale(scale)
     a = _Query("paged_sparse_attention", q, pages, block_table, lengths, starts)
     chosen = _select(a, *sizes)
-    return _attend(a, chosen, scale), chosen
+    return _attend(a, chosen, scale, min(sizes[0], a.P)), chosen  # no row holds more than its table does
 
 
 __all__ = [

@@ -112,7 +112,7 @@ def test_c_entries_refuse_before_any_launch():
     p = ctypes.c_void_p(256)  # never dereferenced
 
     def attend(pool, q=t4, tag=_hip.PFA_F32, B=1, H=2, P=2, n=-1, out=p, lengths=p):
-        return lib.pfa_paged_attn_fwd(q, tag, B, H, pool, p, P, P, lengths, None, None, n, 0.5, out, p, 1 << 40, None)
+        return lib.pfa_paged_attn_fwd(q, tag, B, H, pool, p, P, P, lengths, None, None, max(n, 0), n, 0.5, out, p, 1 << 40, None)
 
     bad = [attend(_c_pool(head_dim=48)), attend(_c_pool(page_size=48)), attend(_c_pool(n_pages=0)),
            attend(_c_pool(dtype=9)), attend(_c_pool(dtype=_hip.PFA_I8)), attend(_c_pool(k=264)),
