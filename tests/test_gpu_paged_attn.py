@@ -392,3 +392,80 @@ def test_offsets_beyond_32_bits():
     want = torch.einsum("bht,bthd->bhd", torch.softmax(s, -1), rv.double())
     # attend_error's bound with sum p |v| <= 5 and sum |q k| scale <= 60
     assert float((out.cpu().double() - want).norm(dim=-1).max()) <= 4 * 2.0 ** -24 * ((math.sqrt(D) + 3) * 60 + 22) * 5 * math.sqrt(D)
+
+
+def test_layouts_and_empty_calls():
+    """Tables and lengths that are slices, keys and queries that are expanded or
+    transposed; calls with nothing to do."""
+    from proteus_attention import (new_kv_pages, paged_attention, paged_sparse_attention, read_kv_pages,
+                                   select_kv_pages, write_kv_pages)
+
+    g = torch.Generator().manual_seed(12)
+    B, H, D, ps = 3, 2, 32, 16
+    pages = new_kv_pages(12, H, ps, D, dtype=torch.float32, bounds=True, device=DEV)
+    pool = {m: t.cpu().clone() for m, t in pages._asdict().items() if t is not None}
+    table = torch.randperm(12, generator=g).view(B, 4).to(torch.int32)
+    lengths = [50, 17, 1]
+    one = torch.randn(1, 50, 1, D, generator=g)
+    k = one.expand(B, 50, H, D)  # every sequence and head the same
+    v = torch.randn(B, H, D, 50, generator=g)
+    want = R.write(pool, k, v.permute(0, 3, 1, 2), table, [0] * B, lengths)
+    wide = torch.zeros(B, 3, dtype=torch.int32)
+    wide[:, 1] = _i32(lengths)
+    n = wide.to(DEV)[:, 1]
+    columns = table.t().contiguous().to(DEV).t()
+    write_kv_pages(pages, one.to(DEV).expand(B, 50, H, D), v.to(DEV).permute(0, 3, 1, 2), columns,
+                   torch.zeros_like(n), counts=n)
+    for m in want:
+        assert _same(getattr(pages, m), want[m]), m
+    q = torch.randn(1, D, generator=g).expand(B, 2 * H, D)
+    qd = q[:1, :1].to(DEV).expand(B, 2 * H, D)
+    ref = R.attend(q, want, table, lengths)
+    assert R.attend_error(paged_attention(qd, pages, columns, n).cpu(), ref, torch.float32, 50) <= 1
+    got, chosen = paged_sparse_attention(qd.transpose(1, 2).contiguous().transpose(1, 2), pages, columns, n, 3)
+    sel = R.select(q, want, table, lengths, None, 3, 1, 1)
+    assert torch.equal(chosen.cpu(), sel)
+    assert R.attend_error(got.cpu(), R.attend(q, want, table, lengths, None, sel), torch.float32, 48) <= 1
+
+    # no sequences, no tokens, no table
+    none, t0, l0 = qd[:0], columns[:0], n[:0]
+    assert paged_attention(none, pages, t0, l0).shape == (0, 2 * H, D)
+    assert select_kv_pages(none, pages, t0, l0, 2).shape == (0, H, 2)
+    assert read_kv_pages(pages, t0, l0, None, 5)[0].shape == (0, 5, H, D)
+    assert read_kv_pages(pages, columns, n, None, 0)[0].shape == (B, 0, H, D)
+    kd = one.to(DEV).expand(B, 50, H, D)
+    write_kv_pages(pages, kd[:0], kd[:0], t0, l0)
+    write_kv_pages(pages, kd[:, :0], kd[:, :0], columns, n)
+    write_kv_pages(pages, kd, kd, columns[:, :0], n)
+    for m in want:
+        assert _same(getattr(pages, m), want[m]), m
+    p0 = columns[:, :0]
+    assert not paged_attention(qd, pages, p0, n).any()
+    out, chosen = paged_sparse_attention(qd, pages, p0, n, 2)
+    assert not out.any() and bool((chosen == -1).all())
+    assert not any(x.any() for x in read_kv_pages(pages, p0, n, None, 7))
+
+
+@pytest.mark.parametrize("ps", [16, 256])
+def test_wide_tables(ps):
+    """Tables far wider than the sequences: more pages than a run of tiles looks
+    up at once, most of them gone."""
+    from proteus_attention import paged_attention, paged_sparse_attention
+
+    g = torch.Generator().manual_seed(13)
+    H, G, D, P = 2, 2, 64, 1500
+    lengths = [P * ps, (P - 3) * ps + 5]
+    pool = R.make_pool(9, H, ps, D, torch.bfloat16, g, bounds=True)
+    table = torch.full((2, P), -1, dtype=torch.int32)
+    for b in range(2):
+        at = torch.randperm(P, generator=g)[:9]
+        table[b, at] = torch.randperm(9, generator=g).to(torch.int32)
+        table[b, P - 1 - 3 * b] = b
+    q = torch.randn(2, H * G, D, generator=g).bfloat16()
+    args = (q.to(DEV), _pages(pool), table.to(DEV), _i32(lengths).to(DEV))
+    ref = R.attend(q, pool, table, lengths)
+    assert R.attend_error(paged_attention(*args).cpu(), ref, torch.bfloat16, 10 * ps) <= 1
+    out, chosen = paged_sparse_attention(*args, 12, first=0, last=1)
+    want = R.select(q, pool, table, lengths, None, 12, 0, 1)
+    assert torch.equal(chosen.cpu(), want)
+    assert R.attend_error(out.cpu(), ref, torch.bfloat16, 10 * ps) <= 1
