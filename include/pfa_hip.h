@@ -686,24 +686,31 @@ int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t
                       const int32_t* counts, void* k_out, void* v_out, int out_dtype,
                       void* stream);
 
-/* Attention of one new token a sequence: q [b][h][d] (H query heads, H a
- * multiple of kv_heads, head h reads key-value head h / (H / kv_heads); s_t
- * unused) over positions starts[b] (NULL: 0) .. lengths[b] - 1, or, with
- * n_selected >= 0, over those of them that lie in the entries of the
- * sequence's table row that `selected` (B, kv_heads, n_selected; rows
- * selected_stride apart) lists (entries outside of it are left out, an entry listed twice counts twice);
- * n_selected < 0: no list.  out (B, H, D) dense, in q's type
- * (PFA_F32 / PFA_BF16 / PFA_F16: the cells' own, or any of the three for
- * 8-bit cells).  A row that sees no key is zero, and so is one all of whose
- * scores are -inf.  Sums and softmax statistics are f32. */
+/* One new token a sequence: queries q [b][h][d] (s_t unused; H heads, a multiple of
+ * kv_heads: head h reads key-value head h / (H / kv_heads)) in dtype PFA_F32 /
+ * PFA_BF16 / PFA_F16 (the cells' own, or any of the three for 8-bit cells),
+ * looking at positions starts[b] (starts NULL: 0) .. lengths[b] - 1.  Lengths
+ * beyond the table's pages count as all of them. */
+typedef struct pfa_paged_query {
+  pfa_kv_pages pages;
+  pfa_tensor4 q;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t *lengths, *starts;
+  int table_pages, B, H, dtype;
+} pfa_paged_query;
+
+/* Attention over those positions, or, with n_selected >= 0, over those of them
+ * that lie in the entries of the sequence's table row that `selected` (B,
+ * kv_heads, n_selected; rows selected_stride apart) lists (entries outside of it
+ * are left out, an entry listed twice counts twice); n_selected < 0: no list.
+ * out (B, H, D) dense, in q's type.  A row that sees no key is zero, and so is
+ * one all of whose scores are -inf.  Sums and softmax statistics are f32. */
 int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
                                   int cell_dtype, int table_pages, int n_selected,
                                   size_t* bytes);
-int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
-                       const int32_t* table, int64_t table_stride, int table_pages,
-                       const int32_t* lengths, const int32_t* starts,
-                       const int32_t* selected, int64_t selected_stride, int n_selected,
-                       float scale, void* out,
+int pfa_paged_attn_fwd(const pfa_paged_query* query, const int32_t* selected,
+                       int64_t selected_stride, int n_selected, float scale, void* out,
                        void* workspace, size_t ws_bytes, void* stream);
 
 /* The `count` pages of each sequence and key-value head with the best bound on
@@ -711,15 +718,12 @@ int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_
  * row in ascending order, -1 behind the last.  A page's score is the largest,
  * over the group's query heads, of sum_d q_d * (q_d > 0 ? max_d : min_d),
  * summed in 64 bits and held in 32; NaN counts below everything.  The `first`
- * first and `last` last entries that hold positions starts[b] ..
- * lengths[b] - 1 come before all others, then the better score, then the
- * lower entry; entries without a page are never chosen. */
+ * first and `last` last entries that hold positions to look at come before all
+ * others, then the better score, then the lower entry; entries without a page
+ * are never chosen. */
 int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes);
-int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
-                        const int32_t* table, int64_t table_stride, int table_pages,
-                        const int32_t* lengths, const int32_t* starts, int count, int first,
-                        int last, int32_t* chosen, void* workspace, size_t ws_bytes,
-                        void* stream);
+int pfa_kv_pages_select(const pfa_paged_query* query, int count, int first, int last,
+                        int32_t* chosen, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -399,13 +399,14 @@ extern "C" int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, co
 
 namespace {
 
-int query_check(const char* what, const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages,
-                const int32_t* lengths) {
-  if (int rc = types_check(dtype, pages->dtype)) return rc;
-  PFA_CHECK_ARG(H > 0 && H <= 65535 && H % pages->kv_heads == 0, "%s: %d query heads over %d key-value heads", what, H,
-                pages->kv_heads);
-  PFA_CHECK_ARG((int64_t)B * H <= 1 << 21, "%s: up to 2^21 rows (got %d x %d)", what, B, H);
-  PFA_CHECK_ARG(B == 0 || (q && q->ptr && lengths), "%s: null argument", what);
+int query_check(const char* what, const pfa_paged_query* a, Pages* p, Table* t) {
+  PFA_CHECK_ARG(a, "%s: null argument", what);
+  if (int rc = paged_check(&a->pages, a->table, a->table_stride, a->table_pages, a->B, p, t)) return rc;
+  if (int rc = types_check(a->dtype, a->pages.dtype)) return rc;
+  PFA_CHECK_ARG(a->H > 0 && a->H <= 65535 && a->H % p->H == 0, "%s: %d query heads over %d key-value heads", what, a->H,
+                p->H);
+  PFA_CHECK_ARG((int64_t)a->B * a->H <= 1 << 21, "%s: up to 2^21 rows (got %d x %d)", what, a->B, a->H);
+  PFA_CHECK_ARG(a->B == 0 || (a->q.ptr && a->lengths), "%s: null argument", what);
   return PFA_OK;
 }
 
@@ -421,29 +422,29 @@ extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table
   return PFA_OK;
 }
 
-extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
-                                   int64_t table_stride, int table_pages, const int32_t* lengths,
-                                   const int32_t* starts, int count, int first, int last, int32_t* chosen,
+extern "C" int pfa_kv_pages_select(const pfa_paged_query* query, int count, int first, int last, int32_t* chosen,
                                    void* workspace, size_t ws_bytes, void* stream) {
   clear_error();
   Pages p;
   Table t;
-  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
-  if (int rc = query_check("kv_pages_select", q, dtype, B, H, pages, lengths)) return rc;
-  PFA_CHECK_ARG(pages->k_bounds, "kv_pages_select: the pool has no key bounds");
+  if (int rc = query_check("kv_pages_select", query, &p, &t)) return rc;
+  PFA_CHECK_ARG(p.bounds, "kv_pages_select: the pool has no key bounds");
   PFA_CHECK_ARG(count > 0 && first >= 0 && last >= 0 && first <= count && last <= count - first,
                 "kv_pages_select: count > 0 pages, the %d first and %d last among them (got %d)", first, last, count);
+  const int B = query->B, H = query->H, D = query->pages.head_dim, P = query->table_pages;
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(chosen, "kv_pages_select: null argument");
   size_t need = 0;
-  pfa_kv_pages_select_workspace_size(B, p.H, table_pages, &need);
+  pfa_kv_pages_select_workspace_size(B, p.H, P, &need);
   if (ws_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16 != 0))) {
     set_error("kv_pages_select: workspace of %zu bytes, %zu needed", ws_bytes, need);
     return PFA_E_WORKSPACE;
   }
   uint32_t* keys = (uint32_t*)workspace;
-  const int D = pages->head_dim, P = table_pages, rows = B * p.H;
-  by_types(dtype, pages->dtype, [&](auto dt, auto ct) {
+  const int rows = B * p.H;
+  const pfa_tensor4* q = &query->q;
+  const int32_t *lengths = query->lengths, *starts = query->starts;
+  by_types(query->dtype, query->pages.dtype, [&](auto dt, auto ct) {
     constexpr int QT = decltype(dt)::value, BT = bound_dtype(decltype(ct)::value);
     const auto* qp = (const typename Elem<QT>::T*)q->ptr;
     by_width(D, [&](auto width) {
@@ -452,13 +453,13 @@ extern "C" int pfa_kv_pages_select(const pfa_tensor4* q, int dtype, int B, int H
       // four waves where two rounds of theirs cover a row
       if (P <= 2 * score_span(4, W, BT) && P <= kFused)
         select_kernel<QT, BT, W, 256><<<rows, 256, 0, as_stream(stream)>>>(
-            p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
+            p, t.ids, t.stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else if (P <= kFused)
         select_kernel<QT, BT, W, 1024><<<rows, 1024, 0, as_stream(stream)>>>(
-            p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
+            p, t.ids, t.stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else
         score_kernel<QT, BT, W><<<dim3(p.H, spans < 65535 ? spans : 65535, B), 256, 0, as_stream(stream)>>>(
-            p, table, table_stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, row_keys(P), keys);
+            p, t.ids, t.stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, row_keys(P), keys);
     });
   });
 #define PFA_CHOOSE(THREADS, K, HELD)                                                                          \
@@ -486,34 +487,32 @@ extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int pag
   return PFA_OK;
 }
 
-extern "C" int pfa_paged_attn_fwd(const pfa_tensor4* q, int dtype, int B, int H, const pfa_kv_pages* pages, const int32_t* table,
-                                  int64_t table_stride, int table_pages, const int32_t* lengths, const int32_t* starts,
-                                  const int32_t* selected, int64_t selected_stride, int n_selected, float scale,
-                                  void* out, void* workspace, size_t ws_bytes, void* stream) {
+extern "C" int pfa_paged_attn_fwd(const pfa_paged_query* query, const int32_t* selected, int64_t selected_stride,
+                                  int n_selected, float scale, void* out, void* workspace, size_t ws_bytes,
+                                  void* stream) {
   clear_error();
   Pages p;
   Table t;
-  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &t)) return rc;
-  if (int rc = query_check("paged_attn", q, dtype, B, H, pages, lengths)) return rc;
-  PFA_CHECK_ARG(n_selected <= 0 || (selected && selected_stride >= n_selected), "paged_attn: lists that are null or overlap");
+  if (int rc = query_check("paged_attn", query, &p, &t)) return rc;
+  PFA_CHECK_ARG(n_selected <= 0 || (selected && selected_stride >= n_selected),
+                "paged_attn: lists that are null or overlap");
   PFA_CHECK_ARG((int64_t)n_selected << p.shift <= (1ll << 30), "paged_attn: lists of up to 2^30 positions");
   const float c = scale * 1.44269504088896340736f;
   PFA_CHECK_ARG(c > 0.0f && c < INFINITY, "paged_attn: scale must be positive and finite");
+  const int B = query->B, H = query->H, D = query->pages.head_dim, ct = query->pages.dtype;
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "paged_attn: null or unaligned argument");
   const int S = n_selected < 0 ? -1 : n_selected;
-  const Plan plan = attend_plan(B, H, p.H, pages->head_dim, p.shift, table_pages, S,
-                                attend_tile(pages->dtype, pages->head_dim));
+  const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D));
   if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
     set_error("paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, plan.bytes);
     return PFA_E_WORKSPACE;
   }
-  const AttendCall a{p, table, table_stride, table_pages, B, H, pages->head_dim, *q, lengths, starts, selected,
-                     selected_stride, S, c, out,
-                     (float*)workspace, as_stream(stream)};
-  if (pages->dtype == PFA_I8) attend_i8(dtype, a);
-  else if (pages->dtype == PFA_E4M3) attend_e4m3(dtype, a);
-  else attend_float(dtype, a);
+  const AttendCall a{p, t.ids, t.stride, t.P, B, H, D, query->q, query->lengths, query->starts, selected,
+                     selected_stride, S, c, out, (float*)workspace, as_stream(stream)};
+  if (ct == PFA_I8) attend_i8(query->dtype, a);
+  else if (ct == PFA_E4M3) attend_e4m3(query->dtype, a);
+  else attend_float(query->dtype, a);
   PFA_CHECK_LAUNCH("paged_attn");
   return PFA_OK;
 }

@@ -78,9 +78,10 @@ def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *
     return KVPages(k, v, *scales, kb)
 
 
-# pfa_kv_pages and pfa_tensor4 of include/pfa_hip.h
+# pfa_kv_pages, pfa_tensor4 and pfa_paged_query of include/pfa_hip.h
 _POOL = struct.Struct("PPPPPqqiiiii4x")
 _TENSOR4 = struct.Struct("Pqqq")
+_QUERY = struct.Struct(_POOL.format + _TENSOR4.format + "PqPPiiii")
 
 
 def _dense(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, name: str) -> int:
@@ -89,8 +90,9 @@ def _dense(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, name: st
     return t.data_ptr()
 
 
-def _pool(pages: KVPages) -> Tuple[bytes, int, int, int]:
-    """The pool for the library, and its heads, page size and head dim."""
+def _pool(pages: KVPages) -> tuple:
+    """The fields of pfa_kv_pages; the last five are pages, heads, page size, head
+    dim and the cells' tag."""
 
     k, v, k_scale, v_scale, bounds = pages
     dtype, shape = k.dtype, k.shape
@@ -120,7 +122,7 @@ def _pool(pages: KVPages) -> Tuple[bytes, int, int, int]:
         bound_dtype = torch.float32
     if bounds is not None:
         b = _dense(bounds, (N, H, 2, D), bound_dtype, "k_bounds")
-    return _POOL.pack(k.data_ptr(), v.data_ptr(), a, c, b, ks[0], vs[0], N, H, ps, D, tag), H, ps, D
+    return k.data_ptr(), v.data_ptr(), a, c, b, ks[0], vs[0], N, H, ps, D, tag
 
 
 def _table(block_table: torch.Tensor, B: int) -> torch.Tensor:
@@ -209,7 +211,8 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     if len(shape) != 4 or v.shape != shape or v.dtype != dtype:
         raise ValueError("k and v must be (B, n, kv_heads, head_dim) tensors of one shape and dtype")
     B, n, H, D = shape
-    pool, pool_heads, _, pool_dim = _pool(pages)
+    pool = _pool(pages)
+    pool_heads, pool_dim = pool[8], pool[10]
     if H != pool_heads or D != pool_dim:
         raise ValueError(f"k and v have {H} heads of {D}, the pages {pool_heads} of {pool_dim}")
     tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
@@ -228,7 +231,7 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     if vs[3] != 1:
         v = v.contiguous()
         vs = v.stride()
-    _call(index, "kv_pages_write", _hip.lib().pfa_kv_pages_write, pool,
+    _call(index, "kv_pages_write", _hip.lib().pfa_kv_pages_write, _POOL.pack(*pool),
           _TENSOR4.pack(k.data_ptr(), ks[0], ks[2], ks[1]), _TENSOR4.pack(v.data_ptr(), vs[0], vs[2], vs[1]), tag, B, n,
           table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(),
           None if counts is None else counts.data_ptr())
@@ -241,7 +244,8 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     ``dtype`` (default: the pages' type, f32 for 8-bit pages).  Rows
     i >= ``counts[b]``, and those without a page, are zero."""
 
-    pool, H, _, D = _pool(pages)
+    pool = _pool(pages)
+    H, D = pool[8], pool[10]
     B, n = block_table.shape[0] if block_table.dim() else 0, int(n)
     table, starts = _table(block_table, B), _per_sequence(starts, B, "starts")
     if counts is not None:
@@ -257,7 +261,7 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     device = table.device
     k = torch.empty((B, n, H, D), dtype=dtype, device=device)
     v = torch.empty((B, n, H, D), dtype=dtype, device=device)
-    _call(index, "kv_pages_read", _hip.lib().pfa_kv_pages_read, pool, B, n, table.data_ptr(), table.stride(0),
+    _call(index, "kv_pages_read", _hip.lib().pfa_kv_pages_read, _POOL.pack(*pool), B, n, table.data_ptr(), table.stride(0),
           table.shape[1], starts.data_ptr(), None if counts is None else counts.data_ptr(), k.data_ptr(), v.data_ptr(),
           tag)
     return k, v
@@ -265,9 +269,9 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
 
 class _Query:
     """The checked arguments that selection and attention share, for the
-    library in ``args``; the tensors stay referenced until the calls are made."""
+    library in ``packed``; the tensors stay referenced until the calls are made."""
 
-    __slots__ = ("args", "B", "H", "Hkv", "ps", "D", "P", "tag", "cells", "q", "table", "lengths", "starts", "index")
+    __slots__ = ("packed", "B", "H", "Hkv", "ps", "D", "P", "cells", "q", "table", "lengths", "starts", "index")
 
     def __init__(self, what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
                  starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None) -> None:
@@ -275,15 +279,15 @@ class _Query:
         if len(shape) != 3:
             raise ValueError("q must be a (B, heads, head_dim) tensor: one new token a sequence")
         self.B, self.H, self.D = B, H, D = shape
-        pool, self.Hkv, self.ps, pool_dim = _pool(pages)
+        pool = _pool(pages)
+        _, self.Hkv, self.ps, pool_dim, self.cells = pool[7:]
         if D != pool_dim or H == 0 or H % self.Hkv:
             raise ValueError(f"q has {H} heads of {D}, the pages {self.Hkv} of {pool_dim}")
         tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
         if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
             raise ValueError(f"queries of {dtype} for pages of {cells}")
-        self.tag, self.cells = tag, _CELL_TAG[cells]
         self.table = table = _table(block_table, B)
-        self.P = table.shape[1]
+        self.P = P = table.shape[1]
         self.lengths = lengths = _per_sequence(lengths, B, "lengths")
         self.starts = starts = None if starts is None else _per_sequence(starts, B, "starts")
         if q.requires_grad and torch.is_grad_enabled():
@@ -294,8 +298,8 @@ class _Query:
             q = q.contiguous()
             s = q.stride()
         self.q = q
-        self.args = (_TENSOR4.pack(q.data_ptr(), s[0], s[1], 0), tag, B, H, pool, table.data_ptr(), table.stride(0),
-                     self.P, lengths.data_ptr(), None if starts is None else starts.data_ptr())
+        self.packed = _QUERY.pack(*pool, q.data_ptr(), s[0], s[1], 0, table.data_ptr(), table.stride(0),
+                                  lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), P, B, H, tag)
 
 
 def _scale(scale: Optional[float]) -> Optional[float]:
@@ -315,7 +319,7 @@ def _attend(a: _Query, selected: Optional[torch.Tensor], scale: Optional[float],
     device = a.table.device
     ws, ws_ptr = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
     out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
-    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, *a.args,
+    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, a.packed,
           None if selected is None else selected.data_ptr(), 0 if selected is None else selected.shape[2], S, scale,
           out.data_ptr(), ws_ptr, 0 if ws is None else ws.numel())
     return out
@@ -360,7 +364,7 @@ def _select(a: _Query, count: int, first: int, last: int) -> torch.Tensor:
     device = a.table.device
     ws, ws_ptr = _scratch(_select_bytes(a.B, a.Hkv, a.P), device)
     chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
-    _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, *a.args, count, first, last, chosen.data_ptr(),
+    _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, a.packed, count, first, last, chosen.data_ptr(),
           ws_ptr, 0 if ws is None else ws.numel())
     return chosen
 

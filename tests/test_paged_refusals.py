@@ -99,41 +99,62 @@ def test_no_backward():
             call()
 
 
-def _c_pool(**kw):
-    a = dict(k=256, v=256, k_scale=None, v_scale=None, k_bounds=None, k_page=2 * 16 * 32, v_page=2 * 16 * 32, n_pages=4,
+_POOL, _TENSOR4, _QUERY = "PPPPPqqiiiii4x", "Pqqq", "PqPPiiii"  # include/pfa_hip.h
+
+
+def _fields(**kw):
+    a = dict(k=256, v=256, k_scale=0, v_scale=0, k_bounds=0, k_page=2 * 16 * 32, v_page=2 * 16 * 32, n_pages=4,
              kv_heads=2, page_size=16, head_dim=32, dtype=_hip.PFA_F32)
     a.update(kw)
-    return struct.pack("PPPPPqqiiiii4x", *(x or 0 for x in a.values()))
+    return list(a.values())
+
+
+def _c_pool(**kw):
+    return struct.pack(_POOL, *_fields(**kw))
+
+
+def _c_query(pool=None, q=256, table=256, lengths=256, P=2, B=1, H=2, tag=_hip.PFA_F32):
+    return struct.pack(_POOL + _TENSOR4 + _QUERY, *_fields(**(pool or {})), q, 64, 32, 0, table, P, lengths, 0, P, B, H, tag)
 
 
 def test_c_entries_refuse_before_any_launch():
     lib = _hip.lib()
-    t4 = struct.pack("Pqqq", 256, 64, 32, 32)
+    t4 = struct.pack(_TENSOR4, 256, 64, 32, 32)
     p = ctypes.c_void_p(256)  # never dereferenced
 
-    def attend(pool, q=t4, tag=_hip.PFA_F32, B=1, H=2, P=2, n=-1, out=p, lengths=p):
-        return lib.pfa_paged_attn_fwd(q, tag, B, H, pool, p, P, P, lengths, None, None, max(n, 0), n, 0.5, out, p, 1 << 40, None)
+    def attend(pool=None, n=-1, out=p, selected=None, stride=0, scale=0.5, **kw):
+        return lib.pfa_paged_attn_fwd(_c_query(pool, **kw), selected, stride, n, scale, out, p, 1 << 40, None)
 
-    bad = [attend(_c_pool(head_dim=48)), attend(_c_pool(page_size=48)), attend(_c_pool(n_pages=0)),
-           attend(_c_pool(dtype=9)), attend(_c_pool(dtype=_hip.PFA_I8)), attend(_c_pool(k=264)),
-           attend(_c_pool(k_page=100)), attend(_c_pool(), B=-1), attend(_c_pool(), B=70000), attend(_c_pool(), H=3),
-           attend(_c_pool(), H=0), attend(_c_pool(), tag=_hip.PFA_BF16), attend(_c_pool(), P=1 << 28),
-           attend(_c_pool(), n=2), attend(_c_pool(), out=None), attend(_c_pool(), lengths=None),
-           lib.pfa_kv_pages_select(t4, 0, 1, 2, _c_pool(), p, 2, 2, p, None, 2, 1, 1, p, p, 1 << 40, None),
-           lib.pfa_kv_pages_select(t4, 0, 1, 2, _c_pool(k_bounds=256), p, 2, 2, p, None, 2, 2, 1, p, p, 1 << 40, None),
+    def select(count, first, last, pool=None, ws=1 << 40, **kw):
+        return lib.pfa_kv_pages_select(_c_query(pool, **kw), count, first, last, p, p, ws, None)
+
+    bad = [attend(dict(head_dim=48)), attend(dict(page_size=48)), attend(dict(n_pages=0)), attend(dict(dtype=9)),
+           attend(dict(dtype=_hip.PFA_I8)), attend(dict(k=264)), attend(dict(k_page=100)), attend(dict(kv_heads=0)),
+           attend(B=-1), attend(B=70000), attend(H=3), attend(H=0), attend(tag=_hip.PFA_BF16), attend(tag=_hip.PFA_I8),
+           attend(P=1 << 28), attend(P=-1), attend(n=2), attend(n=2, selected=p, stride=1),
+           attend(n=1 << 28, selected=p, stride=1 << 28), attend(out=None), attend(lengths=0), attend(q=0),
+           attend(table=0), attend(scale=0.0), attend(scale=math.inf), attend(scale=math.nan), attend(scale=-1.0),
+           attend(B=60000, H=60),
+           lib.pfa_paged_attn_fwd(None, None, 0, -1, 0.5, p, p, 0, None),
+           select(2, 1, 1), select(2, 2, 1, dict(k_bounds=256)), select(0, 0, 0, dict(k_bounds=256)),
+           select(2, -1, 1, dict(k_bounds=256)), lib.pfa_kv_pages_select(None, 2, 1, 1, p, p, 0, None),
            lib.pfa_kv_pages_read(_c_pool(), 1, -1, p, 2, 2, p, p, p, p, 0, None),
            lib.pfa_kv_pages_read(_c_pool(), 1, 5, p, 2, 2, p, p, p, p, _hip.PFA_I8, None),
+           lib.pfa_kv_pages_read(None, 1, 5, p, 2, 2, p, p, p, p, 0, None),
            lib.pfa_kv_pages_write(_c_pool(), t4, t4, _hip.PFA_F16, 1, 3, p, 2, 2, p, p, None),
-           lib.pfa_kv_pages_write(_c_pool(), t4, t4, _hip.PFA_F32, 1, 3, p, 2, 2, None, p, None)]
+           lib.pfa_kv_pages_write(_c_pool(), t4, t4, _hip.PFA_F32, 1, 3, p, 2, 2, None, p, None),
+           lib.pfa_kv_pages_write(_c_pool(), None, t4, _hip.PFA_F32, 1, 3, p, 2, 2, p, p, None)]
     assert bad == [-1] * len(bad)
-    rc = lib.pfa_kv_pages_select(t4, 0, 1, 2, _c_pool(k_bounds=256), p, 600, 600, p, None, 2, 1, 1, p, p, 4, None)
-    assert rc == -3
+    # workspaces: too small, or not aligned
+    assert select(2, 1, 1, dict(k_bounds=256), P=600, ws=4) == -3
+    assert lib.pfa_paged_attn_fwd(_c_query(P=6000), None, 0, -1, 0.5, p, p, 4, None) == -3
+    assert lib.pfa_paged_attn_fwd(_c_query(P=6000), None, 0, -1, 0.5, p, ctypes.c_void_p(264), 1 << 40, None) == -3
     size = ctypes.c_size_t(0)
     sizes = [(1, 4, 2, 16, 32, _hip.PFA_F32, 100, -1), (1, 3, 2, 16, 32, 0, 100, -1), (1, 4, 2, 24, 32, 0, 100, -1),
              (1, 4, 2, 16, 48, 0, 100, -1), (1, 4, 2, 16, 32, 7, 100, -1), (-1, 4, 2, 16, 32, 0, 100, -1)]
     assert [lib.pfa_paged_attn_workspace_size(*x, ctypes.byref(size)) for x in sizes] == [0] + [-1] * 5
     # nothing to do: no launch, no error
-    assert attend(_c_pool(), B=0) == 0
+    assert attend(B=0) == 0
     assert lib.pfa_kv_pages_write(_c_pool(), t4, t4, 0, 1, 0, p, 2, 2, p, p, None) == 0
     assert lib.pfa_kv_pages_read(_c_pool(), 0, 5, p, 2, 2, p, p, p, p, 0, None) == 0
 
