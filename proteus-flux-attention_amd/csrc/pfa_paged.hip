@@ -449,9 +449,9 @@ extern "C" int pfa_kv_pages_select(const pfa_paged_query* query, int count, int 
     const auto* qp = (const typename Elem<QT>::T*)q->ptr;
     by_width(D, [&](auto width) {
       constexpr int W = decltype(width)::value;
-      const int spans = (P + score_span(4, W, BT) - 1) / score_span(4, W, BT);
+      const int spans = (P + score_span(4, W) - 1) / score_span(4, W);
       // four waves where two rounds of theirs cover a row
-      if (P <= 2 * score_span(4, W, BT) && P <= kFused)
+      if (P <= 2 * score_span(4, W) && P <= kFused)
         select_kernel<QT, BT, W, 256><<<rows, 256, 0, as_stream(stream)>>>(
             p, t.ids, t.stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else if (P <= kFused)

@@ -25,9 +25,11 @@ __device__ __forceinline__ Span span_at(const int32_t* lengths, const int32_t* s
 }
 
 constexpr int kScoreHeads = 8;  // query heads in LDS at once
-constexpr int kPair = 1;         // query heads at once
-// pages of a lane at once
-__host__ __device__ constexpr int steps_of(int bt) { return bt == PFA_F32 ? 4 : 4; }
+constexpr int kSteps = 4;        // pages of a lane at once
+// Query heads at once.  f32 bounds leave three waves a SIMD, whose products wait for
+// one another less with two (15.4 -> 14.1 us at 15,000 pages and heads, eight query
+// heads); 16-bit bounds leave eight (27.6 -> 29.2 at 196,608, four query heads).
+__host__ __device__ constexpr int pair_of(int bt) { return bt == PFA_F32 ? 2 : 1; }
 
 // The value of lane ^ MASK, 64 bits: a quad permute, or a swizzle.
 template <int MASK>
@@ -64,7 +66,7 @@ __device__ __forceinline__ void spread(double* sum, int lane) {
 }
 
 // Scores.  D / 8 lanes hold a page's two bounds of a head, eight channels each,
-// of `steps_of` pages at once, and go over the query heads; sums are 64 bits, so
+// of kSteps pages at once, and go over the query heads; sums are 64 bits, so
 // that the order of the summands decides nothing that is not equal to 2^-53:
 // with bf16 or f16 values the sums are as good as always exact.  The bounds are
 // read once for all heads of a group; a channel is a select, a widening and a
@@ -84,7 +86,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
   constexpr int PW = kWave / LP;  // pages of a wave at once
   using BoundT = typename Elem<BT>::T;
   const int tid = threadIdx.x, lane = tid & 63, part = lane % LP;
-  constexpr int STEPS = steps_of(BT);
+  constexpr int STEPS = kSteps, PAIR = pair_of(BT);
   const int page0 = base + (tid >> 6) * STEPS * PW + lane / LP;  // of step s: + s * PW
   // the first heads' queries, on their way before the bounds are waited for
   constexpr int QN = kScoreHeads * D / (WAVES * kWave) > 0 ? kScoreHeads * D / (WAVES * kWave) : 1;
@@ -125,7 +127,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
   }
   // NV sums of a lane, heads first; each exchange leaves a lane half of them, until
   // one is left or the lanes are through: KEEP of them, from value `mine` on
-  constexpr int NV = kPair * STEPS, SPLITS = LP >= NV ? NV : LP, KEEP = NV / SPLITS;
+  constexpr int NV = PAIR * STEPS, SPLITS = LP >= NV ? NV : LP, KEEP = NV / SPLITS;
   float best[KEEP];
   bool nan[KEEP];
 #pragma unroll
@@ -136,12 +138,12 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
     __syncthreads();
     store_q(heads);
     __syncthreads();
-    for (int g = 0; g < (busy ? heads : 0); g += kPair) {
+    for (int g = 0; g < (busy ? heads : 0); g += PAIR) {
       double sum[NV] = {};
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int u = 0; u < kPair; ++u) {
+        for (int u = 0; u < PAIR; ++u) {
           const float x = qs[g + u < heads ? g + u : heads - 1][8 * part + i];  // an odd last head counts twice
           const bool up = x > 0.0f;
           const double xd = x;
@@ -162,7 +164,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
   int mine = 0;
 #pragma unroll
   for (int o = 1; o < SPLITS; o <<= 1) mine += part & o ? NV / (2 * o) : 0;
-  if constexpr (kPair == 2) {
+  if constexpr (PAIR == 2) {
 #pragma unroll
     for (int s = 0; s < KEEP; ++s) {
       best[s] = fmaxf(best[s], __shfl_xor(best[s], 1));
@@ -187,7 +189,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
 }
 
 // Pages of a workgroup of `waves` waves at once.
-__host__ __device__ constexpr int score_span(int waves, int D, int bt) { return waves * (kWave / (D / 8)) * steps_of(bt); }
+__host__ __device__ constexpr int score_span(int waves, int D) { return waves * (kWave / (D / 8)) * kSteps; }
 
 template <int QT, int BT, int D>
 __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __restrict__ table, int64_t table_stride,
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
                                                     int64_t row_keys, uint32_t* __restrict__ keys) {
   const int b = blockIdx.z, h = blockIdx.x;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
-  constexpr int SPAN = score_span(4, D, BT);
+  constexpr int SPAN = score_span(4, D);
   __shared__ float qs[kScoreHeads][D];
   uint32_t* row = keys + ((int64_t)b * pg.H + h) * row_keys;
   for (int base = blockIdx.y * SPAN; base < sp.pe; base += gridDim.y * SPAN) {
@@ -402,7 +404,7 @@ __global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
   __shared__ uint32_t keys[kFused];
-  for (int base = 0; base < P; base += score_span(THREADS / kWave, D, BT))
+  for (int base = 0; base < P; base += score_span(THREADS / kWave, D))
     score_pages<QT, BT, D, THREADS / kWave>(pg, table + b * table_stride, P, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
                                [&](int page, uint32_t key) { keys[page] = key; });
   __syncthreads();
