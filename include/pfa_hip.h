@@ -725,6 +725,15 @@ int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, siz
 int pfa_kv_pages_select(const pfa_paged_query* query, int count, int first, int last,
                         int32_t* chosen, void* workspace, size_t ws_bytes, void* stream);
 
+/* pfa_kv_pages_select, and pfa_paged_attn_fwd over what it chooses: chosen (B,
+ * kv_heads, count) and out (B, H, D).  Short rows take one launch. */
+int pfa_paged_sparse_attn_workspace_size(int B, int H, int kv_heads, int page_size,
+                                         int head_dim, int cell_dtype, int table_pages,
+                                         int count, size_t* bytes);
+int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count, int first, int last,
+                              float scale, int32_t* chosen, void* out, void* workspace,
+                              size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

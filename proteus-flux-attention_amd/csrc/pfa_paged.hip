@@ -422,15 +422,20 @@ extern "C" int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table
   return PFA_OK;
 }
 
+static int choice_check(const char* what, const Pages& p, int count, int first, int last) {
+  PFA_CHECK_ARG(p.bounds, "%s: the pool has no key bounds", what);
+  PFA_CHECK_ARG(count > 0 && first >= 0 && last >= 0 && first <= count && last <= count - first,
+                "%s: count > 0 pages, the %d first and %d last among them (got %d)", what, first, last, count);
+  return PFA_OK;
+}
+
 extern "C" int pfa_kv_pages_select(const pfa_paged_query* query, int count, int first, int last, int32_t* chosen,
                                    void* workspace, size_t ws_bytes, void* stream) {
   clear_error();
   Pages p;
   Table t;
   if (int rc = query_check("kv_pages_select", query, &p, &t)) return rc;
-  PFA_CHECK_ARG(p.bounds, "kv_pages_select: the pool has no key bounds");
-  PFA_CHECK_ARG(count > 0 && first >= 0 && last >= 0 && first <= count && last <= count - first,
-                "kv_pages_select: count > 0 pages, the %d first and %d last among them (got %d)", first, last, count);
+  if (int rc = choice_check("kv_pages_select", p, count, first, last)) return rc;
   const int B = query->B, H = query->H, D = query->pages.head_dim, P = query->table_pages;
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(chosen, "kv_pages_select: null argument");
@@ -451,7 +456,7 @@ extern "C" int pfa_kv_pages_select(const pfa_paged_query* query, int count, int 
       constexpr int W = decltype(width)::value;
       const int spans = (P + score_span(4, W) - 1) / score_span(4, W);
       // four waves where two rounds of theirs cover a row
-      if (P <= 2 * score_span(4, W) && P <= kFused)
+      if (few_pages(P, W))
         select_kernel<QT, BT, W, 256><<<rows, 256, 0, as_stream(stream)>>>(
             p, t.ids, t.stride, P, qp, q->s_b, q->s_h, H / p.H, lengths, starts, first, last, count, chosen);
       else if (P <= kFused)
@@ -487,6 +492,34 @@ extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int pag
   return PFA_OK;
 }
 
+// The workgroups that attend select their pages themselves: a workgroup a pair,
+// 16 query heads at most, and few pages.
+static bool selects_itself(const Plan& plan, int P, int D) {
+  return plan.bytes == 0 && plan.deal.RT == 1 && few_pages(P, D);
+}
+
+static int attend(const char* what, const pfa_paged_query* query, const Pages& p, const Table& t, const int32_t* selected,
+                  int64_t selected_stride, int S, const Choice& choice, float scale, void* out, void* workspace,
+                  size_t ws_bytes, void* stream) {
+  const float c = scale * 1.44269504088896340736f;
+  PFA_CHECK_ARG(c > 0.0f && c < INFINITY, "%s: scale must be positive and finite", what);
+  const int B = query->B, H = query->H, D = query->pages.head_dim, ct = query->pages.dtype;
+  if (B == 0) return PFA_OK;
+  PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "%s: null or unaligned argument", what);
+  const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D));
+  if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
+    set_error("%s: workspace of %zu bytes, %zu needed, 16-byte aligned", what, ws_bytes, plan.bytes);
+    return PFA_E_WORKSPACE;
+  }
+  const AttendCall a{p, t.ids, t.stride, t.P, B, H, D, query->q, query->lengths, query->starts, selected,
+                     selected_stride, S, c, choice, out, (float*)workspace, as_stream(stream)};
+  if (ct == PFA_I8) attend_i8(query->dtype, a);
+  else if (ct == PFA_E4M3) attend_e4m3(query->dtype, a);
+  else attend_float(query->dtype, a);
+  PFA_CHECK_LAUNCH(what);
+  return PFA_OK;
+}
+
 extern "C" int pfa_paged_attn_fwd(const pfa_paged_query* query, const int32_t* selected, int64_t selected_stride,
                                   int n_selected, float scale, void* out, void* workspace, size_t ws_bytes,
                                   void* stream) {
@@ -497,22 +530,43 @@ extern "C" int pfa_paged_attn_fwd(const pfa_paged_query* query, const int32_t* s
   PFA_CHECK_ARG(n_selected <= 0 || (selected && selected_stride >= n_selected),
                 "paged_attn: lists that are null or overlap");
   PFA_CHECK_ARG((int64_t)n_selected << p.shift <= (1ll << 30), "paged_attn: lists of up to 2^30 positions");
-  const float c = scale * 1.44269504088896340736f;
-  PFA_CHECK_ARG(c > 0.0f && c < INFINITY, "paged_attn: scale must be positive and finite");
-  const int B = query->B, H = query->H, D = query->pages.head_dim, ct = query->pages.dtype;
-  if (B == 0) return PFA_OK;
-  PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "paged_attn: null or unaligned argument");
-  const int S = n_selected < 0 ? -1 : n_selected;
-  const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D));
-  if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
-    set_error("paged_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, plan.bytes);
+  return attend("paged_attn", query, p, t, selected, selected_stride, n_selected < 0 ? -1 : n_selected, Choice{}, scale,
+                out, workspace, ws_bytes, stream);
+}
+
+extern "C" int pfa_paged_sparse_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
+                                                    int cell_dtype, int table_pages, int count, size_t* bytes) {
+  size_t select = 0;
+  if (int rc = pfa_paged_attn_workspace_size(B, H, kv_heads, page_size, head_dim, cell_dtype, table_pages,
+                                             count < table_pages ? count : table_pages, bytes))
+    return rc;
+  PFA_CHECK_ARG(count > 0, "paged_sparse_attn: count > 0 pages (got %d)", count);
+  if (int rc = pfa_kv_pages_select_workspace_size(B, kv_heads, table_pages, &select)) return rc;
+  if (select > *bytes) *bytes = select;  // one after the other
+  return PFA_OK;
+}
+
+extern "C" int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count, int first, int last, float scale,
+                                         int32_t* chosen, void* out, void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  Pages p;
+  Table t;
+  if (int rc = query_check("paged_sparse_attn", query, &p, &t)) return rc;
+  if (int rc = choice_check("paged_sparse_attn", p, count, first, last)) return rc;
+  const int B = query->B, H = query->H, D = query->pages.head_dim;
+  PFA_CHECK_ARG(scale > 0.0f && scale < INFINITY, "paged_sparse_attn: scale must be positive and finite");
+  PFA_CHECK_ARG(B == 0 || (chosen && out && (uintptr_t)out % 16 == 0), "paged_sparse_attn: null or unaligned argument");
+  size_t need = 0;
+  if (int rc = pfa_paged_sparse_attn_workspace_size(B, H, p.H, p.ps, D, query->pages.dtype, t.P, count, &need)) return rc;
+  if (ws_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16 != 0))) {
+    set_error("paged_sparse_attn: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
     return PFA_E_WORKSPACE;
   }
-  const AttendCall a{p, t.ids, t.stride, t.P, B, H, D, query->q, query->lengths, query->starts, selected,
-                     selected_stride, S, c, out, (float*)workspace, as_stream(stream)};
-  if (ct == PFA_I8) attend_i8(query->dtype, a);
-  else if (ct == PFA_E4M3) attend_e4m3(query->dtype, a);
-  else attend_float(query->dtype, a);
-  PFA_CHECK_LAUNCH("paged_attn");
-  return PFA_OK;
+  const int S = count < t.P ? count : t.P;  // no row holds more than its table does
+  Choice choice{};
+  if (selects_itself(attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(query->pages.dtype, D)), t.P, D))
+    choice = Choice{count, first, last, chosen};
+  else if (int rc = pfa_kv_pages_select(query, count, first, last, chosen, workspace, ws_bytes, stream))
+    return rc;
+  return attend("paged_sparse_attn", query, p, t, chosen, count, S, choice, scale, out, workspace, ws_bytes, stream);
 }

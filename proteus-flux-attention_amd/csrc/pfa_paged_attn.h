@@ -35,6 +35,7 @@
 #pragma once
 
 #include "pfa_paged.h"
+#include "pfa_paged_select.h"
 
 namespace pfa {
 namespace paged {
@@ -474,12 +475,21 @@ __device__ __forceinline__ float* part_slot(float* parts, int64_t slot, int rows
   return parts + slot * rows * (D + 2);
 }
 
-template <typename F>
+// What paged_sparse_attention chooses before it attends.
+struct Choice {
+  int count, first, last;
+  int32_t* chosen;
+};
+
+// SELECT: the workgroup first selects its pair's pages itself, for a launch and
+// several dependent loads less.
+template <typename F, bool SELECT>
 __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     Pages pg, Deal deal, const int32_t* __restrict__ table, int64_t table_stride,
     const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int q_vec, int G,
     const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts, const int32_t* __restrict__ selected,
-    int64_t selected_stride, float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws, Shared* __restrict__ shared) {
+    int64_t selected_stride, float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws, Shared* __restrict__ shared,
+    Choice choice) {
   constexpr int D = F::D;
   __shared__ float so[kWaves][16][D + 4];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
@@ -563,6 +573,18 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     at = 0;
   }
   const bool lone = !parts_ws;
+  __shared__ int32_t own[SELECT ? kFused : 1];  // the list of an own selection
+  if constexpr (SELECT) {
+    const int h = blockIdx.x % deal.R;
+    int32_t* chosen = choice.chosen + (int64_t)blockIdx.x * choice.count;
+    select_row<F::QT, bound_dtype(F::CT), D, 64 * kWaves>(
+        pg, table + b * table_stride, deal.P, b, h, q + b * q_b, q_h, G, lengths, starts, choice.first, choice.last,
+        choice.count, [&](int i, int entry) {
+          chosen[i] = entry;
+          if (i < deal.S) own[i] = entry;
+        });
+    __syncthreads();
+  }
 
   while (f < f1) {
     const int start = deal.begin(starts, b), len = deal.length(lengths, b);
@@ -600,7 +622,8 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       if (r0 > t0 + ta) __syncthreads();  // the last run's are read
       for (int i = tid; i < n; i += 64 * kWaves) {
         int ordinal = r.first + i;
-        if (deal.S >= 0) ordinal = ordinal < deal.S ? list[ordinal] : -1;
+        if constexpr (SELECT) ordinal = ordinal < deal.S ? own[ordinal] : -1;
+        else if (deal.S >= 0) ordinal = ordinal < deal.S ? list[ordinal] : -1;
         const int id = (uint32_t)ordinal < (uint32_t)deal.P ? ids[ordinal] : -1;
         const bool ok = (uint32_t)id < (uint32_t)pg.n_pages;
         entries[i] = Entry{ok ? id : 0, ok ? ordinal << deal.shift : kNowhere};
@@ -761,6 +784,7 @@ struct AttendCall {
   int64_t selected_stride;
   int S;
   float c;  // scale * log2(e)
+  Choice choice;  // count 0: none
   void* out;
   float* parts;
   hipStream_t stream;
@@ -811,16 +835,19 @@ void attend_launch(const AttendCall& a) {
   using T = typename Elem<QT>::T;
   Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE);
   Deal& deal = p.deal;
-  static const int at_once = resident(reinterpret_cast<const void*>(&attend_kernel<F>), 64 * kWaves);
+  static const int at_once = resident(reinterpret_cast<const void*>(&attend_kernel<F, false>), 64 * kWaves);
   if (deal.groups > at_once) deal.groups = at_once;
   const int G = a.H / a.pg.H;
   const unsigned pairs = (unsigned)(a.B * deal.R);
   Shared* shared = reinterpret_cast<Shared*>(reinterpret_cast<char*>(a.parts) + p.parts);
   const bool q_vec = ((uintptr_t)a.q.ptr | (uintptr_t)(a.q.s_b * sizeof(T)) | (uintptr_t)(a.q.s_h * sizeof(T))) % 16 == 0;
-  attend_kernel<F><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
-      a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts, a.selected,
-      a.selected_stride, a.c,
-      (T*)a.out, p.bytes ? a.parts : nullptr, shared);
+  auto launch = [&](auto select) {
+    attend_kernel<F, decltype(select)::value><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
+        a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts,
+        a.selected, a.selected_stride, a.c, (T*)a.out, p.bytes ? a.parts : nullptr, shared, a.choice);
+  };
+  if (a.choice.count > 0) launch(std::integral_constant<bool, true>{});
+  else launch(std::integral_constant<bool, false>{});
   if (!p.bytes) return;
   const dim3 rows(pairs, pairs >= kMany ? 1 : G < 16 ? G : 16);
   // a row of a few pairs has parts by the hundred

@@ -239,9 +239,10 @@ __device__ __forceinline__ int block_scan(int x, int* sums, int& all) {
 }
 
 // fetch(r, x): the K keys of the thread's entries from + (r * THREADS + thread) * K
-// on in round r, kNone where there are none.
-template <int THREADS, int K, bool HELD, typename Fetch>
-__device__ __forceinline__ void choose_best(int from0, int rounds, int count, int32_t* __restrict__ out, Fetch&& fetch) {
+// on in round r, kNone where there are none.  put(i, entry): the i-th choice, -1
+// behind the last.
+template <int THREADS, int K, bool HELD, typename Fetch, typename Put>
+__device__ __forceinline__ void choose_best(int from0, int rounds, int count, Fetch&& fetch, Put&& put) {
   constexpr int WAVES = THREADS / kWave;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ int hist[kBins];
@@ -352,14 +353,14 @@ __device__ __forceinline__ void choose_best(int from0, int rounds, int count, in
 #pragma unroll
     for (int i = 0; i < K; ++i) {
       const bool tie = ties > 0 && x[i] == over;
-      if (x[i] > over || (tie && eq < ties)) out[at++] = p + i;
+      if (x[i] > over || (tie && eq < ties)) put(at++, p + i);
       eq += tie;
     }
     const int eqs = all & 0xffff, left = ties > tied ? ties - tied : 0;
     base += (all >> 16) + (eqs < left ? eqs : left);
     tied += eqs;
   });
-  for (int i = base + tid; i < count; i += THREADS) out[i] = -1;
+  for (int i = base + tid; i < count; i += THREADS) put(i, -1);
 }
 
 template <int THREADS, int K, bool HELD>
@@ -372,8 +373,8 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
   const Span sp = span_at(lengths, starts, P, shift, blockIdx.x / H);
   const int from0 = HELD ? 0 : sp.p0 & ~3;  // rows of keys are 16-byte aligned
   const int rounds = HELD ? 1 : (sp.pe - from0 + THREADS * K - 1) / (THREADS * K);
-  choose_best<THREADS, K, HELD>(from0, rounds, count, chosen + (int64_t)blockIdx.x * count,
-                                [&](int r, uint32_t (&x)[K]) {
+  int32_t* out = chosen + (int64_t)blockIdx.x * count;
+  auto fetch = [&](int r, uint32_t (&x)[K]) {
     const int p = from0 + (r * THREADS + (int)threadIdx.x) * K;
 #pragma unroll
     for (int i = 0; i < K; i += 4) {
@@ -385,7 +386,8 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
 #pragma unroll
     for (int i = 0; i < K; ++i)
       if (p + i < sp.p0 || p + i >= sp.pe) x[i] = kNone;
-  });
+  };
+  choose_best<THREADS, K, HELD>(from0, rounds, count, fetch, [&](int i, int entry) { out[i] = entry; });
 }
 
 // Both for rows of up to kFused pages, a workgroup a row with the keys in LDS: a
@@ -393,27 +395,43 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
 // channels, 8 rows: 9.1 us against 4.0 + 5.4).
 constexpr int kFused = 512;
 
-template <int QT, int BT, int D, int THREADS>
-__global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t* __restrict__ table,
-                                                      int64_t table_stride, int P,
-                                                      const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
-                                                      int64_t q_h, int G, const int32_t* __restrict__ lengths,
-                                                      const int32_t* __restrict__ starts, int first, int last,
-                                                      int count, int32_t* __restrict__ chosen) {
-  const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H, tid = threadIdx.x;
+// Scores and choice of one row, for a workgroup of THREADS.
+template <int QT, int BT, int D, int THREADS, typename Put>
+__device__ __forceinline__ void select_row(const Pages& pg, const int32_t* __restrict__ ids, int P, int b, int h,
+                                           const typename Elem<QT>::T* __restrict__ q, int64_t q_h, int G,
+                                           const int32_t* lengths, const int32_t* starts, int first, int last, int count,
+                                           Put&& put) {
+  const int tid = threadIdx.x;
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
   __shared__ uint32_t keys[kFused];
   for (int base = 0; base < P; base += score_span(THREADS / kWave, D))
-    score_pages<QT, BT, D, THREADS / kWave>(pg, table + b * table_stride, P, sp, h, q + b * q_b, q_h, G, first, last, base, qs,
-                               [&](int page, uint32_t key) { keys[page] = key; });
+    score_pages<QT, BT, D, THREADS / kWave>(pg, ids, P, sp, h, q, q_h, G, first, last, base, qs,
+                                            [&](int page, uint32_t key) { keys[page] = key; });
   __syncthreads();
   constexpr int K = kFused / THREADS > 0 ? kFused / THREADS : 1;
-  choose_best<THREADS, K, true>(0, 1, count, chosen + (int64_t)blockIdx.x * count, [&](int, uint32_t (&x)[K]) {
+  auto fetch = [&](int, uint32_t (&x)[K]) {
 #pragma unroll
     for (int i = 0; i < K; ++i) x[i] = K * tid + i >= sp.p0 && K * tid + i < sp.pe ? keys[K * tid + i] : kNone;
-  });
+  };
+  choose_best<THREADS, K, true>(0, 1, count, fetch, put);
 }
+
+template <int QT, int BT, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t* __restrict__ table,
+                                                         int64_t table_stride, int P,
+                                                         const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
+                                                         int64_t q_h, int G, const int32_t* __restrict__ lengths,
+                                                         const int32_t* __restrict__ starts, int first, int last,
+                                                         int count, int32_t* __restrict__ chosen) {
+  const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H;
+  int32_t* out = chosen + (int64_t)blockIdx.x * count;
+  select_row<QT, BT, D, THREADS>(pg, table + b * table_stride, P, b, h, q + b * q_b, q_h, G, lengths, starts, first, last,
+                                 count, [&](int i, int entry) { out[i] = entry; });
+}
+
+// Rows that four waves select in two rounds.
+__host__ __device__ constexpr bool few_pages(int P, int D) { return P <= kFused && P <= 2 * score_span(4, D); }
 
 }  // namespace paged
 }  // namespace pfa

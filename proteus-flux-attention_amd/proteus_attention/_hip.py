@@ -79,6 +79,8 @@ EXPORTED_SYMBOLS = (
     "pfa_paged_attn_fwd",
     "pfa_kv_pages_select_workspace_size",
     "pfa_kv_pages_select",
+    "pfa_paged_sparse_attn_workspace_size",
+    "pfa_paged_sparse_attn_fwd",
 )
 
 
@@ -176,6 +178,9 @@ _SIGNATURES = {
     "pfa_paged_attn_fwd": ([_vp, _vp, _i64, _i32, _f32, _vp, _vp, _sz, _vp], _i32),
     "pfa_kv_pages_select_workspace_size": ([_i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_kv_pages_select": ([_vp, _i32, _i32, _i32, _vp, _vp, _sz, _vp], _i32),
+    "pfa_paged_sparse_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)],
+                                             _i32),
+    "pfa_paged_sparse_attn_fwd": ([_vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _sz, _vp], _i32),
 }
 
 

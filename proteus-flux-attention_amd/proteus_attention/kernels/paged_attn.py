@@ -181,14 +181,21 @@ def _select_bytes(*sizes: int) -> int:
     return _size_out(_hip.lib().pfa_kv_pages_select_workspace_size, *sizes)
 
 
-def _scratch(nbytes: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int]]:
+@functools.lru_cache(maxsize=256)
+def _sparse_bytes(*sizes: int) -> int:
+    """Workspace of both: as of attention, with the pages to choose."""
+
+    return _size_out(_hip.lib().pfa_paged_sparse_attn_workspace_size, *sizes)
+
+
+def _scratch(nbytes: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
     """A workspace of the call's own, from torch's allocator on the current
-    stream, and its address."""
+    stream, its address and size."""
 
     if nbytes == 0:
-        return None, None
+        return None, None, 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr()
+    return ws, ws.data_ptr(), nbytes
 
 
 def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor,
@@ -311,20 +318,6 @@ def _scale(scale: Optional[float]) -> Optional[float]:
     return scale
 
 
-def _attend(a: _Query, selected: Optional[torch.Tensor], scale: Optional[float], S: int = -1) -> torch.Tensor:
-    """S: the entries of each list that count."""
-
-    if scale is None:
-        scale = 1.0 / math.sqrt(a.D)
-    device = a.table.device
-    ws, ws_ptr = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
-    out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
-    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, a.packed,
-          None if selected is None else selected.data_ptr(), 0 if selected is None else selected.shape[2], S, scale,
-          out.data_ptr(), ws_ptr, 0 if ws is None else ws.numel())
-    return out
-
-
 def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, *,
                     starts: Optional[torch.Tensor] = None, selected: Optional[torch.Tensor] = None,
                     scale: Optional[float] = None) -> torch.Tensor:
@@ -344,11 +337,18 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
         raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
     scale = _scale(scale)
     a = _Query("paged_attention", q, pages, block_table, lengths, starts, selected)
+    S, selected_ptr = -1, None
     if selected is not None:
         if selected.shape[:2] != (a.B, a.Hkv):
             raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
-        return _attend(a, selected.contiguous(), scale, selected.shape[2])
-    return _attend(a, None, scale)
+        selected = selected.contiguous()
+        S, selected_ptr = selected.shape[2], selected.data_ptr()
+    device = a.table.device
+    ws, ws_ptr, ws_bytes = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
+    out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
+    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, a.packed, selected_ptr, S, S,
+          1.0 / math.sqrt(a.D) if scale is None else scale, out.data_ptr(), ws_ptr, ws_bytes)
+    return out
 
 
 def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, int, int]:
@@ -358,15 +358,6 @@ def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, in
     if count < 1 or first < 0 or last < 0 or first + last > count:
         raise ValueError("count must be positive and hold the first and last pages")
     return count, first, last
-
-
-def _select(a: _Query, count: int, first: int, last: int) -> torch.Tensor:
-    device = a.table.device
-    ws, ws_ptr = _scratch(_select_bytes(a.B, a.Hkv, a.P), device)
-    chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
-    _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, a.packed, count, first, last, chosen.data_ptr(),
-          ws_ptr, 0 if ws is None else ws.numel())
-    return chosen
 
 
 def select_kv_pages(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, count: int, *,
@@ -383,8 +374,14 @@ def select_kv_pages(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     better score wins, ties the lower entry.
     """
 
-    sizes = _counted(pages, count, first, last)
-    return _select(_Query("select_kv_pages", q, pages, block_table, lengths, starts), *sizes)
+    count, first, last = _counted(pages, count, first, last)
+    a = _Query("select_kv_pages", q, pages, block_table, lengths, starts)
+    device = a.table.device
+    ws, ws_ptr, ws_bytes = _scratch(_select_bytes(a.B, a.Hkv, a.P), device)
+    chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
+    _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, a.packed, count, first, last, chosen.data_ptr(),
+          ws_ptr, ws_bytes)
+    return chosen
 
 
 def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
@@ -393,11 +390,16 @@ def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.T
     """:func:`paged_attention` over the pages that :func:`select_kv_pages`
     chooses.  Returns the output and the chosen entries."""
 
-    sizes = _counted(pages, count, first, last)
+    count, first, last = _counted(pages, count, first, last)
     scale = _scale(scale)
     a = _Query("paged_sparse_attention", q, pages, block_table, lengths, starts)
-    chosen = _select(a, *sizes)
-    return _attend(a, chosen, scale, min(sizes[0], a.P)), chosen  # no row holds more than its table does
+    device = a.table.device
+    ws, ws_ptr, ws_bytes = _scratch(_sparse_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, count), device)
+    out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
+    chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
+    _call(a.index, "paged_sparse_attn_fwd", _hip.lib().pfa_paged_sparse_attn_fwd, a.packed, count, first, last,
+          1.0 / math.sqrt(a.D) if scale is None else scale, chosen.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes)
+    return out, chosen
 
 
 __all__ = [

@@ -270,6 +270,35 @@ def test_selection_of_equal_pages():
         assert got.tolist() == want + [-1] * (700 - n)
 
 
+@pytest.mark.parametrize("pair", R.PAIRS, ids=R.pair_id)
+@pytest.mark.parametrize("D", [16, 32, 64, 128])
+def test_sparse_attention(pair, D):
+    """Rows that select and attend in one launch, in several, with more heads than
+    a tile has rows, with more pages asked for than there are, and windows."""
+    from proteus_attention import paged_sparse_attention
+
+    dt, cell = pair
+    g = torch.Generator().manual_seed(14)
+    for H, G, ps, lengths, starts, count, first, last in (
+            (2, 1, 16, [700, 0, 1, 16, 33], None, 6, 1, 1), (1, 16, 32, [1000, 40], [100, 39], 9, 2, 3),
+            (2, 17, 16, [300, 90], None, 4, 0, 1), (3, 2, 64, [64, 3], [0, 7], 50, 1, 1),
+            (1, 2, 16, [9000, 100], [33, 0], 70, 0, 0), (1, 1, 256, [700], None, 2, 1, 1)):
+        B = len(lengths)
+        N = sum(-(-n // ps) for n in lengths) + 1
+        pool = R.make_pool(N, H, ps, D, cell, g, bounds=True)
+        table = R.make_table(lengths, ps, N, g)
+        if H == 2:
+            table[0, 3] = -1
+        q = torch.randn(B, H * G, D, generator=g).to(dt)
+        st = None if starts is None else _i32(starts).to(DEV)
+        out, chosen = paged_sparse_attention(q.to(DEV), _pages(pool), table.to(DEV), _i32(lengths).to(DEV), count,
+                                             first=first, last=last, starts=st, scale=0.15)
+        want = R.select(q, pool, table, lengths, starts, count, first, last)
+        assert torch.equal(chosen.cpu(), want), (H, G, ps)
+        ref = R.attend(q, pool, table, lengths, starts, want, scale=0.15)
+        assert R.attend_error(out.cpu(), ref, dt, count * ps) <= 1, (H, G, ps)
+
+
 # ---------------------------------------------------------------------------
 # as they are used together
 # ---------------------------------------------------------------------------

@@ -128,7 +128,14 @@ def test_c_entries_refuse_before_any_launch():
     def select(count, first, last, pool=None, ws=1 << 40, **kw):
         return lib.pfa_kv_pages_select(_c_query(pool, **kw), count, first, last, p, p, ws, None)
 
-    bad = [attend(dict(head_dim=48)), attend(dict(page_size=48)), attend(dict(n_pages=0)), attend(dict(dtype=9)),
+    def sparse(count, first, last, scale=0.5, chosen=p, out=p, ws=1 << 40, pool=None, **kw):
+        return lib.pfa_paged_sparse_attn_fwd(_c_query(pool or dict(k_bounds=256), **kw), count, first, last, scale, chosen,
+                                             out, p, ws, None)
+
+    bad = [sparse(2, 1, 1, pool=dict(head_dim=32)), sparse(0, 0, 0), sparse(2, 2, 1), sparse(2, 1, 1, scale=0.0),
+           sparse(2, 1, 1, scale=math.nan), sparse(2, 1, 1, chosen=None), sparse(2, 1, 1, out=None), sparse(2, 1, 1, H=3),
+           lib.pfa_paged_sparse_attn_fwd(None, 2, 1, 1, 0.5, p, p, p, 0, None),
+           attend(dict(head_dim=48)), attend(dict(page_size=48)), attend(dict(n_pages=0)), attend(dict(dtype=9)),
            attend(dict(dtype=_hip.PFA_I8)), attend(dict(k=264)), attend(dict(k_page=100)), attend(dict(kv_heads=0)),
            attend(B=-1), attend(B=70000), attend(H=3), attend(H=0), attend(tag=_hip.PFA_BF16), attend(tag=_hip.PFA_I8),
            attend(P=1 << 28), attend(P=-1), attend(n=2), attend(n=2, selected=p, stride=1),
@@ -147,6 +154,7 @@ def test_c_entries_refuse_before_any_launch():
     assert bad == [-1] * len(bad)
     # workspaces: too small, or not aligned
     assert select(2, 1, 1, dict(k_bounds=256), P=600, ws=4) == -3
+    assert sparse(2, 1, 1, P=600, ws=4) == -3 and sparse(2, 1, 1, B=0) == 0
     assert lib.pfa_paged_attn_fwd(_c_query(P=6000), None, 0, -1, 0.5, p, p, 4, None) == -3
     assert lib.pfa_paged_attn_fwd(_c_query(P=6000), None, 0, -1, 0.5, p, ctypes.c_void_p(264), 1 << 40, None) == -3
     size = ctypes.c_size_t(0)
