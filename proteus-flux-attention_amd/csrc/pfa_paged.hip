@@ -487,7 +487,7 @@ extern "C" int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int pag
   if (int rc = sizes_check(kv_heads, page_size, head_dim, cell_dtype, table_pages, B)) return rc;
   PFA_CHECK_ARG(bytes && H > 0 && H % kv_heads == 0, "paged_attn: bad sizes");
   *bytes = attend_plan(B, H, kv_heads, head_dim, shift_of(page_size), table_pages, n_selected < 0 ? -1 : n_selected,
-                       attend_tile(cell_dtype, head_dim))
+                       attend_tile(cell_dtype, head_dim), false)
                .bytes;
   return PFA_OK;
 }
@@ -506,7 +506,7 @@ static int attend(const char* what, const pfa_paged_query* query, const Pages& p
   const int B = query->B, H = query->H, D = query->pages.head_dim, ct = query->pages.dtype;
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "%s: null or unaligned argument", what);
-  const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D));
+  const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D), choice.count > 0);
   if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
     set_error("%s: workspace of %zu bytes, %zu needed, 16-byte aligned", what, ws_bytes, plan.bytes);
     return PFA_E_WORKSPACE;
@@ -564,7 +564,7 @@ extern "C" int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count
   }
   const int S = count < t.P ? count : t.P;  // no row holds more than its table does
   Choice choice{};
-  if (selects_itself(attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(query->pages.dtype, D)), t.P, D))
+  if (selects_itself(attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(query->pages.dtype, D), true), t.P, D))
     choice = Choice{count, first, last, chosen};
   else if (int rc = pfa_kv_pages_select(query, count, first, last, chosen, workspace, ws_bytes, stream))
     return rc;

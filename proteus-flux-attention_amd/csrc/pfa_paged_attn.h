@@ -794,21 +794,28 @@ struct AttendCall {
 // once, at most kGroups.
 constexpr int kGroups = 1024;
 constexpr int kLeast = 8;   // places of a chunk
-// Tiles of a pair that one workgroup takes rather than two launches; with pairs for
-// every second unit, more.
-constexpr int kLone = 16, kLoneMany = 32, kMany = 256;
+constexpr int kMany = 256;
+
+// Tiles of a pair that one workgroup takes, rather than workgroups that share the
+// rows out and a join behind them.  Few pairs leave the chip idle soon; two pairs a
+// unit, of lengths near one another, go through it better whole (512 pairs of 1,800
+// keys of 128 bf16 channels: 101 us shared out, 86 whole; 320 of 3,750 keys of 64
+// int8: 50 and 70), and rows that select their pages themselves save two launches
+// (8 pairs of 14 pages of 64 keys: 18 us and 14).
+inline int lone_tiles(int64_t pairs, bool select) { return pairs >= 512 ? 64 : pairs >= kMany || select ? 32 : 16; }
 
 struct Plan {
   Deal deal;
   size_t parts, bytes;  // of the parts, and of the workspace; 0: a workgroup a pair
 };
 
-inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int S, int tile) {
+// select: the call selects its pages first
+inline Plan attend_plan(int B, int H, int kv_heads, int D, int shift, int P, int S, int tile, bool select) {
   Plan p{};
   const int G = H / kv_heads, RT = (G + 15) / 16;
   const int64_t keys = (int64_t)(S >= 0 ? S : P) << shift, most = (keys + tile - 1) / tile;
   p.deal = Deal{B, kv_heads * RT, RT, S, shift, P, tile, kLeast, 0};
-  if (most > ((int64_t)B * p.deal.R >= kMany ? kLoneMany : kLone)) {
+  if (most > lone_tiles((int64_t)B * p.deal.R, select && RT == 1 && few_pages(P, D))) {
     const int64_t chunks = ((most + kStart) * B * p.deal.R + kLeast - 1) / kLeast;
     p.deal.groups = (int)(chunks < kGroups ? chunks : kGroups);
     p.parts = (size_t)p.deal.groups * 2 * (G < 16 ? G : 16) * (D + 2) * 4;
@@ -833,7 +840,7 @@ template <int QT, int CT, int D>
 void attend_launch(const AttendCall& a) {
   using F = Form<QT, CT, D>;
   using T = typename Elem<QT>::T;
-  Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE);
+  Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE, a.choice.count > 0);
   Deal& deal = p.deal;
   static const int at_once = resident(reinterpret_cast<const void*>(&attend_kernel<F, false>), 64 * kWaves);
   if (deal.groups > at_once) deal.groups = at_once;
