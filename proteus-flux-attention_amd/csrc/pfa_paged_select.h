@@ -72,9 +72,9 @@ __device__ __forceinline__ void spread(double* sum, int lane) {
 // read once for all heads of a group; a channel is a select, a widening and a
 // fused multiply-add.  Heads of one page are neighbours in the grid, as their
 // bounds are in memory.  196,608 pages and heads of 128 bf16 channels (100 MB),
-// four query heads each: 31 us; one query head instead of four: 26 us.  Widening
-// the bounds once and two products of max(q, 0) and min(q, 0) a channel: 35 us (160
-// registers, three waves a SIMD); workgroups of one or two waves: 34 us.
+// four query heads each: 28 us, 3.6 TB/s, of which 3 us are three of the four heads'
+// arithmetic.  Widening the bounds once and two products of max(q, 0) and min(q, 0) a
+// channel: 35 us (160 registers, three waves a SIMD); two pages of a lane at once: 31.
 //
 // Pages base .. base + WAVES * 64 / (D / 8) * kSteps - 1 of a workgroup's row; put
 // gets each page of the span and its key.
@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(256) score_kernel(Pages pg, const int32_t* __r
 // 2,048 bins and the bin that holds the last one to take is cut again, until all
 // of a bin or, among equal keys, the lowest entries are taken: mostly two
 // rounds.  A workgroup a row, a thread K entries in a row, in registers where
-// THREADS * K hold all of them (HELD), else read again from the L2 each time.
+// THREADS * K hold all of them (HELD), else read again from the L2 each time.  32
+// rows of 8,192 pages: 8 us, all of it latency.
 constexpr int kBins = 2048;
 
 // Exclusive sum over the workgroup; `all`: the whole.
@@ -391,8 +392,8 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
 }
 
 // Both for rows of up to kFused pages, a workgroup a row with the keys in LDS: a
-// launch (3.5 us of the host) less, in no more time (251 pages of 64
-// channels, 8 rows: 9.1 us against 4.0 + 5.4).
+// launch (3.6 us of the host) less, and 7.6 us against 4.0 + 5.4 for 8 rows of 251
+// pages of 64 channels.
 constexpr int kFused = 512;
 
 // Scores and choice of one row, for a workgroup of THREADS.

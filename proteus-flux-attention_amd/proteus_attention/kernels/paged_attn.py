@@ -330,7 +330,9 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     counts twice.  ``scale`` defaults to 1 / sqrt(head_dim).
 
     Returns ``(B, heads, head_dim)`` in q's type.  A row that sees no key, or
-    none with a score above -inf, is zero.
+    none with a score above -inf, is zero.  What stands in slots that no
+    sequence sees has no effect, whatever it is; a value that is seen and not
+    finite leaves its channel not finite (inf or NaN).
     """
 
     if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32):
