@@ -698,10 +698,10 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 }
 
 // Joins the parts of a pair's rows, a workgroup a row, or a pair where there are
-// many; writes the rows of sequences that see nothing.  Its time is its chain of
-// loads, 4 to 10 us.  Up to 16 parts are a team
+// many; writes the rows of sequences that see nothing.  Up to 16 parts are a team
 // of min(D, 64) lanes' for each row; of more, every team takes some of a row's, and
-// the teams are joined in LDS.  Eight parts' loads go out at once.
+// the teams are joined in LDS.  Eight parts' loads go out at once.  Its time is its
+// chain of loads, 4 to 10 us.
 template <int QT, int THREADS>
 __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float pscale,
                                                        const int32_t* __restrict__ lengths,

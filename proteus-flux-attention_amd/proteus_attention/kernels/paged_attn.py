@@ -117,8 +117,9 @@ def _pool(pages: KVPages) -> tuple:
     if dtype in _EIGHT_BITS:
         if k_scale is None or v_scale is None:
             raise ValueError("8-bit pages need k_scale and v_scale")
-        a = _dense(k_scale, shape[:3], torch.float32, "k_scale")
-        c = _dense(v_scale, shape[:3], torch.float32, "v_scale")
+        rows = shape[:3]
+        a = _dense(k_scale, rows, torch.float32, "k_scale")
+        c = _dense(v_scale, rows, torch.float32, "v_scale")
         bound_dtype = torch.float32
     if bounds is not None:
         b = _dense(bounds, (N, H, 2, D), bound_dtype, "k_bounds")
@@ -348,7 +349,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     device = a.table.device
     ws, ws_ptr, ws_bytes = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
     out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
-    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, a.packed, selected_ptr, S, S,
+    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, a.packed, selected_ptr, max(S, 0), S,
           1.0 / math.sqrt(a.D) if scale is None else scale, out.data_ptr(), ws_ptr, ws_bytes)
     return out
 
