@@ -721,7 +721,8 @@ int pfa_paged_attn_fwd(const pfa_paged_query* query, const int32_t* selected,
  * first and `last` last entries that hold positions to look at come before all
  * others, then the better score, then the lower entry; entries without a page
  * are never chosen. */
-int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int table_pages, size_t* bytes);
+int pfa_kv_pages_select_workspace_size(int B, int kv_heads, int head_dim, int table_pages,
+                                       size_t* bytes);
 int pfa_kv_pages_select(const pfa_paged_query* query, int count, int first, int last,
                         int32_t* chosen, void* workspace, size_t ws_bytes, void* stream);
 

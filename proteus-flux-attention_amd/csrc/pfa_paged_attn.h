@@ -96,7 +96,8 @@ __device__ __forceinline__ uint32_t cells2_bf16(uint32_t w, int i) {
   }
 }
 
-// 32-key groups of a tile.
+// 32-key groups of a tile: 4 KB of keys for rows of 128 bytes and more.  Two groups of
+// such rows leave no registers: 1,000,003 int8 tokens of 128 channels 195 -> 226 us.
 __host__ __device__ constexpr int tile_groups(int ct, int D) { return D * cell_bytes(ct) >= 128 ? 1 : 2; }
 
 // Cells of a call's kernel, by the types of queries and cells and the head's width.
@@ -587,7 +588,8 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   if constexpr (SELECT) {
     const int h = blockIdx.x % deal.R;
     int32_t* chosen = choice.chosen + (int64_t)blockIdx.x * choice.count;
-    select_row<F::QT, bound_dtype(F::CT), D, 64 * kWaves>(
+    static_assert(kWaves == 4, "select_row has four waves");
+    select_row<F::QT, bound_dtype(F::CT), D>(
         pg, table + b * table_stride, deal.P, b, h, q + b * q_b, q_h, G, lengths, starts, choice.first, choice.last,
         choice.count, [&](int i, int entry) {
           chosen[i] = entry;
@@ -753,7 +755,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
     }
     return a;
   };
-  if (who.n <= 16) {  // a team a row
+  // a team a row (43 x 8 pairs of 5 rows in three parts: 4.5 us, 12 with a row at a time)
+  if (who.n <= 16) {
     for (int row = blockIdx.y * teams + team; row < here; row += gridDim.y * teams) {
       const Sum a = gather(row, 0, 1);
       const float inv = a.l == 0.0f ? 0.0f : 1.0f / (a.l * pscale);
@@ -804,7 +807,8 @@ struct AttendCall {
 // Workgroups of a call that shares its rows out: as many as the chip holds at
 // once, at most kGroups (twice as many: 64 ragged sequences 69 us for 63).
 constexpr int kGroups = 1024;
-constexpr int kLeast = 8;   // places of a chunk
+// Places of a chunk, at least (32 pairs of 4,096 listed keys: 22 us, 25 with 16).
+constexpr int kLeast = 8;
 constexpr int kMany = 256;
 
 // Tiles of a pair that one workgroup takes, rather than workgroups that share the
@@ -868,8 +872,9 @@ void attend_launch(const AttendCall& a) {
   else launch(std::integral_constant<bool, false>{});
   if (!p.bytes) return;
   const dim3 rows(pairs, pairs >= kMany ? 1 : G < 16 ? G : 16);
-  // a row of a few pairs has parts by the hundred
-  if (pairs >= 64)
+  // the rows of a few pairs have parts by the hundred (8 pairs of 60,000 keys: 36.6 us
+  // with 16 waves a row, 37.4 with four; 32 of 25,000: 88.6 and 85.8)
+  if (pairs >= 32)
     join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, shared,
                                                      (T*)a.out);
   else

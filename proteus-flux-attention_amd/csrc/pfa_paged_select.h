@@ -391,13 +391,14 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(int H, int P, int64_t r
   choose_best<THREADS, K, HELD>(from0, rounds, count, fetch, [&](int i, int entry) { out[i] = entry; });
 }
 
-// Both for rows of up to kFused pages, a workgroup a row with the keys in LDS: a
-// launch (3.6 us of the host) less, and 7.6 us against 4.0 + 5.4 for 8 rows of 251
-// pages of 64 channels.
+// Both in one workgroup for rows that four waves score in two rounds, with the keys
+// in LDS: a launch (3.6 us of the host) less, and 7.6 us against 4.0 + 5.4 for 8 rows
+// of 251 pages of 64 channels.  Longer rows are quicker apart (8 rows of 501 pages of
+// 128 channels: 25 us with their attention in one, 22 apart).
 constexpr int kFused = 512;
+__host__ __device__ constexpr bool few_pages(int P, int D) { return P <= kFused && P <= 2 * score_span(4, D); }
 
-// Scores and choice of one row, for a workgroup of THREADS.
-template <int QT, int BT, int D, int THREADS, typename Put>
+template <int QT, int BT, int D, typename Put>
 __device__ __forceinline__ void select_row(const Pages& pg, const int32_t* __restrict__ ids, int P, int b, int h,
                                            const typename Elem<QT>::T* __restrict__ q, int64_t q_h, int G,
                                            const int32_t* lengths, const int32_t* starts, int first, int last, int count,
@@ -406,33 +407,29 @@ __device__ __forceinline__ void select_row(const Pages& pg, const int32_t* __res
   const Span sp = span_at(lengths, starts, P, pg.shift, b);
   __shared__ float qs[kScoreHeads][D];
   __shared__ uint32_t keys[kFused];
-  for (int base = 0; base < P; base += score_span(THREADS / kWave, D))
-    score_pages<QT, BT, D, THREADS / kWave>(pg, ids, P, sp, h, q, q_h, G, first, last, base, qs,
-                                            [&](int page, uint32_t key) { keys[page] = key; });
+  for (int base = 0; base < P; base += score_span(4, D))
+    score_pages<QT, BT, D, 4>(pg, ids, P, sp, h, q, q_h, G, first, last, base, qs,
+                              [&](int page, uint32_t key) { keys[page] = key; });
   __syncthreads();
-  constexpr int K = kFused / THREADS > 0 ? kFused / THREADS : 1;
+  constexpr int K = kFused / 256;
   auto fetch = [&](int, uint32_t (&x)[K]) {
 #pragma unroll
     for (int i = 0; i < K; ++i) x[i] = K * tid + i >= sp.p0 && K * tid + i < sp.pe ? keys[K * tid + i] : kNone;
   };
-  choose_best<THREADS, K, true>(0, 1, count, fetch, put);
+  choose_best<256, K, true>(0, 1, count, fetch, put);
 }
 
-template <int QT, int BT, int D, int THREADS>
-__global__ void __launch_bounds__(THREADS) select_kernel(Pages pg, const int32_t* __restrict__ table,
-                                                         int64_t table_stride, int P,
-                                                         const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
-                                                         int64_t q_h, int G, const int32_t* __restrict__ lengths,
-                                                         const int32_t* __restrict__ starts, int first, int last,
-                                                         int count, int32_t* __restrict__ chosen) {
+template <int QT, int BT, int D>
+__global__ void __launch_bounds__(256) select_kernel(Pages pg, const int32_t* __restrict__ table, int64_t table_stride,
+                                                     int P, const typename Elem<QT>::T* __restrict__ q, int64_t q_b,
+                                                     int64_t q_h, int G, const int32_t* __restrict__ lengths,
+                                                     const int32_t* __restrict__ starts, int first, int last, int count,
+                                                     int32_t* __restrict__ chosen) {
   const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H;
   int32_t* out = chosen + (int64_t)blockIdx.x * count;
-  select_row<QT, BT, D, THREADS>(pg, table + b * table_stride, P, b, h, q + b * q_b, q_h, G, lengths, starts, first, last,
-                                 count, [&](int i, int entry) { out[i] = entry; });
+  select_row<QT, BT, D>(pg, table + b * table_stride, P, b, h, q + b * q_b, q_h, G, lengths, starts, first, last, count,
+                        [&](int i, int entry) { out[i] = entry; });
 }
-
-// Rows that four waves select in two rounds.
-__host__ __device__ constexpr bool few_pages(int P, int D) { return P <= kFused && P <= 2 * score_span(4, D); }
 
 }  // namespace paged
 }  // namespace pfa

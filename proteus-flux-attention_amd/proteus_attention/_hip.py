@@ -176,7 +176,7 @@ _SIGNATURES = {
     "pfa_kv_pages_read": ([_vp, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp], _i32),
     "pfa_paged_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_paged_attn_fwd": ([_vp, _vp, _i64, _i32, _f32, _vp, _vp, _sz, _vp], _i32),
-    "pfa_kv_pages_select_workspace_size": ([_i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
+    "pfa_kv_pages_select_workspace_size": ([_i32, _i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_kv_pages_select": ([_vp, _i32, _i32, _i32, _vp, _vp, _sz, _vp], _i32),
     "pfa_paged_sparse_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)],
                                              _i32),

@@ -177,7 +177,7 @@ def _attend_bytes(*sizes: int) -> int:
 
 @functools.lru_cache(maxsize=256)
 def _select_bytes(*sizes: int) -> int:
-    """Workspace of selection: B, kv heads, the table's pages."""
+    """Workspace of selection: B, kv heads, head dim, the table's pages."""
 
     return _size_out(_hip.lib().pfa_kv_pages_select_workspace_size, *sizes)
 
@@ -210,7 +210,8 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     divided by ``scale = max(absmax / top, 1e-6)`` (top 127 for int8, 448 for
     e4m3) and rounded to nearest even.  A row with a value that is not finite
     gets scale NaN, and reads back as NaN.  The pages' key bounds, where the
-    pool has them, follow: they start anew with a page's first slot.
+    pool has them, follow: they start anew with a page's first slot, so a page
+    is written from there on.
 
     Two sequences of one call must not write to one page.
     """
@@ -380,7 +381,7 @@ def select_kv_pages(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     count, first, last = _counted(pages, count, first, last)
     a = _Query("select_kv_pages", q, pages, block_table, lengths, starts)
     device = a.table.device
-    ws, ws_ptr, ws_bytes = _scratch(_select_bytes(a.B, a.Hkv, a.P), device)
+    ws, ws_ptr, ws_bytes = _scratch(_select_bytes(a.B, a.Hkv, a.D, a.P), device)
     chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
     _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, a.packed, count, first, last, chosen.data_ptr(),
           ws_ptr, ws_bytes)
