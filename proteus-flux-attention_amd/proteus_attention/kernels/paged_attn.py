@@ -276,39 +276,42 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     return k, v
 
 
-class _Query:
-    """The checked arguments that selection and attention share, for the
-    library in ``packed``; the tensors stay referenced until the calls are made."""
+def _query(what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
+           starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None) -> tuple:
+    """The arguments that selection and attention share, checked: packed for the
+    library, (B, heads, kv_heads, page size, head dim, cell tag, the table's pages),
+    the device's index, q, and what must stay referenced until the call is made."""
 
-    __slots__ = ("packed", "B", "H", "Hkv", "ps", "D", "P", "cells", "q", "table", "lengths", "starts", "index")
-
-    def __init__(self, what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
-                 starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None) -> None:
-        shape, dtype = q.shape, q.dtype
-        if len(shape) != 3:
-            raise ValueError("q must be a (B, heads, head_dim) tensor: one new token a sequence")
-        self.B, self.H, self.D = B, H, D = shape
-        pool = _pool(pages)
-        _, self.Hkv, self.ps, pool_dim, self.cells = pool[7:]
-        if D != pool_dim or H == 0 or H % self.Hkv:
-            raise ValueError(f"q has {H} heads of {D}, the pages {self.Hkv} of {pool_dim}")
-        tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
-        if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
-            raise ValueError(f"queries of {dtype} for pages of {cells}")
-        self.table = table = _table(block_table, B)
-        self.P = P = table.shape[1]
-        self.lengths = lengths = _per_sequence(lengths, B, "lengths")
-        self.starts = starts = None if starts is None else _per_sequence(starts, B, "starts")
-        if q.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
-        self.index = _device(what, q, *pages, table, lengths, starts, selected)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
+        raise ValueError("q must be a (B, heads, head_dim) tensor: one new token a sequence")
+    B, H, D = shape
+    pool = _pool(pages)
+    _, _, _, _, _, _, _, _, Hkv, ps, pool_dim, cell_tag = pool
+    if D != pool_dim or H == 0 or H % Hkv:
+        raise ValueError(f"q has {H} heads of {D}, the pages {Hkv} of {pool_dim}")
+    tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
+    if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
+        raise ValueError(f"queries of {dtype} for pages of {cells}")
+    table, lengths = _table(block_table, B), _per_sequence(lengths, B, "lengths")
+    P, starts_ptr = table.shape[1], 0
+    if starts is not None:
+        starts = _per_sequence(starts, B, "starts")
+        starts_ptr = starts.data_ptr()
+    if q.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
+    index = _device(what, q, *pages, table, lengths, starts, selected)
+    s = q.stride()
+    if s[2] != 1:
+        q = q.contiguous()
         s = q.stride()
-        if s[2] != 1:
-            q = q.contiguous()
-            s = q.stride()
-        self.q = q
-        self.packed = _QUERY.pack(*pool, q.data_ptr(), s[0], s[1], 0, table.data_ptr(), table.stride(0),
-                                  lengths.data_ptr(), 0 if starts is None else starts.data_ptr(), P, B, H, tag)
+    packed = _QUERY.pack(*pool, q.data_ptr(), s[0], s[1], 0, table.data_ptr(), table.stride(0), lengths.data_ptr(),
+                         starts_ptr, P, B, H, tag)
+    return packed, (B, H, Hkv, ps, D, cell_tag, P), index, q, (table, lengths, starts)
+
+
+def _output(q: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
 def _scale(scale: Optional[float]) -> Optional[float]:
@@ -340,18 +343,17 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32):
         raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
     scale = _scale(scale)
-    a = _Query("paged_attention", q, pages, block_table, lengths, starts, selected)
+    packed, sizes, index, q, keep = _query("paged_attention", q, pages, block_table, lengths, starts, selected)
     S, selected_ptr = -1, None
     if selected is not None:
-        if selected.shape[:2] != (a.B, a.Hkv):
+        if selected.shape[:2] != (sizes[0], sizes[2]):
             raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
         selected = selected.contiguous()
         S, selected_ptr = selected.shape[2], selected.data_ptr()
-    device = a.table.device
-    ws, ws_ptr, ws_bytes = _scratch(_attend_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, S), device)
-    out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
-    _call(a.index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, a.packed, selected_ptr, max(S, 0), S,
-          1.0 / math.sqrt(a.D) if scale is None else scale, out.data_ptr(), ws_ptr, ws_bytes)
+    ws, ws_ptr, ws_bytes = _scratch(_attend_bytes(*sizes, S), q.device)
+    out = _output(q)
+    _call(index, "paged_attn_fwd", _hip.lib().pfa_paged_attn_fwd, packed, selected_ptr, max(S, 0), S,
+          1.0 / math.sqrt(sizes[4]) if scale is None else scale, out.data_ptr(), ws_ptr, ws_bytes)
     return out
 
 
@@ -379,12 +381,11 @@ def select_kv_pages(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     """
 
     count, first, last = _counted(pages, count, first, last)
-    a = _Query("select_kv_pages", q, pages, block_table, lengths, starts)
-    device = a.table.device
-    ws, ws_ptr, ws_bytes = _scratch(_select_bytes(a.B, a.Hkv, a.D, a.P), device)
-    chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
-    _call(a.index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, a.packed, count, first, last, chosen.data_ptr(),
-          ws_ptr, ws_bytes)
+    packed, (B, _, Hkv, _, D, _, P), index, q, keep = _query("select_kv_pages", q, pages, block_table, lengths, starts)
+    ws, ws_ptr, ws_bytes = _scratch(_select_bytes(B, Hkv, D, P), q.device)
+    chosen = torch.empty((B, Hkv, count), dtype=torch.int32, device=q.device)
+    _call(index, "kv_pages_select", _hip.lib().pfa_kv_pages_select, packed, count, first, last, chosen.data_ptr(), ws_ptr,
+          ws_bytes)
     return chosen
 
 
@@ -396,13 +397,12 @@ def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.T
 
     count, first, last = _counted(pages, count, first, last)
     scale = _scale(scale)
-    a = _Query("paged_sparse_attention", q, pages, block_table, lengths, starts)
-    device = a.table.device
-    ws, ws_ptr, ws_bytes = _scratch(_sparse_bytes(a.B, a.H, a.Hkv, a.ps, a.D, a.cells, a.P, count), device)
-    out = torch.empty((a.B, a.H, a.D), dtype=a.q.dtype, device=device)
-    chosen = torch.empty((a.B, a.Hkv, count), dtype=torch.int32, device=device)
-    _call(a.index, "paged_sparse_attn_fwd", _hip.lib().pfa_paged_sparse_attn_fwd, a.packed, count, first, last,
-          1.0 / math.sqrt(a.D) if scale is None else scale, chosen.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes)
+    packed, sizes, index, q, keep = _query("paged_sparse_attention", q, pages, block_table, lengths, starts)
+    ws, ws_ptr, ws_bytes = _scratch(_sparse_bytes(*sizes, count), q.device)
+    out = _output(q)
+    chosen = torch.empty((sizes[0], sizes[2], count), dtype=torch.int32, device=q.device)
+    _call(index, "paged_sparse_attn_fwd", _hip.lib().pfa_paged_sparse_attn_fwd, packed, count, first, last,
+          1.0 / math.sqrt(sizes[4]) if scale is None else scale, chosen.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes)
     return out, chosen
 
 
