@@ -99,6 +99,19 @@ def test_no_backward():
             call()
 
 
+@pytest.mark.parametrize("name", ["k", "v", "k_bounds"])
+def test_no_backward_of_pools(name):
+    p = _new()
+    p = p._replace(**{name: getattr(p, name).clone().requires_grad_()})
+    for call in (lambda: write_kv_pages(p, KV, KV, TABLE, ONE), lambda: read_kv_pages(p, TABLE, ONE, None, 3),
+                 lambda: paged_attention(Q, p, TABLE, ONE), lambda: select_kv_pages(Q, p, TABLE, ONE, 2),
+                 lambda: paged_sparse_attention(Q, p, TABLE, ONE, 2)):
+        with pytest.raises(NotImplementedError):
+            call()
+        with torch.no_grad(), pytest.raises(_hip.HipLibraryError):  # then only the device is wrong
+            call()
+
+
 _POOL, _TENSOR4, _QUERY = "PPPPPqqiiiii4x", "Pqqq", "PqPPiiii"  # include/pfa_hip.h
 
 
