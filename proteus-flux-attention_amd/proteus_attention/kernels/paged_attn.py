@@ -38,6 +38,9 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 _VALUE_TAG = {torch.float32: _hip.PFA_F32, torch.bfloat16: _hip.PFA_BF16, torch.float16: _hip.PFA_F16}
 _CELL_TAG = {**_VALUE_TAG, torch.int8: _hip.PFA_I8, torch.float8_e4m3fn: _hip.PFA_E4M3}
 _EIGHT_BITS = (torch.int8, torch.float8_e4m3fn)
+# Pages of a table or list, sequences: the library takes them in 32 bits and has limits
+# of its own below these, by the page size and the rows.
+_MOST = 1 << 30
 
 
 class KVPages(NamedTuple):
@@ -132,6 +135,8 @@ def _table(block_table: torch.Tensor, B: int) -> torch.Tensor:
     shape = block_table.shape
     if len(shape) != 2 or shape[0] != B or block_table.dtype != torch.int32:
         raise ValueError(f"block_table must be a ({B}, P) int32 tensor")
+    if B > _MOST or shape[1] > _MOST:
+        raise ValueError(f"a block table of up to {_MOST} sequences and pages (got {tuple(shape)})")
     return block_table if block_table.stride(1) == 1 or shape[1] <= 1 else block_table.contiguous()
 
 
@@ -342,8 +347,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     finite leaves its channel not finite (inf or NaN).
     """
 
-    if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32):
-        raise ValueError("selected must be a (B, kv_heads, S) int32 tensor")
+    if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32 or selected.shape[2] > _MOST):
+        raise ValueError(f"selected must be a (B, kv_heads, S) int32 tensor of up to {_MOST} entries a list")
     scale = _scale(scale)
     packed, sizes, index, q, keep = _query("paged_attention", q, pages, block_table, lengths, starts, selected)
     S, selected_ptr = -1, None
@@ -363,8 +368,8 @@ def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, in
     count, first, last = int(count), int(first), int(last)
     if pages[4] is None:
         raise ValueError("selection needs pages with k_bounds")
-    if count < 1 or first < 0 or last < 0 or first + last > count:
-        raise ValueError("count must be positive and hold the first and last pages")
+    if not 1 <= count <= _MOST or first < 0 or last < 0 or first + last > count:
+        raise ValueError(f"count must be positive, at most {_MOST}, and hold the first and last pages")
     return count, first, last
 
 

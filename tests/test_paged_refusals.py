@@ -112,6 +112,27 @@ def test_no_backward_of_pools(name):
             call()
 
 
+WIDE = 2 ** 32 + 1  # 1 in the library's 32-bit arguments
+
+
+def _wide(*shape):
+    return torch.empty(shape, dtype=torch.int32, device="meta")  # no memory behind it
+
+
+@pytest.mark.parametrize("call", [
+    lambda p: select_kv_pages(Q, p, TABLE, ONE, WIDE),
+    lambda p: paged_sparse_attention(Q, p, TABLE, ONE, WIDE),
+    lambda p: paged_attention(Q, p, TABLE, ONE, selected=_wide(1, 2, WIDE)),
+    lambda p: paged_attention(Q, p, _wide(1, WIDE), ONE),
+    lambda p: read_kv_pages(p, _wide(1, WIDE), ONE, None, 3),
+    lambda p: read_kv_pages(p, _wide(WIDE, 1), _wide(WIDE), None, 3),
+    lambda p: write_kv_pages(p, KV, KV, _wide(1, WIDE), ONE),
+])
+def test_sizes_that_pass_32_bits(call):
+    with pytest.raises(ValueError):
+        call(_new())
+
+
 _POOL, _TENSOR4, _QUERY = "PPPPPqqiiiii4x", "Pqqq", "PqPPiiii"  # include/pfa_hip.h
 
 
