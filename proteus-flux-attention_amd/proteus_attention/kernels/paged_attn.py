@@ -126,7 +126,8 @@ def _pool(pages: KVPages) -> tuple:
         bound_dtype = torch.float32
     if bounds is not None:
         b = _dense(bounds, (N, H, 2, D), bound_dtype, "k_bounds")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in pages):
+    if (k.requires_grad or v.requires_grad or (b and bounds.requires_grad)
+            or (a and (k_scale.requires_grad or v_scale.requires_grad))) and torch.is_grad_enabled():
         raise NotImplementedError("pages have no backward pass: call it under torch.no_grad()")
     return k.data_ptr(), v.data_ptr(), a, c, b, ks[0], vs[0], N, H, ps, D, tag
 
