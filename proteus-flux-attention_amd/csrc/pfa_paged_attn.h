@@ -184,7 +184,8 @@ struct Tile {
 };
 
 // A wave's running state: O^T of head n in lane (n, g), channels
-// VD * (4g + i) + j, and the row's maximum and sum (of the lane's own keys).
+// VD * (4g + i) + j, the row's maximum (of the products as they are: the scale is
+// multiplied on when the maximum is off) and sum (of the lane's own keys).
 template <typename F>
 struct State {
   f32x4_t o[F::VD];
@@ -320,12 +321,11 @@ struct Wave {
       for (int y = 0; y < 4; ++y) load_bytes<F::VB>(base + lane_at + y * F::D * F::E, v[i][y]);
       if constexpr (is8(F::CT)) {
         const int64_t at = ((int64_t)t.b[i].id * pg.H) * pg.ps + slot + 4 * g;
-        s[i] = *reinterpret_cast<const f32x4_t*>(pg.k_scale + at) * c;
+        s[i] = *reinterpret_cast<const f32x4_t*>(pg.k_scale + at);
         vs[i] = *reinterpret_cast<const f32x4_t*>(pg.v_scale + at);
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // V is on its way before K is waited for
-    // t = S * c (with the key's scale): base-2 logarithms of the weights
 #pragma unroll
     for (int i = 0; i < 2 * F::NG; ++i) {
       if constexpr (is8(F::CT)) s[i] = scores(i) * s[i];
@@ -333,7 +333,6 @@ struct Wave {
     }
     load_k(pg, h, next);
     __builtin_amdgcn_sched_barrier(0);
-    const float cc = is8(F::CT) ? 1.0f : c;
     if (!t.whole(r)) {
       // keys that are not seen: no weight, and nothing of what stands there
 #pragma unroll
@@ -354,10 +353,10 @@ struct Wave {
     for (int i = 0; i < 2 * F::NG; ++i)
 #pragma unroll
       for (int y = 0; y < 4; ++y) top = fmaxf(top, s[i][y]);
-    top = max_over_rows4(top) * cc;
+    top = max_over_rows4(top);
     if (__any(top > st.m)) {
       const float m = fmaxf(st.m, top);
-      const float alpha = m == -INFINITY ? 1.0f : exp2_(st.m - m);
+      const float alpha = m == -INFINITY ? 1.0f : exp2_((st.m - m) * c);
       st.m = m;
       st.l *= alpha;
 #pragma unroll
@@ -369,7 +368,9 @@ struct Wave {
     for (int i = 0; i < 2 * F::NG; ++i)
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const float p = exp2_(fmaf(s[i][y], cc, -m));
+        // off the maximum first: no exponent is above zero, however large the scores
+        // (s * c - m * c in one rounding can be, by a rounding of m * c)
+        const float p = exp2_((s[i][y] - m) * c);
         sum += p;
         s[i][y] = is8(F::CT) ? p * vs[i][y] : p * F::PSCALE;
       }
@@ -418,8 +419,8 @@ struct Wave {
 // What a workgroup's waves, and then a row's workgroups, are joined by: the
 // weight of a part with maximum m and sum l under the common maximum.  A part
 // without a score above -inf weighs nothing, unless a NaN is in it.
-__device__ __forceinline__ float part_weight(float m, float l, float top) {
-  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2_(m - top);
+__device__ __forceinline__ float part_weight(float m, float l, float top, float c) {
+  return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2_((m - top) * c);
 }
 
 // How the tiles of all rows are dealt out: a pair is a sequence and 16 heads
@@ -681,7 +682,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       float o = 0.0f, sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < kWaves; ++j) {
-        const float a = part_weight(sm[j][row], sl[j][row], top);
+        const float a = part_weight(sm[j][row], sl[j][row], top, c);
         o += a == 0.0f ? 0.0f : a * so[j][row][d];
         sum += a == 0.0f ? 0.0f : a * sl[j][row];
       }
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 // the teams are joined in LDS.  Eight parts' loads go out at once.  Its time is its
 // chain of loads, 4 to 10 us.
 template <int QT, int THREADS>
-__global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float pscale,
+__global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float c, float pscale,
                                                        const int32_t* __restrict__ lengths,
                                                        const int32_t* __restrict__ starts,
                                                        const float* __restrict__ parts,
@@ -744,12 +745,12 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
       float t = a.m;
 #pragma unroll
       for (int u = 0; u < 8; ++u) t = fmaxf(t, m[u]);
-      const float w = part_weight(a.m, a.l, t);
+      const float w = part_weight(a.m, a.l, t, c);
       a.o0 = w == 0.0f ? 0.0f : w * a.o0, a.o1 = w == 0.0f ? 0.0f : w * a.o1, a.l = w == 0.0f ? 0.0f : w * a.l;
       a.m = t;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float p = part_weight(m[u], l[u], t);
+        const float p = part_weight(m[u], l[u], t, c);
         if (p != 0.0f) a.o0 += p * x[u], a.o1 += p * y[u], a.l += p * l[u];
       }
     }
@@ -774,14 +775,14 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
     if (d == 0) tops[team] = a.m, suml[team] = a.l;
     __syncthreads();
     const int used = who.n < teams ? who.n : teams;
-    for (int c = tid; c < D; c += THREADS) {
+    for (int x = tid; x < D; x += THREADS) {
       float t = -INFINITY, o = 0.0f, l = 0.0f;
       for (int w = 0; w < used; ++w) t = fmaxf(t, tops[w]);
       for (int w = 0; w < used; ++w) {
-        const float p = part_weight(tops[w], suml[w], t);
-        if (p != 0.0f) o += p * acc[w * D + c], l += p * suml[w];
+        const float p = part_weight(tops[w], suml[w], t, c);
+        if (p != 0.0f) o += p * acc[w * D + x], l += p * suml[w];
       }
-      store_f<QT>(to + row * D + c, l == 0.0f ? 0.0f : o / (l * pscale));
+      store_f<QT>(to + row * D + x, l == 0.0f ? 0.0f : o / (l * pscale));
     }
     __syncthreads();
   }
@@ -875,10 +876,10 @@ void attend_launch(const AttendCall& a) {
   // the rows of a few pairs have parts by the hundred (8 pairs of 60,000 keys: 36.6 us
   // with 16 waves a row, 37.4 with four; 32 of 25,000: 88.6 and 85.8)
   if (pairs >= 32)
-    join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, shared,
+    join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared,
                                                      (T*)a.out);
   else
-    join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, F::PSCALE, a.lengths, a.starts, a.parts, shared,
+    join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared,
                                                        (T*)a.out);
 }
 
