@@ -27,11 +27,14 @@
 //
 // Precision: f32 stays on v_mfma_f32_16x16x4f32.  8-bit cells are whole in
 // bf16; their scales multiply S and P in f32.  Queries of f16 or f32 on 8-bit
-// cells are split into two or three bf16 parts, which hold all their bits.  P
-// goes in parts of its own, each what the ones before leave: two parts (bf16: 16
-// bits, f16: 22) where the result has 8 or 11 bits, three (24 bits) where it is
-// f32.  f16 parts are scaled by 2^15, so that a probability is whole down to
-// 2^-39 of the row's largest.  Sums, maxima and O are f32 throughout.
+// cells are split into two or three bf16 parts, which hold all their bits.  P goes
+// in three parts, each cut off from what the ones before leave: all of its 24
+// bits.  f16 parts are of 2^15 P, which has its 24 bits down to 2^-16 of the row's
+// largest and 2^-39 absolutely below.  Two bf16 parts hold 16 bits and put 7 to 19
+// times as many results of bf16 queries, or of f16 queries on 8-bit cells, on the
+// other side of their rounding, and take the same time (1,000,003 int8 tokens: 201
+// us a call with two, 202 with three): the loads are what is waited for.  Sums,
+// maxima and O are f32 throughout.
 //
 // Measured (one MI355X, a large copy at 4.7 TB/s): 1,000,003 int8 tokens of 4 heads
 // of 128, 8 query heads each: 195 us, 5.4 TB/s; 24 windows of up to 6,000 f32 tokens
@@ -73,14 +76,12 @@ __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* o) {
   }
 }
 
-// Two f32 that bf16 holds, or that are rounded to it, in one dword.
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2_t;
-  return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
+// Two f32 cut off to bf16 or f16 in one dword.
+__device__ __forceinline__ uint32_t cut_bf16(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);  // the upper halves
 }
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  typedef __attribute__((__vector_size__(2 * sizeof(_Float16)))) _Float16 f16x2_t;
-  return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b});
+__device__ __forceinline__ uint32_t cut_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
 
 // Cells 2i and 2i + 1 of a dword of 8-bit cells as bf16, exactly.
@@ -88,11 +89,11 @@ template <int CT>
 __device__ __forceinline__ uint32_t cells2_bf16(uint32_t w, int i) {
   if constexpr (CT == PFA_I8) {
     const float a = (float)(int8_t)(w >> (16 * i)), b = (float)(int8_t)(w >> (16 * i + 8));
-    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);  // the upper halves
+    return cut_bf16(a, b);
   } else {
     typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f32x2_;
     const f32x2_ f = i ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-    return __builtin_amdgcn_perm(__float_as_uint(f[1]), __float_as_uint(f[0]), 0x07060302);
+    return cut_bf16(f[0], f[1]);
   }
 }
 
@@ -107,7 +108,7 @@ struct Form {
   static constexpr int E = cell_bytes(CT);
   static constexpr bool F32 = CT == PFA_F32, F16 = CT == PFA_F16;
   static constexpr int NQ = !is8(CT) || QT == PFA_BF16 ? 1 : QT == PFA_F16 ? 2 : 3;  // parts of Q
-  static constexpr int NP = QT == PFA_F32 ? 3 : 2;                                    // parts of P
+  static constexpr int NP = 3;                                                        // parts of P
   static constexpr int EL = D / 4;                     // channels of a lane in S
   static constexpr int U = EL < 16 / E ? EL : 16 / E;  // of one load
   static constexpr int KW = EL * E / 4;                // dwords of a lane's share of 16 keys
@@ -232,7 +233,7 @@ struct Wave {
     }
   }
 
-  // Eight f32 as N 16-bit operands, each what the ones before leave.
+  // Eight f32 as N 16-bit operands, each cut off from what the ones before leave.
   template <int N, bool HALF, typename Put>
   static __device__ __forceinline__ void parts(float (&x)[8], Put&& put) {
 #pragma unroll
@@ -240,7 +241,7 @@ struct Wave {
       u32x4_t w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t u = HALF ? pack_f16(x[2 * i], x[2 * i + 1]) : pack_bf16(x[2 * i], x[2 * i + 1]);
+        const uint32_t u = HALF ? cut_f16(x[2 * i], x[2 * i + 1]) : cut_bf16(x[2 * i], x[2 * i + 1]);
         w[i] = u;
         if (part + 1 < N) {
           if constexpr (HALF) {
