@@ -176,7 +176,7 @@ __device__ __forceinline__ void score_pages(const Pages& pg, const int32_t* __re
     bool ok = false;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) ok = i == s ? have[i] : ok;
-    uint32_t u = __float_as_uint(best[k]);
+    uint32_t u = best[k] == 0.0f ? 0u : __float_as_uint(best[k]);  // -0, a sum that underflows, ties with +0
     u = u & 0x80000000u ? ~u : u | 0x80000000u;  // -inf is 0x007fffff, +inf 0xff800000
     if (nan[k]) u = kNan;
     if (page - sp.p0 < first || sp.pe - page <= last) u = kForced;
