@@ -419,7 +419,9 @@ struct Wave {
 
 // What a workgroup's waves, and then a row's workgroups, are joined by: the
 // weight of a part with maximum m and sum l under the common maximum.  A part
-// without a score above -inf weighs nothing, unless a NaN is in it.
+// without a score above -inf weighs nothing, unless a NaN is in it.  A part that
+// weighs nothing is still added: zero, but for values and sums that are not finite,
+// which are the row's wherever in it they lie.
 __device__ __forceinline__ float part_weight(float m, float l, float top, float c) {
   return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : exp2_((m - top) * c);
 }
@@ -684,8 +686,8 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 #pragma unroll
       for (int j = 0; j < kWaves; ++j) {
         const float a = part_weight(sm[j][row], sl[j][row], top, c);
-        o += a == 0.0f ? 0.0f : a * so[j][row][d];
-        sum += a == 0.0f ? 0.0f : a * sl[j][row];
+        o += a * so[j][row][d];
+        sum += a * sl[j][row];
       }
       if (whole) {
         store_f<F::QT>(out + ((int64_t)b * (deal.R / deal.RT) * G + row0 + row) * D + d,
@@ -741,18 +743,19 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
         // part i is workgroup first + i's
         const float* s = parts + (2 * (int64_t)(who.first + (in ? i : 0)) + (!in || i == 0)) * rows * (D + 2);
         m[u] = in ? s[rows * D + row] : -INFINITY, l[u] = in ? s[rows * (D + 1) + row] : 0.0f;
+        // where there is none, part 0's, which weigh nothing here
         x[u] = s[row * D + d], y[u] = two ? s[row * D + 64 + d] : 0.0f;
       }
       float t = a.m;
 #pragma unroll
       for (int u = 0; u < 8; ++u) t = fmaxf(t, m[u]);
       const float w = part_weight(a.m, a.l, t, c);
-      a.o0 = w == 0.0f ? 0.0f : w * a.o0, a.o1 = w == 0.0f ? 0.0f : w * a.o1, a.l = w == 0.0f ? 0.0f : w * a.l;
+      a.o0 *= w, a.o1 *= w, a.l *= w;
       a.m = t;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float p = part_weight(m[u], l[u], t, c);
-        if (p != 0.0f) a.o0 += p * x[u], a.o1 += p * y[u], a.l += p * l[u];
+        a.o0 += p * x[u], a.o1 += p * y[u], a.l += p * l[u];
       }
     }
     return a;
@@ -761,9 +764,10 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
   if (who.n <= 16) {
     for (int row = blockIdx.y * teams + team; row < here; row += gridDim.y * teams) {
       const Sum a = gather(row, 0, 1);
-      const float inv = a.l == 0.0f ? 0.0f : 1.0f / (a.l * pscale);
-      store_f<QT>(to + row * D + d, a.o0 * inv);
-      if (two) store_f<QT>(to + row * D + 64 + d, a.o1 * inv);
+      const bool none = a.l == 0.0f;  // no score above -inf, whatever the values are
+      const float inv = 1.0f / (a.l * pscale);
+      store_f<QT>(to + row * D + d, none ? 0.0f : a.o0 * inv);
+      if (two) store_f<QT>(to + row * D + 64 + d, none ? 0.0f : a.o1 * inv);
     }
     return;
   }
@@ -781,7 +785,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
       for (int w = 0; w < used; ++w) t = fmaxf(t, tops[w]);
       for (int w = 0; w < used; ++w) {
         const float p = part_weight(tops[w], suml[w], t, c);
-        if (p != 0.0f) o += p * acc[w * D + x], l += p * suml[w];
+        o += p * acc[w * D + x], l += p * suml[w];
       }
       store_f<QT>(to + row * D + x, l == 0.0f ? 0.0f : o / (l * pscale));
     }

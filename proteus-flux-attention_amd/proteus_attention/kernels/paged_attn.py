@@ -345,7 +345,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     Returns ``(B, heads, head_dim)`` in q's type.  A row that sees no key, or
     none with a score above -inf, is zero.  What stands in slots that no
     sequence sees has no effect, whatever it is; a value that is seen and not
-    finite leaves its channel not finite (inf or NaN).
+    finite leaves its channel not finite (inf or NaN) in a row that sees another
+    score than -inf, a score that is NaN or +inf its row NaN.
     """
 
     if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32 or selected.shape[2] > _MOST):
