@@ -228,14 +228,16 @@ struct Wave {
             for (int e = 0; e < (F::EL < 8 ? F::EL : 8); ++e) x[e] = load_f<F::QT>(at + e);
           }
         }
-        parts<F::NQ, F::F16>(x, [&](int part, u32x4_t w) { q[part][c] = w; });
+        parts<F::NQ, F::F16, true>(x, [&](int part, u32x4_t w) { q[part][c] = w; });
       }
     }
   }
 
-  // Eight f32 as N 16-bit operands, each cut off from what the ones before leave.
-  template <int N, bool HALF, typename Put>
+  // Eight f32 as N 16-bit operands, each cut off from what the ones before leave; with
+  // INF an infinity leaves nothing.
+  template <int N, bool HALF, bool INF, typename Put>
   static __device__ __forceinline__ void parts(float (&x)[8], Put&& put) {
+    auto leave = [](float a, float part) { return INF && fabsf(a) == INFINITY ? 0.0f : a - part; };
 #pragma unroll
     for (int part = 0; part < N; ++part) {
       u32x4_t w;
@@ -244,11 +246,9 @@ struct Wave {
         const uint32_t u = HALF ? cut_f16(x[2 * i], x[2 * i + 1]) : cut_bf16(x[2 * i], x[2 * i + 1]);
         w[i] = u;
         if (part + 1 < N) {
-          if constexpr (HALF) {
-            x[2 * i] -= f16_to_f32((uint16_t)u), x[2 * i + 1] -= f16_to_f32((uint16_t)(u >> 16));
-          } else {
-            x[2 * i] -= __uint_as_float(u << 16), x[2 * i + 1] -= __uint_as_float(u & 0xffff0000u);
-          }
+          const float a = HALF ? f16_to_f32((uint16_t)u) : __uint_as_float(u << 16);
+          const float b = HALF ? f16_to_f32((uint16_t)(u >> 16)) : __uint_as_float(u & 0xffff0000u);
+          x[2 * i] = leave(x[2 * i], a), x[2 * i + 1] = leave(x[2 * i + 1], b);
         }
       }
       put(part, w);
@@ -391,7 +391,7 @@ struct Wave {
 #pragma unroll
         for (int y = 0; y < 8; ++y) x[y] = s[i + y / 4][y & 3];
         u32x4_t p[F::NP];
-        parts<F::NP, F::F16>(x, [&](int part, u32x4_t w) { p[part] = w; });
+        parts<F::NP, F::F16, false>(x, [&](int part, u32x4_t w) { p[part] = w; });
         // channels 2jj, 2jj + 1 of the eight keys, as pairs of 16-bit cells
         constexpr int PAIRS = F::VD < 2 ? 1 : F::VD / 2;
 #pragma unroll

@@ -98,3 +98,41 @@ def test_a_key_that_is_not_finite(pair, form):
         assert torch.isnan(got[0, 2:]).all(), bad
         got[0, 2:] = want[0][0, 2:].to(dt)
         assert R.attend_error(got, want, dt, n) <= 1, bad
+
+
+@pytest.mark.parametrize("pair", R.PAIRS, ids=R.pair_id)
+@pytest.mark.parametrize("form", range(len(FORMS)))
+def test_scores_of_minus_infinity(pair, form):
+    """Rows with no score above -inf are zero, whatever their values are; next to
+    other scores a score of -inf weighs nothing.  Queries of -inf on keys above
+    zero, and, in float cells, keys of -inf."""
+    dt, cell = pair
+    B, n, low = FORMS[form]
+    D = 32
+    g = torch.Generator().manual_seed(form + 20)
+    pool, table, q, lengths = _case(pair, B, n, 0, D, g)  # every key 4
+    want = R.attend(q, pool, table, lengths, scale=1.0)
+    minus = q.clone()
+    minus[0, 1, 3] = -math.inf
+    page = int(table[0, 0])
+    if cell in R.TOP:
+        pool["v_scale"][page, 0, 2] = math.nan
+    else:
+        pool["v"][page, 0, 2] = math.nan
+    got = _run(minus, pool, table, lengths, scale=1.0)
+    assert not got[0, 1].any()
+    assert not torch.isfinite(got[0, 0]).any()
+    got[0, :2] = want[0][0, :2].to(dt)
+    assert R.attend_error(got, want, dt, n) <= 1
+    if cell in R.TOP:
+        return
+    pool["v"][page, 0, 2] = 1.0
+    at = table.long()
+    P = at.shape[1]
+    half = max(P // 2, 1)
+    pool["k"][at[:, :half], 1, :, 9] = -math.inf  # the first half of each sequence, head 1
+    pool["k"][at[0], 0, :, 9] = -math.inf  # all of the first one's, head 0
+    got = _run(q, pool, table, lengths, scale=1.0)
+    assert not got[0, :2].any()
+    ref = R.attend(q[:, 2:], {m: t[:, 1:] for m, t in pool.items()}, table, lengths, starts=[half * 16] * B, scale=1.0)
+    assert R.attend_error(got[:, 2:], ref, dt, n) <= 1
