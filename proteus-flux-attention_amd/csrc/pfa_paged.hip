@@ -120,6 +120,7 @@ __device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at,
       float q = x[i] * y;
       q = fmaf(fmaf(-q, s, x[i]), y, q);
       q = fmaf(fmaf(-q, s, x[i]), y, q);
+      if constexpr (CT == PFA_E4M3) q = copysignf(q, x[i]);  // -0 loses its sign in the corrections
       c[i] = ok ? q : 0.0f;
     }
     uint32_t w[2];
