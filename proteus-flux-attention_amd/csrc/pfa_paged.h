@@ -43,10 +43,14 @@ __device__ __forceinline__ int page_at(const Table& t, const Pages& p, int64_t b
   return (uint32_t)id < (uint32_t)p.n_pages ? id : -1;
 }
 
-// Tokens that a sequence holds: no more than its row has pages for.
-__device__ __forceinline__ int64_t length_at(const int32_t* lengths, const Table& t, const Pages& p, int64_t b) {
-  const int64_t n = lengths[b], most = (int64_t)t.P << p.shift;
+// Tokens that a sequence holds: no more than its row has pages for, 2^30 at most.
+__device__ __forceinline__ int length_at(const int32_t* lengths, int P, int shift, int b) {
+  const int n = lengths[b], most = P << shift;
   return n < 0 ? 0 : n < most ? n : most;
+}
+// The first position that it looks at.
+__device__ __forceinline__ int start_at(const int32_t* starts, int b) {
+  return starts && starts[b] > 0 ? starts[b] : 0;
 }
 
 // a / b of positive numbers, in 32 bits where they are enough.
@@ -54,16 +58,8 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
-// One e4m3 cell as f32: v_cvt_f32_fp8 (OCP form on gfx950).
-__device__ __forceinline__ float e4m3_to_f32(uint8_t b) { return __builtin_amdgcn_cvt_f32_fp8((int)b, 0); }
-
-template <int DT>
-__device__ __forceinline__ float cell_f(const typename Cell<DT>::T* p) {
-  if constexpr (DT == PFA_E4M3) return e4m3_to_f32(*p);
-  else return load_f<DT>(p);
-}
-
-// Eight consecutive cells as f32; the address aligned to eight of them.
+// Eight consecutive cells as f32 (e4m3: v_cvt_f32_fp8, the OCP form on gfx950); the
+// address aligned to eight of them.
 template <int DT>
 __device__ __forceinline__ void cells8(const typename Cell<DT>::T* p, float (&o)[8]) {
   if constexpr (DT == PFA_E4M3) {

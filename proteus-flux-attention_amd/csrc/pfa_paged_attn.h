@@ -448,13 +448,7 @@ struct Deal {
     if (S >= 0) return (int)((((int64_t)S << shift) + tile - 1) / tile);
     return start >= len ? 0 : (len + tile - 1) / tile - first_tile(start);
   }
-  __device__ __forceinline__ int length(const int32_t* lengths, int b) const {
-    const int64_t n = lengths[b], most = (int64_t)P << shift;
-    return (int)(n < 0 ? 0 : n < most ? n : most);
-  }
-  __device__ __forceinline__ int begin(const int32_t* starts, int b) const {
-    return starts && starts[b] > 0 ? starts[b] : 0;
-  }
+  __device__ __forceinline__ int length(const int32_t* lengths, int b) const { return length_at(lengths, P, shift, b); }
   // places of a pair
   __device__ __forceinline__ int places(int start, int len) const {
     const int n = tiles(start, len);
@@ -533,7 +527,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   } else if (parts_ws) {
     // places of the sequences up to this thread's, of 256 at a time
     auto places = [&](int i) {
-      return i < deal.B ? deal.places(deal.begin(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
+      return i < deal.B ? deal.places(start_at(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
     };
     int64_t nt, incl, all;
     auto scan = [&](int i) {
@@ -583,7 +577,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     at = uniform(found[1]);
   } else {  // a workgroup a pair
     b = blockIdx.x / deal.R;
-    f = (int64_t)(blockIdx.x % deal.R) * deal.tiles(deal.begin(starts, b), deal.length(lengths, b));
+    f = (int64_t)(blockIdx.x % deal.R) * deal.tiles(start_at(starts, b), deal.length(lengths, b));
     f1 = f + 1;
     at = 0;
   }
@@ -603,7 +597,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   }
 
   while (f < f1) {
-    const int start = deal.begin(starts, b), len = deal.length(lengths, b);
+    const int start = start_at(starts, b), len = deal.length(lengths, b);
     const int nt = deal.tiles(start, len), np = deal.places(start, len);
     if (!lone && nt == 0) {
       ++b;
@@ -721,7 +715,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
   const int rows = G < 16 ? G : 16, here = (h + 1) * G - head0 < 16 ? (h + 1) * G - head0 : 16;
   const Shared who = shared[blockIdx.x];  // nobody's where the sequence has no tiles
   typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head0) * D;
-  if (deal.tiles(deal.begin(starts, b), deal.length(lengths, b)) == 0) {
+  if (deal.tiles(start_at(starts, b), deal.length(lengths, b)) == 0) {
     for (int i = blockIdx.y * D + tid; i < here * D; i += THREADS * gridDim.y) store_f<QT>(to + i, 0.0f);
     return;
   }

@@ -13,9 +13,7 @@ struct Span {
   int p0, pe;
 };
 __device__ __forceinline__ Span span_at(const int32_t* lengths, const int32_t* starts, int P, int shift, int b) {
-  const int64_t n = lengths[b], most = (int64_t)P << shift;
-  const int len = (int)(n < 0 ? 0 : n < most ? n : most);
-  const int start = starts && starts[b] > 0 ? starts[b] : 0;
+  const int len = length_at(lengths, P, shift, b), start = start_at(starts, b);
   if (start >= len) return Span{0, 0};
   return Span{start >> shift, (len + (1 << shift) - 1) >> shift};
 }
