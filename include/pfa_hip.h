@@ -705,7 +705,10 @@ typedef struct pfa_paged_query {
  * kv_heads, n_selected; rows selected_stride apart) lists (entries outside of it
  * are left out, an entry listed twice counts twice); n_selected < 0: no list.
  * out (B, H, D) dense, in q's type.  A row that sees no key is zero, and so is
- * one all of whose scores are -inf.  Sums and softmax statistics are f32. */
+ * one all of whose scores are -inf.  Sums and softmax statistics are f32, and
+ * probabilities multiply the values with all of their 24 bits.  A value that is
+ * seen and not finite leaves its channel not finite, a score that is NaN or +inf
+ * its row NaN. */
 int pfa_paged_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
                                   int cell_dtype, int table_pages, int n_selected,
                                   size_t* bytes);

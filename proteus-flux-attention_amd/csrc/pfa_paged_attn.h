@@ -22,8 +22,10 @@
 // - O^T has head n in lane (n, g) again, so the running maximum's correction is
 //   one factor a lane, and lane (n, g) ends with D / 4 neighbouring channels.
 //
-// No LDS, no barrier and no lane exchange but the maximum over g, two row
-// swaps, until a workgroup's four waves are joined.
+// Keys, values, scores and P pass through no LDS and no lane exchange but the
+// maximum over g, two row swaps, until a workgroup's four waves are joined.  A tile's
+// pages are read from LDS, where the workgroup looks up those of a run of tiles at
+// once, between two barriers (kEntries).
 //
 // Precision: f32 stays on v_mfma_f32_16x16x4f32.  8-bit cells are whole in
 // bf16; their scales multiply S and P in f32.  Queries of f16 or f32 on 8-bit

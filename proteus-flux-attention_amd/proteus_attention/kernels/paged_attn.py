@@ -342,7 +342,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     table row count: entries outside of the row are left out, one listed twice
     counts twice.  ``scale`` defaults to 1 / sqrt(head_dim).
 
-    Returns ``(B, heads, head_dim)`` in q's type.  A row that sees no key, or
+    Returns ``(B, heads, head_dim)`` in q's type; scores, weights and sums are
+    f32, rounded once at the end.  A row that sees no key, or
     none with a score above -inf, is zero.  What stands in slots that no
     sequence sees has no effect, whatever it is; a value that is seen and not
     finite leaves its channel not finite (inf or NaN) in a row that sees another
