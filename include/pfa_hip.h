@@ -41,6 +41,7 @@ extern "C" {
 #define PFA_F16 2
 #define PFA_I8 3   /* symmetric int8 with a float scale per head */
 #define PFA_E4M3 4 /* 8-bit float (OCP e4m3), cells of pfa_kv_pages only */
+#define PFA_E2M1 5 /* 4-bit float (OCP e2m1), cells of pfa_kv_pages only */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int pfa_version(void);
@@ -641,11 +642,16 @@ int pfa_int8_kv_attn_fwd(pfa_tensor4 q, pfa_tensor4 out, int64_t T, int H, int D
  * A pool holds n_pages pages of page_size tokens (16, 32, 64, 128 or 256)
  * for kv_heads heads of head_dim (16, 32, 64 or 128): cells k and v
  * [page][head][slot][d] in `dtype` (PFA_F32 / PFA_BF16 / PFA_F16 / PFA_I8 /
- * PFA_E4M3), pages k_page / v_page cells apart (inner dimensions dense, rows
- * 16-byte aligned).  PFA_I8 and PFA_E4M3 cells have one f32 scale per token
- * and head, k_scale and v_scale [page][head][slot].  k_bounds, or NULL, are
- * the least and the largest stored key of every channel of a page's head,
- * [page][head][2][d], in the cells' type, or f32 for 8-bit cells.
+ * PFA_E4M3 / PFA_E2M1), pages k_page / v_page cells apart (inner dimensions
+ * dense, pages 16-byte aligned).  PFA_I8 and PFA_E4M3 cells have one f32 scale
+ * per token and head, k_scale and v_scale [page][head][slot].  PFA_E2M1 cells
+ * lie two to a byte, the even channel in the lower half, k_page and v_page
+ * count bytes, and 32 neighbouring channels (16 of heads of 16) share a scale
+ * that is a power of two, 2^(byte - 127), 255 for NaN: bytes
+ * [page][head][slot][d / 32].  k_bounds, or NULL, are the least and the largest
+ * stored key of every channel of a page's head, [page][head][2][d], in the
+ * cells' type, f32 for 8-bit cells, bf16 for 4-bit cells (which holds every
+ * one of them).
  *
  * Position t of sequence b lies in slot t % page_size of page
  * table[b * table_stride + t / page_size].  A row of the table has
@@ -656,19 +662,22 @@ int pfa_int8_kv_attn_fwd(pfa_tensor4 q, pfa_tensor4 out, int64_t T, int H, int D
  * ==================================================================== */
 typedef struct pfa_kv_pages {
   void *k, *v;
-  float *k_scale, *v_scale;
+  void *k_scale, *v_scale;
   void* k_bounds;
   int64_t k_page, v_page;
   int n_pages, kv_heads, page_size, head_dim, dtype;
 } pfa_kv_pages;
 
 /* New tokens k, v [b][h][t][d] (n for each of B sequences, dtype PFA_F32 /
- * PFA_BF16 / PFA_F16: the cells' own, or any of the three for 8-bit cells)
- * into their pages: token i < counts[b] (all n where counts is NULL) goes to
+ * PFA_BF16 / PFA_F16: the cells' own, or any of the three for cells of 8 or 4
+ * bits) into their pages: token i < counts[b] (all n where counts is NULL) goes to
  * position starts[b] + i.  Positions below zero or behind the table's last
  * page are left out.  8-bit cells: scale = max(absmax / top, 1e-6), top 127
  * (PFA_I8) or 448 (PFA_E4M3), cell = x / scale rounded to nearest even; a row
- * with a value that is not finite gets scale NaN and zero cells.  k_bounds of
+ * with a value that is not finite gets scale NaN and zero cells.  PFA_E2M1, a
+ * group of channels at a time: scale the least 2^e, -20 <= e <= 125, with
+ * absmax <= 7 * 2^e, cell = x / scale rounded to nearest even, at most 6; not
+ * finite: as there.  k_bounds of
  * a page's head, where the pool has them: those of the written keys as they
  * are stored (a NaN among them gives NaN), joined with what stood there
  * unless the page is written from its first slot on. */
@@ -688,7 +697,7 @@ int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, const int32_t
 
 /* One new token a sequence: queries q [b][h][d] (s_t unused; H heads, a multiple of
  * kv_heads: head h reads key-value head h / (H / kv_heads)) in dtype PFA_F32 /
- * PFA_BF16 / PFA_F16 (the cells' own, or any of the three for 8-bit cells),
+ * PFA_BF16 / PFA_F16 (the cells' own, or any of the three for cells of 8 or 4 bits),
  * looking at positions starts[b] (starts NULL: 0) .. lengths[b] - 1.  Lengths
  * beyond the table's pages count as all of them. */
 typedef struct pfa_paged_query {
@@ -737,6 +746,33 @@ int pfa_paged_sparse_attn_workspace_size(int B, int H, int kv_heads, int page_si
 int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count, int first, int last,
                               float scale, int32_t* chosen, void* out, void* workspace,
                               size_t ws_bytes, void* stream);
+
+/* ====================================================================
+ * Rotary positions of queries and keys.  The reference turns whole heads of
+ * whole sequences (aspa.py:606-618, pfa_rope_qk_inplace); these are the
+ * positions of new tokens of running sequences, in either layout, of part of a
+ * head, at any distance.
+ *
+ * Values q [b][h][t][d] of H heads and k of Hk (0: none), n tokens each of B
+ * sequences, dtype PFA_F32 / PFA_BF16 / PFA_F16, inner dimension dense, to
+ * q_out and k_out, which are the inputs themselves or do not overlap them.
+ * Token t of sequence b is at position positions[b * pos_b] + t, or with
+ * per_token positions[b * pos_b + t * pos_t].  Of each head's head_dim channels
+ * (256 at most) the first `width` (even) turn: pairs (2j, 2j + 1) where they are
+ * interleaved, else (j, j + width / 2), pair j by position * turns[j] / 2^64 turns:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)
+ * computed in f32 and rounded once.  turns: (width / 2) on the device.
+ * ==================================================================== */
+typedef struct pfa_rotary_call {
+  pfa_tensor4 q, k, q_out, k_out;
+  const uint64_t* turns;
+  const int32_t* positions;
+  int64_t pos_b, pos_t, n;
+  int per_token, B, H, Hk, head_dim, width, interleaved, dtype;
+  float magnitude;
+} pfa_rotary_call;
+
+int pfa_rotary(const pfa_rotary_call* call, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,7 @@ from .kernels.paged_attn import (
     select_kv_pages,
     write_kv_pages,
 )
+from .kernels.rotary import RotaryPositions, apply_rotary, new_rotary_positions, rotary_frequencies
 from .kernels.sparse_attn import aspa_sparse_attention, get_last_backend, get_last_backend_info
 from .models.aspa import (
     MLP,
@@ -52,6 +53,10 @@ __all__ = [
     "select_kv_pages",
     "paged_attention",
     "paged_sparse_attention",
+    "RotaryPositions",
+    "new_rotary_positions",
+    "rotary_frequencies",
+    "apply_rotary",
     "__version__",
 ]
 

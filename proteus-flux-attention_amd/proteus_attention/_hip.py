@@ -15,7 +15,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libpfa_hip.so"
 
-PFA_F32, PFA_BF16, PFA_F16, PFA_I8, PFA_E4M3 = 0, 1, 2, 3, 4
+PFA_F32, PFA_BF16, PFA_F16, PFA_I8, PFA_E4M3, PFA_E2M1 = 0, 1, 2, 3, 4, 5
 
 _DTYPE_TAG = {
     torch.float32: PFA_F32,
@@ -81,6 +81,7 @@ EXPORTED_SYMBOLS = (
     "pfa_kv_pages_select",
     "pfa_paged_sparse_attn_workspace_size",
     "pfa_paged_sparse_attn_fwd",
+    "pfa_rotary",
 )
 
 
@@ -181,6 +182,7 @@ _SIGNATURES = {
     "pfa_paged_sparse_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)],
                                              _i32),
     "pfa_paged_sparse_attn_fwd": ([_vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _sz, _vp], _i32),
+    "pfa_rotary": ([_vp, _vp], _i32),
 }
 
 

@@ -9,6 +9,7 @@ from .paged_attn import (
     select_kv_pages,
     write_kv_pages,
 )
+from .rotary import RotaryPositions, apply_rotary, new_rotary_positions, rotary_frequencies
 from .sparse_attn import (
     aspa_sparse_attention,
     build_packed_shortlist_candidates,
@@ -30,4 +31,8 @@ __all__ = [
     "select_kv_pages",
     "paged_attention",
     "paged_sparse_attention",
+    "RotaryPositions",
+    "new_rotary_positions",
+    "rotary_frequencies",
+    "apply_rotary",
 ]
