@@ -15,7 +15,7 @@ static int shift_of(int page_size) {
 }
 
 static int sizes_check(int kv_heads, int page_size, int head_dim, int dtype, int table_pages, int B) {
-  PFA_CHECK_ARG(dtype == PFA_F32 || dtype == PFA_BF16 || dtype == PFA_F16 || is8(dtype), "pages: unknown cell type %d",
+  PFA_CHECK_ARG(dtype == PFA_F32 || dtype == PFA_BF16 || dtype == PFA_F16 || scaled(dtype), "pages: unknown cell type %d",
                 dtype);
   PFA_CHECK_ARG(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128,
                 "pages: head_dim must be 16, 32, 64 or 128 (got %d)", head_dim);
@@ -33,9 +33,9 @@ int paged_check(const pfa_kv_pages* pg, const int32_t* table, int64_t table_stri
   PFA_CHECK_ARG(pg, "pages: null argument");
   if (int rc = sizes_check(pg->kv_heads, pg->page_size, pg->head_dim, pg->dtype, table_pages, B)) return rc;
   PFA_CHECK_ARG(pg->n_pages > 0 && pg->k && pg->v, "pages: an empty pool");
-  PFA_CHECK_ARG(!is8(pg->dtype) || (pg->k_scale && pg->v_scale), "pages: 8-bit cells need k_scale and v_scale");
-  const int64_t cells = (int64_t)pg->kv_heads * pg->page_size * pg->head_dim;
-  const int e = cell_bytes(pg->dtype);
+  PFA_CHECK_ARG(!scaled(pg->dtype) || (pg->k_scale && pg->v_scale), "pages: cells of 8 or 4 bits need k_scale and v_scale");
+  const int64_t cells = (int64_t)pg->kv_heads * pg->page_size * cells_at(pg->dtype, pg->head_dim);
+  const int e = is4(pg->dtype) ? 1 : cells_bytes(pg->dtype, 1);
   PFA_CHECK_ARG(pg->n_pages == 1 || (pg->k_page >= cells && pg->v_page >= cells), "pages: pages overlap");
   PFA_CHECK_ARG((uintptr_t)pg->k % 16 == 0 && (uintptr_t)pg->v % 16 == 0 && pg->k_page * e % 16 == 0 &&
                     pg->v_page * e % 16 == 0 && (uintptr_t)pg->k_scale % 16 == 0 && (uintptr_t)pg->v_scale % 16 == 0 &&
@@ -97,12 +97,41 @@ __device__ __forceinline__ void row8(const NewRows& r, int64_t at, float (&o)[8]
   }
 }
 
-// Eight values of a row of LANES lanes into its cells; with `back`, x comes back as
-// the values that the cells stand for.
+// Eight values, from channel 8 * lane on of a row of LANES lanes, into its cells; with
+// `back`, x comes back as the values that the cells stand for.
 template <int CT, int LANES>
-__device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at, bool first, bool back, float (&x)[8]) {
-  if constexpr (!is8(CT)) {
+__device__ __forceinline__ void put8(typename Cell<CT>::T* dst, void* scales, int64_t slot, int lane, bool back,
+                                     float (&x)[8]) {
+  if constexpr (!scaled(CT)) {
     store8<CT>(dst, x);
+  } else if constexpr (is4(CT)) {
+    // a group's scale is a power of two, so that the quotients are exact and the
+    // hardware's rounding to nearest even, saturating at 6, is the only one
+    constexpr int GROUP = LANES < 4 ? LANES : 4;
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(x[i]));
+    m = max_lanes<GROUP>(m);
+    const bool ok = m < INFINITY;
+    const uint32_t p = ok ? power_for(m) : kNanPower;
+    if (lane % GROUP == 0) ((uint8_t*)scales)[slot * (LANES / GROUP) + lane / GROUP] = (uint8_t)p;
+    const float s = power_of(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = ok ? x[i] : 0.0f;
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+    if (!ok) w = 0;  // whatever a scale that is NaN makes of it
+    if (back) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2_t y = e2m1_f32(w, s, i);
+        x[2 * i] = y[0], x[2 * i + 1] = y[1];
+      }
+    }
+    *reinterpret_cast<uint32_t*>(dst) = w;
   } else {
     float m = 0.0f;
 #pragma unroll
@@ -110,7 +139,7 @@ __device__ __forceinline__ void put8(typename Cell<CT>::T* dst, float* scale_at,
     m = max_lanes<LANES>(m);
     const bool ok = m < INFINITY;
     const float s = ok ? fmaxf(m / top_of(CT), kLeastScale) : __builtin_nanf("");
-    if (first) *scale_at = s;
+    if (lane == 0) ((float*)scales)[slot] = s;
     // x / s to nearest: s >= 1e-6 and at most 448 in size, so that nothing that
     // decides a cell underflows
     const float y = 1.0f / s;
@@ -183,7 +212,8 @@ __global__ void __launch_bounds__(1024) write_kernel(Pages pg, Table tab, NewRow
     const int id = page_at(tab, pg, b, ordinal);
     if (id < 0) continue;
 
-    const int64_t kpage = id * pg.k_page + (int64_t)h * pg.ps * D, vpage = id * pg.v_page + (int64_t)h * pg.ps * D;
+    constexpr int ROW = cells_at(CT, D), UNIT = cells_at(CT, 8);
+    const int64_t kpage = id * pg.k_page + (int64_t)h * pg.ps * ROW, vpage = id * pg.v_page + (int64_t)h * pg.ps * ROW;
     const int64_t spage = ((int64_t)id * pg.H + h) * pg.ps;
     const int64_t k_at = b * k.s_b + h * k.s_h + 8 * lane, v_at = b * v.s_b + h * v.s_h + 8 * lane;
     float lo[8], hi[8];
@@ -195,8 +225,8 @@ __global__ void __launch_bounds__(1024) write_kernel(Pages pg, Table tab, NewRow
       float x[8], y[8];
       row8<DT>(k, k_at + i * k.s_t, x);
       row8<DT>(v, v_at + i * v.s_t, y);
-      put8<CT, LANES>((CellT*)pg.k + kpage + slot * D + 8 * lane, pg.k_scale + spage + slot, lane == 0, back, x);
-      put8<CT, LANES>((CellT*)pg.v + vpage + slot * D + 8 * lane, pg.v_scale + spage + slot, lane == 0, false, y);
+      put8<CT, LANES>((CellT*)pg.k + kpage + slot * ROW + UNIT * lane, pg.k_scale, spage + slot, lane, back, x);
+      put8<CT, LANES>((CellT*)pg.v + vpage + slot * ROW + UNIT * lane, pg.v_scale, spage + slot, lane, false, y);
       if (back) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], x[j]), hi[j] = max_nan(hi[j], x[j]);
@@ -237,7 +267,7 @@ __global__ void __launch_bounds__(1024) write_kernel(Pages pg, Table tab, NewRow
 // ---------------------------------------------------------------------
 // 262,144 rows of 8 heads of 128 e4m3 cells into bf16: two rows 305 us, one 320;
 // 25,600 of int8 into f32: 67 and 59; 3,000 of 8 heads of 32 bf16: 5.0 and 4.2.
-__host__ __device__ constexpr int read_rows(int ct, int ot) { return is8(ct) && ot != PFA_F32 ? 2 : 1; }
+__host__ __device__ constexpr int read_rows(int ct, int ot) { return scaled(ct) && ot != PFA_F32 ? 2 : 1; }
 
 template <int CT, int OT, int D>
 __global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int64_t n, int64_t blocks,
@@ -266,11 +296,26 @@ __global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int64_t 
       for (int j = 0; j < 8; ++j) x[u][j] = y[u][j] = 0.0f;
       if (id >= 0) {
         const int64_t slot = (int64_t)h * pg.ps + (pos & (pg.ps - 1));
-        cells8<CT>((const CellT*)pg.k + id * pg.k_page + slot * D + 8 * lane, x[u]);
-        cells8<CT>((const CellT*)pg.v + id * pg.v_page + slot * D + 8 * lane, y[u]);
+        constexpr int ROW = cells_at(CT, D), UNIT = cells_at(CT, 8);
+        const CellT* kp = (const CellT*)pg.k + id * pg.k_page + slot * ROW + UNIT * lane;
+        const CellT* vp = (const CellT*)pg.v + id * pg.v_page + slot * ROW + UNIT * lane;
+        const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
+        if constexpr (is4(CT)) {
+          constexpr int NS = scales_of(CT, D);
+          const float a = power_of(((const uint8_t*)pg.k_scale)[s * NS + lane / (LANES / NS)]);
+          const float c = power_of(((const uint8_t*)pg.v_scale)[s * NS + lane / (LANES / NS)]);
+          const uint32_t kw = *reinterpret_cast<const uint32_t*>(kp), vw = *reinterpret_cast<const uint32_t*>(vp);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x2_t p = e2m1_f32(kw, a, j), q = e2m1_f32(vw, c, j);
+            x[u][2 * j] = p[0], x[u][2 * j + 1] = p[1], y[u][2 * j] = q[0], y[u][2 * j + 1] = q[1];
+          }
+        } else {
+          cells8<CT>(kp, x[u]);
+          cells8<CT>(vp, y[u]);
+        }
         if constexpr (is8(CT)) {
-          const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
-          const float a = pg.k_scale[s], c = pg.v_scale[s];
+          const float a = ((const float*)pg.k_scale)[s], c = ((const float*)pg.v_scale)[s];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             x[u][j] *= a, y[u][j] *= c;
@@ -293,7 +338,7 @@ __global__ void __launch_bounds__(256) read_kernel(Pages pg, Table tab, int64_t 
 }
 
 // Calls f with the (values, cells) types as template arguments: the cells' own
-// float type, or any of the three with 8-bit cells.
+// float type, or any of the three with cells of 8 or 4 bits.
 template <typename F>
 void by_types(int dt, int ct, F&& f) {
 #define PFA_PAIR(A, C) \
@@ -301,6 +346,7 @@ void by_types(int dt, int ct, F&& f) {
   PFA_PAIR(PFA_F32, PFA_F32) PFA_PAIR(PFA_BF16, PFA_BF16) PFA_PAIR(PFA_F16, PFA_F16)
   PFA_PAIR(PFA_F32, PFA_I8) PFA_PAIR(PFA_BF16, PFA_I8) PFA_PAIR(PFA_F16, PFA_I8)
   PFA_PAIR(PFA_F32, PFA_E4M3) PFA_PAIR(PFA_BF16, PFA_E4M3) PFA_PAIR(PFA_F16, PFA_E4M3)
+  PFA_PAIR(PFA_F32, PFA_E2M1) PFA_PAIR(PFA_BF16, PFA_E2M1) PFA_PAIR(PFA_F16, PFA_E2M1)
 #undef PFA_PAIR
 }
 
@@ -315,7 +361,7 @@ void by_width(int D, F&& f) {
 
 int types_check(int dt, int ct) {
   PFA_CHECK_ARG(dt == PFA_F32 || dt == PFA_BF16 || dt == PFA_F16, "pages: unknown value type %d", dt);
-  PFA_CHECK_ARG(is8(ct) || dt == ct, "pages: values of type %d for cells of type %d", dt, ct);
+  PFA_CHECK_ARG(scaled(ct) || dt == ct, "pages: values of type %d for cells of type %d", dt, ct);
   return PFA_OK;
 }
 
@@ -336,7 +382,7 @@ extern "C" int pfa_kv_pages_write(const pfa_kv_pages* pages, const pfa_tensor4* 
   if (B == 0 || n == 0 || table_pages == 0) return PFA_OK;
   PFA_CHECK_ARG(k && v && k->ptr && v->ptr && starts, "kv_pages_write: null argument");
   const int D = pages->head_dim;
-  const int e = cell_bytes(dtype);
+  const int e = cells_bytes(dtype, 1);
   auto rows = [&](const pfa_tensor4& x) {
     const bool vec = (uintptr_t)x.ptr % 16 == 0 && x.s_b * e % 16 == 0 && x.s_h * e % 16 == 0 && x.s_t * e % 16 == 0;
     return NewRows{x.ptr, x.s_b, x.s_h, x.s_t, vec};
@@ -394,7 +440,8 @@ extern "C" int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, co
     case PFA_BF16: by_out(std::integral_constant<int, PFA_BF16>{}); break;
     case PFA_F16: by_out(std::integral_constant<int, PFA_F16>{}); break;
     case PFA_I8: by_out(std::integral_constant<int, PFA_I8>{}); break;
-    default: by_out(std::integral_constant<int, PFA_E4M3>{}); break;
+    case PFA_E4M3: by_out(std::integral_constant<int, PFA_E4M3>{}); break;
+    default: by_out(std::integral_constant<int, PFA_E2M1>{}); break;
   }
   PFA_CHECK_LAUNCH("kv_pages_read");
   return PFA_OK;
@@ -515,6 +562,7 @@ static int attend(const char* what, const pfa_paged_query* query, const Pages& p
                      selected_stride, S, c, choice, out, (float*)workspace, as_stream(stream)};
   if (ct == PFA_I8) attend_i8(query->dtype, a);
   else if (ct == PFA_E4M3) attend_e4m3(query->dtype, a);
+  else if (ct == PFA_E2M1) attend_e2m1(query->dtype, a);
   else attend_float(query->dtype, a);
   PFA_CHECK_LAUNCH(what);
   return PFA_OK;

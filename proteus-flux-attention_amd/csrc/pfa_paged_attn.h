@@ -101,22 +101,24 @@ __device__ __forceinline__ uint32_t cells2_bf16(uint32_t w, int i) {
 
 // 32-key groups of a tile: 4 KB of keys for rows of 128 bytes and more.  Two groups of
 // such rows leave no registers: 1,000,003 int8 tokens of 128 channels 195 -> 226 us.
-__host__ __device__ constexpr int tile_groups(int ct, int D) { return D * cell_bytes(ct) >= 128 ? 1 : 2; }
+__host__ __device__ constexpr int tile_groups(int ct, int D) { return cells_bytes(ct, D) >= 128 ? 1 : 2; }
 
 // Cells of a call's kernel, by the types of queries and cells and the head's width.
 template <int QT_, int CT_, int D_>
 struct Form {
   static constexpr int QT = QT_, CT = CT_, D = D_;
-  static constexpr int E = cell_bytes(CT);
+  static constexpr int BITS = cell_bits(CT), ROW = cells_bytes(CT, D);
   static constexpr bool F32 = CT == PFA_F32, F16 = CT == PFA_F16;
-  static constexpr int NQ = !is8(CT) || QT == PFA_BF16 ? 1 : QT == PFA_F16 ? 2 : 3;  // parts of Q
+  static constexpr int NS = scales_of(CT, D);  // scales of a row
+  static constexpr int NQ = !scaled(CT) || QT == PFA_BF16 ? 1 : QT == PFA_F16 ? 2 : 3;  // parts of Q
   static constexpr int NP = 3;                                                        // parts of P
   static constexpr int EL = D / 4;                     // channels of a lane in S
-  static constexpr int U = EL < 16 / E ? EL : 16 / E;  // of one load
-  static constexpr int KW = EL * E / 4;                // dwords of a lane's share of 16 keys
+  static constexpr int U = EL < 128 / BITS ? EL : 128 / BITS;  // of one load
+  static constexpr int UB = U * BITS / 8;                      // their bytes
+  static constexpr int KW = EL * BITS < 32 ? 1 : EL * BITS / 32;  // dwords of a lane's share of 16 keys
   static constexpr int NC = F32 ? EL : EL < 8 ? 1 : EL / 8;  // products over it
   static constexpr int VD = D / 16;                    // channels of a lane in O
-  static constexpr int VB = VD * E;                    // their bytes of a key
+  static constexpr int VB = VD * BITS < 8 ? 1 : VD * BITS / 8;  // their bytes of a key
   static constexpr int VW = VB < 4 ? 1 : VB / 4;
   static constexpr int NG = tile_groups(CT, D);  // 32-key groups that a wave loads at once
   static constexpr int TILE = 32 * NG;
@@ -201,6 +203,7 @@ struct Wave {
   u32x4_t q[F::F32 ? 1 : F::NQ][F::F32 ? 1 : F::NC];
   float qf[F::F32 ? F::EL : 1];
   uint32_t k[2 * F::NG][F::KW];
+  uint32_t ks[is4(F::CT) ? 2 * F::NG : 1];  // scales of 4-bit cells: of the lane's channels, which are of one group
 
   // Channel of a lane's element x: unit x / U of 4U channels, one U a lane group.
   __device__ __forceinline__ int channel(int x) const { return x / F::U * 4 * F::U + g * F::U + x % F::U; }
@@ -266,15 +269,21 @@ struct Wave {
                                                      0, 0, 0);
   }
 
+  static __device__ __forceinline__ const uint8_t* page_of(const void* cells, int64_t page, int id) {
+    return (const uint8_t*)cells + (int64_t)id * page * (int64_t)sizeof(typename Cell<F::CT>::T);
+  }
+
   __device__ __forceinline__ void load_k(const Pages& pg, int h, const Tile<F>& t) {
-    const int lane_at = (n * F::D + g * F::U) * F::E;
+    const int lane_at = n * F::ROW + g * F::UB;
 #pragma unroll
     for (int i = 0; i < 2 * F::NG; ++i) {
-      const uint8_t* base =
-          (const uint8_t*)pg.k + ((int64_t)t.b[i].id * pg.k_page + (int64_t)(h * pg.ps + t.b[i].slot) * F::D) * F::E;
+      const uint8_t* base = page_of(pg.k, pg.k_page, t.b[i].id) + (int64_t)(h * pg.ps + t.b[i].slot) * F::ROW;
 #pragma unroll
-      for (int u = 0; u < F::EL / F::U; ++u)
-        load_bytes<F::U * F::E>(base + lane_at + u * 4 * F::U * F::E, &k[i][u * F::U * F::E / 4]);
+      for (int u = 0; u < F::EL / F::U; ++u) load_bytes<F::UB>(base + lane_at + u * 4 * F::UB, &k[i][u * F::UB / 4]);
+      if constexpr (is4(F::CT)) {
+        const int64_t row = ((int64_t)t.b[i].id * pg.H + h) * pg.ps + t.b[i].slot;
+        ks[i] = ((const uint8_t*)pg.k_scale)[row * F::NS + n * F::NS + g * F::EL / 32];
+      }
     }
   }
 
@@ -293,7 +302,10 @@ struct Wave {
 #pragma unroll
       for (int c = 0; c < F::NC; ++c) {
         u32x4_t a = {0, 0, 0, 0};
-        if constexpr (is8(F::CT)) {
+        if constexpr (is4(F::CT)) {
+#pragma unroll
+          for (int w = 0; w < (F::EL < 8 ? 2 : 4); ++w) a[w] = e2m1_bf16(k[i][c], power_of(ks[i]), w);
+        } else if constexpr (is8(F::CT)) {
 #pragma unroll
           for (int w = 0; w < (F::EL < 8 ? 2 : 4); ++w) a[w] = cells2_bf16<F::CT>(k[i][2 * c + w / 2], w & 1);
         } else {
@@ -315,18 +327,20 @@ struct Wave {
                                        const Tile<F>& next, State<F>& st) {
     uint32_t v[2 * F::NG][4][F::VW];
     f32x4_t s[2 * F::NG], vs[2 * F::NG];
-    const int lane_at = 4 * g * F::D * F::E + n * F::VB;
+    [[maybe_unused]] uint32_t raw[2 * F::NG][F::NS];  // V's scales of 4-bit cells: four keys'
+    const int lane_at = 4 * g * F::ROW + n * F::VD * F::BITS / 8;
 #pragma unroll
     for (int i = 0; i < 2 * F::NG; ++i) {
       const int64_t slot = (int64_t)(h * pg.ps + t.b[i].slot);
-      const uint8_t* base = (const uint8_t*)pg.v + ((int64_t)t.b[i].id * pg.v_page + slot * F::D) * F::E;
+      const uint8_t* base = page_of(pg.v, pg.v_page, t.b[i].id) + slot * F::ROW;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) load_bytes<F::VB>(base + lane_at + y * F::D * F::E, v[i][y]);
+      for (int y = 0; y < 4; ++y) load_bytes<F::VB>(base + lane_at + y * F::ROW, v[i][y]);
+      const int64_t at = ((int64_t)t.b[i].id * pg.H) * pg.ps + slot + 4 * g;
       if constexpr (is8(F::CT)) {
-        const int64_t at = ((int64_t)t.b[i].id * pg.H) * pg.ps + slot + 4 * g;
-        s[i] = *reinterpret_cast<const f32x4_t*>(pg.k_scale + at);
-        vs[i] = *reinterpret_cast<const f32x4_t*>(pg.v_scale + at);
+        s[i] = *reinterpret_cast<const f32x4_t*>((const float*)pg.k_scale + at);
+        vs[i] = *reinterpret_cast<const f32x4_t*>((const float*)pg.v_scale + at);
       }
+      if constexpr (is4(F::CT)) load_bytes<4 * F::NS>((const uint8_t*)pg.v_scale + at * F::NS, raw[i]);
     }
     __builtin_amdgcn_sched_barrier(0);  // V is on its way before K is waited for
 #pragma unroll
@@ -336,6 +350,17 @@ struct Wave {
     }
     load_k(pg, h, next);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (is4(F::CT)) {
+      // byte y * NS + (the lane's group) of the four keys', as the exponent of an f32
+      const int group = n * F::VD / 32;
+#pragma unroll
+      for (int i = 0; i < 2 * F::NG; ++i)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          vs[i][y] = power_of(raw[i][y * F::NS / 4] >> (8 * (y * F::NS % 4) + 8 * group) & 255u);
+          if constexpr (F::VD == 1) v[i][y][0] = v[i][y][0] >> 4 * (n & 1) & 15u;
+        }
+    }
     if (!t.whole(r)) {
       // keys that are not seen: no weight, and nothing of what stands there
 #pragma unroll
@@ -345,7 +370,7 @@ struct Wave {
         for (int y = 0; y < 4; ++y) {
           const bool seen = pos + y >= r.start && pos + y < r.len;
           s[i][y] = seen ? s[i][y] : -INFINITY;
-          if constexpr (is8(F::CT)) vs[i][y] = seen ? vs[i][y] : 0.0f;
+          if constexpr (scaled(F::CT)) vs[i][y] = seen ? vs[i][y] : 0.0f;
 #pragma unroll
           for (int w = 0; w < F::VW; ++w) v[i][y][w] = seen ? v[i][y][w] : 0u;
         }
@@ -401,7 +426,8 @@ struct Wave {
           uint32_t w[8];
 #pragma unroll
           for (int y = 0; y < 8; ++y) {
-            if constexpr (is8(F::CT)) w[y] = cells2_bf16<F::CT>(v[i + y / 4][y & 3][jj / 2], jj & 1);
+            if constexpr (is4(F::CT)) w[y] = e2m1_bf16(v[i + y / 4][y & 3][jj / 4], vs[i + y / 4][y & 3], jj & 3);
+            else if constexpr (is8(F::CT)) w[y] = cells2_bf16<F::CT>(v[i + y / 4][y & 3][jj / 2], jj & 1);
             else w[y] = v[i + y / 4][y & 3][jj];
           }
 #pragma unroll
@@ -898,6 +924,7 @@ void attend_by_width(const AttendCall& a) {
 void attend_float(int qt, const AttendCall& a);
 void attend_i8(int qt, const AttendCall& a);
 void attend_e4m3(int qt, const AttendCall& a);
+void attend_e2m1(int qt, const AttendCall& a);
 
 }  // namespace paged
 }  // namespace pfa

@@ -4,7 +4,7 @@
 that generates holds the keys and values of what it has read and written, and
 asks for one token's attention at a time:
 
-* :func:`new_kv_pages` -- a pool of pages, in the values' type or in 8 bits;
+* :func:`new_kv_pages` -- a pool of pages, in the values' type or in 8 or 4 bits;
 * :func:`write_kv_pages` -- new tokens into their sequences' pages, quantised as
   they are written;
 * :func:`read_kv_pages` -- a range of every sequence back out of its pages;
@@ -36,8 +36,13 @@ HEAD_DIMS = (16, 32, 64, 128)
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
 _VALUE_TAG = {torch.float32: _hip.PFA_F32, torch.bfloat16: _hip.PFA_BF16, torch.float16: _hip.PFA_F16}
-_CELL_TAG = {**_VALUE_TAG, torch.int8: _hip.PFA_I8, torch.float8_e4m3fn: _hip.PFA_E4M3}
-_EIGHT_BITS = (torch.int8, torch.float8_e4m3fn)
+_CELL_TAG = {**_VALUE_TAG, torch.int8: _hip.PFA_I8, torch.float8_e4m3fn: _hip.PFA_E4M3,
+             torch.float4_e2m1fn_x2: _hip.PFA_E2M1}
+_FOUR_BITS = torch.float4_e2m1fn_x2  # two cells an element
+_SCALED = (torch.int8, torch.float8_e4m3fn, _FOUR_BITS)
+# Type of the scales and of the key bounds of cells that have scales.
+_SCALE_TYPE = {torch.int8: torch.float32, torch.float8_e4m3fn: torch.float32, _FOUR_BITS: torch.float8_e8m0fnu}
+_BOUND_TYPE = {torch.int8: torch.float32, torch.float8_e4m3fn: torch.float32, _FOUR_BITS: torch.bfloat16}
 # Pages of a table or list, sequences: the library takes them in 32 bits and has limits
 # of its own below these, by the page size and the rows.
 _MOST = 1 << 30
@@ -45,18 +50,27 @@ _MOST = 1 << 30
 
 class KVPages(NamedTuple):
     """A pool of pages.  ``k``, ``v``: ``(pages, kv_heads, page_size,
-    head_dim)`` cells, f32, bf16, f16, int8 or float8_e4m3fn (a stride between
-    pages is fine, the inner dimensions are dense).  ``k_scale``, ``v_scale``:
-    ``(pages, kv_heads, page_size)`` f32 for 8-bit cells.  ``k_bounds``: the
-    least and the largest stored key of every channel, ``(pages, kv_heads, 2,
-    head_dim)`` in the cells' type, f32 for 8-bit cells; needed for selection
-    alone."""
+    head_dim)`` cells, f32, bf16, f16, int8 or float8_e4m3fn, or ``(pages,
+    kv_heads, page_size, head_dim / 2)`` float4_e2m1fn_x2, two cells an element
+    (a stride between pages is fine, the inner dimensions are dense).
+    ``k_scale``, ``v_scale``: ``(pages, kv_heads, page_size)`` f32 for 8-bit
+    cells; ``(pages, kv_heads, page_size, head_dim / 32)`` float8_e8m0fnu for
+    4-bit cells, a power of two for 32 neighbouring channels (one for all of a
+    head of 16).  ``k_bounds``: the least and the largest stored key of every
+    channel, ``(pages, kv_heads, 2, head_dim)`` in the cells' type, f32 for 8-bit
+    and bf16 for 4-bit cells; needed for selection alone."""
 
     k: torch.Tensor
     v: torch.Tensor
     k_scale: Optional[torch.Tensor] = None
     v_scale: Optional[torch.Tensor] = None
     k_bounds: Optional[torch.Tensor] = None
+
+
+def _scales(head_dim: int) -> int:
+    """Scales of a row of 4-bit cells."""
+
+    return max(head_dim // 32, 1)
 
 
 def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *,
@@ -69,15 +83,18 @@ def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *
         raise ValueError(f"head_dim must be one of {HEAD_DIMS} and page_size one of {PAGE_SIZES}")
     if num_pages < 1 or kv_heads < 1:
         raise ValueError("a pool needs pages and heads")
-    shape = (num_pages, kv_heads, page_size, head_dim)
-    k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+    four = dtype is _FOUR_BITS
+    shape = (num_pages, kv_heads, page_size, head_dim // 2 if four else head_dim)
+    k, v = (torch.zeros(shape, dtype=torch.uint8 if four else dtype, device=device).view(dtype) for _ in range(2))
     scales = (None, None)
-    if dtype in _EIGHT_BITS:
+    if four:
+        scales = tuple(torch.zeros(*shape[:3], _scales(head_dim), dtype=torch.uint8, device=device).view(_SCALE_TYPE[dtype])
+                       for _ in range(2))
+    elif dtype in _SCALED:
         scales = tuple(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
     kb = None
     if bounds:
-        kb = torch.zeros(num_pages, kv_heads, 2, head_dim, device=device,
-                         dtype=torch.float32 if dtype in _EIGHT_BITS else dtype)
+        kb = torch.zeros(num_pages, kv_heads, 2, head_dim, device=device, dtype=_BOUND_TYPE.get(dtype, dtype))
     return KVPages(k, v, *scales, kb)
 
 
@@ -104,26 +121,29 @@ def _pool(pages: KVPages) -> tuple:
         raise ValueError(f"k and v pages must share one of {tuple(_CELL_TAG)} (got {dtype}, {v.dtype})")
     if len(shape) != 4 or v.shape != shape:
         raise ValueError("k and v pages must be (pages, kv_heads, page_size, head_dim) tensors of one shape")
-    N, H, ps, D = shape
+    N, H, ps, row = shape
+    D = 2 * row if dtype is _FOUR_BITS else row
     if D not in HEAD_DIMS or ps not in PAGE_SIZES:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS} and page_size one of {PAGE_SIZES} (got {D}, {ps})")
     if N == 0 or H == 0:
         raise ValueError("an empty pool")
     ks, vs = k.stride(), v.stride()
-    dense = (ps * D, D, 1)
+    dense = (ps * row, row, 1)
     if ks[1:] != dense or vs[1:] != dense:
         for s in (ks, vs):
             if s[2:] != dense[1:] or (H > 1 and s[1] != dense[0]):
                 raise ValueError("a page's heads, slots and channels must be dense")
     a = c = b = 0
     bound_dtype = dtype
-    if dtype in _EIGHT_BITS:
+    if dtype in _SCALED:
         if k_scale is None or v_scale is None:
-            raise ValueError("8-bit pages need k_scale and v_scale")
-        rows = shape[:3]
-        a = _dense(k_scale, rows, torch.float32, "k_scale")
-        c = _dense(v_scale, rows, torch.float32, "v_scale")
-        bound_dtype = torch.float32
+            raise ValueError("pages of 8 or 4 bits need k_scale and v_scale")
+        rows, scale_dtype = shape[:3], _SCALE_TYPE[dtype]
+        if dtype is _FOUR_BITS:
+            rows = (N, H, ps, _scales(D))
+        a = _dense(k_scale, rows, scale_dtype, "k_scale")
+        c = _dense(v_scale, rows, scale_dtype, "v_scale")
+        bound_dtype = _BOUND_TYPE[dtype]
     if bounds is not None:
         b = _dense(bounds, (N, H, 2, D), bound_dtype, "k_bounds")
     if (k.requires_grad or v.requires_grad or (b and bounds.requires_grad)
@@ -214,10 +234,14 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     without ``counts``), goes to position ``starts[b] + i``.  Positions below
     zero, behind the table's last page or without a page are left out.
 
-    Values have the pages' type, or f32, bf16 or f16 for 8-bit pages: a row is
-    divided by ``scale = max(absmax / top, 1e-6)`` (top 127 for int8, 448 for
-    e4m3) and rounded to nearest even.  A row with a value that is not finite
-    gets scale NaN, and reads back as NaN.  The pages' key bounds, where the
+    Values have the pages' type, or f32, bf16 or f16 for pages of 8 or 4 bits: a
+    row is divided by ``scale = max(absmax / top, 1e-6)`` (top 127 for int8, 448
+    for e4m3) and rounded to nearest even.  In 4 bits every group of 32 channels
+    (16 of a head of 16) is divided by the least power of two from 2^-20 to 2^125
+    that is a seventh of its absmax or more, and rounded to the nearest of 0, 0.5,
+    1, 1.5, 2, 3, 4, 6 (ties to the even one of these: 0, 1, 2, 4) and their
+    negatives.  A row or group with a value that is not finite gets scale NaN,
+    and reads back as NaN.  The pages' key bounds, where the
     pool has them, follow: they start anew with a page's first slot, so a page
     is written from there on.
 
@@ -233,7 +257,7 @@ def write_kv_pages(pages: KVPages, k: torch.Tensor, v: torch.Tensor, block_table
     if H != pool_heads or D != pool_dim:
         raise ValueError(f"k and v have {H} heads of {D}, the pages {pool_heads} of {pool_dim}")
     tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
-    if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
+    if tag is None or (cells != dtype and cells not in _SCALED):
         raise ValueError(f"values of {dtype} for pages of {cells}")
     table, starts = _table(block_table, B), _per_sequence(starts, B, "starts")
     if counts is not None:
@@ -258,7 +282,7 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
                   n: int, *, dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Positions ``starts[b] .. starts[b] + counts[b] - 1`` (``counts`` None:
     n of them) of every sequence: k and v ``(B, n, kv_heads, head_dim)`` in
-    ``dtype`` (default: the pages' type, f32 for 8-bit pages).  Rows
+    ``dtype`` (default: the pages' type, f32 for pages of 8 or 4 bits).  Rows
     i >= ``counts[b]``, and those without a page, are zero."""
 
     pool = _pool(pages)
@@ -270,7 +294,7 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     if n < 0:
         raise ValueError("n must not be negative")
     if dtype is None:
-        dtype = torch.float32 if pages[0].dtype in _EIGHT_BITS else pages[0].dtype
+        dtype = torch.float32 if pages[0].dtype in _SCALED else pages[0].dtype
     tag = _VALUE_TAG.get(dtype)
     if tag is None:
         raise ValueError(f"unsupported value dtype {dtype}")
@@ -299,7 +323,7 @@ def _query(what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor
     if D != pool_dim or H == 0 or H % Hkv:
         raise ValueError(f"q has {H} heads of {D}, the pages {Hkv} of {pool_dim}")
     tag, cells = _VALUE_TAG.get(dtype), pages[0].dtype
-    if tag is None or (cells != dtype and cells not in _EIGHT_BITS):
+    if tag is None or (cells != dtype and cells not in _SCALED):
         raise ValueError(f"queries of {dtype} for pages of {cells}")
     table, lengths = _table(block_table, B), _per_sequence(lengths, B, "lengths")
     P, starts_ptr = table.shape[1], 0
