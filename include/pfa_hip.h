@@ -747,6 +747,42 @@ int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count, int first
                               float scale, int32_t* chosen, void* out, void* workspace,
                               size_t ws_bytes, void* stream);
 
+/* pfa_paged_attn_fwd without lists that also adds to every key that it sees what
+ * attention it got: weights (B, kv_heads, weights_n) f32, rows weights_b and
+ * weights_h apart, of at least table_pages * page_size positions; position t of a
+ * key-value head gets the sum, over the query heads that share it, of
+ * exp(score_t - max) / sum, added in f32 in the heads' order.  Positions that are
+ * not seen, or have no page, stay as they are; a row that is NaN gives NaN.  No
+ * rows of weights may overlap.  The workspace holds the scores: 4 bytes for each
+ * query head and position of the table, of every sequence. */
+int pfa_paged_weigh_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
+                                        int cell_dtype, int table_pages, size_t* bytes);
+int pfa_paged_weigh_attn_fwd(const pfa_paged_query* query, float* weights, int64_t weights_b,
+                             int64_t weights_h, int64_t weights_n, float scale, void* out,
+                             void* workspace, size_t ws_bytes, void* stream);
+
+/* The `count` positions below lengths[b] (and n) of each sequence and head with the
+ * largest weights (B, H, n): kept (B, H, count) int32, ascending, -1 behind the
+ * last.  The `first` first and `last` last positions come before all others, then
+ * the larger weight, then the lower position; NaN counts below everything, -0 and
+ * +0 alike. */
+int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int64_t weights_h, int64_t n,
+                         int B, int H, const int32_t* lengths, int count, int first, int last,
+                         int32_t* kept, void* stream);
+
+/* That choice among the positions that have a page, and a move: the i-th kept
+ * position's cells and scales, of every head, into slot i of the pages that `into`
+ * (B, into_pages, at least count positions) names, its weight into fresh (B,
+ * kv_heads, n) dense, zeros behind the last.  k_bounds of the new pages, where the
+ * pool has them, are those of their kept keys.  Entries of `into` without a page
+ * take nothing.  No page of `into` may be one of the call's `table`, or named
+ * twice: the other pages stay as they are. */
+int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weights, int64_t weights_b,
+                        int64_t weights_h, int64_t n, int B, const int32_t* table,
+                        int64_t table_stride, int table_pages, const int32_t* lengths, int count,
+                        int first, int last, const int32_t* into, int64_t into_stride,
+                        int into_pages, int32_t* kept, float* fresh, void* stream);
+
 /* ====================================================================
  * Rotary positions of queries and keys.  The reference turns whole heads of
  * whole sequences (aspa.py:606-618, pfa_rope_qk_inplace); these are the

@@ -2,6 +2,8 @@
 // and attend to them.
 #pragma once
 
+#include <type_traits>
+
 #include "pfa_common.h"
 
 namespace pfa {
@@ -115,6 +117,58 @@ __device__ __forceinline__ void cells8(const typename Cell<DT>::T* p, float (&o)
     }
   } else {
     load8<DT>(p, o);
+  }
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The bounds of a page's rows over a workgroup, whose threads hold eight channels of
+// some rows each, D / 8 neighbours a row: put(d, least, largest) for every channel.
+template <int D, int WAVES, typename Put>
+__device__ __forceinline__ void join_bounds(float (&lo)[8], float (&hi)[8], float (&part)[2][WAVES][D], Put&& put) {
+  constexpr int LANES = D / 8;
+  const int lane = threadIdx.x % LANES, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int o = LANES; o < kWave; o <<= 1) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo[j] = min_nan(lo[j], __shfl_xor(lo[j], o));
+      hi[j] = max_nan(hi[j], __shfl_xor(hi[j], o));
+    }
+  }
+  if (threadIdx.x % kWave < LANES) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[0][wave][8 * lane + j] = lo[j], part[1][wave][8 * lane + j] = hi[j];
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float a = part[0][0][d], z = part[1][0][d];
+    for (int w = 1; w < (int)blockDim.x / kWave; ++w) a = min_nan(a, part[0][w][d]), z = max_nan(z, part[1][w][d]);
+    put(d, a, z);
+  }
+  __syncthreads();
+}
+
+// Calls f with the head's width as a template argument.
+template <typename F>
+void by_width(int D, F&& f) {
+  if (D == 16) f(std::integral_constant<int, 16>{});
+  else if (D == 32) f(std::integral_constant<int, 32>{});
+  else if (D == 64) f(std::integral_constant<int, 64>{});
+  else f(std::integral_constant<int, 128>{});
+}
+
+// Calls f with the cells' type as a template argument.
+template <typename F>
+void by_cells(int ct, F&& f) {
+  switch (ct) {
+    case PFA_F32: return f(std::integral_constant<int, PFA_F32>{});
+    case PFA_BF16: return f(std::integral_constant<int, PFA_BF16>{});
+    case PFA_F16: return f(std::integral_constant<int, PFA_F16>{});
+    case PFA_I8: return f(std::integral_constant<int, PFA_I8>{});
+    case PFA_E4M3: return f(std::integral_constant<int, PFA_E4M3>{});
+    default: return f(std::integral_constant<int, PFA_E2M1>{});
   }
 }
 

@@ -64,9 +64,6 @@ namespace {
 // quotient.  25,600 rows of 8 heads of 128 bf16 values into int8 pages with bounds:
 // 41 to 52 us, 162 MB (58 with divisions and selects for NaN).
 // ---------------------------------------------------------------------
-__device__ __forceinline__ float min_nan(float a, float b) { return __builtin_elementwise_minimum(a, b); }
-__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-
 // The largest over 2, 4, 8 or 16 lanes that lie together.
 template <int LANES>
 __device__ __forceinline__ float max_lanes(float x) {
@@ -199,7 +196,7 @@ __global__ void __launch_bounds__(1024) write_kernel(Pages pg, Table tab, NewRow
   count = count < 0 ? 0 : count < n ? count : n;
   const int64_t first = start < 0 ? 0 : start;  // positions written: [first, end)
   const int64_t end = start + count;
-  const int lane = threadIdx.x % LANES, rows = blockDim.x / LANES, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % LANES, rows = blockDim.x / LANES;
   const bool back = pg.bounds != nullptr;
   __shared__ float part[2][16][D];
   // heads of one page are neighbours, as their new rows are in memory
@@ -233,30 +230,14 @@ __global__ void __launch_bounds__(1024) write_kernel(Pages pg, Table tab, NewRow
       }
     }
     if (!back) continue;
-#pragma unroll
-    for (int o = LANES; o < kWave; o <<= 1) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        lo[j] = min_nan(lo[j], __shfl_xor(lo[j], o));
-        hi[j] = max_nan(hi[j], __shfl_xor(hi[j], o));
-      }
-    }
-    if (threadIdx.x % kWave < LANES) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) part[0][wave][8 * lane + j] = lo[j], part[1][wave][8 * lane + j] = hi[j];
-    }
-    __syncthreads();
     constexpr int BT = bound_dtype(CT);
     using BoundT = typename Elem<BT>::T;
     BoundT* out = (BoundT*)pg.bounds + ((int64_t)id * pg.H + h) * 2 * D;
-    for (int d = threadIdx.x; d < D; d += blockDim.x) {
-      float a = part[0][0][d], z = part[1][0][d];
-      for (int w = 1; w < (int)blockDim.x / kWave; ++w) a = min_nan(a, part[0][w][d]), z = max_nan(z, part[1][w][d]);
+    join_bounds<D>(lo, hi, part, [&](int d, float a, float z) {
       if (from > base) a = min_nan(a, load_f<BT>(out + d)), z = max_nan(z, load_f<BT>(out + D + d));
       store_f<BT>(out + d, a);
       store_f<BT>(out + D + d, z);
-    }
-    __syncthreads();
+    });
   }
 }
 
@@ -350,15 +331,6 @@ void by_types(int dt, int ct, F&& f) {
 #undef PFA_PAIR
 }
 
-// Calls f with the head's width as a template argument.
-template <typename F>
-void by_width(int D, F&& f) {
-  if (D == 16) f(std::integral_constant<int, 16>{});
-  else if (D == 32) f(std::integral_constant<int, 32>{});
-  else if (D == 64) f(std::integral_constant<int, 64>{});
-  else f(std::integral_constant<int, 128>{});
-}
-
 int types_check(int dt, int ct) {
   PFA_CHECK_ARG(dt == PFA_F32 || dt == PFA_BF16 || dt == PFA_F16, "pages: unknown value type %d", dt);
   PFA_CHECK_ARG(scaled(ct) || dt == ct, "pages: values of type %d for cells of type %d", dt, ct);
@@ -435,14 +407,7 @@ extern "C" int pfa_kv_pages_read(const pfa_kv_pages* pages, int B, int64_t n, co
     else if (out_dtype == PFA_BF16) launch(ct, std::integral_constant<int, PFA_BF16>{});
     else launch(ct, std::integral_constant<int, PFA_F16>{});
   };
-  switch (pages->dtype) {
-    case PFA_F32: by_out(std::integral_constant<int, PFA_F32>{}); break;
-    case PFA_BF16: by_out(std::integral_constant<int, PFA_BF16>{}); break;
-    case PFA_F16: by_out(std::integral_constant<int, PFA_F16>{}); break;
-    case PFA_I8: by_out(std::integral_constant<int, PFA_I8>{}); break;
-    case PFA_E4M3: by_out(std::integral_constant<int, PFA_E4M3>{}); break;
-    default: by_out(std::integral_constant<int, PFA_E2M1>{}); break;
-  }
+  by_cells(pages->dtype, by_out);
   PFA_CHECK_LAUNCH("kv_pages_read");
   return PFA_OK;
 }
@@ -545,21 +510,34 @@ static bool selects_itself(const Plan& plan, int P, int D) {
   return plan.bytes == 0 && plan.deal.RT == 1 && few_pages(P, D);
 }
 
+// Behind a call's own workspace, where it weighs its keys: the scores and the rows'
+// statistics.
+static size_t weigh_bytes(int B, int H, int P, int shift) {
+  return (size_t)B * H * (((size_t)P << shift) * sizeof(float) + sizeof(float2));
+}
+static size_t aligned16(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
+
 static int attend(const char* what, const pfa_paged_query* query, const Pages& p, const Table& t, const int32_t* selected,
-                  int64_t selected_stride, int S, const Choice& choice, float scale, void* out, void* workspace,
-                  size_t ws_bytes, void* stream) {
+                  int64_t selected_stride, int S, const Choice& choice, Weigh weigh, float scale, void* out,
+                  void* workspace, size_t ws_bytes, void* stream) {
   const float c = scale * 1.44269504088896340736f;
   PFA_CHECK_ARG(c > 0.0f && c < INFINITY, "%s: scale must be positive and finite", what);
   const int B = query->B, H = query->H, D = query->pages.head_dim, ct = query->pages.dtype;
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "%s: null or unaligned argument", what);
   const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D), choice.count > 0);
-  if (ws_bytes < plan.bytes || (plan.bytes && (!workspace || (uintptr_t)workspace % 16 != 0))) {
-    set_error("%s: workspace of %zu bytes, %zu needed, 16-byte aligned", what, ws_bytes, plan.bytes);
+  const size_t need = weigh.weights ? aligned16(plan.bytes) + weigh_bytes(B, H, t.P, p.shift) : plan.bytes;
+  if (ws_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16 != 0))) {
+    set_error("%s: workspace of %zu bytes, %zu needed, 16-byte aligned", what, ws_bytes, need);
     return PFA_E_WORKSPACE;
   }
+  if (weigh.weights) {
+    weigh.cap = (int64_t)t.P << p.shift;
+    weigh.scores = (float*)((char*)workspace + aligned16(plan.bytes));
+    weigh.stats = (float2*)(weigh.scores + (int64_t)B * H * weigh.cap);
+  }
   const AttendCall a{p, t.ids, t.stride, t.P, B, H, D, query->q, query->lengths, query->starts, selected,
-                     selected_stride, S, c, choice, out, (float*)workspace, as_stream(stream)};
+                     selected_stride, S, c, choice, weigh, out, (float*)workspace, as_stream(stream)};
   if (ct == PFA_I8) attend_i8(query->dtype, a);
   else if (ct == PFA_E4M3) attend_e4m3(query->dtype, a);
   else if (ct == PFA_E2M1) attend_e2m1(query->dtype, a);
@@ -578,8 +556,33 @@ extern "C" int pfa_paged_attn_fwd(const pfa_paged_query* query, const int32_t* s
   PFA_CHECK_ARG(n_selected <= 0 || (selected && selected_stride >= n_selected),
                 "paged_attn: lists that are null or overlap");
   PFA_CHECK_ARG((int64_t)n_selected << p.shift <= (1ll << 30), "paged_attn: lists of up to 2^30 positions");
-  return attend("paged_attn", query, p, t, selected, selected_stride, n_selected < 0 ? -1 : n_selected, Choice{}, scale,
+  return attend("paged_attn", query, p, t, selected, selected_stride, n_selected < 0 ? -1 : n_selected, Choice{}, Weigh{}, scale,
                 out, workspace, ws_bytes, stream);
+}
+
+extern "C" int pfa_paged_weigh_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim, int cell_dtype,
+                                                   int table_pages, size_t* bytes) {
+  if (int rc = pfa_paged_attn_workspace_size(B, H, kv_heads, page_size, head_dim, cell_dtype, table_pages, -1, bytes))
+    return rc;
+  *bytes = aligned16(*bytes) + weigh_bytes(B, H, table_pages, shift_of(page_size));
+  return PFA_OK;
+}
+
+extern "C" int pfa_paged_weigh_attn_fwd(const pfa_paged_query* query, float* weights, int64_t weights_b, int64_t weights_h,
+                                        int64_t weights_n, float scale, void* out, void* workspace, size_t ws_bytes,
+                                        void* stream) {
+  clear_error();
+  Pages p;
+  Table t;
+  if (int rc = query_check("paged_weigh_attn", query, &p, &t)) return rc;
+  PFA_CHECK_ARG(weights || query->B == 0 || t.P == 0, "paged_weigh_attn: null argument");
+  PFA_CHECK_ARG((uintptr_t)weights % 4 == 0 && weights_n >= (int64_t)t.P << p.shift,
+                "paged_weigh_attn: weights of %lld positions for a table of %lld", (long long)weights_n,
+                (long long)((int64_t)t.P << p.shift));
+  if (t.P == 0) weights = nullptr;  // no keys to weigh
+  const bool vec = (uintptr_t)weights % 16 == 0 && weights_b % 4 == 0 && weights_h % 4 == 0;
+  const Weigh weigh{weights, weights_b, weights_h, vec, nullptr, 0, nullptr};
+  return attend("paged_weigh_attn", query, p, t, nullptr, 0, -1, Choice{}, weigh, scale, out, workspace, ws_bytes, stream);
 }
 
 extern "C" int pfa_paged_sparse_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
@@ -616,5 +619,5 @@ extern "C" int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count
     choice = Choice{count, first, last, chosen};
   else if (int rc = pfa_kv_pages_select(query, count, first, last, chosen, workspace, ws_bytes, stream))
     return rc;
-  return attend("paged_sparse_attn", query, p, t, chosen, count, S, choice, scale, out, workspace, ws_bytes, stream);
+  return attend("paged_sparse_attn", query, p, t, chosen, count, S, choice, Weigh{}, scale, out, workspace, ws_bytes, stream);
 }

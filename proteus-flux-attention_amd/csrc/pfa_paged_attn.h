@@ -323,8 +323,10 @@ struct Wave {
   // keys, P, and O.  The next keys are loaded whether or not there is a next tile
   // (`next` is this one then): a load under a condition would have the wait for V
   // wait for them, too.
+  // With KEEP it stores the scores, where `scores_at`, the lane's row of them, is one.
+  template <bool KEEP>
   __device__ __forceinline__ void step(const Pages& pg, const Row& r, int h, float c, const Tile<F>& t,
-                                       const Tile<F>& next, State<F>& st) {
+                                       const Tile<F>& next, State<F>& st, float* __restrict__ scores_at) {
     uint32_t v[2 * F::NG][4][F::VW];
     f32x4_t s[2 * F::NG], vs[2 * F::NG];
     [[maybe_unused]] uint32_t raw[2 * F::NG][F::NS];  // V's scales of 4-bit cells: four keys'
@@ -350,6 +352,11 @@ struct Wave {
     }
     load_k(pg, h, next);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int i = 0; i < 2 * F::NG; ++i)
+        if (scores_at && t.b[i].pos < kNowhere) *reinterpret_cast<f32x4_t*>(scores_at + t.b[i].pos + 4 * g) = s[i];
+    }
     if constexpr (is4(F::CT)) {
       // byte y * NS + (the lane's group) of the four keys', as the exponent of an f32
       const int group = n * F::VD / 32;
@@ -512,27 +519,96 @@ __device__ __forceinline__ float* part_slot(float* parts, int64_t slot, int rows
   return parts + slot * rows * (D + 2);
 }
 
+// Attention that every key got, summed over the query heads of its head: what a call
+// adds to.  The weight of a key is exp2((s - m) c) / l, and m and l are known when
+// all keys are through: the scores are kept, G of them for a key, and read again
+// behind the join.  K again instead would be 64 to 512 bytes for 4 G.
+struct Weigh {
+  float* weights;  // (B, H, T), rows apart by
+  int64_t s_b, s_h;
+  int vec;         // rows are aligned to four
+  float* scores;   // (B * query heads, cap): the products, before the scale
+  int64_t cap;
+  float2* stats;   // (B * query heads): the maximum, and one over the sum
+};
+
+// A row's statistics, as the weights of its keys need them: a row without a score
+// above -inf has none.
+__device__ __forceinline__ float2 row_stats(float m, float l) {
+  return make_float2(m == -INFINITY ? 0.0f : m, l == 0.0f ? 0.0f : 1.0f / l);
+}
+
+// Adds the weights of positions first, first + 4 * step, ... before `end`, four at a
+// time, of the G rows from `row` on, in their order: the same bits every time.
+template <typename Stats>
+__device__ __forceinline__ void add_weights(const Weigh& w, const Pages& pg, const int32_t* __restrict__ ids, int b, int h,
+                                            int64_t row, int G, float c, int start, int len, int64_t first, int step,
+                                            Stats&& stats) {
+  float* to = w.weights + b * w.s_b + h * w.s_h;
+  for (int64_t p = first; p < len; p += 4 * step) {
+    if ((uint32_t)ids[p >> pg.shift] >= (uint32_t)pg.n_pages) continue;
+    float sum[4] = {};
+    const float* at = w.scores + row * w.cap + p;
+#pragma unroll 4
+    for (int g = 0; g < G; ++g) {
+      const f32x4_t s = *reinterpret_cast<const f32x4_t*>(at + g * w.cap);
+      const float2 st = stats(g);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) sum[y] += exp2_((s[y] - st.x) * c) * st.y;
+    }
+    if (w.vec && p >= start && p + 4 <= len) {
+      f32x4_t x = *reinterpret_cast<const f32x4_t*>(to + p);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[y] += sum[y];
+      *reinterpret_cast<f32x4_t*>(to + p) = x;
+    } else {
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (p + y >= start && p + y < len) to[p + y] += sum[y];
+    }
+  }
+}
+
+// Behind the join: a workgroup four times its threads' positions of a sequence and
+// key-value head.
+static __global__ void __launch_bounds__(256) weigh_kernel(Weigh w, Pages pg, const int32_t* __restrict__ table,
+                                                           int64_t table_stride, int P, int G, float c,
+                                                           const int32_t* __restrict__ lengths,
+                                                           const int32_t* __restrict__ starts) {
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int len = length_at(lengths, P, pg.shift, b), start = start_at(starts, b);
+  const int64_t row = ((int64_t)b * pg.H + h) * G;
+  const int64_t first = (start & ~3) + 4 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
+  add_weights(w, pg, table + b * table_stride, b, h, row, G, c, start, len, first, (int)(gridDim.x * blockDim.x),
+              [&](int g) { return w.stats[row + g]; });
+}
+
 // What paged_sparse_attention chooses before it attends.
 struct Choice {
   int count, first, last;
   int32_t* chosen;
 };
 
-// SELECT: the workgroup first selects its pair's pages itself, for a launch and
-// several dependent loads less.
-template <typename F, bool SELECT>
+// What a call does beside attending.  SELECT: the workgroup first selects its pair's
+// pages itself, for a launch and several dependent loads less.  WEIGH: it keeps the
+// scores, and where a workgroup has all of a key's rows it adds their weights itself.
+enum class Also { NOTHING, SELECT, WEIGH };
+
+template <typename F, Also ALSO>
 __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     Pages pg, Deal deal, const int32_t* __restrict__ table, int64_t table_stride,
     const typename Elem<F::QT>::T* __restrict__ q, int64_t q_b, int64_t q_h, int q_vec, int G,
     const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts, const int32_t* __restrict__ selected,
     int64_t selected_stride, float c, typename Elem<F::QT>::T* __restrict__ out, float* __restrict__ parts_ws, Shared* __restrict__ shared,
-    Choice choice) {
+    Choice choice, Weigh weigh) {
   constexpr int D = F::D;
+  constexpr bool SELECT = ALSO == Also::SELECT, WEIGH = ALSO == Also::WEIGH;
   __shared__ float so[kWaves][16][D + 4];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ Entry entries[kEntries + 1];
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found[2];
+  __shared__ float2 stats[WEIGH ? 16 : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Wave<F> w;
@@ -645,6 +721,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     const int here = (h + 1) * G - row0 < 16 ? (h + 1) * G - row0 : 16;
 
     w.load_q(q + b * q_b + (row0 + w.n) * q_h, w.n < here, q_vec);
+    float* scores_at = nullptr;
+    if (WEIGH && w.n < here)
+      scores_at = weigh.scores + ((int64_t)b * (deal.R / deal.RT) * G + row0 + w.n) * weigh.cap;
     State<F> st;
 #pragma unroll
     for (int j = 0; j < F::VD; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -676,7 +755,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
           Tile<F> found;
           t = found.find_seen(r, t + kWaves, re);
           if (t < re) next = found;
-          w.step(pg, r, h, c, cur, next, st);
+          w.template step<WEIGH>(pg, r, h, c, cur, next, st, scores_at);
           cur = next;
         }
       }
@@ -712,14 +791,25 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
         sum += a * sl[j][row];
       }
       if (whole) {
-        store_f<F::QT>(out + ((int64_t)b * (deal.R / deal.RT) * G + row0 + row) * D + d,
-                       sum == 0.0f ? 0.0f : o / (sum * F::PSCALE));
+        const int64_t out_row = (int64_t)b * (deal.R / deal.RT) * G + row0 + row;
+        store_f<F::QT>(out + out_row * D + d, sum == 0.0f ? 0.0f : o / (sum * F::PSCALE));
+        if (WEIGH && d == 0) {
+          if (lone && deal.RT == 1) stats[row] = row_stats(top, sum);
+          else weigh.stats[out_row] = row_stats(top, sum);
+        }
       } else {
         slot[i] = o;
         if (d == 0) slot[rows * D + row] = top, slot[rows * (D + 1) + row] = sum;
       }
     }
-    if (lone) return;
+    if (lone) {
+      if (WEIGH && deal.RT == 1) {
+        __syncthreads();
+        add_weights(weigh, pg, ids, b, h, (int64_t)b * (deal.R / deal.RT) * G + row0, G, c, start, len,
+                    (start & ~3) + 4 * tid, 64 * kWaves, [&](int g) { return stats[g]; });
+      }
+      return;
+    }
     if (ends && pair + 1 == deal.R) ++b;
     __syncthreads();
   }
@@ -736,13 +826,15 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
                                                        const int32_t* __restrict__ starts,
                                                        const float* __restrict__ parts,
                                                        const Shared* __restrict__ shared,
-                                                       typename Elem<QT>::T* __restrict__ out) {
+                                                       typename Elem<QT>::T* __restrict__ out,
+                                                       float2* __restrict__ stats) {
   const int tid = threadIdx.x;
   const int b = blockIdx.x / deal.R, pair = blockIdx.x % deal.R;
   const int h = pair / deal.RT, head0 = h * G + 16 * (pair % deal.RT);
   const int rows = G < 16 ? G : 16, here = (h + 1) * G - head0 < 16 ? (h + 1) * G - head0 : 16;
   const Shared who = shared[blockIdx.x];  // nobody's where the sequence has no tiles
-  typename Elem<QT>::T* to = out + ((int64_t)b * (deal.R / deal.RT) * G + head0) * D;
+  const int64_t row0 = (int64_t)b * (deal.R / deal.RT) * G + head0;
+  typename Elem<QT>::T* to = out + row0 * D;
   if (deal.tiles(start_at(starts, b), deal.length(lengths, b)) == 0) {
     for (int i = blockIdx.y * D + tid; i < here * D; i += THREADS * gridDim.y) store_f<QT>(to + i, 0.0f);
     return;
@@ -789,6 +881,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
       const bool none = a.l == 0.0f;  // no score above -inf, whatever the values are
       const float inv = 1.0f / (a.l * pscale);
       store_f<QT>(to + row * D + d, none ? 0.0f : a.o0 * inv);
+      if (stats && d == 0) stats[row0 + row] = row_stats(a.m, a.l);
       if (two) store_f<QT>(to + row * D + 64 + d, none ? 0.0f : a.o1 * inv);
     }
     return;
@@ -810,6 +903,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
         o += p * acc[w * D + x], l += p * suml[w];
       }
       store_f<QT>(to + row * D + x, l == 0.0f ? 0.0f : o / (l * pscale));
+      if (stats && x == 0) stats[row0 + row] = row_stats(t, l);
     }
     __syncthreads();
   }
@@ -827,6 +921,7 @@ struct AttendCall {
   int S;
   float c;  // scale * log2(e)
   Choice choice;  // count 0: none
+  Weigh weigh;    // weights null: none
   void* out;
   float* parts;
   hipStream_t stream;
@@ -879,35 +974,48 @@ inline int resident(const void* kernel, int threads) {
   return units * each;
 }
 
+inline void weigh_launch(const AttendCall& a, int G) {
+  const int64_t blocks = (a.weigh.cap + 1023) / 1024;
+  weigh_kernel<<<dim3((unsigned)(blocks < 65535 ? blocks : 65535), a.pg.H, a.B), 256, 0, a.stream>>>(
+      a.weigh, a.pg, a.table, a.table_stride, a.P, G, a.c, a.lengths, a.starts);
+}
+
 template <int QT, int CT, int D>
 void attend_launch(const AttendCall& a) {
   using F = Form<QT, CT, D>;
   using T = typename Elem<QT>::T;
   Plan p = attend_plan(a.B, a.H, a.pg.H, D, a.pg.shift, a.P, a.S, F::TILE, a.choice.count > 0);
   Deal& deal = p.deal;
-  static const int at_once = resident(reinterpret_cast<const void*>(&attend_kernel<F, false>), 64 * kWaves);
+  static const int at_once =
+      resident(reinterpret_cast<const void*>(&attend_kernel<F, Also::NOTHING>), 64 * kWaves);
   if (deal.groups > at_once) deal.groups = at_once;
   const int G = a.H / a.pg.H;
   const unsigned pairs = (unsigned)(a.B * deal.R);
   Shared* shared = reinterpret_cast<Shared*>(reinterpret_cast<char*>(a.parts) + p.parts);
   const bool q_vec = ((uintptr_t)a.q.ptr | (uintptr_t)(a.q.s_b * sizeof(T)) | (uintptr_t)(a.q.s_h * sizeof(T))) % 16 == 0;
-  auto launch = [&](auto select) {
-    attend_kernel<F, decltype(select)::value><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
+  const bool weighs = a.weigh.weights != nullptr;
+  auto launch = [&](auto also) {
+    attend_kernel<F, decltype(also)::value><<<p.bytes ? deal.groups : pairs, 64 * kWaves, 0, a.stream>>>(
         a.pg, deal, a.table, a.table_stride, (const T*)a.q.ptr, a.q.s_b, a.q.s_h, q_vec, G, a.lengths, a.starts,
-        a.selected, a.selected_stride, a.c, (T*)a.out, p.bytes ? a.parts : nullptr, shared, a.choice);
+        a.selected, a.selected_stride, a.c, (T*)a.out, p.bytes ? a.parts : nullptr, shared, a.choice, a.weigh);
   };
-  if (a.choice.count > 0) launch(std::integral_constant<bool, true>{});
-  else launch(std::integral_constant<bool, false>{});
-  if (!p.bytes) return;
+  if (a.choice.count > 0) launch(std::integral_constant<Also, Also::SELECT>{});
+  else if (weighs) launch(std::integral_constant<Also, Also::WEIGH>{});
+  else launch(std::integral_constant<Also, Also::NOTHING>{});
+  if (!p.bytes) {
+    if (weighs && deal.RT > 1) weigh_launch(a, G);
+    return;
+  }
   const dim3 rows(pairs, pairs >= kMany ? 1 : G < 16 ? G : 16);
   // the rows of a few pairs have parts by the hundred (8 pairs of 60,000 keys: 36.6 us
   // with 16 waves a row, 37.4 with four; 32 of 25,000: 88.6 and 85.8)
   if (pairs >= 32)
     join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared,
-                                                     (T*)a.out);
+                                                     (T*)a.out, a.weigh.stats);
   else
     join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared,
-                                                       (T*)a.out);
+                                                       (T*)a.out, a.weigh.stats);
+  if (weighs) weigh_launch(a, G);
 }
 
 template <int QT, int CT>

@@ -8,11 +8,13 @@ hand-written gfx950 HIP kernels in ``lib/libpfa_hip.so`` (C ABI declared in
 
 from .kernels.paged_attn import (
     KVPages,
+    evict_kv_tokens,
     new_kv_pages,
     paged_attention,
     paged_sparse_attention,
     read_kv_pages,
     select_kv_pages,
+    select_kv_tokens,
     write_kv_pages,
 )
 from .kernels.rotary import RotaryPositions, apply_rotary, new_rotary_positions, rotary_frequencies
@@ -53,6 +55,8 @@ __all__ = [
     "select_kv_pages",
     "paged_attention",
     "paged_sparse_attention",
+    "select_kv_tokens",
+    "evict_kv_tokens",
     "RotaryPositions",
     "new_rotary_positions",
     "rotary_frequencies",

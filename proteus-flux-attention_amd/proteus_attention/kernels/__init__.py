@@ -2,11 +2,13 @@
 
 from .paged_attn import (
     KVPages,
+    evict_kv_tokens,
     new_kv_pages,
     paged_attention,
     paged_sparse_attention,
     read_kv_pages,
     select_kv_pages,
+    select_kv_tokens,
     write_kv_pages,
 )
 from .rotary import RotaryPositions, apply_rotary, new_rotary_positions, rotary_frequencies
@@ -31,6 +33,8 @@ __all__ = [
     "select_kv_pages",
     "paged_attention",
     "paged_sparse_attention",
+    "select_kv_tokens",
+    "evict_kv_tokens",
     "RotaryPositions",
     "new_rotary_positions",
     "rotary_frequencies",

@@ -11,7 +11,9 @@ asks for one token's attention at a time:
 * :func:`paged_attention` -- one new token a sequence over its cache, over a
   window of it, or over listed pages of it;
 * :func:`select_kv_pages` -- the pages whose keys promise the largest scores;
-* :func:`paged_sparse_attention` -- attention over those.
+* :func:`paged_sparse_attention` -- attention over those;
+* :func:`select_kv_tokens`, :func:`evict_kv_tokens` -- the tokens that
+  :func:`paged_attention` has given most weight, and their move into fresh pages.
 
 A block table ``(B, P)`` int32 names each sequence's pages in the order of its
 positions; entries that name no page (-1) hold no keys.  ``lengths``,
@@ -217,6 +219,13 @@ def _sparse_bytes(*sizes: int) -> int:
     return _size_out(_hip.lib().pfa_paged_sparse_attn_workspace_size, *sizes)
 
 
+@functools.lru_cache(maxsize=256)
+def _weigh_bytes(*sizes: int) -> int:
+    """Workspace of attention that weighs its keys: as of attention, without lists."""
+
+    return _size_out(_hip.lib().pfa_paged_weigh_attn_workspace_size, *sizes)
+
+
 def _scratch(nbytes: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
     """A workspace of the call's own, from torch's allocator on the current
     stream, its address and size."""
@@ -308,8 +317,32 @@ def read_kv_pages(pages: KVPages, block_table: torch.Tensor, starts: torch.Tenso
     return k, v
 
 
+def _apart(stride: Tuple[int, ...], shape: Tuple[int, ...]) -> bool:
+    """Whether the rows of a (B, H, T) tensor are dense and no two of them overlap."""
+
+    (B, H, T), (b, h, t) = shape, stride
+    if T > 1 and t != 1:
+        return False
+    if H > 1 and B > 1 and h > b:
+        B, H, b, h = H, B, h, b
+    if H > 1 and h < T:
+        return False
+    return B <= 1 or b >= h * (H - 1) * (H > 1) + T
+
+
+def _key_weights(t: torch.Tensor, B: int, H: Optional[int], what: str) -> torch.Tensor:
+    if t.dim() != 3 or t.dtype != torch.float32 or t.shape[0] != B or (H is not None and t.shape[1] != H):
+        raise ValueError(f"key_weights must be a ({B}, {'kv_heads' if H is None else H}, T) f32 tensor")
+    if t.shape[2] > _MOST:
+        raise ValueError(f"key_weights of up to {_MOST} positions")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
+    return t
+
+
 def _query(what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor,
-           starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None) -> tuple:
+           starts: Optional[torch.Tensor], selected: Optional[torch.Tensor] = None,
+           key_weights: Optional[torch.Tensor] = None) -> tuple:
     """The arguments that selection and attention share, checked: packed for the
     library, (B, heads, kv_heads, page size, head dim, cell tag, the table's pages),
     the device's index, q, and what must stay referenced until the call is made."""
@@ -332,7 +365,13 @@ def _query(what: str, q: torch.Tensor, pages: KVPages, block_table: torch.Tensor
         starts_ptr = starts.data_ptr()
     if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{what} has no backward pass: call it under torch.no_grad()")
-    index = _device(what, q, *pages, table, lengths, starts, selected)
+    if key_weights is not None:
+        _key_weights(key_weights, B, Hkv, what)
+        if key_weights.shape[2] < P * ps:
+            raise ValueError(f"key_weights of {key_weights.shape[2]} positions for a table of {P * ps}")
+        if not _apart(key_weights.stride(), key_weights.shape):
+            raise ValueError("key_weights needs rows of its own, each dense")
+    index = _device(what, q, *pages, table, lengths, starts, selected, key_weights)
     s = q.stride()
     if s[2] != 1:
         q = q.contiguous()
@@ -355,9 +394,20 @@ def _scale(scale: Optional[float]) -> Optional[float]:
     return scale
 
 
+def _attend_and_weigh(q, pages, block_table, lengths, starts, scale, key_weights) -> torch.Tensor:
+    packed, (B, H, Hkv, ps, D, cell_tag, P), index, q, keep = _query("paged_attention", q, pages, block_table, lengths,
+                                                                      starts, None, key_weights)
+    stride = key_weights.stride()
+    ws, ws_ptr, ws_bytes = _scratch(_weigh_bytes(B, H, Hkv, ps, D, cell_tag, P), q.device)
+    out = _output(q)
+    _call(index, "paged_attn_fwd", _hip.lib().pfa_paged_weigh_attn_fwd, packed, key_weights.data_ptr(), stride[0],
+          stride[1], key_weights.shape[2], 1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(), ws_ptr, ws_bytes)
+    return out
+
+
 def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, *,
                     starts: Optional[torch.Tensor] = None, selected: Optional[torch.Tensor] = None,
-                    scale: Optional[float] = None) -> torch.Tensor:
+                    scale: Optional[float] = None, key_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token a sequence, ``q`` ``(B, heads, head_dim)``,
     over positions ``starts[b] .. lengths[b] - 1`` of its cache (``starts``
     None: from 0).  ``heads`` is a multiple of the pages' kv_heads, each of
@@ -372,8 +422,19 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     sequence sees has no effect, whatever it is; a value that is seen and not
     finite leaves its channel not finite (inf or NaN) in a row that sees another
     score than -inf, a score that is NaN or +inf its row NaN.
+
+    ``key_weights`` ``(B, kv_heads, T)`` f32, T at least the table's positions,
+    rows dense and apart, is added to: position t of a key-value head gets the
+    sum of its softmax weights over the query heads that share it, in f32 and in
+    their order.  Positions that are not seen stay as they are; rows that are
+    NaN give NaN.  It takes a workspace of 4 bytes for each query head and
+    position of the table, and is not combined with ``selected``.
     """
 
+    if key_weights is not None:
+        if selected is not None:
+            raise ValueError("key_weights are of all positions: not with selected")
+        return _attend_and_weigh(q, pages, block_table, lengths, starts, _scale(scale), key_weights)
     if selected is not None and (selected.dim() != 3 or selected.dtype != torch.int32 or selected.shape[2] > _MOST):
         raise ValueError(f"selected must be a (B, kv_heads, S) int32 tensor of up to {_MOST} entries a list")
     scale = _scale(scale)
@@ -391,13 +452,17 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     return out
 
 
-def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, int, int]:
+def _held(count: int, first: int, last: int, what: str) -> Tuple[int, int, int]:
     count, first, last = int(count), int(first), int(last)
+    if not 1 <= count <= _MOST or first < 0 or last < 0 or first + last > count:
+        raise ValueError(f"count must be positive, at most {_MOST}, and hold the first and last {what}")
+    return count, first, last
+
+
+def _counted(pages: KVPages, count: int, first: int, last: int) -> Tuple[int, int, int]:
     if pages[4] is None:
         raise ValueError("selection needs pages with k_bounds")
-    if not 1 <= count <= _MOST or first < 0 or last < 0 or first + last > count:
-        raise ValueError(f"count must be positive, at most {_MOST}, and hold the first and last pages")
-    return count, first, last
+    return _held(count, first, last, "pages")
 
 
 def select_kv_pages(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, lengths: torch.Tensor, count: int, *,
@@ -440,6 +505,74 @@ def paged_sparse_attention(q: torch.Tensor, pages: KVPages, block_table: torch.T
     return out, chosen
 
 
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous()
+
+
+def select_kv_tokens(key_weights: torch.Tensor, lengths: torch.Tensor, count: int, *, first: int = 1,
+                     last: int = 1) -> torch.Tensor:
+    """The ``count`` positions below ``lengths[b]`` of each sequence and key-value
+    head that have the largest ``key_weights`` ``(B, kv_heads, T)``: ``(B,
+    kv_heads, count)`` int32, ascending, -1 behind the last.
+
+    The ``first`` first and ``last`` last positions are always taken; then the
+    larger weight wins, ties the lower position, NaN below everything.
+    """
+
+    count, first, last = _held(count, first, last, "tokens")
+    B = key_weights.shape[0] if key_weights.dim() else 0
+    weights = _dense_rows(_key_weights(key_weights, B, None, "select_kv_tokens"))
+    H, T = weights.shape[1:]
+    if H == 0:
+        raise ValueError("key_weights needs a head")
+    lengths = _per_sequence(lengths, B, "lengths")
+    index = _device("select_kv_tokens", weights, lengths)
+    kept = torch.empty((B, H, count), dtype=torch.int32, device=weights.device)
+    _call(index, "kv_tokens_select", _hip.lib().pfa_kv_tokens_select, weights.data_ptr(), weights.stride(0),
+          weights.stride(1), T, B, H, lengths.data_ptr(), count, first, last, kept.data_ptr())
+    return kept
+
+
+def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                    count: int, into: torch.Tensor, *, first: int = 1,
+                    last: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keeps ``count`` tokens of each sequence and key-value head: those that
+    :func:`select_kv_tokens` takes, of the positions that have a page, move into
+    the pages that ``into`` ``(B, pages)`` int32 names, in their order, from its
+    first slot on.  Cells and scales move as they are, with the pages' key bounds
+    where the pool has them.
+
+    Returns the positions that were kept ``(B, kv_heads, count)``, -1 behind the
+    last, and their key weights, zeros behind them, in a tensor of
+    ``key_weights``' shape: sequences go on with ``into`` for a table, these
+    weights, and ``lengths`` of up to ``count``.  The pages of ``block_table``
+    stay as they are, so that others may share them; no page may be in both
+    tables, or in ``into`` twice.  Tokens for entries of ``into`` that name no page
+    are lost.  Keys keep the rotary positions that they were written with.
+    """
+
+    count, first, last = _held(count, first, last, "tokens")
+    pool = _pool(pages)
+    Hkv, ps = pool[8], pool[9]
+    B = block_table.shape[0] if block_table.dim() else 0
+    table, fresh_table = _table(block_table, B), _table(into, B)
+    if fresh_table.shape[1] * ps < count:
+        raise ValueError(f"{count} tokens into {fresh_table.shape[1]} pages of {ps}")
+    if B and table.data_ptr() == fresh_table.data_ptr():
+        raise ValueError("into must name other pages than block_table")
+    weights = _dense_rows(_key_weights(key_weights, B, Hkv, "evict_kv_tokens"))
+    T = weights.shape[2]
+    lengths = _per_sequence(lengths, B, "lengths")
+    index = _device("evict_kv_tokens", *pages, table, fresh_table, weights, lengths)
+    kept = torch.empty((B, Hkv, count), dtype=torch.int32, device=weights.device)
+    fresh = torch.empty((B, Hkv, T), dtype=torch.float32, device=weights.device)
+    _call(index, "kv_tokens_evict", _hip.lib().pfa_kv_tokens_evict, _POOL.pack(*pool), weights.data_ptr(),
+          weights.stride(0), weights.stride(1), T, B, table.data_ptr(), table.stride(0), table.shape[1],
+          lengths.data_ptr(), count, first, last, fresh_table.data_ptr(), fresh_table.stride(0), fresh_table.shape[1],
+          kept.data_ptr(), fresh.data_ptr())
+    return kept, fresh
+
+
 __all__ = [
     "KVPages",
     "new_kv_pages",
@@ -448,4 +581,6 @@ __all__ = [
     "select_kv_pages",
     "paged_attention",
     "paged_sparse_attention",
+    "select_kv_tokens",
+    "evict_kv_tokens",
 ]
