@@ -15,7 +15,13 @@
 //
 // Bytes bound it: every value is read and written once.  A workgroup takes some tokens
 // of a sequence and computes their sines and cosines into LDS once for all heads, with
-// its first rows already on their way.
+// its first rows already on their way.  65,536 f16 tokens of 16 heads of 64, a fused
+// projection's slices (268 MB): 48 us, 5.6 TB/s, where a copy of them takes 55; lanes
+// that hold both units of a pair, and channels that stay in lanes with half the work:
+// 117.  128 tokens of 40 heads of 128: 4.6 us, one of 16 heads of 64: 2.5, both the
+// chain of position, sine, LDS and store.
+#include <type_traits>
+
 #include "pfa_common.h"
 
 namespace pfa {
@@ -36,9 +42,9 @@ struct Call {
   int H[2];
   int width, D;
   float magnitude;
-  int turning, units, shift;  // units of a row that turn, all of them, and log2 of the lanes of a row
-  int tile, heads;            // tokens and heads of a workgroup
-  uint32_t inverse;           // ceil(2^20 / heads)
+  int units, shift;   // of a row, and log2 of its lanes
+  int tile, heads;    // tokens and heads of a workgroup: several tokens only with all heads
+  uint32_t inverse;   // ceil(2^20 / heads): quotients of up to 1,024 rows
 };
 
 // The angle of a position in turns of 2^-64: its cosine and sine.
@@ -61,129 +67,189 @@ __device__ __forceinline__ float2 cos_sin(int64_t position, uint64_t turns, floa
   return make_float2(((quarter + 1) & 2 ? -a : a) * magnitude, (quarter & 2 ? -b : b) * magnitude);
 }
 
-// N elements (8 of them aligned to 16 bytes, or one) as f32.
-template <int DT, int N>
-__device__ __forceinline__ void get(const void* p, int64_t at, float* x) {
-  const auto* q = (const typename Elem<DT>::T*)p + at;
-  if constexpr (N == 8) {
-    float y[8];
-    load8<DT>(q, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = y[i];
-  } else {
-    x[0] = load_f<DT>(q);
-  }
-}
+// A workgroup's share: some tokens of a sequence, and heads.
+struct Share {
+  int b, h0, tokens, heads, rows;
+  int64_t t0;
 
-template <int DT, int N>
-__device__ __forceinline__ void put(void* p, int64_t at, const float* x) {
-  auto* q = (typename Elem<DT>::T*)p + at;
-  if constexpr (N == 8 && DT == PFA_BF16) {
-    typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
-    bf16x8 y;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = (__bf16)x[i];
-    *reinterpret_cast<bf16x8*>(q) = y;
-  } else if constexpr (N == 8) {
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
-    store8<DT>(q, y);
-  } else {
-    store_f<DT>(q, x[0]);
+  __device__ __forceinline__ explicit Share(const Call& a) {
+    b = blockIdx.y, h0 = blockIdx.z * a.heads;
+    t0 = (int64_t)blockIdx.x * a.tile;
+    tokens = a.n - t0 < a.tile ? (int)(a.n - t0) : a.tile;
+    heads = a.H[0] + a.H[1] - h0 < a.heads ? a.H[0] + a.H[1] - h0 : a.heads;
+    rows = tokens * heads;
   }
-}
+  // Cosines and sines of its tokens' pairs.  Loads come back in order: those for a
+  // thread's first are sent before the rows, so that the rows are not waited for.
+  struct Angle {
+    int64_t position;
+    uint64_t turns;
+  };
+  __device__ __forceinline__ Angle angle(const Call& a, int i) const {
+    const int half = a.width / 2, token = i / half;
+    const int32_t* at = a.positions + b * a.pos_b;
+    if (i >= tokens * half) return Angle{0, 0};
+    return Angle{a.per_token ? (int64_t)at[(t0 + token) * a.pos_t] : *at + t0 + token, a.turns[i - token * half]};
+  }
+  __device__ __forceinline__ void angles(const Call& a, Angle x, float2* table) const {
+    for (int i = threadIdx.x; i < tokens * (a.width / 2); i += blockDim.x) {
+      if (i > (int)threadIdx.x) x = angle(a, i);
+      table[i] = cos_sin(x.position, x.turns, a.magnitude);
+    }
+  }
+};
 
-// VEC: rows of all four tensors are aligned to 16 bytes and fall into units of eight
-// elements; else a unit is a pair, or one of the channels that stay.
-template <int DT, bool HALVES, bool VEC>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(Call a) {
+// Where a row of it is.
+struct Place {
+  const void* in;
+  void* out;
+  int token;
+
+  __device__ __forceinline__ Place(const Call& a, const Share& s, int r, int bytes) {
+    token = (int)((uint32_t)r * a.inverse >> 20);
+    const int head = s.h0 + r - token * s.heads;
+    const bool keys = head >= a.H[0];
+    const int h = keys ? head - a.H[0] : head;
+    // Field by field: a choice between tensors has every lane read them from memory
+    // (65,536 f16 tokens of 16 heads of 64: 66 us, 47 so).
+    auto at = [&](const pfa_tensor4& x, const pfa_tensor4& y) {
+      const int64_t s_h = keys ? y.s_h : x.s_h, s_t = keys ? y.s_t : x.s_t;
+      char* const p0 = (char*)x.ptr + (s.b * x.s_b + s.t0 * x.s_t) * bytes;
+      char* const p1 = (char*)y.ptr + (s.b * y.s_b + s.t0 * y.s_t) * bytes;
+      return (keys ? p1 : p0) + (h * s_h + token * s_t) * bytes;
+    };
+    in = at(a.in[0], a.in[1]);
+    out = at(a.out[0], a.out[1]);
+  }
+};
+
+// Eight elements as they are in memory, and as f32.
+template <int DT>
+struct Eight {
+  uint4 w[DT == PFA_F32 ? 2 : 1];
+
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    const uint4* q = reinterpret_cast<const uint4*>((const typename Elem<DT>::T*)p + at);
+    w[0] = q[0];
+    if constexpr (DT == PFA_F32) w[1] = q[1];
+  }
+  __device__ __forceinline__ void store(void* p, int64_t at) const {
+    uint4* q = reinterpret_cast<uint4*>((typename Elem<DT>::T*)p + at);
+    q[0] = w[0];
+    if constexpr (DT == PFA_F32) q[1] = w[1];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    load8<DT>(reinterpret_cast<const typename Elem<DT>::T*>(w), x);
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    if constexpr (DT == PFA_F32) {
+      store8<DT>(reinterpret_cast<float*>(w), x);
+    } else {
+      using T = std::conditional_t<DT == PFA_BF16, __bf16, _Float16>;
+      typedef __attribute__((__vector_size__(8 * sizeof(T)))) T V;
+      V y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (T)x[i];
+      w[0] = __builtin_bit_cast(uint4, y);
+    }
+  }
+};
+
+// Rows of all four tensors aligned to 16 bytes, in units of eight channels that lie
+// together and turn alike: a lane a unit.  In halves its partner's unit is read, too
+// (from the L1: another lane of the wave reads it), so that all lanes have the same
+// work, whatever part of the head turns.  A row's lanes are of one wave, and their
+// loads are through before the first of its stores: it may turn in place.
+template <int DT, bool HALVES>
+__global__ void __launch_bounds__(kThreads) rows_kernel(Call a) {
   extern __shared__ float2 table[];
-  constexpr int N = VEC ? 8 : 1;                      // elements of a load
-  constexpr int PAIRS = HALVES ? N : VEC ? 4 : 1;     // of a unit
-  constexpr int LOADS = HALVES || !VEC ? 2 : 1;       // of a unit that turns
-  const int b = blockIdx.y, h0 = blockIdx.z * a.heads;
-  const int64_t t0 = (int64_t)blockIdx.x * a.tile;
-  const int tokens = a.n - t0 < a.tile ? (int)(a.n - t0) : a.tile;
-  const int heads = a.H[0] + a.H[1] - h0 < a.heads ? a.H[0] + a.H[1] - h0 : a.heads;
-  const int rows = tokens * heads, step = blockDim.x >> a.shift;
-  const int unit = threadIdx.x & ((1 << a.shift) - 1);
-  const bool turn = unit < a.turning;
-  const int half = a.width / 2;
-  const int at0 = !turn ? a.width + (unit - a.turning) * N : unit * (HALVES ? N : VEC ? 8 : 2);
-  const int at1 = HALVES ? at0 + half : at0 + 1;  // of the second load
-  int row = unit < a.units ? threadIdx.x >> a.shift : rows;
-
-  struct Place {
-    int64_t in, out;
-    int token, which;
-  };
-  auto place = [&](int r) {
-    const int token = (int)((uint32_t)r * a.inverse >> 20);
-    const int head = h0 + r - token * heads;
-    const int which = head >= a.H[0];
-    const int h = head - (which ? a.H[0] : 0);
-    const pfa_tensor4 &x = a.in[which], &y = a.out[which];
-    return Place{b * x.s_b + h * x.s_h + (t0 + token) * x.s_t, b * y.s_b + h * y.s_h + (t0 + token) * y.s_t, token,
-                 which};
-  };
-  float x[kAtOnce][LOADS * N];
-  auto fetch = [&](int first) {
+  const Share s(a);
+  const int step = blockDim.x >> a.shift, unit = threadIdx.x & ((1 << a.shift) - 1), half = a.width / 2;
+  const bool turn = 8 * unit < a.width, upper = HALVES && 8 * unit >= half;
+  const int partner = upper ? 8 * unit - half : 8 * unit + half;
+  const float2* mine = table + (HALVES ? (upper ? partner : 8 * unit) : 4 * unit);
+  int row = unit < a.units ? (int)threadIdx.x >> a.shift : s.rows;
+  Eight<DT> x[kAtOnce], y[HALVES ? kAtOnce : 1];
+  auto fetch = [&]() {
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int r = first + i * step;
-      if (r >= rows) continue;
-      const Place p = place(r);
-      get<DT, N>(a.in[p.which].ptr, p.in + at0, x[i]);
-      if (LOADS == 2 && turn) get<DT, N>(a.in[p.which].ptr, p.in + at1, x[i] + N);
+      if (row + i * step >= s.rows) continue;
+      const Place p(a, s, row + i * step, sizeof(typename Elem<DT>::T));
+      x[i].load(p.in, 8 * unit);
+      if (HALVES && turn) y[i].load(p.in, partner);
     }
   };
-  fetch(row);
-  for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
-    const int token = i / half, pair = i - token * half;
-    const int32_t* at = a.positions + b * a.pos_b;
-    const int64_t position = a.per_token ? (int64_t)at[(t0 + token) * a.pos_t] : *at + t0 + token;
-    table[i] = cos_sin(position, a.turns[pair], a.magnitude);
-  }
+  const Share::Angle first = s.angle(a, threadIdx.x);
+  fetch();
+  s.angles(a, first, table);
   __syncthreads();
-  while (row < rows) {
+  while (row < s.rows) {
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int r = row + i * step;
-      if (r >= rows) continue;
-      const Place p = place(r);
-      void* to = a.out[p.which].ptr;
-      if (!turn) {
-        put<DT, N>(to, p.out + at0, x[i]);
-        continue;
-      }
-      const float2* cs = table + p.token * half + unit * PAIRS;
-      float y[LOADS * N];
+      if (row + i * step >= s.rows) continue;
+      const Place p(a, s, row + i * step, sizeof(typename Elem<DT>::T));
+      if (turn) {
+        const float2* cs = mine + p.token * half;
+        float u[8], o[8];
+        x[i].get(u);
+        if constexpr (HALVES) {
+          float v[8];
+          y[i].get(v);
 #pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        const int u = HALVES ? j : 2 * j, v = HALVES ? j + N : 2 * j + 1;
-        const float2 z = cs[j];
-        y[u] = fmaf(x[i][u], z.x, -(x[i][v] * z.y));
-        y[v] = fmaf(x[i][v], z.x, x[i][u] * z.y);
+          for (int j = 0; j < 8; ++j) {
+            const float vs = v[j] * cs[j].y;
+            o[j] = fmaf(u[j], cs[j].x, upper ? vs : -vs);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            o[j] = fmaf(u[j], cs[j / 2].x, -(u[j + 1] * cs[j / 2].y));
+            o[j + 1] = fmaf(u[j + 1], cs[j / 2].x, u[j] * cs[j / 2].y);
+          }
+        }
+        x[i].set(o);
       }
-      put<DT, N>(to, p.out + at0, y);
-      if (LOADS == 2) put<DT, N>(to, p.out + at1, y + N);
+      x[i].store(p.out, 8 * unit);
     }
     row += kAtOnce * step;
-    if (row < rows) fetch(row);
+    if (row < s.rows) fetch();
+  }
+}
+
+// Any other rows: a lane a pair, or one of the channels that stay.
+template <int DT>
+__global__ void __launch_bounds__(kThreads) pairs_kernel(Call a, int halves) {
+  extern __shared__ float2 table[];
+  using T = typename Elem<DT>::T;
+  const Share s(a);
+  s.angles(a, s.angle(a, threadIdx.x), table);
+  __syncthreads();
+  const int step = blockDim.x >> a.shift, unit = threadIdx.x & ((1 << a.shift) - 1), half = a.width / 2;
+  const int at = unit >= half ? unit + half : halves ? unit : 2 * unit, other = halves ? at + half : at + 1;
+  for (int row = unit < a.units ? (int)threadIdx.x >> a.shift : s.rows; row < s.rows; row += step) {
+    const Place p(a, s, row, sizeof(T));
+    const T* in = (const T*)p.in;
+    T* out = (T*)p.out;
+    if (unit >= half) {
+      out[at] = in[at];
+      continue;
+    }
+    const float u = load_f<DT>(in + at), v = load_f<DT>(in + other);
+    const float2 cs = table[p.token * half + unit];
+    store_f<DT>(out + at, fmaf(u, cs.x, -(v * cs.y)));
+    store_f<DT>(out + other, fmaf(v, cs.x, u * cs.y));
   }
 }
 
 template <int DT>
 void launch(Call a, int B, bool halves, bool vec, hipStream_t stream) {
-  const int heads = a.H[0] + a.H[1], half = a.width / 2, pairs = halves ? 8 : 4;
-  a.turning = vec ? half / pairs : half;
-  a.units = a.turning + (a.D - a.width) / (vec ? 8 : 1);
+  const int heads = a.H[0] + a.H[1], half = a.width / 2;
+  a.units = vec ? a.D / 8 : half + a.D - a.width;
   while ((1 << a.shift) < a.units) ++a.shift;
   // heads of a workgroup, then tokens
   const int most = kUnits >> a.shift;
   a.heads = heads < most ? heads : most;
-  int64_t tile = most / a.heads;
+  int64_t tile = a.heads < heads ? 1 : most / a.heads;
   if (tile > kPairs / half) tile = kPairs / half;
   if (tile > a.n) tile = a.n;
   a.tile = (int)tile;
@@ -192,12 +258,9 @@ void launch(Call a, int B, bool halves, bool vec, hipStream_t stream) {
   const int threads = lanes >= kThreads ? kThreads : (int)((lanes + kWave - 1) / kWave * kWave);
   const dim3 grid((unsigned)((a.n + tile - 1) / tile), B, (heads + a.heads - 1) / a.heads);
   const size_t lds = (size_t)tile * half * sizeof(float2);
-#define PFA_ROTARY(HALVES, VEC) rotary_kernel<DT, HALVES, VEC><<<grid, threads, lds, stream>>>(a)
-  if (halves && vec) PFA_ROTARY(true, true);
-  else if (halves) PFA_ROTARY(true, false);
-  else if (vec) PFA_ROTARY(false, true);
-  else PFA_ROTARY(false, false);
-#undef PFA_ROTARY
+  if (!vec) pairs_kernel<DT><<<grid, threads, lds, stream>>>(a, halves);
+  else if (halves) rows_kernel<DT, true><<<grid, threads, lds, stream>>>(a);
+  else rows_kernel<DT, false><<<grid, threads, lds, stream>>>(a);
 }
 
 }  // namespace

@@ -117,16 +117,27 @@ def new_rotary_positions(width: int, *, base: float = 10000.0, interleaved: bool
 
 
 _CALL = struct.Struct("PqqqPqqqPqqqPqqqPPqqqiiiiiiiif4x")  # pfa_rotary_call of include/pfa_hip.h
+_NONE = (0, 0, 0, 0)
 
 
-def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
-    """(B, n, heads, head_dim) with a dense last dimension."""
+def _sides(x: torch.Tensor, inplace: bool) -> Tuple[torch.Tensor, torch.Tensor, tuple, tuple]:
+    """x with a dense last dimension, the result, and the library's descriptions of both."""
 
-    if x.dim() == 3:
-        x = x.unsqueeze(1)
-    if x.dim() != 4:
-        raise ValueError(f"{name} must be (B, n, heads, head_dim), or (B, heads, head_dim): one new token a sequence")
-    return x
+    shape, s = x.shape, x.stride()
+    if s[-1] != 1 and shape[-1] > 1:
+        if inplace:
+            raise ValueError("inplace needs a dense last dimension")
+        x = x.contiguous()
+        s = x.stride()
+    many = len(shape) == 4
+    source = (x.data_ptr(), s[0], s[2], s[1]) if many else (x.data_ptr(), s[0], s[1], 0)
+    if inplace:
+        if 0 in s and any(stride == 0 and size > 1 for stride, size in zip(s, shape)):
+            raise ValueError("inplace needs rows of their own: an expanded tensor has none")
+        return x, x, source, source
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    s = y.stride()
+    return x, y, source, (y.data_ptr(), s[0], s[2], s[1]) if many else (y.data_ptr(), s[0], s[1], 0)
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: RotaryPositions, *,
@@ -145,60 +156,42 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
     turns, magnitude, interleaved = rotary
     shape, dtype = q.shape, q.dtype
-    q4 = _rows(q, "q")
-    B, n, H, D = q4.shape
+    if len(shape) == 4:
+        B, n, H, D = shape
+    elif len(shape) == 3:
+        (B, H, D), n = shape, 1
+    else:
+        raise ValueError("q must be (B, n, heads, head_dim), or (B, heads, head_dim): one new token a sequence")
     tag = _VALUE_TAG.get(dtype)
     if tag is None:
         raise ValueError(f"unsupported value dtype {dtype}")
-    width = 2 * turns.shape[0] if turns.dim() == 1 else 0
-    if turns.dtype != torch.int64 or width == 0 or not turns.is_contiguous():
+    width = 2 * turns.numel()
+    if turns.dtype != torch.int64 or turns.dim() != 1 or width == 0 or not turns.is_contiguous():
         raise ValueError("turns must be a contiguous (width / 2,) int64 tensor")
     if not 0 < D <= WIDEST_HEAD or width > D or H == 0:
         raise ValueError(f"q has {H} heads of {D} channels for {width} that turn: up to {WIDEST_HEAD}, and a head at least")
-    k4, Hk = None, 0
+    Hk = 0
     if k is not None:
-        if k.dim() != q.dim() or k.dtype != dtype:
-            raise ValueError("q and k must have one dtype and as many dimensions")
-        k4 = _rows(k, "k")
-        if k4.shape[:2] != (B, n) or k4.shape[3] != D or k4.shape[2] == 0:
-            raise ValueError(f"k must be ({B}, {n}, kv_heads, {D}) (got {tuple(k4.shape)})")
-        Hk = k4.shape[2]
-    if positions.dtype != torch.int32 or positions.shape not in ((B,), (B, n)):
+        other = k.shape
+        Hk = other[-2] if len(other) == len(shape) else 0
+        if k.dtype != dtype or Hk == 0 or other[:-2] != shape[:-2] or other[-1] != D:
+            raise ValueError(f"k must be {tuple(shape[:-2])} x kv_heads x {D} of {dtype} (got {tuple(other)}, {k.dtype})")
+    at = positions.shape
+    if positions.dtype != torch.int32 or (at != (B,) and at != (B, n)):
         raise ValueError(f"positions must be a ({B},) or ({B}, {n}) int32 tensor")
     if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("apply_rotary has no backward pass: call it under torch.no_grad()")
     index = _device("apply_rotary", q, k, positions, turns)
-    per_token = positions.dim() == 2
     pos = positions.stride()
-    sources, targets, results = [], [], []
-    for x, x4 in ((q, q4), (k, k4)):
-        if x is None:
-            sources.append((0, 0, 0, 0)), targets.append((0, 0, 0, 0)), results.append(None)
-            continue
-        s = x4.stride()
-        if inplace:
-            if s[3] != 1 and D > 1:
-                raise ValueError("inplace needs a dense last dimension")
-            for size, stride in zip(x4.shape[:3], s[:3]):
-                if stride == 0 and size > 1:
-                    raise ValueError("inplace needs rows of their own: an expanded tensor has none")
-            y = x
-            t = s
-        else:
-            if s[3] != 1:
-                x4 = x4.contiguous()
-                s = x4.stride()
-            y = torch.empty(x.shape, dtype=dtype, device=x.device)
-            h = x4.shape[2]
-            t = (n * h * D, h * D, D, 1)
-        sources.append((x4, s)), targets.append((y.data_ptr(), t[0], t[2], t[1])), results.append(y)
-    (q4, qs), ks = sources[0], sources[1]
-    src_q = (q4.data_ptr(), qs[0], qs[2], qs[1])
-    src_k = ks if k is None else (ks[0].data_ptr(), ks[1][0], ks[1][2], ks[1][1])
-    packed = _CALL.pack(*src_q, *src_k, *targets[0], *targets[1], turns.data_ptr(), positions.data_ptr(), pos[0],
+    q, q_out, q_from, q_to = _sides(q, inplace)
+    k_out, k_from, k_to = None, _NONE, _NONE
+    if Hk:
+        k, k_out, k_from, k_to = _sides(k, inplace)
+    per_token = len(pos) == 2
+    packed = _CALL.pack(*q_from, *k_from, *q_to, *k_to, turns.data_ptr(), positions.data_ptr(), pos[0],
                         pos[1] if per_token else 0, n, per_token, B, H, Hk, D, width, interleaved, tag, magnitude)
     _call(index, "rotary", _hip.lib().pfa_rotary, packed)
-    return results[0], results[1]
+    return q_out, k_out
 
 
 __all__ = ["RotaryPositions", "new_rotary_positions", "rotary_frequencies", "apply_rotary"]
