@@ -18,60 +18,229 @@ struct Weights {
 };
 
 // ---------------------------------------------------------------------
-// Choice: a workgroup a sequence and head, choose_best over its weights' bits in
-// order.  Positions without a page (where there is a table) are no candidates.
+// Choice: a workgroup a sequence and head.  The weights' bits in their order are keys;
+// their range is cut into 2,048 bins and the bin that holds the last one to take is
+// cut again, as choose_best does it for pages, mostly twice.  A thread holds four
+// neighbours of every 4 * THREADS positions, so that loads are in one piece, and a
+// position's place among the kept is counted by ballots: within its wave, then over
+// the waves of all pieces.  All is LDS and latency: 48 rows of up to 20,480 positions
+// in registers, 8,192 kept: XX us (choose_best with 32 neighbours a thread: 23).
+// Positions without a page (where there is a table) are no candidates.
 // ---------------------------------------------------------------------
-template <int THREADS, int K, bool HELD>
+template <int THREADS, int C, bool HELD>
 __global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Weights w, Table tab, int shift, int n_pages, int H,
                                                                 const int32_t* __restrict__ lengths, int count, int first,
-                                                                int last, int32_t* __restrict__ kept,
-                                                                float* __restrict__ fresh) {
+                                                                int last, int32_t* __restrict__ kept) {
+  constexpr int WAVES = THREADS / kWave, PIECE = 4 * THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / H, h = blockIdx.x % H;
   const float* row = w.p + b * w.s_b + h * w.s_h;
   const int n = lengths[b], len = n < 0 ? 0 : n < w.most ? n : w.most;
   const int32_t* ids = tab.ids ? tab.ids + b * tab.stride : nullptr;
-  int32_t* out = kept + (int64_t)blockIdx.x * count;
-  float* moved = fresh ? fresh + (int64_t)blockIdx.x * w.T : nullptr;
-  const int rounds = HELD ? 1 : (len + THREADS * K - 1) / (THREADS * K);
-  auto fetch = [&](int r, uint32_t (&x)[K]) {
-    const int p0 = (r * THREADS + (int)threadIdx.x) * K;
-    float v[K];
+  const int rounds = HELD ? 1 : (len + C * PIECE - 1) / (C * PIECE);
+  __shared__ int hist[kBins];
+  __shared__ int sums[3][WAVES];
+  __shared__ uint32_t range[2][WAVES];
+  __shared__ int cut[3];
+  __shared__ int taken[2][C * WAVES + 1];
+
+  // One CU has a row's arithmetic to itself: pieces behind the last position are left
+  // out, and those without an end of the row or a position that is always taken go
+  // without the comparisons for them.
+  uint32_t x[C][4];
+  auto piece = [&](int r, int c) { return (r * C + c) * PIECE; };
+  auto fetch = [&](int r) {
+    float4 v[C];
+    int id[C];
 #pragma unroll
-    for (int i = 0; i < K; i += 4) {
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-      const int p = p0 + i;
+    for (int c = 0; c < C; ++c) {
+      const int p = piece(r, c) + 4 * tid;
+      id[c] = ids && p < len ? ids[p >> shift] : 0;
+      v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (w.vec) {
-        if (p < len) a = *reinterpret_cast<const float4*>(row + p);
+        if (p < len) v[c] = *reinterpret_cast<const float4*>(row + p);
       } else {
-        if (p < len) a.x = row[p];
-        if (p + 1 < len) a.y = row[p + 1];
-        if (p + 2 < len) a.z = row[p + 2];
-        if (p + 3 < len) a.w = row[p + 3];
+        if (p < len) v[c].x = row[p];
+        if (p + 1 < len) v[c].y = row[p + 1];
+        if (p + 2 < len) v[c].z = row[p + 2];
+        if (p + 3 < len) v[c].w = row[p + 3];
       }
-      v[i] = a.x, v[i + 1] = a.y, v[i + 2] = a.z, v[i + 3] = a.w;
     }
 #pragma unroll
-    for (int i = 0; i < K; ++i) {
-      const int p = p0 + i;
-      uint32_t u = v[i] == 0.0f ? 0u : __float_as_uint(v[i]);  // -0 ties with +0
-      u = u & 0x80000000u ? ~u : u | 0x80000000u;
-      if (v[i] != v[i]) u = kNan;
-      if (p < first || len - p <= last) u = kForced;
-      x[i] = p < len ? u : kNone;
-    }
-    if (ids) {  // pages hold 16 tokens or more
+    for (int c = 0; c < C; ++c) {
+      const int p0 = piece(r, c);
+      if (p0 >= len) continue;
+      const bool have = (uint32_t)id[c] < (uint32_t)n_pages || !ids;
+      const float y[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-      for (int i = 0; i < K; i += K < 16 ? K : 16) {
-        const bool gone = p0 + i < len && (uint32_t)ids[(p0 + i) >> shift] >= (uint32_t)n_pages;
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = __float_as_uint(y[j] + 0.0f);  // -0 ties with +0
+        const uint32_t key = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+        x[c][j] = !have ? kNone : y[j] != y[j] ? kNan : key;
+      }
+      if (p0 < first || p0 + PIECE > len - last) {
 #pragma unroll
-        for (int j = 0; j < (K < 16 ? K : 16); ++j) x[i + j] = gone ? kNone : x[i + j];
+        for (int j = 0; j < 4; ++j) {
+          const int p = p0 + 4 * tid + j;
+          if (have && (p < first || len - p <= last)) x[c][j] = kForced;
+          if (p >= len) x[c][j] = kNone;
+        }
       }
     }
   };
-  choose_best<THREADS, K, HELD>(0, rounds, count, fetch, [&](int i, int entry) {
-    out[i] = entry;
-    if (moved && i < w.T) moved[i] = entry >= 0 ? row[entry] : 0.0f;
+  if constexpr (HELD) fetch(0);
+  auto each = [&](auto&& f) {
+    for (int r = 0; r < rounds; ++r) {
+      if constexpr (!HELD) fetch(r);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (piece(r, c) >= len) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f(x[c][j]);
+      }
+    }
+  };
+
+  uint32_t lo = 0xffffffffu, hi = 0;
+  int forced = 0, others = 0;
+  each([&](uint32_t key) {
+    const bool normal = key != kNone && key != kForced;
+    forced += key == kForced;
+    others += normal;
+    if (normal) lo = key < lo ? key : lo, hi = key > hi ? key : hi;
   });
+  for (int i = tid; i < kBins; i += THREADS) hist[i] = 0;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t a = __shfl_xor(lo, o), z = __shfl_xor(hi, o);
+    lo = a < lo ? a : lo, hi = z > hi ? z : hi;
+    forced += __shfl_xor(forced, o), others += __shfl_xor(others, o);
+  }
+  if (lane == 0) range[0][wave] = lo, range[1][wave] = hi, sums[0][wave] = forced, sums[1][wave] = others;
+  __syncthreads();
+  forced = others = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    lo = range[0][i] < lo ? range[0][i] : lo, hi = range[1][i] > hi ? range[1][i] : hi;
+    forced += sums[0][i], others += sums[1][i];
+  }
+  // taken: keys above `over`, and the lowest `ties` positions of those that equal it
+  int need = count - forced, ties = 0;
+  uint32_t over = 0;
+  if (need >= others) {
+    over = kNone;
+  } else if (need <= 0) {
+    over = kForced - 1;
+  } else {
+    while (true) {
+      if (hi == lo) {
+        over = lo, ties = need;
+        break;
+      }
+      const int bits = 32 - __clz(hi - lo), cutshift = bits > 11 ? bits - 11 : 0;
+      each([&](uint32_t key) {
+        if (key - lo <= hi - lo) atomicAdd(&hist[(key - lo) >> cutshift], 1);
+      });
+      __syncthreads();
+      // bins from the top: thread t's are kBins - 1 - PER * t ...
+      constexpr int PER = kBins / THREADS;
+      int bin_n[PER], mine = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        int& bin = hist[kBins - 1 - PER * tid - i];
+        mine += bin_n[i] = bin;
+        bin = 0;
+      }
+      int all;
+      int above = block_scan<THREADS>(mine, sums[2], all);
+      if (above < need && above + mine >= need) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          if (above < need && above + bin_n[i] >= need)
+            cut[0] = kBins - 1 - PER * tid - i, cut[1] = need - above, cut[2] = bin_n[i];
+          above += bin_n[i];
+        }
+      }
+      __syncthreads();
+      need = cut[1];
+      const uint32_t from = lo + ((uint32_t)cut[0] << cutshift), to = from + ((1u << cutshift) - 1u);
+      if (cut[2] == need) {  // all of the bin
+        over = from - 1;
+        break;
+      }
+      lo = from, hi = to < hi ? to : hi;
+    }
+  }
+
+  int32_t* out = kept + (int64_t)blockIdx.x * count;
+  int base = 0, tied = 0;  // keys above and equal ones of the rounds before
+  for (int r = 0; r < rounds; ++r) {
+    if constexpr (!HELD) {
+      fetch(r);
+      __syncthreads();  // the last round's places are read
+    }
+    // of the lanes before this one, above in the lower half and equal in the upper
+    uint32_t before[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      uint32_t mine = 0, whole = 0;
+      auto vote = [&](bool yes, int at) {
+        const uint64_t m = __ballot(yes);
+        mine += __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0)) << at;
+        whole += __popcll(m) << at;
+      };
+      if (piece(r, c) < len) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vote(x[c][j] > over, 0);
+        if (ties > 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vote(x[c][j] == over, 16);
+        }
+      }
+      before[c] = mine;
+      if (lane == 0) taken[0][c * WAVES + wave] = whole & 0xffff, taken[1][c * WAVES + wave] = whole >> 16;
+    }
+    __syncthreads();
+    if (wave < 2) {  // sums of those before, a wave each
+      constexpr int N = C * WAVES, PER = (N + kWave - 1) / kWave;
+      int v[PER], mine = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = lane * PER + i;
+        v[i] = at < N ? taken[wave][at] : 0;
+        mine += v[i];
+      }
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int y = __shfl_up(incl, o);
+        if (lane >= o) incl += y;
+      }
+      int sum = incl - mine;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = lane * PER + i;
+        if (at < N) taken[wave][at] = sum;
+        sum += v[i];
+      }
+      if (lane == 63) taken[wave][N] = incl;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (piece(r, c) >= len) continue;
+      int at = base + taken[0][c * WAVES + wave] + (int)(before[c] & 0xffff);
+      int eq = tied + taken[1][c * WAVES + wave] + (int)(before[c] >> 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool above = x[c][j] > over, tie = ties > 0 && x[c][j] == over;
+        if (above || (tie && eq < ties)) out[at + (eq < ties ? eq : ties)] = piece(r, c) + 4 * tid + j;
+        at += above, eq += tie;
+      }
+    }
+    base += taken[0][C * WAVES], tied += taken[1][C * WAVES];
+  }
+  for (int i = base + (tied < ties ? tied : ties) + tid; i < count; i += THREADS) out[i] = -1;
 }
 
 // ---------------------------------------------------------------------
@@ -130,16 +299,19 @@ __device__ __forceinline__ void copy_out(uint8_t* p, const uint32_t* w) {
 }
 
 template <int CT, int D>
-__global__ void __launch_bounds__(256) move_kernel(Pages pg, Table from, Table to, const int32_t* __restrict__ kept, int count,
-                                                   float* __restrict__ fresh, int T) {
+__global__ void __launch_bounds__(256) move_kernel(Pages pg, Table from, Table to, Weights w, const int32_t* __restrict__ kept,
+                                                   int count, float* __restrict__ fresh) {
   constexpr int LANES = D / 8, ROWS = 256 / LANES, UB = cells_bytes(CT, 8), ROW = cells_bytes(CT, D);
   constexpr int NS = scales_of(CT, D), PER = LANES / NS;  // scales of a row, lanes of one
   constexpr int ES = (int)sizeof(typename Cell<CT>::T);
   const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % LANES;
   const int64_t list = (int64_t)b * pg.H + h;
-  // the weights behind the kept ones
-  for (int64_t i = count + (int64_t)blockIdx.x * 256 + threadIdx.x; i < T; i += (int64_t)gridDim.x * 256)
-    fresh[list * T + i] = 0.0f;
+  // the weights of the kept ones, and zeros behind them
+  const float* weights = w.p + b * w.s_b + h * w.s_h;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < w.T; i += (int64_t)gridDim.x * 256) {
+    const int src = i < count ? kept[list * count + i] : -1;
+    fresh[list * w.T + i] = src >= 0 ? weights[src] : 0.0f;
+  }
   __shared__ float part[2][4][D];
   for (int64_t ordinal = blockIdx.x; ordinal << pg.shift < count; ordinal += gridDim.x) {
     const int64_t at = ordinal << pg.shift;
@@ -219,14 +391,16 @@ int tokens_check(const char* what, const float* weights, int64_t n, int B, int H
 }
 
 void choose_tokens(const Weights& w, const Table& t, int shift, int n_pages, int B, int H, const int32_t* lengths, int count,
-                   int first, int last, int32_t* kept, float* fresh, hipStream_t stream) {
-#define PFA_CHOOSE(THREADS, K, HELD)                                                                                    \
-  choose_tokens_kernel<THREADS, K, HELD><<<B * H, THREADS, 0, stream>>>(w, t, shift, n_pages, H, lengths, count, first, \
-                                                                        last, kept, fresh)
-  if (w.most <= 256 * 4) PFA_CHOOSE(256, 4, true);
-  else if (w.most <= 1024 * 4) PFA_CHOOSE(1024, 4, true);
-  else if (w.most <= 1024 * 16) PFA_CHOOSE(1024, 16, true);
-  else PFA_CHOOSE(1024, 16, false);
+                   int first, int last, int32_t* kept, hipStream_t stream) {
+#define PFA_CHOOSE(THREADS, C, HELD)                                                                                    \
+  choose_tokens_kernel<THREADS, C, HELD><<<B * H, THREADS, 0, stream>>>(w, t, shift, n_pages, H, lengths, count, first, \
+                                                                        last, kept)
+  if (w.most <= 256 * 4) PFA_CHOOSE(256, 1, true);
+  else if (w.most <= 1024 * 4) PFA_CHOOSE(1024, 1, true);
+  else if (w.most <= 1024 * 16) PFA_CHOOSE(1024, 4, true);
+  else if (w.most <= 1024 * 32) PFA_CHOOSE(1024, 8, true);
+  else if (w.most <= 1024 * 64) PFA_CHOOSE(1024, 16, true);
+  else PFA_CHOOSE(1024, 8, false);
 #undef PFA_CHOOSE
 }
 
@@ -243,7 +417,7 @@ extern "C" int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int
   PFA_CHECK_ARG(lengths && kept, "kv_tokens_select: null argument");
   const bool vec = (uintptr_t)weights % 16 == 0 && weights_b % 4 == 0 && weights_h % 4 == 0 && n % 4 == 0;
   choose_tokens(Weights{weights, weights_b, weights_h, (int)n, (int)n, vec}, Table{nullptr, 0, 0}, 0, 0, B, H, lengths, count, first,
-                last, kept, nullptr, as_stream(stream));
+                last, kept, as_stream(stream));
   PFA_CHECK_LAUNCH("kv_tokens_select");
   return PFA_OK;
 }
@@ -266,13 +440,13 @@ extern "C" int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weigh
   hipStream_t s = as_stream(stream);
   const int64_t held = (int64_t)table_pages << p.shift;
   const Weights w{weights, weights_b, weights_h, (int)n, (int)(held < n ? held : n), vec};
-  choose_tokens(w, from, p.shift, p.n_pages, B, p.H, lengths, count, first, last, kept, fresh, s);
+  choose_tokens(w, from, p.shift, p.n_pages, B, p.H, lengths, count, first, last, kept, s);
   const int64_t fresh_pages = ((int64_t)count + p.ps - 1) >> p.shift;
   const dim3 grid((unsigned)(fresh_pages < 65535 ? fresh_pages : 65535), p.H, B);
   by_cells(pages->dtype, [&](auto ct) {
     by_width(pages->head_dim, [&](auto width) {
       move_kernel<decltype(ct)::value, decltype(width)::value>
-          <<<grid, 256, 0, s>>>(p, from, to, kept, count, fresh, (int)n);
+          <<<grid, 256, 0, s>>>(p, from, to, w, kept, count, fresh);
     });
   });
   PFA_CHECK_LAUNCH("kv_tokens_evict");

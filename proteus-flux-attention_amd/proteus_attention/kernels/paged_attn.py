@@ -527,7 +527,7 @@ def select_kv_tokens(key_weights: torch.Tensor, lengths: torch.Tensor, count: in
         raise ValueError("key_weights needs a head")
     lengths = _per_sequence(lengths, B, "lengths")
     index = _device("select_kv_tokens", weights, lengths)
-    kept = torch.empty((B, H, count), dtype=torch.int32, device=weights.device)
+    kept = lengths.new_empty((B, H, count))
     _call(index, "kv_tokens_select", _hip.lib().pfa_kv_tokens_select, weights.data_ptr(), weights.stride(0),
           weights.stride(1), T, B, H, lengths.data_ptr(), count, first, last, kept.data_ptr())
     return kept
@@ -564,8 +564,8 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     T = weights.shape[2]
     lengths = _per_sequence(lengths, B, "lengths")
     index = _device("evict_kv_tokens", *pages, table, fresh_table, weights, lengths)
-    kept = torch.empty((B, Hkv, count), dtype=torch.int32, device=weights.device)
-    fresh = torch.empty((B, Hkv, T), dtype=torch.float32, device=weights.device)
+    kept = table.new_empty((B, Hkv, count))
+    fresh = torch.empty_like(weights, memory_format=torch.contiguous_format)
     _call(index, "kv_tokens_evict", _hip.lib().pfa_kv_tokens_evict, _POOL.pack(*pool), weights.data_ptr(),
           weights.stride(0), weights.stride(1), T, B, table.data_ptr(), table.stride(0), table.shape[1],
           lengths.data_ptr(), count, first, last, fresh_table.data_ptr(), fresh_table.stride(0), fresh_table.shape[1],
