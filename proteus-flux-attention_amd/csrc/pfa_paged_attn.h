@@ -358,13 +358,15 @@ struct Wave {
         if (scores_at && t.b[i].pos < kNowhere) *reinterpret_cast<f32x4_t*>(scores_at + t.b[i].pos + 4 * g) = s[i];
     }
     if constexpr (is4(F::CT)) {
-      // byte y * NS + (the lane's group) of the four keys', as the exponent of an f32
-      const int group = n * F::VD / 32;
+      // byte y * NS + (the lane's group) of the four keys', turned to where an f32 has its
+      // exponent: what else comes with it is no part of that
+      const int turn = 8 * (n * F::VD / 32) + 9;
 #pragma unroll
       for (int i = 0; i < 2 * F::NG; ++i)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          vs[i][y] = power_of(raw[i][y * F::NS / 4] >> (8 * (y * F::NS % 4) + 8 * group) & 255u);
+          const uint32_t w = raw[i][y * F::NS / 4];
+          vs[i][y] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, 8 * (y * F::NS % 4) + turn));
           if constexpr (F::VD == 1) v[i][y][0] = v[i][y][0] >> 4 * (n & 1) & 15u;
         }
     }
@@ -569,8 +571,8 @@ __device__ __forceinline__ void add_weights(const Weigh& w, const Pages& pg, con
   }
 }
 
-// Behind the join: a workgroup four times its threads' positions of a sequence and
-// key-value head.
+// Rows of more heads than a tile has, behind the join: a workgroup four times its
+// threads' positions of a sequence and key-value head.
 static __global__ void __launch_bounds__(256) weigh_kernel(Weigh w, Pages pg, const int32_t* __restrict__ table,
                                                            int64_t table_stride, int P, int G, float c,
                                                            const int32_t* __restrict__ lengths,
@@ -700,6 +702,13 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     __syncthreads();
   }
 
+  // The chip gives a unit's oldest wave its turn first, so that of three workgroups with
+  // the same work the first is through in 60 % of the last one's time, which then has
+  // the unit for itself and does not fill it.  A wave's priority falls with each quarter
+  // of its chunk: they go on side by side (1,000,003 4-bit tokens: 124 -> 119 us; 64
+  // ragged sequences: 44.9 -> 44.0).
+  const int64_t f0 = f;
+  const int quarter = (int)((f1 - f + 3) >> 2);
   while (f < f1) {
     const int start = start_at(starts, b), len = deal.length(lengths, b);
     const int nt = deal.tiles(start, len), np = deal.places(start, len);
@@ -751,6 +760,13 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       if (t < re) {
         w.load_k(pg, h, cur);
         while (t < re) {
+          if (!lone) {
+            const int done = (int)(pair_at - f0) + t - t0;
+            if (done < quarter) __builtin_amdgcn_s_setprio(3);
+            else if (done < 2 * quarter) __builtin_amdgcn_s_setprio(2);
+            else if (done < 3 * quarter) __builtin_amdgcn_s_setprio(1);
+            else __builtin_amdgcn_s_setprio(0);
+          }
           next = cur;
           Tile<F> found;
           t = found.find_seen(r, t + kWaves, re);
@@ -821,22 +837,20 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 // the teams are joined in LDS.  Eight parts' loads go out at once.  Its time is its
 // chain of loads, 4 to 10 us.
 template <int QT, int THREADS>
-__global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float c, float pscale,
-                                                       const int32_t* __restrict__ lengths,
-                                                       const int32_t* __restrict__ starts,
-                                                       const float* __restrict__ parts,
-                                                       const Shared* __restrict__ shared,
-                                                       typename Elem<QT>::T* __restrict__ out,
-                                                       float2* __restrict__ stats) {
+__device__ __forceinline__ void join_rows(const Deal& deal, int G, int D, float c, float pscale,
+                                          const int32_t* __restrict__ lengths, const int32_t* __restrict__ starts,
+                                          const float* __restrict__ parts, const Shared* __restrict__ shared,
+                                          typename Elem<QT>::T* __restrict__ out, float2* __restrict__ stats, int block,
+                                          int first, int step) {
   const int tid = threadIdx.x;
-  const int b = blockIdx.x / deal.R, pair = blockIdx.x % deal.R;
+  const int b = block / deal.R, pair = block % deal.R;
   const int h = pair / deal.RT, head0 = h * G + 16 * (pair % deal.RT);
   const int rows = G < 16 ? G : 16, here = (h + 1) * G - head0 < 16 ? (h + 1) * G - head0 : 16;
-  const Shared who = shared[blockIdx.x];  // nobody's where the sequence has no tiles
+  const Shared who = shared[block];  // nobody's where the sequence has no tiles
   const int64_t row0 = (int64_t)b * (deal.R / deal.RT) * G + head0;
   typename Elem<QT>::T* to = out + row0 * D;
   if (deal.tiles(start_at(starts, b), deal.length(lengths, b)) == 0) {
-    for (int i = blockIdx.y * D + tid; i < here * D; i += THREADS * gridDim.y) store_f<QT>(to + i, 0.0f);
+    for (int i = first * D + tid; i < here * D; i += THREADS * step) store_f<QT>(to + i, 0.0f);
     return;
   }
   if (who.n == 1) return;  // written by its one workgroup
@@ -845,14 +859,14 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
   struct Sum {
     float m, l, o0, o1;
   };
-  // parts i0, i0 + step, ... of a row, this lane's channels
-  auto gather = [&](int row, int i0, int step) {
+  // parts i0, i0 + stride, ... of a row, this lane's channels
+  auto gather = [&](int row, int i0, int stride) {
     Sum a{-INFINITY, 0.0f, 0.0f, 0.0f};
-    for (; i0 < who.n; i0 += 8 * step) {
+    for (; i0 < who.n; i0 += 8 * stride) {
       float m[8], l[8], x[8], y[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * step;
+        const int i = i0 + u * stride;
         const bool in = i < who.n;
         // part i is workgroup first + i's
         const float* s = parts + (2 * (int64_t)(who.first + (in ? i : 0)) + (!in || i == 0)) * rows * (D + 2);
@@ -876,7 +890,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
   };
   // a team a row (43 x 8 pairs of 5 rows in three parts: 4.5 us, 12 with a row at a time)
   if (who.n <= 16) {
-    for (int row = blockIdx.y * teams + team; row < here; row += gridDim.y * teams) {
+    for (int row = first * teams + team; row < here; row += step * teams) {
       const Sum a = gather(row, 0, 1);
       const bool none = a.l == 0.0f;  // no score above -inf, whatever the values are
       const float inv = 1.0f / (a.l * pscale);
@@ -888,7 +902,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
   }
   constexpr int TEAMS = THREADS / 16;  // at most
   __shared__ float acc[THREADS * 2], tops[TEAMS], suml[TEAMS];
-  for (int row = blockIdx.y; row < here; row += gridDim.y) {
+  for (int row = first; row < here; row += step) {
     const Sum a = gather(row, team, teams);
     acc[team * D + d] = a.o0;
     if (two) acc[team * D + 64 + d] = a.o1;
@@ -907,6 +921,69 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
     }
     __syncthreads();
   }
+}
+
+template <int QT, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, float c, float pscale,
+                                                       const int32_t* __restrict__ lengths,
+                                                       const int32_t* __restrict__ starts,
+                                                       const float* __restrict__ parts,
+                                                       const Shared* __restrict__ shared,
+                                                       typename Elem<QT>::T* __restrict__ out,
+                                                       float2* __restrict__ stats) {
+  join_rows<QT, THREADS>(deal, G, D, c, pscale, lengths, starts, parts, shared, out, stats, blockIdx.x, blockIdx.y,
+                         gridDim.y);
+}
+
+// The join and the weights beside it: `joins` workgroups join, as join_kernel's do, the
+// others take four positions a thread and work their rows' statistics out of the parts
+// themselves, which costs less than to wait for the join (32 ragged sequences of up to
+// 16,384 int8 tokens: 85 -> 79 us).  16 rows of a key-value head at most.
+template <int QT, int THREADS>
+__global__ void __launch_bounds__(THREADS) join_weigh_kernel(Deal deal, int G, int D, float c, float pscale,
+                                                             const int32_t* __restrict__ lengths,
+                                                             const int32_t* __restrict__ starts,
+                                                             const float* __restrict__ parts,
+                                                             const Shared* __restrict__ shared,
+                                                             typename Elem<QT>::T* __restrict__ out, int joins,
+                                                             int rows_at_once, Weigh w, Pages pg,
+                                                             const int32_t* __restrict__ table, int64_t table_stride,
+                                                             int pieces) {
+  if ((int)blockIdx.x < joins) {
+    join_rows<QT, THREADS>(deal, G, D, c, pscale, lengths, starts, parts, shared, out, nullptr, blockIdx.x / rows_at_once,
+                           blockIdx.x % rows_at_once, rows_at_once);
+    return;
+  }
+  const int block = (int)blockIdx.x - joins, pair = block / pieces, b = pair / pg.H, h = pair % pg.H;
+  const int len = deal.length(lengths, b), start = start_at(starts, b);
+  const int64_t first = (start & ~3) + 4 * (int64_t)(block % pieces) * THREADS;
+  if (first >= len) return;
+  const int64_t row0 = (int64_t)pair * G;
+  __shared__ float2 stats[16];
+  const Shared who = shared[pair];
+  const int lane = threadIdx.x & 63;
+  for (int g = threadIdx.x >> 6; g < G; g += THREADS / kWave) {
+    if (who.n == 1) {  // left by the one workgroup that had the row
+      if (lane == 0) stats[g] = w.stats[row0 + g];
+      continue;
+    }
+    float m = -INFINITY, l = 0.0f;
+    auto with = [&](float m2, float l2) {
+      const float t = fmaxf(m, m2);
+      l = l * part_weight(m, l, t, c) + l2 * part_weight(m2, l2, t, c);
+      m = t;
+    };
+    for (int i = lane; i < who.n; i += kWave) {
+      const float* s = parts + (2 * (int64_t)(who.first + i) + (i == 0)) * G * (D + 2) + G * D + g;
+      with(s[0], s[G]);
+    }
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) with(__shfl_xor(m, o), __shfl_xor(l, o));
+    if (lane == 0) stats[g] = row_stats(m, l);
+  }
+  __syncthreads();
+  add_weights(w, pg, table + b * table_stride, b, h, row0, G, c, start, len, first + 4 * threadIdx.x, pieces * THREADS,
+              [&](int g) { return stats[g]; });
 }
 
 // A call's arguments behind its checks.
@@ -1006,16 +1083,27 @@ void attend_launch(const AttendCall& a) {
     if (weighs && deal.RT > 1) weigh_launch(a, G);
     return;
   }
-  const dim3 rows(pairs, pairs >= kMany ? 1 : G < 16 ? G : 16);
+  const int rows = pairs >= kMany ? 1 : G < 16 ? G : 16;
+  auto join = [&](auto threads) {
+    constexpr int THREADS = decltype(threads)::value;
+    if (weighs && deal.RT == 1) {
+      // pieces of a row: all of it at once, but no more workgroups than go through soon
+      const int64_t all = (a.weigh.cap + 4 * THREADS - 1) / (4 * THREADS), most = 8192 / pairs;
+      const int pieces = (int)(all < most ? all : most > 0 ? most : 1);
+      const int joins = (int)pairs * rows;
+      join_weigh_kernel<QT, THREADS><<<joins + (int)pairs * pieces, THREADS, 0, a.stream>>>(
+          deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared, (T*)a.out, joins, rows, a.weigh, a.pg, a.table,
+          a.table_stride, pieces);
+    } else {
+      join_kernel<QT, THREADS><<<dim3(pairs, rows), THREADS, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts,
+                                                                           a.parts, shared, (T*)a.out, a.weigh.stats);
+      if (weighs) weigh_launch(a, G);
+    }
+  };
   // the rows of a few pairs have parts by the hundred (8 pairs of 60,000 keys: 36.6 us
   // with 16 waves a row, 37.4 with four; 32 of 25,000: 88.6 and 85.8)
-  if (pairs >= 32)
-    join_kernel<QT, 256><<<rows, 256, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared,
-                                                     (T*)a.out, a.weigh.stats);
-  else
-    join_kernel<QT, 1024><<<rows, 1024, 0, a.stream>>>(deal, G, D, a.c, F::PSCALE, a.lengths, a.starts, a.parts, shared,
-                                                       (T*)a.out, a.weigh.stats);
-  if (weighs) weigh_launch(a, G);
+  if (pairs >= 32) join(std::integral_constant<int, 256>{});
+  else join(std::integral_constant<int, 1024>{});
 }
 
 template <int QT, int CT>
