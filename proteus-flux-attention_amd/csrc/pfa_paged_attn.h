@@ -591,6 +591,13 @@ struct Choice {
   int32_t* chosen;
 };
 
+// A barrier for what passes through LDS: stores to memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // What a call does beside attending.  SELECT: the workgroup first selects its pair's
 // pages itself, for a launch and several dependent loads less.  WEIGH: it keeps the
 // scores, and where a workgroup has all of a key's rows it adds their weights itself.
@@ -611,6 +618,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found[2];
   __shared__ float2 stats[WEIGH ? 16 : 1];
+  deal.tile = F::TILE;  // as it is, and known
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Wave<F> w;
@@ -644,7 +652,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
         if (lane >= o) incl += x;
       }
       if (lane == 63) sums[wave] = incl;
-      __syncthreads();
+      lds_barrier();
       all = 0;
 #pragma unroll
       for (int j = 0; j < kWaves; ++j) {
@@ -658,9 +666,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       int64_t mine = 0;
       for (int i = tid + 64 * kWaves; i < deal.B; i += 64 * kWaves) mine += places(i);
       mine = wave_sum(mine);
-      __syncthreads();
+      lds_barrier();
       if (lane == 0) sums[wave] = mine;
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) total += sums[i];
     }
@@ -675,10 +683,10 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       before += all;
       if (f < before) break;
       base += 64 * kWaves;
-      __syncthreads();
+      lds_barrier();
       scan(base + tid);
     }
-    __syncthreads();
+    lds_barrier();
     b = (int)uniform(found[0]);
     at = uniform(found[1]);
   } else {  // a workgroup a pair
@@ -699,7 +707,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
           chosen[i] = entry;
           if (i < deal.S) own[i] = entry;
         });
-    __syncthreads();
+    lds_barrier();
   }
 
   // The chip gives a unit's oldest wave its turn first, so that of three workgroups with
@@ -709,9 +717,16 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   // ragged sequences: 44.9 -> 44.0).
   const int64_t f0 = f;
   const int quarter = (int)((f1 - f + 3) >> 2);
+  // of the sequence at hand, and the tiles whose pages are in LDS: the next pair of a
+  // short sequence, which has the same, goes on without waiting for either
+  int at_hand = -1, start = 0, len = 0, nt = 0, np = 0;
+  int looked_up = -1, first_up = 0, end_up = 0;
   while (f < f1) {
-    const int start = start_at(starts, b), len = deal.length(lengths, b);
-    const int nt = deal.tiles(start, len), np = deal.places(start, len);
+    if (b != at_hand) {
+      at_hand = b;
+      start = start_at(starts, b), len = deal.length(lengths, b);
+      nt = deal.tiles(start, len), np = deal.places(start, len);
+    }
     if (!lone && nt == 0) {
       ++b;
       continue;
@@ -744,8 +759,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     for (int r0 = t0 + ta; r0 < te; r0 += run) {
       const int re = te - r0 < run ? te : r0 + run;
       const Row r{entries, r0 * F::TILE >> deal.shift, deal.shift, start, len};
-      const int n = ((re * F::TILE - 1) >> deal.shift) - r.first + 1;
-      if (r0 > t0 + ta) __syncthreads();  // the last run's are read
+      const bool there = !SELECT && deal.S < 0 && looked_up == b && first_up == r0 && end_up >= re;
+      const int n = there ? 0 : ((re * F::TILE - 1) >> deal.shift) - r.first + 1;
+      if (r0 > t0 + ta) lds_barrier();  // the last run's are read
       for (int i = tid; i < n; i += 64 * kWaves) {
         int ordinal = r.first + i;
         if constexpr (SELECT) ordinal = ordinal < deal.S ? own[ordinal] : -1;
@@ -754,7 +770,8 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
         const bool ok = (uint32_t)id < (uint32_t)pg.n_pages;
         entries[i] = Entry{ok ? id : 0, ok ? ordinal << deal.shift : kNowhere};
       }
-      __syncthreads();
+      if (!there) lds_barrier();
+      looked_up = b, first_up = r0, end_up = there ? end_up : re;
       Tile<F> cur, next;
       int t = cur.find_seen(r, r0 + wave, re);
       if (t < re) {
@@ -788,7 +805,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
 #pragma unroll
         for (int j = 0; j < F::VD; ++j) so[wave][w.n][F::VD * (4 * w.g + y) + j] = st.o[j][y];
     }
-    __syncthreads();
+    lds_barrier();
     const bool ends = tb == nt, whole = ta == 0 && ends;
     if (!lone && ta == 0 && tid == 0)
       shared[(int64_t)b * deal.R + pair] =
@@ -820,14 +837,14 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     }
     if (lone) {
       if (WEIGH && deal.RT == 1) {
-        __syncthreads();
+        __syncthreads();  // the scores are in memory
         add_weights(weigh, pg, ids, b, h, (int64_t)b * (deal.R / deal.RT) * G + row0, G, c, start, len,
                     (start & ~3) + 4 * tid, 64 * kWaves, [&](int g) { return stats[g]; });
       }
       return;
     }
     if (ends && pair + 1 == deal.R) ++b;
-    __syncthreads();
+    lds_barrier();
   }
 }
 
