@@ -714,7 +714,8 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   // the same work the first is through in 60 % of the last one's time, which then has
   // the unit for itself and does not fill it.  A wave's priority falls with each quarter
   // of its chunk: they go on side by side (1,000,003 4-bit tokens: 124 -> 119 us; 64
-  // ragged sequences: 44.9 -> 44.0).
+  // ragged sequences: 44.9 -> 44.0).  f32 cells keep the units' order: a workgroup's
+  // loads fill a unit (24 windows of 6,000 tokens: 77 us, 78 side by side).
   const int64_t f0 = f;
   const int quarter = (int)((f1 - f + 3) >> 2);
   // of the sequence at hand, and the tiles whose pages are in LDS: the next pair of a
@@ -777,7 +778,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
       if (t < re) {
         w.load_k(pg, h, cur);
         while (t < re) {
-          if (!lone) {
+          if (!lone && !F::F32) {
             const int done = (int)(pair_at - f0) + t - t0;
             if (done < quarter) __builtin_amdgcn_s_setprio(3);
             else if (done < 2 * quarter) __builtin_amdgcn_s_setprio(2);

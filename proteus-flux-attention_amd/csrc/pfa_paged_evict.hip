@@ -24,19 +24,28 @@ struct Weights {
 // neighbours of every 4 * THREADS positions, so that loads are in one piece, and a
 // position's place among the kept is counted by ballots: within its wave, then over
 // the waves of all pieces.  All is LDS and latency: 48 rows of up to 20,480 positions
-// in registers, 8,192 kept: XX us (choose_best with 32 neighbours a thread: 23).
+// in registers, 8,192 kept: 16 us (choose_best with 32 neighbours a thread: 23).
 // Positions without a page (where there is a table) are no candidates.
 // ---------------------------------------------------------------------
-template <int THREADS, int C, bool HELD>
-__global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Weights w, Table tab, int shift, int n_pages, int H,
-                                                                const int32_t* __restrict__ lengths, int count, int first,
-                                                                int last, int32_t* __restrict__ kept) {
+// What is chosen from, and how.
+struct Keep {
+  Weights w;
+  Table tab;
+  int shift, n_pages, H;
+  const int32_t* lengths;
+  int count, first, last;
+};
+
+// put(i, position): the i-th kept position, -1 behind the last.
+template <int THREADS, int C, bool HELD, typename Put>
+__device__ __forceinline__ void choose_tokens(const Keep& k, int b, int h, Put&& put) {
   constexpr int WAVES = THREADS / kWave, PIECE = 4 * THREADS;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x / H, h = blockIdx.x % H;
+  const Weights& w = k.w;
+  const int first = k.first, last = k.last, count = k.count, shift = k.shift, n_pages = k.n_pages;
   const float* row = w.p + b * w.s_b + h * w.s_h;
-  const int n = lengths[b], len = n < 0 ? 0 : n < w.most ? n : w.most;
-  const int32_t* ids = tab.ids ? tab.ids + b * tab.stride : nullptr;
+  const int n = k.lengths[b], len = n < 0 ? 0 : n < w.most ? n : w.most;
+  const int32_t* ids = k.tab.ids ? k.tab.ids + b * k.tab.stride : nullptr;
   const int rounds = HELD ? 1 : (len + C * PIECE - 1) / (C * PIECE);
   __shared__ int hist[kBins];
   __shared__ int sums[3][WAVES];
@@ -172,7 +181,6 @@ __global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Weights w, Table
     }
   }
 
-  int32_t* out = kept + (int64_t)blockIdx.x * count;
   int base = 0, tied = 0;  // keys above and equal ones of the rounds before
   for (int r = 0; r < rounds; ++r) {
     if constexpr (!HELD) {
@@ -234,13 +242,19 @@ __global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Weights w, Table
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const bool above = x[c][j] > over, tie = ties > 0 && x[c][j] == over;
-        if (above || (tie && eq < ties)) out[at + (eq < ties ? eq : ties)] = piece(r, c) + 4 * tid + j;
+        if (above || (tie && eq < ties)) put(at + (eq < ties ? eq : ties), piece(r, c) + 4 * tid + j);
         at += above, eq += tie;
       }
     }
     base += taken[0][C * WAVES], tied += taken[1][C * WAVES];
   }
-  for (int i = base + (tied < ties ? tied : ties) + tid; i < count; i += THREADS) out[i] = -1;
+  for (int i = base + (tied < ties ? tied : ties) + tid; i < count; i += THREADS) put(i, -1);
+}
+
+template <int THREADS, int C, bool HELD>
+__global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Keep k, int32_t* __restrict__ kept) {
+  int32_t* out = kept + (int64_t)blockIdx.x * k.count;
+  choose_tokens<THREADS, C, HELD>(k, blockIdx.x / k.H, blockIdx.x % k.H, [&](int i, int position) { out[i] = position; });
 }
 
 // ---------------------------------------------------------------------
@@ -298,13 +312,60 @@ __device__ __forceinline__ void copy_out(uint8_t* p, const uint32_t* w) {
   }
 }
 
+// The lanes' eight channels of kMoveRows rows on their way from slots of one page to
+// slots of another.
+template <int CT, int D>
+struct Moving {
+  static constexpr int LANES = D / 8, UB = cells_bytes(CT, 8), ROW = cells_bytes(CT, D);
+  static constexpr int NS = scales_of(CT, D), PER = LANES / NS;  // scales of a row, lanes of one
+  static constexpr int ES = (int)sizeof(typename Cell<CT>::T);
+  int page[kMoveRows];
+  uint32_t k[kMoveRows][UB / 4], v[kMoveRows][UB / 4];
+  float ks[kMoveRows], vs[kMoveRows];
+
+  // src[u]: the row's position, -1 for none
+  __device__ __forceinline__ void load(const Pages& pg, const Table& from, int b, int h, const int (&src)[kMoveRows]) {
+    const int lane = threadIdx.x % LANES;
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) page[u] = src[u] >= 0 ? page_at(from, pg, b, src[u] >> pg.shift) : -1;
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      if (page[u] < 0) continue;
+      const int64_t slot = (int64_t)h * pg.ps + (src[u] & (pg.ps - 1));
+      copy_in<UB>((const uint8_t*)pg.k + page[u] * pg.k_page * ES + slot * ROW + lane * UB, k[u]);
+      copy_in<UB>((const uint8_t*)pg.v + page[u] * pg.v_page * ES + slot * ROW + lane * UB, v[u]);
+      const int64_t s = (int64_t)page[u] * pg.H * pg.ps + slot;
+      if constexpr (is8(CT)) ks[u] = ((const float*)pg.k_scale)[s], vs[u] = ((const float*)pg.v_scale)[s];
+      if constexpr (is4(CT)) {
+        ks[u] = power_of(((const uint8_t*)pg.k_scale)[s * NS + lane / PER]);
+        vs[u] = power_of(((const uint8_t*)pg.v_scale)[s * NS + lane / PER]);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const Pages& pg, int id, int h, int at, int u) const {
+    const int lane = threadIdx.x % LANES;
+    const int64_t slot = (int64_t)h * pg.ps + at;
+    copy_out<UB>((uint8_t*)pg.k + id * pg.k_page * ES + slot * ROW + lane * UB, k[u]);
+    copy_out<UB>((uint8_t*)pg.v + id * pg.v_page * ES + slot * ROW + lane * UB, v[u]);
+    const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
+    if constexpr (is8(CT)) {
+      if (lane == 0) ((float*)pg.k_scale)[s] = ks[u], ((float*)pg.v_scale)[s] = vs[u];
+    }
+    if constexpr (is4(CT)) {
+      if (lane % PER == 0) {
+        ((uint8_t*)pg.k_scale)[s * NS + lane / PER] = (uint8_t)(__float_as_uint(ks[u]) >> 23);
+        ((uint8_t*)pg.v_scale)[s * NS + lane / PER] = (uint8_t)(__float_as_uint(vs[u]) >> 23);
+      }
+    }
+  }
+};
+
 template <int CT, int D>
 __global__ void __launch_bounds__(256) move_kernel(Pages pg, Table from, Table to, Weights w, const int32_t* __restrict__ kept,
                                                    int count, float* __restrict__ fresh) {
-  constexpr int LANES = D / 8, ROWS = 256 / LANES, UB = cells_bytes(CT, 8), ROW = cells_bytes(CT, D);
-  constexpr int NS = scales_of(CT, D), PER = LANES / NS;  // scales of a row, lanes of one
-  constexpr int ES = (int)sizeof(typename Cell<CT>::T);
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % LANES;
+  using M = Moving<CT, D>;
+  constexpr int ROWS = 256 / M::LANES;
+  const int b = blockIdx.z, h = blockIdx.y;
   const int64_t list = (int64_t)b * pg.H + h;
   // the weights of the kept ones, and zeros behind them
   const float* weights = w.p + b * w.s_b + h * w.s_h;
@@ -320,50 +381,22 @@ __global__ void __launch_bounds__(256) move_kernel(Pages pg, Table from, Table t
     float lo[8], hi[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-    for (int r0 = threadIdx.x / LANES; r0 < pg.ps; r0 += kMoveRows * ROWS) {
+    for (int r0 = threadIdx.x / M::LANES; r0 < pg.ps; r0 += kMoveRows * ROWS) {
       int src[kMoveRows];
-      int page[kMoveRows];
 #pragma unroll
       for (int u = 0; u < kMoveRows; ++u) {
         const int r = r0 + u * ROWS;
         src[u] = r < pg.ps && at + r < count ? kept[list * count + at + r] : -1;
       }
-#pragma unroll
-      for (int u = 0; u < kMoveRows; ++u) page[u] = src[u] >= 0 ? page_at(from, pg, b, src[u] >> pg.shift) : -1;
-      uint32_t k[kMoveRows][UB / 4], v[kMoveRows][UB / 4];
-      [[maybe_unused]] float ks[kMoveRows], vs[kMoveRows];
+      M m;
+      m.load(pg, from, b, h, src);
 #pragma unroll
       for (int u = 0; u < kMoveRows; ++u) {
-        if (page[u] < 0) continue;
-        const int64_t slot = (int64_t)h * pg.ps + (src[u] & (pg.ps - 1));
-        copy_in<UB>((const uint8_t*)pg.k + page[u] * pg.k_page * ES + slot * ROW + lane * UB, k[u]);
-        copy_in<UB>((const uint8_t*)pg.v + page[u] * pg.v_page * ES + slot * ROW + lane * UB, v[u]);
-        const int64_t s = (int64_t)page[u] * pg.H * pg.ps + slot;
-        if constexpr (is8(CT)) ks[u] = ((const float*)pg.k_scale)[s], vs[u] = ((const float*)pg.v_scale)[s];
-        if constexpr (is4(CT)) {
-          ks[u] = power_of(((const uint8_t*)pg.k_scale)[s * NS + lane / PER]);
-          vs[u] = power_of(((const uint8_t*)pg.v_scale)[s * NS + lane / PER]);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kMoveRows; ++u) {
-        if (page[u] < 0) continue;
-        const int64_t slot = (int64_t)h * pg.ps + r0 + u * ROWS;
-        copy_out<UB>((uint8_t*)pg.k + id * pg.k_page * ES + slot * ROW + lane * UB, k[u]);
-        copy_out<UB>((uint8_t*)pg.v + id * pg.v_page * ES + slot * ROW + lane * UB, v[u]);
-        const int64_t s = (int64_t)id * pg.H * pg.ps + slot;
-        if constexpr (is8(CT)) {
-          if (lane == 0) ((float*)pg.k_scale)[s] = ks[u], ((float*)pg.v_scale)[s] = vs[u];
-        }
-        if constexpr (is4(CT)) {
-          if (lane % PER == 0) {
-            ((uint8_t*)pg.k_scale)[s * NS + lane / PER] = (uint8_t)(__float_as_uint(ks[u]) >> 23);
-            ((uint8_t*)pg.v_scale)[s * NS + lane / PER] = (uint8_t)(__float_as_uint(vs[u]) >> 23);
-          }
-        }
+        if (m.page[u] < 0) continue;
+        m.store(pg, id, h, r0 + u * ROWS, u);
         if (pg.bounds) {
           float x[8];
-          values8<CT>(k[u], scaled(CT) ? ks[u] : 1.0f, x);
+          values8<CT>(m.k[u], scaled(CT) ? m.ks[u] : 1.0f, x);
 #pragma unroll
           for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], x[j]), hi[j] = max_nan(hi[j], x[j]);
         }
@@ -380,6 +413,44 @@ __global__ void __launch_bounds__(256) move_kernel(Pages pg, Table from, Table t
   }
 }
 
+// Both in one workgroup for a few rows without bounds, with the kept positions in LDS: a
+// launch less, which is 3.6 us of the host (8 rows of 700 positions, 512 kept, 256 bytes
+// each: 15.4 us a call, 11.8 so).  One unit moves 128 KB in 4 us; with more of it than
+// kSmallBytes the launch is the cheaper.
+constexpr int kSmall = 1024;
+constexpr int64_t kSmallBytes = 256 << 10;
+template <int CT, int D>
+__global__ void __launch_bounds__(1024) evict_kernel(Keep k, Pages pg, Table to, int32_t* __restrict__ kept,
+                                                     float* __restrict__ fresh) {
+  using M = Moving<CT, D>;
+  constexpr int ROWS = 1024 / M::LANES;
+  const int b = blockIdx.x / pg.H, h = blockIdx.x % pg.H;
+  const Weights& w = k.w;
+  __shared__ int32_t list[kSmall];
+  int32_t* out = kept + (int64_t)blockIdx.x * k.count;
+  choose_tokens<1024, 1, true>(k, b, h, [&](int i, int position) { out[i] = list[i] = position; });
+  __syncthreads();
+  const float* weights = w.p + b * w.s_b + h * w.s_h;
+  for (int i = threadIdx.x; i < w.T; i += 1024) {
+    const int src = i < k.count ? list[i] : -1;
+    fresh[(int64_t)blockIdx.x * w.T + i] = src >= 0 ? weights[src] : 0.0f;
+  }
+  for (int i0 = threadIdx.x / M::LANES; i0 < k.count; i0 += kMoveRows * ROWS) {
+    int src[kMoveRows], id[kMoveRows];
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      const int i = i0 + u * ROWS;
+      id[u] = i < k.count ? page_at(to, pg, b, i >> pg.shift) : -1;
+      src[u] = id[u] >= 0 ? list[i] : -1;
+    }
+    M m;
+    m.load(pg, k.tab, b, h, src);
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u)
+      if (m.page[u] >= 0) m.store(pg, id[u], h, (i0 + u * ROWS) & (pg.ps - 1), u);
+  }
+}
+
 int tokens_check(const char* what, const float* weights, int64_t n, int B, int H, int count, int first, int last) {
   PFA_CHECK_ARG(B >= 0 && B <= 65535 && H > 0 && H <= 65535, "%s: 0 to 65535 sequences and 1 to 65535 heads", what);
   PFA_CHECK_ARG((int64_t)B * H <= 1 << 21, "%s: up to 2^21 rows (got %d x %d)", what, B, H);
@@ -390,16 +461,13 @@ int tokens_check(const char* what, const float* weights, int64_t n, int B, int H
   return PFA_OK;
 }
 
-void choose_tokens(const Weights& w, const Table& t, int shift, int n_pages, int B, int H, const int32_t* lengths, int count,
-                   int first, int last, int32_t* kept, hipStream_t stream) {
-#define PFA_CHOOSE(THREADS, C, HELD)                                                                                    \
-  choose_tokens_kernel<THREADS, C, HELD><<<B * H, THREADS, 0, stream>>>(w, t, shift, n_pages, H, lengths, count, first, \
-                                                                        last, kept)
-  if (w.most <= 256 * 4) PFA_CHOOSE(256, 1, true);
-  else if (w.most <= 1024 * 4) PFA_CHOOSE(1024, 1, true);
-  else if (w.most <= 1024 * 16) PFA_CHOOSE(1024, 4, true);
-  else if (w.most <= 1024 * 32) PFA_CHOOSE(1024, 8, true);
-  else if (w.most <= 1024 * 64) PFA_CHOOSE(1024, 16, true);
+void choose_launch(const Keep& k, int rows, int32_t* kept, hipStream_t stream) {
+#define PFA_CHOOSE(THREADS, C, HELD) choose_tokens_kernel<THREADS, C, HELD><<<rows, THREADS, 0, stream>>>(k, kept)
+  if (k.w.most <= 256 * 4) PFA_CHOOSE(256, 1, true);
+  else if (k.w.most <= 1024 * 4) PFA_CHOOSE(1024, 1, true);
+  else if (k.w.most <= 1024 * 16) PFA_CHOOSE(1024, 4, true);
+  else if (k.w.most <= 1024 * 32) PFA_CHOOSE(1024, 8, true);
+  else if (k.w.most <= 1024 * 64) PFA_CHOOSE(1024, 16, true);
   else PFA_CHOOSE(1024, 8, false);
 #undef PFA_CHOOSE
 }
@@ -416,8 +484,9 @@ extern "C" int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(lengths && kept, "kv_tokens_select: null argument");
   const bool vec = (uintptr_t)weights % 16 == 0 && weights_b % 4 == 0 && weights_h % 4 == 0 && n % 4 == 0;
-  choose_tokens(Weights{weights, weights_b, weights_h, (int)n, (int)n, vec}, Table{nullptr, 0, 0}, 0, 0, B, H, lengths, count, first,
-                last, kept, as_stream(stream));
+  choose_launch(Keep{Weights{weights, weights_b, weights_h, (int)n, (int)n, vec}, Table{nullptr, 0, 0}, 0, 0, H, lengths, count,
+                     first, last},
+                B * H, kept, as_stream(stream));
   PFA_CHECK_LAUNCH("kv_tokens_select");
   return PFA_OK;
 }
@@ -440,13 +509,17 @@ extern "C" int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weigh
   hipStream_t s = as_stream(stream);
   const int64_t held = (int64_t)table_pages << p.shift;
   const Weights w{weights, weights_b, weights_h, (int)n, (int)(held < n ? held : n), vec};
-  choose_tokens(w, from, p.shift, p.n_pages, B, p.H, lengths, count, first, last, kept, s);
+  const Keep keep{w, from, p.shift, p.n_pages, p.H, lengths, count, first, last};
+  const int64_t bytes = (int64_t)count * 2 * cells_bytes(pages->dtype, pages->head_dim);
+  const bool small = !p.bounds && count <= kSmall && w.most <= 1024 * 4 && bytes <= kSmallBytes;
+  if (!small) choose_launch(keep, B * p.H, kept, s);
   const int64_t fresh_pages = ((int64_t)count + p.ps - 1) >> p.shift;
   const dim3 grid((unsigned)(fresh_pages < 65535 ? fresh_pages : 65535), p.H, B);
   by_cells(pages->dtype, [&](auto ct) {
     by_width(pages->head_dim, [&](auto width) {
-      move_kernel<decltype(ct)::value, decltype(width)::value>
-          <<<grid, 256, 0, s>>>(p, from, to, w, kept, count, fresh);
+      constexpr int CT = decltype(ct)::value, D = decltype(width)::value;
+      if (small) evict_kernel<CT, D><<<B * p.H, 1024, 0, s>>>(keep, p, to, kept, fresh);
+      else move_kernel<CT, D><<<grid, 256, 0, s>>>(p, from, to, w, kept, count, fresh);
     });
   });
   PFA_CHECK_LAUNCH("kv_tokens_evict");
