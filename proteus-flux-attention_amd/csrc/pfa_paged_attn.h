@@ -122,8 +122,9 @@ struct Form {
   static constexpr int VW = VB < 4 ? 1 : VB / 4;
   static constexpr int NG = tile_groups(CT, D);  // 32-key groups that a wave loads at once
   static constexpr int TILE = 32 * NG;
-  // waves of a SIMD, at least, that the registers leave without spills
-  static constexpr int AT_LEAST = QT == PFA_F32 && D == 128 ? 2 : 3;
+  // waves of a SIMD, at least, that the registers leave without spills (f16 queries on
+  // 1,000,003 4-bit tokens of 128 channels: 135 us with three, 126 with two)
+  static constexpr int AT_LEAST = D == 128 && (QT == PFA_F32 || (is4(CT) && QT == PFA_F16)) ? 2 : 3;
   static constexpr float PSCALE = F16 ? 32768.0f : 1.0f;
 };
 
@@ -579,6 +580,7 @@ static __global__ void __launch_bounds__(256) weigh_kernel(Weigh w, Pages pg, co
                                                            const int32_t* __restrict__ starts) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int len = length_at(lengths, P, pg.shift, b), start = start_at(starts, b);
+  if (start >= len) return;
   const int64_t row = ((int64_t)b * pg.H + h) * G;
   const int64_t first = (start & ~3) + 4 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
   add_weights(w, pg, table + b * table_stride, b, h, row, G, c, start, len, first, (int)(gridDim.x * blockDim.x),
@@ -956,7 +958,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
 // The join and the weights beside it: `joins` workgroups join, as join_kernel's do, the
 // others take four positions a thread and work their rows' statistics out of the parts
 // themselves, which costs less than to wait for the join (32 ragged sequences of up to
-// 16,384 int8 tokens: 85 -> 79 us).  16 rows of a key-value head at most.
+// 16,384 int8 tokens: 85 -> 83 us; 700 tokens of 8 heads: 19 -> 16).  16 rows of a key-value head at most.
 template <int QT, int THREADS>
 __global__ void __launch_bounds__(THREADS) join_weigh_kernel(Deal deal, int G, int D, float c, float pscale,
                                                              const int32_t* __restrict__ lengths,
@@ -975,7 +977,7 @@ __global__ void __launch_bounds__(THREADS) join_weigh_kernel(Deal deal, int G, i
   const int block = (int)blockIdx.x - joins, pair = block / pieces, b = pair / pg.H, h = pair % pg.H;
   const int len = deal.length(lengths, b), start = start_at(starts, b);
   const int64_t first = (start & ~3) + 4 * (int64_t)(block % pieces) * THREADS;
-  if (first >= len) return;
+  if (start >= len || first >= len) return;  // a row without tiles has no parts
   const int64_t row0 = (int64_t)pair * G;
   __shared__ float2 stats[16];
   const Shared who = shared[pair];

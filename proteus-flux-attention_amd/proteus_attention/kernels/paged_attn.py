@@ -539,8 +539,9 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     """Keeps ``count`` tokens of each sequence and key-value head: those that
     :func:`select_kv_tokens` takes, of the positions that have a page, move into
     the pages that ``into`` ``(B, pages)`` int32 names, in their order, from its
-    first slot on.  Cells and scales move as they are, with the pages' key bounds
-    where the pool has them.
+    first slot on.  Positions from T on, which have no weight, are not kept.
+    Cells and scales move as they are, with the pages' key bounds where the pool
+    has them.
 
     Returns the positions that were kept ``(B, kv_heads, count)``, -1 behind the
     last, and their key weights, zeros behind them, in a tensor of

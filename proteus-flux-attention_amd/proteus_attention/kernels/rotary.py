@@ -125,15 +125,11 @@ def _sides(x: torch.Tensor, inplace: bool) -> Tuple[torch.Tensor, torch.Tensor, 
 
     shape, s = x.shape, x.stride()
     if s[-1] != 1 and shape[-1] > 1:
-        if inplace:
-            raise ValueError("inplace needs a dense last dimension")
         x = x.contiguous()
         s = x.stride()
     many = len(shape) == 4
     source = (x.data_ptr(), s[0], s[2], s[1]) if many else (x.data_ptr(), s[0], s[1], 0)
     if inplace:
-        if 0 in s and any(stride == 0 and size > 1 for stride, size in zip(s, shape)):
-            raise ValueError("inplace needs rows of their own: an expanded tensor has none")
         return x, x, source, source
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     s = y.stride()
@@ -151,7 +147,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     The first ``width`` channels of a head turn, the others stay.  Angles are
     exact at any position, products f32, rounded once at the end.  Returns
     contiguous tensors in the inputs' type, or with ``inplace`` the inputs,
-    written over.
+    written over: their rows must not overlap, and q and k not be the same.
     """
 
     turns, magnitude, interleaved = rotary
@@ -181,6 +177,14 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
         raise ValueError(f"positions must be a ({B},) or ({B}, {n}) int32 tensor")
     if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("apply_rotary has no backward pass: call it under torch.no_grad()")
+    if inplace:
+        for x in (q, k) if Hk else (q,):
+            if x.stride(-1) != 1 and D > 1:
+                raise ValueError("inplace needs a dense last dimension")
+            if any(stride == 0 and size > 1 for stride, size in zip(x.stride(), x.shape)):
+                raise ValueError("inplace needs rows of their own: an expanded tensor has none")
+        if Hk and q.data_ptr() == k.data_ptr() and q.numel():
+            raise ValueError("inplace needs q and k apart: one tensor would be turned twice")
     index = _device("apply_rotary", q, k, positions, turns)
     pos = positions.stride()
     q, q_out, q_from, q_to = _sides(q, inplace)

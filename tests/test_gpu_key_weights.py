@@ -152,6 +152,32 @@ def test_windows_and_pages_that_are_gone(pair):
             assert bool(seen.any())
 
 
+@pytest.mark.parametrize("pair", [PAIRS[0], PAIRS[1], PAIRS[4], PAIRS[-1]], ids=R.pair_id)
+def test_windows_of_rows_that_are_shared_out(pair):
+    """Rows cut over many workgroups beside rows that see nothing: windows that start at,
+    behind and next to their ends, a row of one key, sequences without tokens."""
+    from proteus_attention import paged_attention
+
+    dt, cell = pair
+    g = torch.Generator().manual_seed(21)
+    for D, ps, H, G in ((64, 16, 1, 4), (128, 64, 2, 1), (32, 16, 1, 18)):
+        lengths = [9001, 4097, 9, 0, 4098, 5, 2050, 3]
+        starts = [103, 4097, 10, 3, 4097, 7, 2047, -9]
+        N = sum(-(-n // ps) for n in lengths) + 1
+        table = R.make_table(lengths, ps, N, g)
+        table[0, 7] = -1
+        pool = _pool(cell, N, H, ps, D, g)
+        q = torch.randn(len(lengths), H * G, D, generator=g).to(dt)
+        ref = weights(q, _plain(cell, pool), table, lengths, starts)
+        before = torch.rand(len(lengths), H, table.shape[1] * ps, generator=g)
+        w = before.to(DEV)
+        args = (q.to(DEV), _pages(cell, pool), table.to(DEV), _i32(lengths).to(DEV))
+        out = paged_attention(*args, starts=_i32(starts).to(DEV), key_weights=w)
+        assert torch.equal(out, paged_attention(*args, starts=_i32(starts).to(DEV)))
+        assert holds(w.cpu(), before, ref, G, D, 9001), (D, ps)
+        assert not out[[1, 2, 3, 5]].any()
+
+
 def test_rows_without_a_weight_and_rows_that_are_not_numbers():
     """Scores of -inf alone leave nothing; a NaN among a row's scores makes its weights NaN,
     in its own head alone."""
@@ -209,7 +235,7 @@ def choose(w, lengths, count, first, last, have=None):
     return kept
 
 
-@pytest.mark.parametrize("T", [1, 7, 64, 1023, 1024, 1025, 4096, 5000, 16384, 16385, 40003])
+@pytest.mark.parametrize("T", [1, 7, 64, 1023, 1024, 1025, 4096, 5000, 16384, 16385, 40003, 65536, 65537, 140001])
 def test_select_tokens(T):
     from proteus_attention import select_kv_tokens
 

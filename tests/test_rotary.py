@@ -90,6 +90,9 @@ POS = torch.zeros(2, dtype=torch.int32)
     lambda: apply_rotary(Q, K, POS, ROT._replace(turns=ROT.turns.int())),
     lambda: apply_rotary(Q, K, POS, ROT._replace(turns=ROT.turns[:0])),
     lambda: apply_rotary(Q, K, POS, ROT._replace(turns=ROT.turns[::2])),
+    lambda: apply_rotary(Q, Q, POS, ROT, inplace=True),
+    lambda: apply_rotary(Q, Q[:, :, :2], POS, ROT, inplace=True),
+    lambda: apply_rotary(Q[:, :, :1].expand(2, 3, 4, 32), None, POS, ROT, inplace=True),
 ])
 def test_arguments_that_do_not_fit(call):
     with pytest.raises(ValueError):
