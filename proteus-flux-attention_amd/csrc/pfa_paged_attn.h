@@ -619,6 +619,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   __shared__ Entry entries[kEntries + 1];
   __shared__ int64_t sums[kWaves];
   __shared__ int64_t found[2];
+  __shared__ int found_at[2];
   __shared__ float2 stats[WEIGH ? 16 : 1];
   deal.tile = F::TILE;  // as it is, and known
   const int tid = threadIdx.x, lane = tid & 63;
@@ -631,6 +632,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   // first pair begins at `at`
   int64_t f, f1, at, chunk = 1;
   int b;
+  // of the sequence at hand, and below the tiles whose pages are in LDS: the next pair of
+  // a short sequence, which has the same, goes on without waiting for either
+  int at_hand = -1, start = 0, len = 0, nt = 0, np = 0;
   if (parts_ws && deal.S >= 0) {  // all sequences alike
     const int np = deal.places(0, 1);
     const int64_t total = (int64_t)deal.B * deal.R * np;
@@ -642,12 +646,14 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     at = (int64_t)b * deal.R * np;
   } else if (parts_ws) {
     // places of the sequences up to this thread's, of 256 at a time
+    int its_start = 0, its_len = 0;
     auto places = [&](int i) {
-      return i < deal.B ? deal.places(start_at(starts, i), deal.length(lengths, i)) * (int64_t)deal.R : 0;
+      its_start = i < deal.B ? start_at(starts, i) : 0, its_len = i < deal.B ? deal.length(lengths, i) : 0;
+      return deal.places(its_start, its_len) * (int64_t)deal.R;
     };
-    int64_t nt, incl, all;
+    int64_t incl, all, mine;
     auto scan = [&](int i) {
-      incl = nt = places(i);
+      incl = mine = places(i);
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) {
         const int64_t x = __shfl_up(incl, o);
@@ -665,14 +671,16 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     scan(tid);
     int64_t total = all;
     if (deal.B > 64 * kWaves) {
-      int64_t mine = 0;
-      for (int i = tid + 64 * kWaves; i < deal.B; i += 64 * kWaves) mine += places(i);
-      mine = wave_sum(mine);
+      const int start0 = its_start, len0 = its_len;
+      int64_t rest = 0;
+      for (int i = tid + 64 * kWaves; i < deal.B; i += 64 * kWaves) rest += places(i);
+      rest = wave_sum(rest);
       lds_barrier();
-      if (lane == 0) sums[wave] = mine;
+      if (lane == 0) sums[wave] = rest;
       lds_barrier();
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) total += sums[i];
+      its_start = start0, its_len = len0;
     }
     total = uniform(total);
     chunk = deal.chunk(total);
@@ -681,7 +689,10 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     f1 = f + chunk < total ? f + chunk : total;
     int64_t before = 0;
     for (int base = 0;;) {
-      if (nt > 0 && before + incl - nt <= f && f < before + incl) found[0] = base + tid, found[1] = before + incl - nt;
+      if (mine > 0 && before + incl - mine <= f && f < before + incl) {
+        found[0] = base + tid, found[1] = before + incl - mine;
+        found_at[0] = its_start, found_at[1] = its_len;
+      }
       before += all;
       if (f < before) break;
       base += 64 * kWaves;
@@ -691,6 +702,9 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     lds_barrier();
     b = (int)uniform(found[0]);
     at = uniform(found[1]);
+    at_hand = b;
+    start = __builtin_amdgcn_readfirstlane(found_at[0]), len = __builtin_amdgcn_readfirstlane(found_at[1]);
+    nt = deal.tiles(start, len), np = deal.places(start, len);
   } else {  // a workgroup a pair
     b = blockIdx.x / deal.R;
     f = (int64_t)(blockIdx.x % deal.R) * deal.tiles(start_at(starts, b), deal.length(lengths, b));
@@ -720,9 +734,6 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
   // loads fill a unit (24 windows of 6,000 tokens: 77 us, 78 side by side).
   const int64_t f0 = f;
   const int quarter = (int)((f1 - f + 3) >> 2);
-  // of the sequence at hand, and the tiles whose pages are in LDS: the next pair of a
-  // short sequence, which has the same, goes on without waiting for either
-  int at_hand = -1, start = 0, len = 0, nt = 0, np = 0;
   int looked_up = -1, first_up = 0, end_up = 0;
   while (f < f1) {
     if (b != at_hand) {
