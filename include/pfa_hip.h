@@ -754,7 +754,8 @@ int pfa_paged_sparse_attn_fwd(const pfa_paged_query* query, int count, int first
  * exp(score_t - max) / sum, added in f32 in the heads' order.  Positions that are
  * not seen, or have no page, stay as they are; a row that is NaN gives NaN.  No
  * rows of weights may overlap.  The workspace holds the scores: 4 bytes for each
- * query head and position of the table, of every sequence. */
+ * query head (whole 16s of them where more than 16 share a key-value head) and
+ * position of the table, of every sequence. */
 int pfa_paged_weigh_attn_workspace_size(int B, int H, int kv_heads, int page_size, int head_dim,
                                         int cell_dtype, int table_pages, size_t* bytes);
 int pfa_paged_weigh_attn_fwd(const pfa_paged_query* query, float* weights, int64_t weights_b,
@@ -772,10 +773,10 @@ int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int64_t weight
 
 /* That choice among the positions that have a page, and a move: the i-th kept
  * position's cells and scales, of every head, into slot i of the pages that `into`
- * (B, into_pages, at least count positions) names, its weight into fresh (B,
- * kv_heads, n) dense, zeros behind the last.  k_bounds of the new pages, where the
+ * (B, into_pages) names, its weight into fresh (B, kv_heads, n) dense, zeros
+ * behind the last.  k_bounds of the new pages, where the
  * pool has them, are those of their kept keys.  Entries of `into` without a page
- * take nothing.  No page of `into` may be one of the call's `table`, or named
+ * take nothing, and what is behind its last is left out.  No page of `into` may be one of the call's `table`, or named
  * twice: the other pages stay as they are. */
 int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weights, int64_t weights_b,
                         int64_t weights_h, int64_t n, int B, const int32_t* table,

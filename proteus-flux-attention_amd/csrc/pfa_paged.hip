@@ -512,8 +512,13 @@ static bool selects_itself(const Plan& plan, int P, int D) {
 
 // Behind a call's own workspace, where it weighs its keys: the scores and the rows'
 // statistics.
-static size_t weigh_bytes(int B, int H, int P, int shift) {
-  return (size_t)B * H * (((size_t)P << shift) * sizeof(float) + sizeof(float2));
+static int score_rows(int G) { return G < 16 ? G : 16; }
+static size_t score_count(int B, int H, int kv_heads, int P, int shift) {
+  const int G = H / kv_heads;
+  return (size_t)B * kv_heads * ((G + 15) / 16) * score_rows(G) * ((size_t)P << shift);
+}
+static size_t weigh_bytes(int B, int H, int kv_heads, int P, int shift) {
+  return score_count(B, H, kv_heads, P, shift) * sizeof(float) + (size_t)B * H * sizeof(float2);
 }
 static size_t aligned16(size_t bytes) { return (bytes + 15) & ~(size_t)15; }
 
@@ -526,7 +531,7 @@ static int attend(const char* what, const pfa_paged_query* query, const Pages& p
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(out && (uintptr_t)out % 16 == 0, "%s: null or unaligned argument", what);
   const Plan plan = attend_plan(B, H, p.H, D, p.shift, t.P, S, attend_tile(ct, D), choice.count > 0);
-  const size_t need = weigh.weights ? aligned16(plan.bytes) + weigh_bytes(B, H, t.P, p.shift) : plan.bytes;
+  const size_t need = weigh.weights ? aligned16(plan.bytes) + weigh_bytes(B, H, p.H, t.P, p.shift) : plan.bytes;
   if (ws_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16 != 0))) {
     set_error("%s: workspace of %zu bytes, %zu needed, 16-byte aligned", what, ws_bytes, need);
     return PFA_E_WORKSPACE;
@@ -534,7 +539,8 @@ static int attend(const char* what, const pfa_paged_query* query, const Pages& p
   if (weigh.weights) {
     weigh.cap = (int64_t)t.P << p.shift;
     weigh.scores = (float*)((char*)workspace + aligned16(plan.bytes));
-    weigh.stats = (float2*)(weigh.scores + (int64_t)B * H * weigh.cap);
+    weigh.rows = score_rows(H / p.H);
+    weigh.stats = (float2*)(weigh.scores + score_count(B, H, p.H, t.P, p.shift));
   }
   const AttendCall a{p, t.ids, t.stride, t.P, B, H, D, query->q, query->lengths, query->starts, selected,
                      selected_stride, S, c, choice, weigh, out, (float*)workspace, as_stream(stream)};
@@ -564,7 +570,7 @@ extern "C" int pfa_paged_weigh_attn_workspace_size(int B, int H, int kv_heads, i
                                                    int table_pages, size_t* bytes) {
   if (int rc = pfa_paged_attn_workspace_size(B, H, kv_heads, page_size, head_dim, cell_dtype, table_pages, -1, bytes))
     return rc;
-  *bytes = aligned16(*bytes) + weigh_bytes(B, H, table_pages, shift_of(page_size));
+  *bytes = aligned16(*bytes) + weigh_bytes(B, H, kv_heads, table_pages, shift_of(page_size));
   return PFA_OK;
 }
 
@@ -581,7 +587,7 @@ extern "C" int pfa_paged_weigh_attn_fwd(const pfa_paged_query* query, float* wei
                 (long long)((int64_t)t.P << p.shift));
   if (t.P == 0) weights = nullptr;  // no keys to weigh
   const bool vec = (uintptr_t)weights % 16 == 0 && weights_b % 4 == 0 && weights_h % 4 == 0;
-  const Weigh weigh{weights, weights_b, weights_h, vec, nullptr, 0, nullptr};
+  const Weigh weigh{weights, weights_b, weights_h, vec, nullptr, 0, 0, nullptr};
   return attend("paged_weigh_attn", query, p, t, nullptr, 0, -1, Choice{}, weigh, scale, out, workspace, ws_bytes, stream);
 }
 

@@ -501,8 +501,6 @@ extern "C" int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weigh
   if (int rc = paged_check(pages, into, into_stride, into_pages, B, &p, &to)) return rc;
   if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &from)) return rc;
   if (int rc = tokens_check("kv_tokens_evict", weights, n, B, p.H, count, first, last)) return rc;
-  PFA_CHECK_ARG((int64_t)into_pages << p.shift >= count, "kv_tokens_evict: %d tokens into %d pages of %d", count, into_pages,
-                p.ps);
   if (B == 0) return PFA_OK;
   PFA_CHECK_ARG(lengths && kept && (fresh || n == 0), "kv_tokens_evict: null argument");
   const bool vec = (uintptr_t)weights % 16 == 0 && weights_b % 4 == 0 && weights_h % 4 == 0 && n % 4 == 0;

@@ -548,17 +548,15 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     ``key_weights``' shape: sequences go on with ``into`` for a table, these
     weights, and ``lengths`` of up to ``count``.  The pages of ``block_table``
     stay as they are, so that others may share them; no page may be in both
-    tables, or in ``into`` twice.  Tokens for entries of ``into`` that name no page
-    are lost.  Keys keep the rotary positions that they were written with.
+    tables, or in ``into`` twice.  Tokens for entries of ``into`` that name no page,
+    and those behind its last, are left out.  Keys keep the rotary positions that they were written with.
     """
 
     count, first, last = _held(count, first, last, "tokens")
     pool = _pool(pages)
-    Hkv, ps = pool[8], pool[9]
+    Hkv = pool[8]
     B = block_table.shape[0] if block_table.dim() else 0
     table, fresh_table = _table(block_table, B), _table(into, B)
-    if fresh_table.shape[1] * ps < count:
-        raise ValueError(f"{count} tokens into {fresh_table.shape[1]} pages of {ps}")
     if B and table.data_ptr() == fresh_table.data_ptr():
         raise ValueError("into must name other pages than block_table")
     weights = _dense_rows(_key_weights(key_weights, B, Hkv, "evict_kv_tokens"))

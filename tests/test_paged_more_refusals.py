@@ -76,7 +76,6 @@ def test_cpu_tensors_fail_loudly():
     lambda p: evict_kv_tokens(p, W, TABLE, ONE, 0, INTO),
     lambda p: evict_kv_tokens(p, W, TABLE, ONE, 3, INTO, first=2, last=2),
     lambda p: evict_kv_tokens(p, W, TABLE, ONE, 3, INTO, last=-1),
-    lambda p: evict_kv_tokens(p, W, TABLE, ONE, 33, INTO),
     lambda p: evict_kv_tokens(p, W, TABLE, ONE, 3, INTO.long()),
     lambda p: evict_kv_tokens(p, W, TABLE, ONE, 3, INTO[0]),
     lambda p: evict_kv_tokens(p, W, TABLE, ONE, 3, TABLE),
@@ -137,7 +136,7 @@ def test_c_entries_refuse_before_any_launch():
            weigh(B=-1), weigh(head_dim=48), lib.pfa_paged_weigh_attn_fwd(None, p, 64, 32, 32, 0.5, p, p, 1 << 40, None),
            evict(w=None), evict(w=ctypes.c_void_p(257)), evict(n=-1), evict(n=(1 << 30) + 1), evict(B=-1), evict(table=None),
            evict(P=-1), evict(lengths=None), evict(count=0), evict(count=1), evict(first=3), evict(last=-1), evict(into=None),
-           evict(P2=0), evict(P2=2, count=33), evict(kept=None), evict(fresh=None), evict(v_scale=0), evict(dtype=6),
+           evict(P2=-1), evict(P2=1 << 28), evict(kept=None), evict(fresh=None), evict(v_scale=0), evict(dtype=6),
            select(w=None), select(n=-1), select(B=70000), select(B=60000, H=60), select(H=0), select(lengths=None),
            select(count=0), select(count=-3, first=0, last=0), select(kept=None), select(last=3)]
     assert bad == [-1] * len(bad)
