@@ -778,11 +778,18 @@ int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int64_t weight
  * pool has them, are those of their kept keys.  Entries of `into` without a page
  * take nothing, and what is behind its last is left out.  No page of `into` may be one of the call's `table`, or named
  * twice: the other pages stay as they are. */
-int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weights, int64_t weights_b,
-                        int64_t weights_h, int64_t n, int B, const int32_t* table,
-                        int64_t table_stride, int table_pages, const int32_t* lengths, int count,
-                        int first, int last, const int32_t* into, int64_t into_stride,
-                        int into_pages, int32_t* kept, float* fresh, void* stream);
+typedef struct pfa_kv_evict {
+  pfa_kv_pages pages;
+  const float* weights;
+  int64_t weights_b, weights_h, n;
+  const int32_t *table, *into, *lengths;
+  int64_t table_stride, into_stride;
+  int32_t* kept;
+  float* fresh;
+  int table_pages, into_pages, B, count, first, last;
+} pfa_kv_evict;
+
+int pfa_kv_tokens_evict(const pfa_kv_evict* call, void* stream);
 
 /* ====================================================================
  * Rotary positions of queries and keys.  The reference turns whole heads of

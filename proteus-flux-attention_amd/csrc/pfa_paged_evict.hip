@@ -491,30 +491,33 @@ extern "C" int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int
   return PFA_OK;
 }
 
-extern "C" int pfa_kv_tokens_evict(const pfa_kv_pages* pages, const float* weights, int64_t weights_b, int64_t weights_h,
-                                   int64_t n, int B, const int32_t* table, int64_t table_stride, int table_pages,
-                                   const int32_t* lengths, int count, int first, int last, const int32_t* into,
-                                   int64_t into_stride, int into_pages, int32_t* kept, float* fresh, void* stream) {
+extern "C" int pfa_kv_tokens_evict(const pfa_kv_evict* c, void* stream) {
   clear_error();
+  PFA_CHECK_ARG(c, "kv_tokens_evict: null argument");
+  const int B = c->B, count = c->count;
+  const float* weights = c->weights;
+  const int64_t n = c->n;
+  int32_t* kept = c->kept;
+  float* fresh = c->fresh;
   Pages p;
   Table from, to;
-  if (int rc = paged_check(pages, into, into_stride, into_pages, B, &p, &to)) return rc;
-  if (int rc = paged_check(pages, table, table_stride, table_pages, B, &p, &from)) return rc;
-  if (int rc = tokens_check("kv_tokens_evict", weights, n, B, p.H, count, first, last)) return rc;
+  if (int rc = paged_check(&c->pages, c->into, c->into_stride, c->into_pages, B, &p, &to)) return rc;
+  if (int rc = paged_check(&c->pages, c->table, c->table_stride, c->table_pages, B, &p, &from)) return rc;
+  if (int rc = tokens_check("kv_tokens_evict", weights, n, B, p.H, count, c->first, c->last)) return rc;
   if (B == 0) return PFA_OK;
-  PFA_CHECK_ARG(lengths && kept && (fresh || n == 0), "kv_tokens_evict: null argument");
-  const bool vec = (uintptr_t)weights % 16 == 0 && weights_b % 4 == 0 && weights_h % 4 == 0 && n % 4 == 0;
+  PFA_CHECK_ARG(c->lengths && kept && (fresh || n == 0), "kv_tokens_evict: null argument");
+  const bool vec = (uintptr_t)weights % 16 == 0 && c->weights_b % 4 == 0 && c->weights_h % 4 == 0 && n % 4 == 0;
   hipStream_t s = as_stream(stream);
-  const int64_t held = (int64_t)table_pages << p.shift;
-  const Weights w{weights, weights_b, weights_h, (int)n, (int)(held < n ? held : n), vec};
-  const Keep keep{w, from, p.shift, p.n_pages, p.H, lengths, count, first, last};
-  const int64_t bytes = (int64_t)count * 2 * cells_bytes(pages->dtype, pages->head_dim);
+  const int64_t held = (int64_t)from.P << p.shift;
+  const Weights w{weights, c->weights_b, c->weights_h, (int)n, (int)(held < n ? held : n), vec};
+  const Keep keep{w, from, p.shift, p.n_pages, p.H, c->lengths, count, c->first, c->last};
+  const int64_t bytes = (int64_t)count * 2 * cells_bytes(c->pages.dtype, c->pages.head_dim);
   const bool small = !p.bounds && count <= kSmall && w.most <= 1024 * 4 && bytes <= kSmallBytes;
   if (!small) choose_launch(keep, B * p.H, kept, s);
   const int64_t fresh_pages = ((int64_t)count + p.ps - 1) >> p.shift;
   const dim3 grid((unsigned)(fresh_pages < 65535 ? fresh_pages : 65535), p.H, B);
-  by_cells(pages->dtype, [&](auto ct) {
-    by_width(pages->head_dim, [&](auto width) {
+  by_cells(c->pages.dtype, [&](auto ct) {
+    by_width(c->pages.head_dim, [&](auto width) {
       constexpr int CT = decltype(ct)::value, D = decltype(width)::value;
       if (small) evict_kernel<CT, D><<<B * p.H, 1024, 0, s>>>(keep, p, to, kept, fresh);
       else move_kernel<CT, D><<<grid, 256, 0, s>>>(p, from, to, w, kept, count, fresh);

@@ -100,10 +100,11 @@ def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *
     return KVPages(k, v, *scales, kb)
 
 
-# pfa_kv_pages, pfa_tensor4 and pfa_paged_query of include/pfa_hip.h
+# pfa_kv_pages, pfa_tensor4, pfa_paged_query and pfa_kv_evict of include/pfa_hip.h
 _POOL = struct.Struct("PPPPPqqiiiii4x")
 _TENSOR4 = struct.Struct("Pqqq")
 _QUERY = struct.Struct(_POOL.format + _TENSOR4.format + "PqPPiiii")
+_EVICT = struct.Struct(_POOL.format + "PqqqPPPqqPPiiiiii")
 
 
 def _dense(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, name: str) -> int:
@@ -565,10 +566,11 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     index = _device("evict_kv_tokens", *pages, table, fresh_table, weights, lengths)
     kept = table.new_empty((B, Hkv, count))
     fresh = torch.empty_like(weights, memory_format=torch.contiguous_format)
-    _call(index, "kv_tokens_evict", _hip.lib().pfa_kv_tokens_evict, _POOL.pack(*pool), weights.data_ptr(),
-          weights.stride(0), weights.stride(1), T, B, table.data_ptr(), table.stride(0), table.shape[1],
-          lengths.data_ptr(), count, first, last, fresh_table.data_ptr(), fresh_table.stride(0), fresh_table.shape[1],
-          kept.data_ptr(), fresh.data_ptr())
+    apart = weights.stride()
+    packed = _EVICT.pack(*pool, weights.data_ptr(), apart[0], apart[1], T, table.data_ptr(), fresh_table.data_ptr(),
+                         lengths.data_ptr(), table.stride(0), fresh_table.stride(0), kept.data_ptr(), fresh.data_ptr(),
+                         table.shape[1], fresh_table.shape[1], B, count, first, last)
+    _call(index, "kv_tokens_evict", _hip.lib().pfa_kv_tokens_evict, packed)
     return kept, fresh
 
 

@@ -124,9 +124,10 @@ def test_c_entries_refuse_before_any_launch():
     def weigh(w=p, n=32, scale=0.5, out=p, ws=p, size=1 << 40, **kw):
         return lib.pfa_paged_weigh_attn_fwd(query(**kw), w, 64, 32, n, scale, out, ws, size, None)
 
-    def evict(w=p, n=32, B=1, table=p, P=2, lengths=p, count=3, first=1, last=1, into=p, P2=2, kept=p, fresh=p, **kw):
-        return lib.pfa_kv_tokens_evict(struct.pack(_POOL, *_fields(**kw)), w, 64, 32, n, B, table, P, P, lengths, count,
-                                       first, last, into, P2, P2, kept, fresh, None)
+    def evict(w=256, n=32, B=1, table=256, P=2, lengths=256, count=3, first=1, last=1, into=256, P2=2, kept=256, fresh=256,
+              **kw):
+        return lib.pfa_kv_tokens_evict(struct.pack(_POOL + "PqqqPPPqqPPiiiiii", *_fields(**kw), w, 64, 32, n, table, into,
+                                                   lengths, P, P2, kept, fresh, P, P2, B, count, first, last), None)
 
     def select(w=p, n=32, B=1, H=2, lengths=p, count=3, first=1, last=1, kept=p):
         return lib.pfa_kv_tokens_select(w, 64, 32, n, B, H, lengths, count, first, last, kept, None)
@@ -134,9 +135,9 @@ def test_c_entries_refuse_before_any_launch():
     bad = [weigh(w=None), weigh(w=ctypes.c_void_p(258)), weigh(n=31), weigh(scale=0.0), weigh(scale=math.nan), weigh(out=None),
            weigh(H=3), weigh(k_scale=0), weigh(k_page=2 * 16 * 32 - 16), weigh(v_page=2 * 16 * 32 + 8), weigh(k=264),
            weigh(B=-1), weigh(head_dim=48), lib.pfa_paged_weigh_attn_fwd(None, p, 64, 32, 32, 0.5, p, p, 1 << 40, None),
-           evict(w=None), evict(w=ctypes.c_void_p(257)), evict(n=-1), evict(n=(1 << 30) + 1), evict(B=-1), evict(table=None),
-           evict(P=-1), evict(lengths=None), evict(count=0), evict(count=1), evict(first=3), evict(last=-1), evict(into=None),
-           evict(P2=-1), evict(P2=1 << 28), evict(kept=None), evict(fresh=None), evict(v_scale=0), evict(dtype=6),
+           lib.pfa_kv_tokens_evict(None, None), evict(w=0), evict(w=257), evict(n=-1), evict(n=(1 << 30) + 1), evict(B=-1), evict(table=0),
+           evict(P=-1), evict(lengths=0), evict(count=0), evict(count=1), evict(first=3), evict(last=-1), evict(into=0),
+           evict(P2=-1), evict(P2=1 << 28), evict(kept=0), evict(fresh=0), evict(v_scale=0), evict(dtype=6),
            select(w=None), select(n=-1), select(B=70000), select(B=60000, H=60), select(H=0), select(lengths=None),
            select(count=0), select(count=-3, first=0, last=0), select(kept=None), select(last=3)]
     assert bad == [-1] * len(bad)
