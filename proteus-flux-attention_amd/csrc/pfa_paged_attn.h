@@ -28,18 +28,23 @@
 // once, between two barriers (kEntries).
 //
 // Precision: f32 stays on v_mfma_f32_16x16x4f32.  8-bit cells are whole in
-// bf16; their scales multiply S and P in f32.  Queries of f16 or f32 on 8-bit
-// cells are split into two or three bf16 parts, which hold all their bits.  P goes
+// bf16; their scales multiply S and P in f32.  4-bit cells with their scales, which are
+// powers of two, are whole in bf16, too: the conversion multiplies them.  Queries of f16
+// or f32 on cells of 8 or 4 bits are split into two or three bf16 parts, which hold all
+// their bits.  P goes
 // in three parts, each cut off from what the ones before leave: all of its 24
 // bits.  f16 parts are of 2^15 P, which has its 24 bits down to 2^-16 of the row's
 // largest and 2^-39 absolutely below.  Two bf16 parts hold 16 bits and put 7 to 19
 // times as many results of bf16 queries, or of f16 queries on 8-bit cells, on the
 // other side of their rounding, and take the same time (1,000,003 int8 tokens: 201
-// us a call with two, 202 with three): the loads are what is waited for.  Sums,
+// us a call with two, 202 with three): the loads are what is waited for.  4-bit cells
+// are near what the arithmetic takes (118 us for 124 with two of them).  Sums,
 // maxima and O are f32 throughout.
 //
-// Measured (one MI355X, a large copy at 4.7 TB/s): 1,000,003 int8 tokens of 4 heads
-// of 128, 8 query heads each: 195 us, 5.4 TB/s; 24 windows of up to 6,000 f32 tokens
+// Measured (one MI355X, a large copy at 4.7 to 5.1 TB/s): 1,000,003 tokens of 4 heads
+// of 128, 8 query heads each: int8 190 us, 5.5 TB/s, 4 bits 104 us, 5.2 TB/s; 64 ragged
+// sequences of up to 16,384 4-bit tokens of 8 heads of 128, 4 query heads each: 35 us,
+// 3.5 TB/s; 24 windows of up to 6,000 f32 tokens
 // of 8 heads of 64: 75 us, 5.0 TB/s; 64 ragged sequences of up to 8,192 bf16 tokens of
 // 8 heads of 128, 4 query heads each: 57 us, 4.3 TB/s; 8 heads of 64 over 173 tokens:
 // 8 us, of which the launch and four loads one behind the other (length, table, key,
