@@ -774,10 +774,10 @@ int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int64_t weight
 /* That choice among the positions that have a page, and a move: the i-th kept
  * position's cells and scales, of every head, into slot i of the pages that `into`
  * (B, into_pages) names, its weight into fresh (B, kv_heads, n) dense, zeros
- * behind the last.  k_bounds of the new pages, where the
- * pool has them, are those of their kept keys.  Entries of `into` without a page
- * take nothing, and what is behind its last is left out.  No page of `into` may be one of the call's `table`, or named
- * twice: the other pages stay as they are. */
+ * behind the last.  k_bounds of the new pages, where the pool has them, are those
+ * of their kept keys.  Entries of `into` without a page take nothing, and what is
+ * behind its last is left out.  No page of `into` may be one of the call's `table`,
+ * or named twice: the other pages stay as they are. */
 typedef struct pfa_kv_evict {
   pfa_kv_pages pages;
   const float* weights;

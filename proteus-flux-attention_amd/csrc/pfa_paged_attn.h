@@ -985,7 +985,8 @@ __global__ void __launch_bounds__(THREADS) join_kernel(Deal deal, int G, int D, 
 // The join and the weights beside it: `joins` workgroups join, as join_kernel's do, the
 // others take four positions a thread and work their rows' statistics out of the parts
 // themselves, which costs less than to wait for the join (32 ragged sequences of up to
-// 16,384 int8 tokens: 85 -> 83 us; 700 tokens of 8 heads: 19 -> 16).  16 rows of a key-value head at most.
+// 16,384 int8 tokens: 85 -> 83 us; 700 tokens of 8 heads: 19 -> 16).  16 rows of a
+// key-value head at most.
 template <int QT, int THREADS>
 __global__ void __launch_bounds__(THREADS) join_weigh_kernel(Deal deal, int G, int D, float c, float pscale,
                                                              const int32_t* __restrict__ lengths,

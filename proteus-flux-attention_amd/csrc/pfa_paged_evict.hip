@@ -514,8 +514,11 @@ extern "C" int pfa_kv_tokens_evict(const pfa_kv_evict* c, void* stream) {
   const int64_t bytes = (int64_t)count * 2 * cells_bytes(c->pages.dtype, c->pages.head_dim);
   const bool small = !p.bounds && count <= kSmall && w.most <= 1024 * 4 && bytes <= kSmallBytes;
   if (!small) choose_launch(keep, B * p.H, kept, s);
-  const int64_t fresh_pages = ((int64_t)count + p.ps - 1) >> p.shift;
-  const dim3 grid((unsigned)(fresh_pages < 65535 ? fresh_pages : 65535), p.H, B);
+  // a workgroup a page, but no more than 4,096 of the weights to each (8 rows of
+  // 1,048,576, two pages of 256 kept: the move takes 330 us with two workgroups a row, 49 so)
+  const int64_t fresh_pages = ((int64_t)count + p.ps - 1) >> p.shift, fills = (n + 4095) / 4096;
+  const int64_t blocks = fresh_pages > fills ? fresh_pages : fills;
+  const dim3 grid((unsigned)(blocks < 65535 ? blocks : 65535), p.H, B);
   by_cells(c->pages.dtype, [&](auto ct) {
     by_width(c->pages.head_dim, [&](auto width) {
       constexpr int CT = decltype(ct)::value, D = decltype(width)::value;

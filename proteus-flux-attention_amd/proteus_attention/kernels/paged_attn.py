@@ -547,10 +547,12 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     Returns the positions that were kept ``(B, kv_heads, count)``, -1 behind the
     last, and their key weights, zeros behind them, in a tensor of
     ``key_weights``' shape: sequences go on with ``into`` for a table, these
-    weights, and ``lengths`` of up to ``count``.  The pages of ``block_table``
-    stay as they are, so that others may share them; no page may be in both
-    tables, or in ``into`` twice.  Tokens for entries of ``into`` that name no page,
-    and those behind its last, are left out.  Keys keep the rotary positions that they were written with.
+    weights, and as many tokens as were kept, ``(kept[:, 0] >= 0).sum(-1)``, for
+    lengths: the lesser of ``lengths[b]`` and ``count`` where every position has a
+    page and a weight.  The pages of ``block_table`` stay as they are, so that others
+    may share them; no page may be in both tables, or in ``into`` twice.  Tokens for
+    entries of ``into`` that name no page, and those behind its last, are left out.
+    Keys keep the rotary positions that they were written with.
     """
 
     count, first, last = _held(count, first, last, "tokens")

@@ -110,7 +110,7 @@ def new_rotary_positions(width: int, *, base: float = 10000.0, interleaved: bool
     length = length if magnitude is None else float(magnitude)
     if not 0.0 < length < math.inf:
         raise ValueError("magnitude must be positive and finite")
-    # a frequency is a whole number of 2^-64 turns, as exactly as 64 bits hold it
+    # a frequency is a whole number of 2^-64 turns: what a double's radians leave, off by 2^-53 of it and half a unit
     turns = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for f in radians]
     turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=device)
     return RotaryPositions(turns, length, bool(interleaved))
