@@ -766,10 +766,11 @@ int pfa_paged_weigh_attn_fwd(const pfa_paged_query* query, float* weights, int64
  * largest weights (B, H, n): kept (B, H, count) int32, ascending, -1 behind the
  * last.  The `first` first and `last` last positions come before all others, then
  * the larger weight, then the lower position; NaN counts below everything, -0 and
- * +0 alike. */
+ * +0 alike.  Rows of more than 65,536 positions need a workspace. */
+int pfa_kv_tokens_workspace_size(int B, int H, int64_t n, size_t* bytes);
 int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int64_t weights_h, int64_t n,
                          int B, int H, const int32_t* lengths, int count, int first, int last,
-                         int32_t* kept, void* stream);
+                         int32_t* kept, void* workspace, size_t ws_bytes, void* stream);
 
 /* That choice among the positions that have a page, and a move: the i-th kept
  * position's cells and scales, of every head, into slot i of the pages that `into`
@@ -777,7 +778,8 @@ int pfa_kv_tokens_select(const float* weights, int64_t weights_b, int64_t weight
  * behind the last.  k_bounds of the new pages, where the pool has them, are those
  * of their kept keys.  Entries of `into` without a page take nothing, and what is
  * behind its last is left out.  No page of `into` may be one of the call's `table`,
- * or named twice: the other pages stay as they are. */
+ * or named twice: the other pages stay as they are.  The workspace is that of the
+ * choice, of n positions or the table's if they are fewer. */
 typedef struct pfa_kv_evict {
   pfa_kv_pages pages;
   const float* weights;
@@ -786,6 +788,8 @@ typedef struct pfa_kv_evict {
   int64_t table_stride, into_stride;
   int32_t* kept;
   float* fresh;
+  void* workspace;
+  size_t ws_bytes;
   int table_pages, into_pages, B, count, first, last;
 } pfa_kv_evict;
 

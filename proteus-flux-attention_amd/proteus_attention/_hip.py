@@ -83,6 +83,7 @@ EXPORTED_SYMBOLS = (
     "pfa_paged_sparse_attn_fwd",
     "pfa_paged_weigh_attn_workspace_size",
     "pfa_paged_weigh_attn_fwd",
+    "pfa_kv_tokens_workspace_size",
     "pfa_kv_tokens_select",
     "pfa_kv_tokens_evict",
     "pfa_rotary",
@@ -188,7 +189,8 @@ _SIGNATURES = {
     "pfa_paged_sparse_attn_fwd": ([_vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _sz, _vp], _i32),
     "pfa_paged_weigh_attn_workspace_size": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_sz)], _i32),
     "pfa_paged_weigh_attn_fwd": ([_vp, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _sz, _vp], _i32),
-    "pfa_kv_tokens_select": ([_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp], _i32),
+    "pfa_kv_tokens_workspace_size": ([_i32, _i32, _i64, ctypes.POINTER(_sz)], _i32),
+    "pfa_kv_tokens_select": ([_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _sz, _vp], _i32),
     "pfa_kv_tokens_evict": ([_vp, _vp], _i32),
     "pfa_rotary": ([_vp, _vp], _i32),
 }

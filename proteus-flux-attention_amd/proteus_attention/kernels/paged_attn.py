@@ -104,7 +104,7 @@ def new_kv_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int, *
 _POOL = struct.Struct("PPPPPqqiiiii4x")
 _TENSOR4 = struct.Struct("Pqqq")
 _QUERY = struct.Struct(_POOL.format + _TENSOR4.format + "PqPPiiii")
-_EVICT = struct.Struct(_POOL.format + "PqqqPPPqqPPiiiiii")
+_EVICT = struct.Struct(_POOL.format + "PqqqPPPqqPPPqiiiiii")
 
 
 def _dense(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, name: str) -> int:
@@ -225,6 +225,13 @@ def _weigh_bytes(*sizes: int) -> int:
     """Workspace of attention that weighs its keys: as of attention, without lists."""
 
     return _size_out(_hip.lib().pfa_paged_weigh_attn_workspace_size, *sizes)
+
+
+@functools.lru_cache(maxsize=256)
+def _tokens_bytes(*sizes: int) -> int:
+    """Workspace of a choice of tokens: rows that one workgroup holds need none."""
+
+    return _size_out(_hip.lib().pfa_kv_tokens_workspace_size, *sizes)
 
 
 def _scratch(nbytes: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
@@ -529,8 +536,9 @@ def select_kv_tokens(key_weights: torch.Tensor, lengths: torch.Tensor, count: in
     lengths = _per_sequence(lengths, B, "lengths")
     index = _device("select_kv_tokens", weights, lengths)
     kept = lengths.new_empty((B, H, count))
+    ws, ws_ptr, ws_bytes = _scratch(_tokens_bytes(B, H, T), weights.device)
     _call(index, "kv_tokens_select", _hip.lib().pfa_kv_tokens_select, weights.data_ptr(), weights.stride(0),
-          weights.stride(1), T, B, H, lengths.data_ptr(), count, first, last, kept.data_ptr())
+          weights.stride(1), T, B, H, lengths.data_ptr(), count, first, last, kept.data_ptr(), ws_ptr, ws_bytes)
     return kept
 
 
@@ -569,9 +577,10 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     kept = table.new_empty((B, Hkv, count))
     fresh = torch.empty_like(weights, memory_format=torch.contiguous_format)
     apart = weights.stride()
+    ws, ws_ptr, ws_bytes = _scratch(_tokens_bytes(B, Hkv, min(T, table.shape[1] * pool[9])), weights.device)
     packed = _EVICT.pack(*pool, weights.data_ptr(), apart[0], apart[1], T, table.data_ptr(), fresh_table.data_ptr(),
                          lengths.data_ptr(), table.stride(0), fresh_table.stride(0), kept.data_ptr(), fresh.data_ptr(),
-                         table.shape[1], fresh_table.shape[1], B, count, first, last)
+                         ws_ptr or 0, ws_bytes, table.shape[1], fresh_table.shape[1], B, count, first, last)
     _call(index, "kv_tokens_evict", _hip.lib().pfa_kv_tokens_evict, packed)
     return kept, fresh
 

@@ -257,6 +257,73 @@ def test_select_tokens(T):
     assert torch.equal(select_kv_tokens(odd, _i32([-5, 10 ** 9, 0]).to(DEV), 5).cpu(), choose(w, [0, T, 0], 5, 1, 1))
 
 
+def choose_long(w, lengths, count, first, last):
+    """choose() of whole rows, by a stable sort of their bits' order."""
+    B, H, T = w.shape
+    u = (w + 0.0).view(torch.int32).long()
+    key = torch.where(w != w, -2 ** 40, torch.where(u < 0, -1 - (u & 0x7fffffff), u))
+    kept = torch.full((B, H, count), -1, dtype=torch.int32)
+    for b in range(B):
+        n = min(max(int(lengths[b]), 0), T)
+        row = key[b, :, :n].clone()
+        row[:, :first] = row[:, max(n - last, 0):] = 2 ** 40
+        take = row.sort(dim=1, descending=True, stable=True).indices[:, :count].sort(1).values
+        kept[b, :, :take.shape[1]] = take.int()
+    return kept
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 1 << 20), (2, 3, 300007), (2, 130, 70001), (1, 40, 262144)], ids=str)
+def test_select_tokens_of_long_rows(shape):
+    """Rows of one to 32 slices: all distinct, few distinct, one value, numbers of either
+    sign and none, the key to cut at in the first, a middle and the last bits."""
+    from proteus_attention import select_kv_tokens
+
+    B, H, T = shape
+    g = torch.Generator().manual_seed(T)
+    lengths = [T, 65000][:B]
+    for kind in range(5):
+        w = torch.rand(shape, generator=g)
+        if kind == 1:
+            w = torch.randint(0, 5, shape, generator=g).float()
+        elif kind == 2:
+            w.fill_(0.25)
+        elif kind == 3:
+            w = torch.exp(20 * torch.randn(shape, generator=g)) * torch.randn(shape, generator=g).sign()
+            w[..., ::7] = math.nan
+            w[..., 1::11], w[..., 2::5] = -0.0, 0.0
+        elif kind == 4:  # neighbours in the last bits
+            w = (torch.randint(0, 3000, shape, generator=g, dtype=torch.int32) + 0x3f000000).view(torch.float32)
+            w[..., 5] = 1e30
+        for count, first, last in ((1, 0, 0), (4096, 4, 64), (T // 3, 1, 1), (T + 9, 0, 1)):
+            got = select_kv_tokens(w.to(DEV), _i32(lengths).to(DEV), count, first=first, last=last).cpu()
+            assert torch.equal(got, choose_long(w, lengths, count, first, last)), (kind, count)
+
+
+def test_evict_from_long_rows():
+    from proteus_attention import evict_kv_tokens
+
+    g = torch.Generator().manual_seed(5)
+    cell, D, H, ps = torch.bfloat16, 16, 2, 256
+    for lengths, count, bounds in (([70000, 300], 66000, True), ([140000], 257, False)):
+        B, N = len(lengths), sum(-(-n // ps) for n in lengths) + len(lengths) * (-(-count // ps)) + 1
+        pool = _pool(cell, N, H, ps, D, g, bounds=bounds)
+        both = R.make_table(lengths + [count] * B, ps, N, g)
+        table, into = both[:B].clone(), both[B:].contiguous()
+        table[0, 7] = -1
+        w = torch.rand(B, H, table.shape[1] * ps, generator=g)
+        have = (torch.arange(w.shape[2]) // ps != 7).expand(B, -1).clone()
+        have[1:] = True
+        kept = choose(w, lengths, count, 2, 5, have)
+        raw = _bytes(cell, pool)
+        want, weights_after = moved(raw, kept, w, table, into, _values(cell))
+        pages = _pages(cell, pool)
+        got, after = evict_kv_tokens(pages, w.to(DEV), table.to(DEV), _i32(lengths).to(DEV), count, into.to(DEV), first=2,
+                                     last=5)
+        assert torch.equal(got.cpu(), kept) and torch.equal(after.cpu(), weights_after)
+        for m in want:
+            assert torch.equal(getattr(pages, m).cpu(), want[m]), m
+
+
 def moved(raw, kept, w, table, into, cells_of):
     """Pool and weights after the move; cells_of(pool, page, head, slots): key values."""
     raw = {m: t.clone() for m, t in raw.items()}

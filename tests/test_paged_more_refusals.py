@@ -125,12 +125,12 @@ def test_c_entries_refuse_before_any_launch():
         return lib.pfa_paged_weigh_attn_fwd(query(**kw), w, 64, 32, n, scale, out, ws, size, None)
 
     def evict(w=256, n=32, B=1, table=256, P=2, lengths=256, count=3, first=1, last=1, into=256, P2=2, kept=256, fresh=256,
-              **kw):
-        return lib.pfa_kv_tokens_evict(struct.pack(_POOL + "PqqqPPPqqPPiiiiii", *_fields(**kw), w, 64, 32, n, table, into,
-                                                   lengths, P, P2, kept, fresh, P, P2, B, count, first, last), None)
+              ws=256, size=1 << 40, **kw):
+        return lib.pfa_kv_tokens_evict(struct.pack(_POOL + "PqqqPPPqqPPPqiiiiii", *_fields(**kw), w, 64, 32, n, table, into,
+                                                   lengths, P, P2, kept, fresh, ws, size, P, P2, B, count, first, last), None)
 
-    def select(w=p, n=32, B=1, H=2, lengths=p, count=3, first=1, last=1, kept=p):
-        return lib.pfa_kv_tokens_select(w, 64, 32, n, B, H, lengths, count, first, last, kept, None)
+    def select(w=p, n=32, B=1, H=2, lengths=p, count=3, first=1, last=1, kept=p, ws=p, size=1 << 40):
+        return lib.pfa_kv_tokens_select(w, 64, 32, n, B, H, lengths, count, first, last, kept, ws, size, None)
 
     bad = [weigh(w=None), weigh(w=ctypes.c_void_p(258)), weigh(n=31), weigh(scale=0.0), weigh(scale=math.nan), weigh(out=None),
            weigh(H=3), weigh(k_scale=0), weigh(k_page=2 * 16 * 32 - 16), weigh(v_page=2 * 16 * 32 + 8), weigh(k=264),
@@ -142,7 +142,15 @@ def test_c_entries_refuse_before_any_launch():
            select(count=0), select(count=-3, first=0, last=0), select(kept=None), select(last=3)]
     assert bad == [-1] * len(bad)
     assert weigh(size=8) == -3 and weigh(ws=ctypes.c_void_p(264)) == -3 and weigh(ws=None) == -3
+    long = dict(n=70000, P=4400)
+    assert [evict(ws=0, **long), evict(ws=264, **long), evict(size=4096, **long)] == [-3] * 3
+    assert [select(n=70000, ws=None), select(n=70000, ws=ctypes.c_void_p(264)), select(n=70000, size=4096)] == [-3] * 3
     size = ctypes.c_size_t(0)
+    assert lib.pfa_kv_tokens_workspace_size(3, 8, 65536, ctypes.byref(size)) == 0 and size.value == 0
+    assert lib.pfa_kv_tokens_workspace_size(3, 8, 65537, ctypes.byref(size)) == 0 and size.value >= 3 * 8 * 2 * 8192
+    assert lib.pfa_kv_tokens_workspace_size(0, 8, 1 << 30, ctypes.byref(size)) == 0 and size.value == 0
+    assert lib.pfa_kv_tokens_workspace_size(1, 8, (1 << 30) + 1, ctypes.byref(size)) == -1
+    assert lib.pfa_kv_tokens_workspace_size(60000, 60, 9, ctypes.byref(size)) == -1
     assert lib.pfa_paged_weigh_attn_workspace_size(1, 4, 2, 16, 64, _hip.PFA_E2M1, 100, ctypes.byref(size)) == 0
     assert size.value >= 4 * 4 * 1600
     assert lib.pfa_paged_weigh_attn_workspace_size(1, 3, 2, 16, 64, _hip.PFA_E2M1, 100, ctypes.byref(size)) == -1
