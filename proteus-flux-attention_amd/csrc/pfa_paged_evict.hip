@@ -318,11 +318,13 @@ __global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Keep k, int32_t*
 // each time: the third leaves single keys); how many of a slice are taken; their
 // places.  A launch adds the slices' bins up in each of its workgroups, a cache's
 // reads (8 KB a slice), and has no atomics in memory and nothing to clear.
-// MEASURED
-constexpr int kSlices = 32;    // of a row, at most
+// 8 rows of 65,536 positions by a workgroup each: 30 us; of 131,072: 87, 46 cut; of
+// 1,048,576: 630, 71 cut, eight to twelve a launch, the bins' sum (256 KB of them) half
+// of it.
+constexpr int kSlices = 32;    // of a row, at most (1,048,576: 85 us with 16, 106 with 64)
 constexpr int kHeld = 65536;   // positions of a row that one workgroup takes
-constexpr int kPieces = 4;     // of a thread at once
-constexpr int kEnough = 512;   // workgroups of a launch: more of them only read one another's bins
+constexpr int kPieces = 2;     // of a thread at once (512 rows of 70,000: 152 us, 164 with 4, 195 with 8)
+constexpr int kEnough = 256;   // workgroups of a launch, where rows are fewer (32 rows of 100,000: 44 us, 56 with 512)
 struct Split {
   int slices, length;  // of a row, and positions of each
   uint4* ranges;       // (rows, slices)

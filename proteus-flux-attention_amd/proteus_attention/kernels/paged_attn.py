@@ -227,11 +227,12 @@ def _weigh_bytes(*sizes: int) -> int:
     return _size_out(_hip.lib().pfa_paged_weigh_attn_workspace_size, *sizes)
 
 
-@functools.lru_cache(maxsize=256)
-def _tokens_bytes(*sizes: int) -> int:
-    """Workspace of a choice of tokens: rows that one workgroup holds need none."""
+def _tokens_scratch(B: int, H: int, T: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    """Workspace of a choice of tokens: only rows of more than 65,536 need one."""
 
-    return _size_out(_hip.lib().pfa_kv_tokens_workspace_size, *sizes)
+    if T <= 65536:
+        return None, 0, 0
+    return _scratch(_size_out(_hip.lib().pfa_kv_tokens_workspace_size, B, H, T), device)
 
 
 def _scratch(nbytes: int, device: torch.device) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
@@ -536,7 +537,7 @@ def select_kv_tokens(key_weights: torch.Tensor, lengths: torch.Tensor, count: in
     lengths = _per_sequence(lengths, B, "lengths")
     index = _device("select_kv_tokens", weights, lengths)
     kept = lengths.new_empty((B, H, count))
-    ws, ws_ptr, ws_bytes = _scratch(_tokens_bytes(B, H, T), weights.device)
+    ws, ws_ptr, ws_bytes = _tokens_scratch(B, H, T, weights.device)
     _call(index, "kv_tokens_select", _hip.lib().pfa_kv_tokens_select, weights.data_ptr(), weights.stride(0),
           weights.stride(1), T, B, H, lengths.data_ptr(), count, first, last, kept.data_ptr(), ws_ptr, ws_bytes)
     return kept
@@ -577,7 +578,7 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     kept = table.new_empty((B, Hkv, count))
     fresh = torch.empty_like(weights, memory_format=torch.contiguous_format)
     apart = weights.stride()
-    ws, ws_ptr, ws_bytes = _scratch(_tokens_bytes(B, Hkv, min(T, table.shape[1] * pool[9])), weights.device)
+    ws, ws_ptr, ws_bytes = _tokens_scratch(B, Hkv, min(T, table.shape[1] * pool[9]), weights.device)
     packed = _EVICT.pack(*pool, weights.data_ptr(), apart[0], apart[1], T, table.data_ptr(), fresh_table.data_ptr(),
                          lengths.data_ptr(), table.stride(0), fresh_table.stride(0), kept.data_ptr(), fresh.data_ptr(),
                          ws_ptr or 0, ws_bytes, table.shape[1], fresh_table.shape[1], B, count, first, last)
