@@ -522,3 +522,76 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for x in got for a, b in zip(x, want))
     assert all(a is None or torch.equal(a, b) for a, b in zip(*own))
+
+
+def test_captured_choice_of_long_rows():
+    from proteus_attention import select_kv_tokens
+
+    g = torch.Generator().manual_seed(10)
+    w, lengths = torch.zeros(2, 2, 70003, device=DEV), _i32([70003, 69000]).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        select_kv_tokens(w, lengths, 5000)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    held = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            held.append(select_kv_tokens(w, lengths, 5000))
+    for t in range(4):
+        w.copy_(torch.rand(w.shape, generator=g) ** (t + 1))
+        want = select_kv_tokens(w, lengths, 5000)
+        torch.cuda.synchronize()
+        graphs[t % 2].replay()
+        graphs[1 - t % 2].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held[0], want) and torch.equal(held[1], want), t
+        lengths -= 17
+
+
+def test_eviction_of_pages_beyond_32_bits():
+    """A pool of more than 2^32 cells, from its last pages to its first and back."""
+    from proteus_attention import KVPages, evict_kv_tokens
+
+    H, ps, D = 2, 256, 128
+    N = (1 << 32) // (H * ps * D) + 30
+    k, v = (torch.empty(N, H, ps, D, dtype=torch.int8, device=DEV) for _ in range(2))
+    scales = [torch.empty(N, H, ps, device=DEV) for _ in range(2)]
+    pages = KVPages(k, v, *scales, torch.empty(N, H, 2, D, device=DEV))
+    g = torch.Generator().manual_seed(11)
+    some = [N - 1, 2, N - 9, 5, N - 3, 1]
+    small = _pool(torch.int8, len(some), H, ps, D, g, bounds=True)
+    for i, page in enumerate(some):
+        for m, t in small.items():
+            getattr(pages, m)[page] = t[i].to(DEV)
+    table, into, lengths, count = _i32([[0, 1], [2, 3]]), _i32([[5], [4]]), [500, 300], 200
+    w = torch.rand(2, H, 2 * ps, generator=g)
+    kept = choose(w, lengths, count, 1, 3)
+    want, fresh = moved(small, kept, w, table, into, _values(torch.int8))
+    names = _i32(some)
+    got, after = evict_kv_tokens(pages, w.to(DEV), names[table.long()].to(DEV), _i32(lengths).to(DEV), count,
+                                 names[into.long()].to(DEV), last=3)
+    assert torch.equal(got.cpu(), kept) and torch.equal(after.cpu(), fresh)
+    for i, page in enumerate(some):
+        for m in want:
+            assert torch.equal(getattr(pages, m)[page].cpu(), want[m][i]), (m, page)
+
+
+@pytest.mark.parametrize("G", [16, 32])
+def test_scores_beyond_32_bits(G):
+    """A workspace of more than 2^32 bytes: the weights of its last sequence's keys."""
+    from proteus_attention import paged_attention
+
+    g = torch.Generator().manual_seed(12)
+    B, D, ps, N = 80, 32, 256, 50
+    T = 1 << 20
+    pool = _pool(torch.bfloat16, N, 1, ps, D, g)
+    table = torch.randint(0, N, (B, T // ps), generator=g, dtype=torch.int32)
+    lengths = [1] * (B - 1) + [T - 5]
+    q = torch.randn(B, G, D, generator=g).bfloat16()
+    before = torch.zeros(B, 1, T, device=DEV)
+    paged_attention(q.to(DEV), _pages(torch.bfloat16, pool), table.to(DEV), _i32(lengths).to(DEV), key_weights=before)
+    assert bool((before[:-1, 0, 0] == G).all()) and not before[:-1, :, 1:].any() and not before[-1, :, T - 5:].any()
+    ref = weights(q[-1:], pool, table[-1:], lengths[-1:])
+    assert holds(before[-1:].cpu(), torch.zeros(1, 1, T), ref, G, D, T)

@@ -204,3 +204,24 @@ def test_captured_and_on_two_streams():
                 got.append(apply_rotary(q, k, pos, rotary))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for x in got for a, b in zip(x, want))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows of a tensor of more than 2^32 elements, in place: the others stay as they are."""
+    from proteus_attention import apply_rotary, new_rotary_positions
+
+    g = torch.Generator().manual_seed(12)
+    B, n, H, D, apart = 3, 5, 2, 64, (1 << 31) + 4096
+    rotary = new_rotary_positions(D, device=DEV)
+    far = torch.empty((B - 1) * apart + 4 * n * H * D, dtype=torch.float16, device=DEV)
+    x = torch.randn(B, n, H, D, generator=g).half()
+    rows = far.as_strided((B, n, H, D), (apart, 2 * H * D, D, 1))
+    between = far.as_strided((B, n, H, D), (apart, 2 * H * D, D, 1), H * D)
+    rows.copy_(x)
+    between.fill_(7.0)
+    positions = torch.tensor([5, 2 ** 31 - 9, -4], dtype=torch.int32)
+    every = positions.long()[:, None] + torch.arange(n)
+    out, _ = apply_rotary(rows, None, positions.to(DEV), rotary)
+    assert holds(out, x, every, rotary)
+    apply_rotary(rows, None, positions.to(DEV), rotary, inplace=True)
+    assert torch.equal(rows, out) and bool((between == 7.0).all())
