@@ -318,9 +318,9 @@ __global__ void __launch_bounds__(THREADS) choose_tokens_kernel(Keep k, int32_t*
 // each time: the third leaves single keys); how many of a slice are taken; their
 // places.  A launch adds the slices' bins up in each of its workgroups, a cache's
 // reads (8 KB a slice), and has no atomics in memory and nothing to clear.
-// 8 rows of 65,536 positions by a workgroup each: 30 us; of 131,072: 87, 46 cut; of
-// 1,048,576: 630, 71 cut, eight to twelve a launch, the bins' sum (256 KB of them) half
-// of it.
+// 8 rows of 65,536 positions by a workgroup each: 32 us, cut 37 (128 rows: 34 and 58);
+// of 131,072, which one workgroup has to read again each time: 87, 46 cut; of 1,048,576:
+// 630, 71 cut, eight to twelve a launch, the bins' sum (256 KB of them) half of it.
 constexpr int kSlices = 32;    // of a row, at most (1,048,576: 85 us with 16, 106 with 64)
 constexpr int kHeld = 65536;   // positions of a row that one workgroup takes
 constexpr int kPieces = 2;     // of a thread at once (512 rows of 70,000: 152 us, 164 with 4, 195 with 8)
