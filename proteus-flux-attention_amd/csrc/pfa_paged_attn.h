@@ -130,6 +130,12 @@ struct Form {
   // waves of a SIMD, at least, that the registers leave without spills (f16 queries on
   // 1,000,003 4-bit tokens of 128 channels: 135 us with three, 126 with two)
   static constexpr int AT_LEAST = D == 128 && (QT == PFA_F32 || (is4(CT) && QT == PFA_F16)) ? 2 : 3;
+  // Whether a wave that keeps scores holds those of some tiles back in LDS: a wait for
+  // loads waits for the stores before them, too.  32 ragged sequences of up to 16,384
+  // tokens, int8 of 128 channels: 82.3 -> 80.1 us, bf16 of 64 76.6 -> 73.9.  Elsewhere
+  // it takes registers that are not there (4 bits of 128: 64.9 -> 68.1, bf16 of 128:
+  // 121.4 -> 126.8) or a wave of a SIMD.
+  static constexpr bool HOLDS = NG == 1 && (D < 128 || is8(CT));
   static constexpr float PSCALE = F16 ? 32768.0f : 1.0f;
 };
 
@@ -329,12 +335,12 @@ struct Wave {
   // keys, P, and O.  The next keys are loaded whether or not there is a next tile
   // (`next` is this one then): a load under a condition would have the wait for V
   // wait for them, too.
-  // With KEEP it stores the scores to `scores_at`, if that is anywhere: the lane's place
-  // of 16 keys' scores of `score_rows` rows.
+  // With KEEP it leaves the scores of `score_rows` rows, 16 keys of all rows together:
+  // HOLDS in `kept`, LDS, and those keys' positions in `kept_at`, else in the workspace,
+  // of whose rows `kept` is the lane's place, if it has one.
   template <bool KEEP>
   __device__ __forceinline__ void step(const Pages& pg, const Row& r, int h, float c, const Tile<F>& t,
-                                       const Tile<F>& next, State<F>& st, float* __restrict__ scores_at,
-                                       int score_rows) {
+                                       const Tile<F>& next, State<F>& st, float* kept, int* kept_at, int score_rows) {
     uint32_t v[2 * F::NG][4][F::VW];
     f32x4_t s[2 * F::NG], vs[2 * F::NG];
     [[maybe_unused]] uint32_t raw[2 * F::NG][F::NS];  // V's scales of 4-bit cells: four keys'
@@ -362,9 +368,15 @@ struct Wave {
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (KEEP) {
 #pragma unroll
-      for (int i = 0; i < 2 * F::NG; ++i)
-        if (scores_at && t.b[i].pos < kNowhere)
-          *reinterpret_cast<f32x4_t*>(scores_at + (int64_t)t.b[i].pos * score_rows) = s[i];
+      for (int i = 0; i < 2 * F::NG; ++i) {
+        if constexpr (F::HOLDS) {
+          if (n < score_rows) *reinterpret_cast<f32x4_t*>(kept + (i * score_rows + n) * 16 + 4 * g) = s[i];
+          if (n == 0 && g == 0) kept_at[i] = t.b[i].pos;
+        } else {
+          if (kept && t.b[i].pos < kNowhere)
+            *reinterpret_cast<f32x4_t*>(kept + (int64_t)t.b[i].pos * score_rows) = s[i];
+        }
+      }
     }
     if constexpr (is4(F::CT)) {
       // byte y * NS + (the lane's group) of the four keys', turned to where an f32 has its
@@ -540,7 +552,7 @@ struct Weigh {
   int vec;         // rows are aligned to four
   // (pairs, cap / 16, rows, 16): the products, before the scale.  16 keys of all rows lie
   // together, which is what a wave stores at once: 1,000,003 int8 tokens of four heads,
-  // eight query heads each, 310 us with a row in one piece, 297 so (200 without weights).
+  // eight query heads each, 310 us with a row in one piece, 295 so (200 without weights).
   float* scores;
   int64_t cap;
   int rows;        // of a pair
@@ -616,10 +628,15 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Between what lanes of a wave leave in LDS and what others of it read: an order, no wait.
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 // What a call does beside attending.  SELECT: the workgroup first selects its pair's
 // pages itself, for a launch and several dependent loads less.  WEIGH: it keeps the
 // scores, and where a workgroup has all of a key's rows it adds their weights itself.
 enum class Also { NOTHING, SELECT, WEIGH };
+
+constexpr int kKept = 8;  // tiles whose scores a wave holds back, at most
 
 template <typename F, Also ALSO>
 __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
@@ -630,7 +647,11 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     Choice choice, Weigh weigh) {
   constexpr int D = F::D;
   constexpr bool SELECT = ALSO == Also::SELECT, WEIGH = ALSO == Also::WEIGH;
-  __shared__ float so[kWaves][16][D + 4];
+  constexpr bool HOLDS = WEIGH && F::HOLDS;
+  // a wave's O, and before that the scores of some of its tiles
+  __shared__ __attribute__((aligned(16))) float so[kWaves][16][D + 4];
+  static_assert(!HOLDS || D + 4 >= F::TILE, "a tile's scores of 16 rows");
+  __shared__ int kept_at[HOLDS ? kWaves : 1][HOLDS ? kKept * 2 * F::NG : 1];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ Entry entries[kEntries + 1];
   __shared__ int64_t sums[kWaves];
@@ -775,9 +796,26 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     const int here = (h + 1) * G - row0 < 16 ? (h + 1) * G - row0 : 16;
 
     w.load_q(q + b * q_b + (row0 + w.n) * q_h, w.n < here, q_vec);
-    float* scores_at = nullptr;
-    if (WEIGH && w.n < here)
-      scores_at = weigh.scores + ((int64_t)b * deal.R + pair) * weigh.cap * weigh.rows + 16 * w.n + 4 * w.g;
+    float* scores = nullptr;
+    if constexpr (WEIGH) {
+      scores = weigh.scores + ((int64_t)b * deal.R + pair) * weigh.cap * rows;
+      if (!HOLDS) scores = w.n < here ? scores + 16 * w.n + 4 * w.g : nullptr;
+    }
+    int kept = 0;  // tiles that are held back
+    const int tile_kept = F::TILE * rows, room = 16 * (D + 4) / tile_kept;
+    auto put_out = [&]() {
+      wave_fence();
+      const float* from = &so[wave][0][0];
+      const int each = 4 * rows, inverse = ((1 << 20) + each - 1) / each;  // quotients of up to 2,048
+      for (int u = lane; u < kept * 2 * F::NG * each; u += kWave) {
+        const int block = u * inverse >> 20, pos = kept_at[wave][block];
+        if (pos < kNowhere)
+          *reinterpret_cast<f32x4_t*>(scores + (int64_t)pos * rows + 4 * (u - block * each)) =
+              *reinterpret_cast<const f32x4_t*>(from + 4 * u);
+      }
+      wave_fence();
+      kept = 0;
+    };
     State<F> st;
 #pragma unroll
     for (int j = 0; j < F::VD; ++j) st.o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -818,9 +856,16 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
           Tile<F> found;
           t = found.find_seen(r, t + kWaves, re);
           if (t < re) next = found;
-          w.template step<WEIGH>(pg, r, h, c, cur, next, st, scores_at, weigh.rows);
+          if constexpr (HOLDS) {
+            w.template step<true>(pg, r, h, c, cur, next, st, &so[wave][0][0] + kept * tile_kept,
+                                  &kept_at[wave][kept * 2 * F::NG], rows);
+            if (++kept == kKept || kept == room) put_out();
+          } else {
+            w.template step<WEIGH>(pg, r, h, c, cur, next, st, scores, nullptr, rows);
+          }
           cur = next;
         }
+        if (HOLDS && kept) put_out();
       }
     }
 
