@@ -565,14 +565,18 @@ __device__ __forceinline__ float2 row_stats(float m, float l) {
   return make_float2(m == -INFINITY ? 0.0f : m, l == 0.0f ? 0.0f : 1.0f / l);
 }
 
-// Adds the weights of positions first, first + 4 * step, ... before `len`, four at a
-// time, of the G rows of a key-value head in their order: the same bits every time.
+// Adds the weights of the positions [start, len), of the G rows of a key-value head in
+// their order: the same bits every time.  A thread takes four neighbours of every
+// 4 * step, the first of them `unit` fours behind the four that hold the start.  A start
+// may be any number of 32 bits: at or behind the length there is nothing to add, and 4 *
+// unit more than it is a number of 64.
 template <typename Stats>
 __device__ __forceinline__ void add_weights(const Weigh& w, const Pages& pg, const int32_t* __restrict__ ids, int b, int h,
-                                            int G, float c, int start, int len, int64_t first, int step, Stats&& stats) {
+                                            int G, float c, int start, int len, int64_t unit, int step, Stats&& stats) {
+  if (start >= len) return;
   float* to = w.weights + b * w.s_b + h * w.s_h;
   const int pairs = (G + 15) / 16;
-  for (int64_t p = first; p < len; p += 4 * step) {
+  for (int64_t p = (start & ~3) + 4 * unit; p < len; p += 4 * (int64_t)step) {
     if ((uint32_t)ids[p >> pg.shift] >= (uint32_t)pg.n_pages) continue;
     float sum[4] = {};
     for (int g0 = 0; g0 < G; g0 += 16) {
@@ -608,11 +612,9 @@ static __global__ void __launch_bounds__(256) weigh_kernel(Weigh w, Pages pg, co
                                                            const int32_t* __restrict__ starts) {
   const int b = blockIdx.z, h = blockIdx.y;
   const int len = length_at(lengths, P, pg.shift, b), start = start_at(starts, b);
-  if (start >= len) return;
   const int64_t row = ((int64_t)b * pg.H + h) * G;
-  const int64_t first = (start & ~3) + 4 * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
-  add_weights(w, pg, table + b * table_stride, b, h, G, c, start, len, first, (int)(gridDim.x * blockDim.x),
-              [&](int g) { return w.stats[row + g]; });
+  add_weights(w, pg, table + b * table_stride, b, h, G, c, start, len, (int64_t)blockIdx.x * blockDim.x + threadIdx.x,
+              (int)(gridDim.x * blockDim.x), [&](int g) { return w.stats[row + g]; });
 }
 
 // What paged_sparse_attention chooses before it attends.
@@ -913,8 +915,7 @@ __global__ void __launch_bounds__(64 * kWaves, F::AT_LEAST) attend_kernel(
     if (lone) {
       if (WEIGH && deal.RT == 1) {
         __syncthreads();  // the scores are in memory
-        add_weights(weigh, pg, ids, b, h, G, c, start, len, (start & ~3) + 4 * tid, 64 * kWaves,
-                    [&](int g) { return stats[g]; });
+        add_weights(weigh, pg, ids, b, h, G, c, start, len, tid, 64 * kWaves, [&](int g) { return stats[g]; });
       }
       return;
     }
@@ -1049,8 +1050,8 @@ __global__ void __launch_bounds__(THREADS) join_weigh_kernel(Deal deal, int G, i
   }
   const int block = (int)blockIdx.x - joins, pair = block / pieces, b = pair / pg.H, h = pair % pg.H;
   const int len = deal.length(lengths, b), start = start_at(starts, b);
-  const int64_t first = (start & ~3) + 4 * (int64_t)(block % pieces) * THREADS;
-  if (start >= len || first >= len) return;  // a row without tiles has no parts
+  const int64_t first = (int64_t)(block % pieces) * THREADS;  // of the workgroup, in units of four positions
+  if (start >= len || (start & ~3) + 4 * first >= len) return;  // a row without tiles has no parts
   const int64_t row0 = (int64_t)pair * G;
   __shared__ float2 stats[16];
   const Shared who = shared[pair];
@@ -1075,7 +1076,7 @@ __global__ void __launch_bounds__(THREADS) join_weigh_kernel(Deal deal, int G, i
     if (lane == 0) stats[g] = row_stats(m, l);
   }
   __syncthreads();
-  add_weights(w, pg, table + b * table_stride, b, h, G, c, start, len, first + 4 * threadIdx.x, pieces * THREADS,
+  add_weights(w, pg, table + b * table_stride, b, h, G, c, start, len, first + threadIdx.x, pieces * THREADS,
               [&](int g) { return stats[g]; });
 }
 

@@ -1,0 +1,45 @@
+"""Key weights and evictions at the ends of what their calls allow, on the GPU against
+plain torch on the CPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import four_bits_reference as F
+import paged_reference as R
+from test_gpu_key_weights import DEV, _i32, _pages, _plain, _pool, holds, weights
+
+pytestmark = pytest.mark.gpu
+
+# what sees nothing: at the length, behind it, and the last starts of 32 bits, from which
+# a workgroup's 1,024 positions leave them
+NOTHING = [0, 1, 2 ** 31 - 1, 2 ** 31 - 4, 2 ** 31 - 1020, 2 ** 31 - 1024, 2 ** 31 - 1025, 2 ** 30]
+
+
+@pytest.mark.parametrize("pair", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.int8), (torch.float16, F.FP4)],
+                         ids=R.pair_id)
+@pytest.mark.parametrize("longest", [300, 4500])  # a workgroup a pair, and rows shared out
+@pytest.mark.parametrize("G", [1, 4, 18])
+def test_starts_that_see_nothing(pair, longest, G):
+    """Beside rows that see keys: output rows of zeros, weights that keep their bits."""
+    from proteus_attention import paged_attention
+
+    dt, cell = pair
+    g = torch.Generator().manual_seed(G)
+    H, D, ps = 2, 64, 16
+    lengths = [longest, 40] + [min(longest, 90 + 7 * i) for i in range(len(NOTHING))] + [33, 33, 10 ** 9]
+    starts = [3, -2 ** 31] + [n if n > 1 else lengths[2 + i] + n for i, n in enumerate(NOTHING)] + [32, 33, 2 ** 31 - 2]
+    N = sum(-(-min(n, longest) // ps) for n in lengths) + 1
+    table = R.make_table([min(n, longest) for n in lengths], ps, N, g)
+    pool = _pool(cell, N, H, ps, D, g)
+    q = torch.randn(len(lengths), H * G, D, generator=g).to(dt)
+    ref = weights(q, _plain(cell, pool), table, lengths, starts)
+    before = torch.rand(len(lengths), H, table.shape[1] * ps, generator=g)
+    w, wide = before.to(DEV), torch.zeros(*before.shape[:2], before.shape[2] + 1, device=DEV)[..., 1:].copy_(before)
+    args, kw = (q.to(DEV), _pages(cell, pool), table.to(DEV), _i32(lengths).to(DEV)), dict(starts=_i32(starts).to(DEV))
+    out = paged_attention(*args, key_weights=w, **kw)
+    assert torch.equal(out, paged_attention(*args, key_weights=wide, **kw)) and torch.equal(out, paged_attention(*args, **kw))
+    blind = [b for b, (s, n) in enumerate(zip(starts, lengths)) if s >= min(n, table.shape[1] * ps)]
+    assert len(blind) == len(NOTHING) + 2 and not out[blind].any() and bool(out[[0, 1, -3]].any(-1).all())
+    assert torch.equal(w[blind].cpu(), before[blind]) and torch.equal(w, wide)
+    assert holds(w.cpu(), before, ref, G, D, longest)
