@@ -38,6 +38,7 @@ struct Call {
   const uint64_t* turns;
   const int32_t* positions;
   int64_t pos_b, pos_t, n;
+  int64_t from;  // a launch's first token
   int per_token;
   int H[2];
   int width, D;
@@ -74,7 +75,7 @@ struct Share {
 
   __device__ __forceinline__ explicit Share(const Call& a) {
     b = blockIdx.y, h0 = blockIdx.z * a.heads;
-    t0 = (int64_t)blockIdx.x * a.tile;
+    t0 = a.from + (int64_t)blockIdx.x * a.tile;
     tokens = a.n - t0 < a.tile ? (int)(a.n - t0) : a.tile;
     heads = a.H[0] + a.H[1] - h0 < a.heads ? a.H[0] + a.H[1] - h0 : a.heads;
     rows = tokens * heads;
@@ -256,11 +257,16 @@ void launch(Call a, int B, bool halves, bool vec, hipStream_t stream) {
   a.inverse = ((1u << 20) + a.heads - 1) / a.heads;
   const int64_t lanes = (tile * a.heads) << a.shift;
   const int threads = lanes >= kThreads ? kThreads : (int)((lanes + kWave - 1) / kWave * kWave);
-  const dim3 grid((unsigned)((a.n + tile - 1) / tile), B, (heads + a.heads - 1) / a.heads);
   const size_t lds = (size_t)tile * half * sizeof(float2);
-  if (!vec) pairs_kernel<DT><<<grid, threads, lds, stream>>>(a, halves);
-  else if (halves) rows_kernel<DT, true><<<grid, threads, lds, stream>>>(a);
-  else rows_kernel<DT, false><<<grid, threads, lds, stream>>>(a);
+  // a grid has fewer than 2^32 threads along x: from 2^24 workgroups on, several launches
+  const int64_t all = (a.n + tile - 1) / tile, once = (1ll << 32) / threads - 1;
+  for (int64_t at = 0; at < all; at += once) {
+    a.from = at * tile;
+    const dim3 grid((unsigned)(all - at < once ? all - at : once), B, (heads + a.heads - 1) / a.heads);
+    if (!vec) pairs_kernel<DT><<<grid, threads, lds, stream>>>(a, halves);
+    else if (halves) rows_kernel<DT, true><<<grid, threads, lds, stream>>>(a);
+    else rows_kernel<DT, false><<<grid, threads, lds, stream>>>(a);
+  }
 }
 
 }  // namespace
