@@ -569,7 +569,7 @@ def evict_kv_tokens(pages: KVPages, key_weights: torch.Tensor, block_table: torc
     Hkv = pool[8]
     B = block_table.shape[0] if block_table.dim() else 0
     table, fresh_table = _table(block_table, B), _table(into, B)
-    if B and table.data_ptr() == fresh_table.data_ptr():
+    if table.numel() and table.data_ptr() == fresh_table.data_ptr():  # empty ones have no address
         raise ValueError("into must name other pages than block_table")
     weights = _dense_rows(_key_weights(key_weights, B, Hkv, "evict_kv_tokens"))
     T = weights.shape[2]

@@ -43,3 +43,13 @@ def test_starts_that_see_nothing(pair, longest, G):
     assert len(blind) == len(NOTHING) + 2 and not out[blind].any() and bool(out[[0, 1, -3]].any(-1).all())
     assert torch.equal(w[blind].cpu(), before[blind]) and torch.equal(w, wide)
     assert holds(w.cpu(), before, ref, G, D, longest)
+
+
+def test_eviction_from_no_pages_into_none():
+    from proteus_attention import evict_kv_tokens, new_kv_pages
+
+    pages = new_kv_pages(4, 2, 16, 32, bounds=True, device=DEV)
+    none, w = torch.zeros(2, 0, dtype=torch.int32, device=DEV), torch.ones(2, 2, 40, device=DEV)
+    kept, fresh = evict_kv_tokens(pages, w, none, _i32([5, 0]).to(DEV), 9, none)
+    assert kept.shape == (2, 2, 9) and bool((kept == -1).all()) and fresh.shape == w.shape and not fresh.any()
+    assert not any(t.any() for t in pages if t is not None)
