@@ -593,9 +593,16 @@ __global__ void __launch_bounds__(256) move_kernel(Pages pg, Table from, Table t
 // Both in one workgroup for a few rows without bounds, with the kept positions in LDS: a
 // launch less, which is 3.6 us of the host (8 rows of 700 positions, 512 kept, 256 bytes
 // each: 15.4 us a call, 11.8 so).  One unit moves 128 KB in 4 us; with more of it than
-// kSmallBytes the launch is the cheaper.
+// kSmallBytes the launch is the cheaper.  It also fills the weights behind the kept ones,
+// which may be many more than the table has positions: beyond kSmallFill of them the launch
+// is the cheaper where rows leave units free (8 rows, 4,096 positions, weights of 16,384:
+// 12.6 us in one launch, 12.9 in two; of 65,536 18.3 and 13.1; of 1,048,576 130 and 18.5;
+// 64 rows of 1,048,576: 132 and 70), but not from kSmallRows on (128 rows of 32,768: 15.0
+// and 19.2, of 1,048,576 136 and 137; 512 rows: 26.4 and 44.5, 396 and 523).
 constexpr int kSmall = 1024;
 constexpr int64_t kSmallBytes = 256 << 10;
+constexpr int64_t kSmallFill = 16384;
+constexpr int kSmallRows = 128;
 template <int CT, int D>
 __global__ void __launch_bounds__(1024) evict_kernel(Keep k, Pages pg, Table to, int32_t* __restrict__ kept,
                                                      float* __restrict__ fresh) {
@@ -739,7 +746,8 @@ extern "C" int pfa_kv_tokens_evict(const pfa_kv_evict* c, void* stream) {
   const Weights w{weights, c->weights_b, c->weights_h, (int)n, (int)(held < n ? held : n), vec};
   const Keep keep{w, from, p.shift, p.n_pages, p.H, c->lengths, count, c->first, c->last};
   const int64_t bytes = (int64_t)count * 2 * cells_bytes(c->pages.dtype, c->pages.head_dim);
-  const bool small = !p.bounds && count <= kSmall && w.most <= 1024 * 4 && bytes <= kSmallBytes;
+  const bool small = !p.bounds && count <= kSmall && w.most <= 1024 * 4 && bytes <= kSmallBytes &&
+                     (n <= kSmallFill || B * p.H >= kSmallRows);
   if (!small)
     if (int rc = choose_launch("kv_tokens_evict", keep, B * p.H, kept, c->workspace, c->ws_bytes, s)) return rc;
   // a workgroup a page, but no more than 4,096 of the weights to each (8 rows of
