@@ -2,6 +2,8 @@
 plain torch on the CPU."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -98,3 +100,74 @@ def test_weights_far_wider_than_the_table(shape):
     pool = _pool(torch.bfloat16, N, H, ps, D, g)
     w = torch.rand(B, H, T, generator=g) + 1.0
     evicts(torch.bfloat16, pool, table, into, w, lengths, count, 1, 3)
+
+
+def _odd_rows(w):
+    """w on the device, rows off a 16-byte line and heads apart by a stride of their own."""
+    B, H, T = w.shape
+    return torch.zeros(H, B, T + 2, device=DEV).transpose(0, 1)[..., 1:T + 1].copy_(w)
+
+
+@pytest.mark.parametrize("cell", [torch.float32, torch.bfloat16, torch.int8, torch.float8_e4m3fn, F.FP4], ids=str)
+@pytest.mark.parametrize("kind", ["one launch", "two", "bounds"])
+@pytest.mark.parametrize("more", [5, -7, 0])
+def test_weights_that_the_table_does_not_fit(cell, kind, more):
+    """Weights of more positions than the table has, and of fewer, with lengths beyond
+    them: what has no weight is not kept, and `last` counts from the last that has one."""
+    g = torch.Generator().manual_seed(17)
+    ps, D, H = 16, 32, 2
+    count = 70 if kind != "two" else 1100
+    lengths = [10 ** 9, 200, 37] if kind != "two" else [10 ** 9, 1500, 300]
+    P = 25 if kind != "two" else 110
+    pages = -(-count // ps)
+    N = 3 * (P + pages)
+    both = torch.randperm(N, generator=g).to(torch.int32)
+    table, into = both[:3 * P].view(3, P).clone(), both[3 * P:].view(3, pages).clone()
+    table[0, 2], table[1, P - 1], table[2, 1], into[1, 1] = -1, -1, N, -1
+    pool = _pool(cell, N, H, ps, D, g, bounds=kind == "bounds")
+    T = P * ps + more
+    w = torch.rand(3, H, T, generator=g)
+    w[:, :, 3::7] = 0.25
+    w[0, 0, 40:60], w[1, 1, ::3], w[0, 1, -1], w[2] = math.nan, math.nan, math.inf, -w[2]
+    for last in (0, 9):
+        for before in (None, _odd_rows(w)):
+            kept = evicts(cell, pool, table, into, w, lengths, count, 2, last, before)
+            assert int(kept.max()) < min(T, P * ps)
+            if last and more < 0:  # the last of the clamped length
+                assert kept[0, 0, -1] == T - 1 and (kept[0, 0, -last:] >= T - last).all()
+
+
+@pytest.mark.parametrize("more", [0, 5, -7])
+def test_long_weights_that_the_table_does_not_fit(more):
+    """Rows that are cut in slices, with pages that are gone."""
+    g = torch.Generator().manual_seed(23)
+    ps, D, H, P, count = 256, 16, 2, 275, 700
+    pages = 3
+    N = P + pages + 1
+    both = torch.randperm(N, generator=g).to(torch.int32)
+    table, into = both[:P].view(1, P).clone(), both[P:P + pages].view(1, pages)
+    table[0, 40], table[0, 3] = -1, N
+    pool = _pool(torch.bfloat16, N, H, ps, D, g, bounds=True)
+    T = P * ps + more
+    w = torch.rand(1, H, T, generator=g)
+    w[0, 0, 9000:9500], w[0, 1, ::2], w[0, 0, 70001] = math.nan, 0.75, -1.0
+    for before in (None, _odd_rows(w)):
+        evicts(torch.bfloat16, pool, table, into, w, [2 ** 31 - 1], count, 4, 11, before)
+
+
+@pytest.mark.parametrize("cell", [torch.float32, torch.bfloat16, torch.float16, torch.int8, torch.float8_e4m3fn, F.FP4], ids=str)
+def test_keys_that_are_not_numbers_move_with_their_bounds(cell):
+    g = torch.Generator().manual_seed(29)
+    ps, D, H, N = 16, 64, 2, 8
+    pool = _pool(cell, N, H, ps, D, g, bounds=True)
+    table, into = _i32([[3, 0, 6]]), _i32([[1, 5]])
+    if cell == F.FP4:
+        pool["k_scale"][3, 0, 2, 1] = pool["v_scale"][6, 1, 3, 0] = 255
+    elif cell in R.TOP:
+        pool["k_scale"][3, 0, 2] = pool["v_scale"][6, 1, 3] = math.nan
+    else:
+        pool["k"][3, 0, 2, 7], pool["v"][6, 1, 3, 0], pool["k"][6, 0, 1, 9] = math.nan, math.nan, -math.inf
+    w = torch.rand(1, H, 3 * ps, generator=g)
+    w[0, 0, 2], w[0, 0, 2 * ps + 1] = 9.0, 8.0  # kept, in the first fresh page and the second
+    kept = evicts(cell, pool, table, into, w, [40], 20, 0, 3)
+    assert 2 in kept[0, 0].tolist()
