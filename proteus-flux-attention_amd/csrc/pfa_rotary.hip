@@ -8,18 +8,19 @@
 // Angles.  A frequency comes as turns a position, w / 2 pi, in units of 2^-64: the
 // product with the position, modulo 2^64, is the angle's fraction of a turn, exactly,
 // at any position of 32 bits.  No table of positions is read, and none limits them.
-// The fraction's first three bits give the octant; what is left, at most pi / 4, is
-// rounded to f32 once, and its sine and cosine are their Taylor series, cut off where
-// the next term is below 2^-25 of the value (x^11 / 11! and x^12 / 12! at pi / 4: 2^-29
-// and 2^-33).
+// The nearest quarter turn is taken off exactly; what is left, pi / 4 at most to either
+// side, is rounded to f32 as a fraction and once more as an angle, and its sine and cosine
+// are their Taylor series, cut off where the next term is below 2^-25 of the value (x^11 /
+// 11! and x^12 / 12! at pi / 4: 2^-29 and 2^-33).
 //
 // Bytes bound it: every value is read and written once.  A workgroup takes some tokens
 // of a sequence and computes their sines and cosines into LDS once for all heads, with
 // its first rows already on their way.  65,536 f16 tokens of 16 heads of 64, a fused
-// projection's slices (268 MB): 48 us, 5.6 TB/s, where a copy of them takes 55; lanes
-// that hold both units of a pair, and channels that stay in lanes with half the work:
-// 117.  128 tokens of 40 heads of 128: 4.6 us, one of 16 heads of 64: 2.5, both the
-// chain of position, sine, LDS and store.
+// projection's slices (268 MB): 43 to 44 us on two sets in turn, of which the last-level
+// cache holds a part (6.1 TB/s, where a copy of them takes 55 us); lanes that hold both
+// units of a pair, and channels that stay in lanes with half the work: 117.  128 tokens
+// of 40 heads of 128: 4.2 us, one of 16 heads of 64: 2.5, both the chain of position,
+// sine, LDS and store.
 #include <type_traits>
 
 #include "pfa_common.h"
