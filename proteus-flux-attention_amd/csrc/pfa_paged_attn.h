@@ -38,18 +38,19 @@
 // times as many results of bf16 queries, or of f16 queries on 8-bit cells, on the
 // other side of their rounding, and take the same time (1,000,003 int8 tokens: 201
 // us a call with two, 202 with three): the loads are what is waited for.  4-bit cells
-// are near what the arithmetic takes (118 us for 124 with two of them).  Sums,
-// maxima and O are f32 throughout.
+// are near what the arithmetic takes (1,000,003 tokens: 115 us a call with two, 117.5 with
+// three; 64 ragged sequences: 39.8 and 41.2).  Sums, maxima and O are f32 throughout.
 //
-// Measured (one MI355X, a large copy at 4.7 to 5.1 TB/s): 1,000,003 tokens of 4 heads
-// of 128, 8 query heads each: int8 190 us, 5.5 TB/s, 4 bits 104 us, 5.2 TB/s; 64 ragged
-// sequences of up to 16,384 4-bit tokens of 8 heads of 128, 4 query heads each: 35 us,
-// 3.5 TB/s; 24 windows of up to 6,000 f32 tokens
+// Measured (one MI355X, a large copy at 4.7 to 5.1 TB/s; this kernel alone, averages of 20
+// launches): 1,000,003 tokens of 4 heads of 128, 8 query heads each: int8 191 us, 5.5
+// TB/s, 4 bits 108 us, 5.0 TB/s; 64 ragged sequences of up to 16,384 4-bit tokens of 8
+// heads of 128, 4 query heads each: 37 us, 3.3 TB/s; 24 windows of up to 6,000 f32 tokens
 // of 8 heads of 64: 75 us, 5.0 TB/s; 64 ragged sequences of up to 8,192 bf16 tokens of
-// 8 heads of 128, 4 query heads each: 57 us, 4.3 TB/s; 8 heads of 64 over 173 tokens:
-// 8 us, of which the launch and four loads one behind the other (length, table, key,
+// 8 heads of 128, 4 query heads each: 59 us, 4.2 TB/s; 8 heads of 64 over 173 tokens:
+// 7 to 8 us, of which the launch and four loads one behind the other (length, table, key,
 // value) are nearly all.  A key at a time with a lane exchange for its score, as these
-// kernels began: 1,150,000, 7,400 and 13,700 us.
+// kernels began, a million int8 tokens, the windows and the ragged bf16: 1,150,000, 7,400
+// and 13,700 us.
 #pragma once
 
 #include "pfa_paged.h"
@@ -127,8 +128,13 @@ struct Form {
   static constexpr int VW = VB < 4 ? 1 : VB / 4;
   static constexpr int NG = tile_groups(CT, D);  // 32-key groups that a wave loads at once
   static constexpr int TILE = 32 * NG;
-  // waves of a SIMD, at least, that the registers leave without spills (f16 queries on
-  // 1,000,003 4-bit tokens of 128 channels: 135 us with three, 126 with two)
+  // Waves of a SIMD, at least: three, but two where three would spill what a tile reads
+  // (f16 queries on 1,000,003 4-bit tokens of 128 channels: 135 us a call with three, 126
+  // with two).  bf16 queries on 4-bit cells of 128 channels spill 8 bytes a lane at three,
+  // 32 where scores are kept, none at two: 1,000,003 tokens 118.5 us with three, 121.5 with
+  // two, 64 ragged sequences 41.5 and 42.0; with weights 192 and 188, 32 ragged sequences
+  // 54.4 and 54.0.  f16 cells of 128 channels spill 8 where scores are kept: 32 ragged
+  // sequences with weights 133 with three, 140 with two, 400,003 tokens 207 and 221.
   static constexpr int AT_LEAST = D == 128 && (QT == PFA_F32 || (is4(CT) && QT == PFA_F16)) ? 2 : 3;
   // Whether a wave that keeps scores holds those of some tiles back in LDS: a wait for
   // loads waits for the stores before them, too.  32 ragged sequences of up to 16,384
