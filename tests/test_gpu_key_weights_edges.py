@@ -171,3 +171,85 @@ def test_keys_that_are_not_numbers_move_with_their_bounds(cell):
     w[0, 0, 2], w[0, 0, 2 * ps + 1] = 9.0, 8.0  # kept, in the first fresh page and the second
     kept = evicts(cell, pool, table, into, w, [40], 20, 0, 3)
     assert 2 in kept[0, 0].tolist()
+
+
+@pytest.mark.parametrize("cell", [torch.float32, torch.bfloat16, torch.int8, torch.float8_e4m3fn, F.FP4], ids=str)
+@pytest.mark.parametrize("bounds", [False, True])
+def test_pools_and_tables_with_strides(cell, bounds):
+    """k and v side by side in one tensor, tables that are columns of a wider one: the bits
+    of dense ones, and nothing else written."""
+    from proteus_attention import evict_kv_tokens, paged_attention
+
+    g = torch.Generator().manual_seed(31)
+    ps, D, H, N, count = 16, 32, 2, 40, 37
+    pool = _pool(cell, N, H, ps, D, g, bounds=bounds)
+    both = torch.randperm(N, generator=g).to(torch.int32).view(2, 20).to(DEV)
+    table, into, lengths = both[:, 2:14], both[:, 15:18], _i32([190, 77]).to(DEV)
+    q = torch.randn(2, 3 * H, D, generator=g).to(torch.bfloat16 if cell in (torch.int8, torch.float8_e4m3fn, F.FP4) else cell)
+    dense, apart = _pages(cell, pool), _pages(cell, pool)
+    byte = torch.uint8 if cell == F.FP4 else cell
+    wide = torch.stack([apart.k.view(byte).view(torch.uint8), torch.full_like(apart.k.view(byte).view(torch.uint8), 99),
+                        apart.v.view(byte).view(torch.uint8)], 1).contiguous()
+    apart = apart._replace(k=wide[:, 0].view(byte).view(cell), v=wide[:, 2].view(byte).view(cell))
+    assert apart.k.stride(0) == 3 * dense.k.stride(0)
+    got = []
+    for pages, t, into_ in ((dense, table.contiguous(), into.contiguous()), (apart, table, into)):
+        w = torch.zeros(2, H, 12 * ps, device=DEV)
+        out = paged_attention(q.to(DEV), pages, t, lengths, key_weights=w)
+        got.append([out, w, *evict_kv_tokens(pages, w, t, lengths, count, into_, last=5)])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and bool((got[0][2] >= 0).all())
+    for a, b in zip(dense, apart):
+        if a is not None:
+            a, b = (x.view(torch.uint8) if x.dtype in (F.FP4, F.E8M0) else x for x in (a, b))
+            assert torch.equal(a.cpu(), b.cpu())
+    assert bool((wide[:, 1] == 99).all())
+
+
+@pytest.mark.parametrize("pair", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, F.FP4)], ids=R.pair_id)
+@pytest.mark.parametrize("G", [2, 17])
+def test_weights_of_many_sequences(pair, G):
+    """More sequences than a workgroup has threads, rows of a key to rows shared out."""
+    from proteus_attention import paged_attention
+
+    dt, cell = pair
+    g = torch.Generator().manual_seed(37)
+    B, H, D, ps, N, T = 600, 1, 32, 16, 320, 4096
+    lengths = [int(n) for n in torch.exp(torch.rand(B, generator=g) * math.log(300)).int()]
+    lengths[7], lengths[300], lengths[599], lengths[11] = T, T - 1, 3000, 0
+    table = torch.randint(0, N, (B, T // ps), generator=g, dtype=torch.int32)
+    pool = _pool(cell, N, H, ps, D, g)
+    q = torch.randn(B, H * G, D, generator=g).to(dt)
+    before = torch.rand(B, H, T, generator=g)
+    w = before.to(DEV)
+    args = (q.to(DEV), _pages(cell, pool), table.to(DEV), _i32(lengths).to(DEV))
+    assert torch.equal(paged_attention(*args, key_weights=w), paged_attention(*args))
+    assert holds(w.cpu(), before, weights(q, _plain(cell, pool), table, lengths), G, D, T)
+
+
+@pytest.mark.parametrize("lengths", [[200, 90], [6000, 90]], ids=str)
+def test_scores_of_plus_infinity(lengths):
+    """One in a row of a group's: its output and the weights of the keys it sees are NaN,
+    wherever the row is cut; the other key-value head's are as they were."""
+    from proteus_attention import KVPages, paged_attention
+
+    g = torch.Generator().manual_seed(41)
+    ps, D, H, N = 16, 32, 2, sum(-(-n // 16) for n in lengths) + 1
+    k, v = (torch.randn(N, H, ps, D, generator=g) for _ in range(2))
+    table = R.make_table(lengths, ps, N, g)
+    k[int(table[0, 5]), 1, 3, 2] = math.inf
+    q = torch.rand(2, 2 * H, D, generator=g) + 0.5
+    w, clean = (torch.zeros(2, H, table.shape[1] * ps, device=DEV) for _ in range(2))
+    rest = (table.to(DEV), _i32(lengths).to(DEV))
+    out = paged_attention(q.to(DEV), KVPages(k.to(DEV), v.to(DEV)), *rest, key_weights=w)
+    same = paged_attention(q.to(DEV), KVPages(k.nan_to_num(posinf=0.0).to(DEV), v.to(DEV)), *rest, key_weights=clean)
+    assert out[0, 2:].isnan().all() and w[0, 1, :lengths[0]].isnan().all() and not w[0, 1, lengths[0]:].any()
+    assert torch.equal(out[0, :2], same[0, :2]) and torch.equal(out[1], same[1])
+    assert torch.equal(w[0, 0], clean[0, 0]) and torch.equal(w[1], clean[1])
+
+
+def test_more_kept_than_there_are():
+    g = torch.Generator().manual_seed(43)
+    for count, bounds in ((900, False), (1500, False), (900, True)):
+        pool = _pool(torch.bfloat16, 120, 2, 16, 32, g, bounds=bounds)
+        table, into = _i32([[3, 1, 2]]), torch.arange(10, 10 + -(-count // 16), dtype=torch.int32)[None]
+        evicts(torch.bfloat16, pool, table, into, torch.rand(1, 2, 48, generator=g), [41], count, 300, 500)
